@@ -314,6 +314,80 @@ int32_t egnn_radius_graph(const double* pos, int64_t N, const int32_t* seg_ptr, 
                           double cutoff, int32_t max_nb, int32_t* rowptr, int32_t* col, int64_t col_capacity,
                           void* tmp, size_t tmp_bytes, int64_t* n_edges, void* stream);
 
+/* ---- attention over the nodes of a graph -------------------------------------
+ * No counterpart in the reference.  The graphs of a batch lie back to back: the
+ * queries of segment b are rows q_ptr[b] .. q_ptr[b + 1] - 1 of q, its keys rows
+ * kv_ptr[b] .. kv_ptr[b + 1] - 1 of k and v (both device int32, n_seg + 1
+ * non-decreasing entries).  With G = Hq / Hkv query heads on each key head, for a
+ * query i and head h (key head h / G) of a segment:
+ *   s_j = scale q_i . k_j,  lse_i = log sum_j e^s_j,  out_i = sum_j e^(s_j - lse_i) v_j
+ * over the keys j of i's segment with key_mask[j] != 0 (NULL: all).  A row without
+ * any key (an empty or fully masked segment, a row outside every segment) has
+ * out = 0, lse = -inf and no gradient; what a masked key, another segment or a row
+ * outside holds, NaN and infinities included, reaches nothing.  Offsets are
+ * clamped to the rows there are, so no access leaves the tensors whatever they
+ * hold; offsets that decrease give unspecified results.
+ * Sums, softmax statistics and lse (Hq, Nq) are fp32; bf16 rounds the
+ * probabilities and their gradients once, for the second product. */
+typedef struct EgnnAttnDims {
+  int64_t Nq, Nk;        /* rows of q, and of k and v; Nq Hq and Nk below 2^31 - 1024 */
+  int32_t n_seg;
+  int32_t Hq, Hkv;       /* heads; Hq a multiple of Hkv */
+  int32_t D;             /* head width, a multiple of 8 up to 128 */
+  int32_t dtype;         /* EGNN_F32 or EGNN_BF16, of q, k, v, out and the gradients */
+  float scale;           /* finite and not 0 */
+} EgnnAttnDims;
+
+/* Strides in elements; a head's D values are contiguous and start 16-byte
+ * aligned (parts of one projection's rows need no copy).  The forward reads the
+ * first eight.  Outputs must not overlap themselves. */
+typedef struct EgnnAttnStrides {
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  int64_t grad_out_row, grad_out_head, grad_q_row, grad_q_head, grad_k_row, grad_k_head, grad_v_row, grad_v_head;
+} EgnnAttnStrides;
+
+/* Workspace bytes; 0 where none is needed (or the dims are refused). */
+size_t egnn_attn_fwd_workspace_bytes(const EgnnAttnDims* dims);
+size_t egnn_attn_bwd_workspace_bytes(const EgnnAttnDims* dims);
+/* Forward.  lse may be NULL (inference). */
+int32_t egnn_attn_fwd(const EgnnAttnDims* dims, const EgnnAttnStrides* strides, const void* q, const void* k, const void* v,
+                      const int32_t* q_ptr, const int32_t* kv_ptr, const uint8_t* key_mask, void* out, float* lse,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* Backward: recomputes the probabilities from lse.  Writes grad_q, grad_k and
+ * grad_v (the last two summed over the heads of a group); deterministic, no
+ * atomics. */
+int32_t egnn_attn_bwd(const EgnnAttnDims* dims, const EgnnAttnStrides* strides, const void* q, const void* k, const void* v,
+                      const void* out, const float* lse, const void* grad_out, const int32_t* q_ptr, const int32_t* kv_ptr,
+                      const uint8_t* key_mask, void* grad_q, void* grad_k, void* grad_v,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- layer norm ----------------------------------------------------------------
+ * No counterpart in the reference.  Over the C values of each of N rows:
+ *   s = x (+ residual),  mu = mean s,  rstd = (mean (s - mu)^2 + eps)^-1/2,
+ *   y = (s - mu) rstd weight + bias
+ * Any C from 1 to 2^20 and any row stride; 16-byte aligned rows and widths are
+ * read and written in 16-byte pieces.  weight and bias may be NULL (1 and 0), in
+ * the dtype of x.  Statistics and sums are fp32; y is made from the unrounded s. */
+typedef struct EgnnNormDims {
+  int64_t N;             /* below 2^31 */
+  int32_t C;
+  int32_t dtype;
+  float eps;             /* >= 0 */
+} EgnnNormDims;
+
+/* Writes y (N, C) and, with a residual, s (N, C) to `sum` (both contiguous);
+ * mean and rstd (N each) for the backward, or both NULL. */
+int32_t egnn_norm_fwd(const EgnnNormDims* dims, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                      const void* weight, const void* bias, void* y, void* sum, float* mean, float* rstd, void* stream);
+size_t egnn_norm_bwd_workspace_bytes(const EgnnNormDims* dims);
+/* Backward from s (the forward's sum, or x without a residual).  grad_x (N, C)
+ * contiguous is the gradient of x and of the residual, grad_sum (may be NULL) the
+ * gradient that reached s directly, added to it.  grad_weight and grad_bias (C)
+ * may be NULL, and need the workspace otherwise; fixed-order sums, no atomics. */
+int32_t egnn_norm_bwd(const EgnnNormDims* dims, const void* grad_y, int64_t ldg, const void* sum, int64_t lds,
+                      const void* weight, const float* mean, const float* rstd, const void* grad_sum, int64_t ldgs,
+                      void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

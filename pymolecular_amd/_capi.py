@@ -6,7 +6,7 @@ There is no fallback: if the library is missing every entry point raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_int32, c_int64, c_size_t, c_void_p, c_char_p
+from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p, c_char_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libpymolecular_egnn.so")
@@ -28,6 +28,8 @@ EXPORTED = (
     "egnn_dense_fwd", "egnn_dense_dgrad", "egnn_dense_wgrad_workspace_bytes", "egnn_dense_wgrad",
     "egnn_profile_enable", "egnn_profile_read",
     "egnn_graph_tmp_bytes", "egnn_knn_graph", "egnn_radius_graph",
+    "egnn_attn_fwd_workspace_bytes", "egnn_attn_bwd_workspace_bytes", "egnn_attn_fwd", "egnn_attn_bwd",
+    "egnn_norm_fwd", "egnn_norm_bwd_workspace_bytes", "egnn_norm_bwd",
 )
 
 # kernel classes of the instrumentation hook
@@ -59,9 +61,23 @@ class EgnnNodeDims(ctypes.Structure):
                 ("residual", c_int32), ("dtype", c_int32)]
 
 
+class EgnnAttnDims(ctypes.Structure):
+    _fields_ = [("Nq", c_int64), ("Nk", c_int64), ("n_seg", c_int32), ("Hq", c_int32), ("Hkv", c_int32),
+                ("D", c_int32), ("dtype", c_int32), ("scale", c_float)]
+
+
+class EgnnAttnStrides(ctypes.Structure):
+    _fields_ = [(n + x, c_int64) for n in ("q", "k", "v", "out", "grad_out", "grad_q", "grad_k", "grad_v")
+                for x in ("_row", "_head")]
+
+
+class EgnnNormDims(ctypes.Structure):
+    _fields_ = [("N", c_int64), ("C", c_int32), ("dtype", c_int32), ("eps", c_float)]
+
+
 _lib = None
 
-ABI_VERSION = 9   # include/egnn.h egnn_abi_version()
+ABI_VERSION = 10   # include/egnn.h egnn_abi_version()
 
 
 def _check_stamp(path=None, stamp=None, digest=None, what="other sources") -> None:
@@ -153,6 +169,21 @@ def lib() -> ctypes.CDLL:
     L.egnn_profile_enable.argtypes = [c_int32]
     L.egnn_profile_read.restype = c_int32
     L.egnn_profile_read.argtypes = [c_int32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(c_int64)]
+    AD, AS, MD = ctypes.POINTER(EgnnAttnDims), ctypes.POINTER(EgnnAttnStrides), ctypes.POINTER(EgnnNormDims)
+    L.egnn_attn_fwd_workspace_bytes.restype = c_size_t
+    L.egnn_attn_fwd_workspace_bytes.argtypes = [AD]
+    L.egnn_attn_bwd_workspace_bytes.restype = c_size_t
+    L.egnn_attn_bwd_workspace_bytes.argtypes = [AD]
+    L.egnn_attn_fwd.restype = c_int32
+    L.egnn_attn_fwd.argtypes = [AD, AS] + [P] * 9 + [c_size_t, P]
+    L.egnn_attn_bwd.restype = c_int32
+    L.egnn_attn_bwd.argtypes = [AD, AS] + [P] * 13 + [c_size_t, P]
+    L.egnn_norm_fwd.restype = c_int32
+    L.egnn_norm_fwd.argtypes = [MD, P, c_int64, P, c_int64] + [P] * 7
+    L.egnn_norm_bwd_workspace_bytes.restype = c_size_t
+    L.egnn_norm_bwd_workspace_bytes.argtypes = [MD]
+    L.egnn_norm_bwd.restype = c_int32
+    L.egnn_norm_bwd.argtypes = [MD, P, c_int64, P, c_int64, P, P, P, P, c_int64, P, P, P, P, c_size_t, P]
     _lib = L
     return L
 

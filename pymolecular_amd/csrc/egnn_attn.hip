@@ -1,0 +1,136 @@
+// C entries of the segment attention: checks, how the axes are cut, workspaces.
+#include "egnn_attn.h"
+
+namespace egnn {
+namespace attn {
+namespace {
+
+bool dims_ok(const EgnnAttnDims* d) {
+  const int64_t top = INT32_MAX - 1024;
+  return d && d->Nq >= 0 && d->Nk >= 0 && d->n_seg >= 0 && d->Hq >= 1 && d->Hkv >= 1 && d->Hq % d->Hkv == 0 && d->D >= 8 &&
+         d->D <= 128 && d->D % 8 == 0 && (d->dtype == EGNN_F32 || d->dtype == EGNN_BF16) && d->scale - d->scale == 0.f &&
+         d->scale != 0.f && d->Nk <= top && d->n_seg <= top && d->Nq <= top && d->Nq * d->Hq <= top;
+}
+
+// own: (virtual) rows of the axis that is cut into tiles, other: rows of the axis a tile walks
+Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads) {
+  const int64_t segs = n_seg > 0 ? n_seg : 1;
+  Plan p;
+  p.waves = own <= 48 * segs ? 1 : 4;
+  const int BQ = 16 * p.waves;
+  p.slots = own / BQ + n_seg + 2;
+  const int64_t tiles = cdiv(own, BQ) > n_seg ? cdiv(own, BQ) : n_seg, blocks = (tiles > 0 ? tiles : 1) * heads;
+  const int64_t len = other / segs;
+  p.nsplit = 1;
+  if (blocks < 512 && len >= 512) {
+    const int64_t want = cdiv(p.waves == 1 ? 4096 : 1024, blocks), most = len / 256;
+    p.nsplit = (int)(want < most ? want : most);
+  }
+  return p;
+}
+Plan plan_q(const EgnnAttnDims* d) { return make_plan(d->Nq * (d->Hq / d->Hkv), d->Nk, d->n_seg, d->Hkv); }
+Plan plan_k(const EgnnAttnDims* d) { return make_plan(d->Nk, d->Nq * (d->Hq / d->Hkv), d->n_seg, d->Hkv); }
+
+size_t fwd_bytes(const EgnnAttnDims* d) {
+  const Plan p = plan_q(d);
+  return p.nsplit == 1 ? 0 : (size_t)p.nsplit * d->Nq * d->Hq * (padded(d->D) + 2) * 4;
+}
+size_t delta_bytes(const EgnnAttnDims* d) { return align_up((size_t)d->Nq * d->Hq * 4); }
+size_t bwd_bytes(const EgnnAttnDims* d) {
+  const Plan pq = plan_q(d), pk = plan_k(d);
+  const size_t q = pq.nsplit == 1 ? 0 : (size_t)pq.nsplit * d->Nq * d->Hq * padded(d->D) * 4;
+  const size_t k = pk.nsplit == 1 ? 0 : (size_t)pk.nsplit * d->Nk * d->Hkv * 2 * padded(d->D) * 4;
+  return delta_bytes(d) + (q > k ? q : k);
+}
+
+bool grid_ok(const EgnnAttnDims* d, const Plan& p) { return p.slots * d->Hkv * p.nsplit <= INT32_MAX; }
+
+// rows and heads 16-byte aligned, heads of a row apart from each other (inputs may overlap, outputs not)
+int check_view(const void* p, int64_t rows, int heads, int D, int64_t rs, int64_t hs, int esz, bool output) {
+  if (rows == 0) return EGNN_OK;
+  if (!p) return EGNN_ERR_NULL;
+  if (rs < 0 || hs < 0 || (rs * esz) % 16 || (hs * esz) % 16) return EGNN_ERR_STRIDE;
+  if (output && ((heads > 1 && hs < D) || (rows > 1 && rs < D))) return EGNN_ERR_STRIDE;
+  return (uintptr_t)p % 16 ? EGNN_ERR_ALIGN : EGNN_OK;
+}
+
+Args make_args(const EgnnAttnDims* d, const EgnnAttnStrides* s) {
+  Args a{};
+  a.q_r = s->q_row; a.q_h = s->q_head; a.k_r = s->k_row; a.k_h = s->k_head; a.v_r = s->v_row; a.v_h = s->v_head;
+  a.o_r = s->out_row; a.o_h = s->out_head; a.go_r = s->grad_out_row; a.go_h = s->grad_out_head;
+  a.gq_r = s->grad_q_row; a.gq_h = s->grad_q_head; a.gk_r = s->grad_k_row; a.gk_h = s->grad_k_head;
+  a.gv_r = s->grad_v_row; a.gv_h = s->grad_v_head;
+  a.Nq = (int32_t)d->Nq; a.Nk = (int32_t)d->Nk; a.B = d->n_seg; a.Hq = d->Hq; a.Hkv = d->Hkv; a.G = d->Hq / d->Hkv; a.D = d->D;
+  a.scale = d->scale < 0 ? -d->scale : d->scale;
+  a.c2 = a.scale * kLog2e;
+  a.flip = d->scale < 0 ? 0x80000000u : 0u;
+  return a;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace egnn
+
+using namespace egnn::attn;
+
+extern "C" {
+
+size_t egnn_attn_fwd_workspace_bytes(const EgnnAttnDims* d) { return dims_ok(d) ? fwd_bytes(d) : 0; }
+size_t egnn_attn_bwd_workspace_bytes(const EgnnAttnDims* d) { return dims_ok(d) ? bwd_bytes(d) : 0; }
+
+#define EGNN_TRY(x) do { const int rc_ = (x); if (rc_ != EGNN_OK) return rc_; } while (0)
+
+int32_t egnn_attn_fwd(const EgnnAttnDims* d, const EgnnAttnStrides* s, const void* q, const void* k, const void* v,
+                      const int32_t* q_ptr, const int32_t* kv_ptr, const uint8_t* key_mask, void* out, float* lse, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  if (!d || !s) return EGNN_ERR_NULL;
+  if (!dims_ok(d)) return EGNN_ERR_DIMS;
+  const int esz = d->dtype == EGNN_F32 ? 4 : 2;
+  if (!q_ptr || !kv_ptr) return EGNN_ERR_NULL;
+  EGNN_TRY(check_view(q, d->Nq, d->Hq, d->D, s->q_row, s->q_head, esz, false));
+  EGNN_TRY(check_view(k, d->Nk, d->Hkv, d->D, s->k_row, s->k_head, esz, false));
+  EGNN_TRY(check_view(v, d->Nk, d->Hkv, d->D, s->v_row, s->v_head, esz, false));
+  EGNN_TRY(check_view(out, d->Nq, d->Hq, d->D, s->out_row, s->out_head, esz, true));
+  const Plan p = plan_q(d);
+  if (!grid_ok(d, p)) return EGNN_ERR_DIMS;
+  const size_t need = fwd_bytes(d);
+  if (need && (!workspace || workspace_bytes < need)) return EGNN_ERR_WORKSPACE;
+  if (need && (uintptr_t)workspace % 16) return EGNN_ERR_ALIGN;
+  if (d->Nq == 0) return EGNN_OK;
+  Args a = make_args(d, s);
+  a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.q_ptr = q_ptr; a.kv_ptr = kv_ptr; a.mask = key_mask;
+  a.nsplit = p.nsplit;
+  a.part = (float*)workspace;
+  return launch_fwd(a, d->dtype == EGNN_BF16, p, (hipStream_t)stream) ? EGNN_ERR_HIP : EGNN_OK;
+}
+
+int32_t egnn_attn_bwd(const EgnnAttnDims* d, const EgnnAttnStrides* s, const void* q, const void* k, const void* v, const void* out,
+                      const float* lse, const void* grad_out, const int32_t* q_ptr, const int32_t* kv_ptr, const uint8_t* key_mask,
+                      void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!d || !s) return EGNN_ERR_NULL;
+  if (!dims_ok(d)) return EGNN_ERR_DIMS;
+  const int esz = d->dtype == EGNN_F32 ? 4 : 2;
+  if (!q_ptr || !kv_ptr || (d->Nq && !lse)) return EGNN_ERR_NULL;
+  EGNN_TRY(check_view(q, d->Nq, d->Hq, d->D, s->q_row, s->q_head, esz, false));
+  EGNN_TRY(check_view(k, d->Nk, d->Hkv, d->D, s->k_row, s->k_head, esz, false));
+  EGNN_TRY(check_view(v, d->Nk, d->Hkv, d->D, s->v_row, s->v_head, esz, false));
+  EGNN_TRY(check_view(out, d->Nq, d->Hq, d->D, s->out_row, s->out_head, esz, false));
+  EGNN_TRY(check_view(grad_out, d->Nq, d->Hq, d->D, s->grad_out_row, s->grad_out_head, esz, false));
+  EGNN_TRY(check_view(grad_q, d->Nq, d->Hq, d->D, s->grad_q_row, s->grad_q_head, esz, true));
+  EGNN_TRY(check_view(grad_k, d->Nk, d->Hkv, d->D, s->grad_k_row, s->grad_k_head, esz, true));
+  EGNN_TRY(check_view(grad_v, d->Nk, d->Hkv, d->D, s->grad_v_row, s->grad_v_head, esz, true));
+  const Plan pq = plan_q(d), pk = plan_k(d);
+  if (!grid_ok(d, pq) || !grid_ok(d, pk)) return EGNN_ERR_DIMS;
+  const size_t need = bwd_bytes(d);
+  if (need && (!workspace || workspace_bytes < need)) return EGNN_ERR_WORKSPACE;
+  if (need && (uintptr_t)workspace % 16) return EGNN_ERR_ALIGN;
+  if (d->Nq == 0 && d->Nk == 0) return EGNN_OK;
+  Args a = make_args(d, s);
+  a.q = q; a.k = k; a.v = v; a.o = out; a.lse = (float*)lse; a.go = grad_out; a.gq = grad_q; a.gk = grad_k; a.gv = grad_v;
+  a.q_ptr = q_ptr; a.kv_ptr = kv_ptr; a.mask = key_mask;
+  a.delta = (float*)workspace;
+  a.part = (float*)((char*)workspace + delta_bytes(d));
+  return launch_bwd(a, d->dtype == EGNN_BF16, pq, pk, (hipStream_t)stream) ? EGNN_ERR_HIP : EGNN_OK;
+}
+
+}  // extern "C"

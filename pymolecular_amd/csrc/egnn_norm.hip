@@ -1,0 +1,381 @@
+// Layer norm over the last axis, with the residual sum in front of it, and its backward.
+//   s = x (+ r), mu = mean s, rstd = (mean (s - mu)^2 + eps)^-1/2, xh = (s - mu) rstd, y = xh w + b
+//   t = gy w, gs = rstd (t - mean t - xh mean(t xh)) (+ g_sum), gw = sum_rows gy xh, gb = sum_rows gy
+// A row lives in the registers of LPR lanes, so it is read once and the variance is taken around the mean.  The backward's
+// blocks walk the rows with a fixed stride; a lane keeps the sums of gw and gb of its columns in fp32 registers, a
+// block's row groups are joined in LDS and its sums leave as one partial row, which a second launch adds up in order.
+#include "egnn_device.h"
+#include "egnn_internal.h"
+
+namespace egnn {
+namespace norm {
+
+struct Args {
+  const void *x, *r, *w, *b, *gy, *gsum;
+  void *y, *s, *gx, *gw, *gb;
+  float *mean, *rstd, *part;
+  int64_t N, ldx, ldr, ldg, ldgs;
+  int32_t C;
+  float eps;
+};
+
+template <typename T, int VEC> struct Vec;
+template <> struct Vec<float, 4> {
+  static __device__ __forceinline__ void load(const float* p, float* v) {
+    const f32x4 t = load4_f32(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = t[i];
+  }
+  static __device__ __forceinline__ void store(float* p, const float* v) { *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]}; }
+};
+template <> struct Vec<bf16, 8> {
+  static __device__ __forceinline__ void load(const bf16* p, float* v) {
+    const bf16x8 t = load_chunk(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+  }
+  static __device__ __forceinline__ void store(bf16* p, const float* v) {
+    bf16x8 t;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = (bf16)v[i];
+    store_chunk(p, t);
+  }
+};
+template <typename T> struct Vec<T, 1> {
+  static __device__ __forceinline__ void load(const T* p, float* v) { v[0] = to_f32(*p); }
+  static __device__ __forceinline__ void store(T* p, const float* v) { *p = from_f32<T>(v[0]); }
+};
+
+template <int LPR> __device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int x = LPR / 2; x; x >>= 1) v += shfl_xor(v, x);
+  return v;
+}
+
+constexpr int NT = 256;
+
+template <typename T, int VEC, int LPR, int VPL>
+__global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
+  const int lane = threadIdx.x % LPR;
+  const int64_t n = (int64_t)blockIdx.x * (NT / LPR) + threadIdx.x / LPR;
+  const bool live = n < a.N;
+  float v[VPL][VEC];
+  float sum = 0.f;
+#pragma unroll
+  for (int p = 0; p < VPL; ++p) {
+    const int f = (p * LPR + lane) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[p][i] = 0.f;
+    if (live && f < a.C) {
+      Vec<T, VEC>::load((const T*)a.x + n * a.ldx + f, v[p]);
+      if (a.r) {
+        float r[VEC];
+        Vec<T, VEC>::load((const T*)a.r + n * a.ldr + f, r);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[p][i] += r[i];
+        Vec<T, VEC>::store((T*)a.s + n * a.C + f, v[p]);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum += v[p][i];
+    }
+  }
+  const float mean = row_sum<LPR>(sum) / a.C;
+  float sq = 0.f;
+#pragma unroll
+  for (int p = 0; p < VPL; ++p)
+    if ((p * LPR + lane) * VEC < a.C) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { const float d = v[p][i] - mean; sq = __builtin_fmaf(d, d, sq); }
+    }
+  const float rstd = 1.0f / sqrtf(row_sum<LPR>(sq) / a.C + a.eps);
+  if (!live) return;
+  if (lane == 0 && a.mean) { a.mean[n] = mean; a.rstd[n] = rstd; }
+#pragma unroll
+  for (int p = 0; p < VPL; ++p) {
+    const int f = (p * LPR + lane) * VEC;
+    if (f < a.C) {
+      float w[VEC], b[VEC], y[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { w[i] = 1.f; b[i] = 0.f; }
+      if (a.w) Vec<T, VEC>::load((const T*)a.w + f, w);
+      if (a.b) Vec<T, VEC>::load((const T*)a.b + f, b);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) y[i] = __builtin_fmaf((v[p][i] - mean) * rstd, w[i], b[i]);
+      Vec<T, VEC>::store((T*)a.y + n * a.C + f, y);
+    }
+  }
+}
+
+template <typename T, int VEC, int LPR, int VPL>
+__global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
+  constexpr int RG = NT / LPR, W = LPR * VPL * VEC;
+  __shared__ float red[RG][W];
+  const int lane = threadIdx.x % LPR, rg = threadIdx.x / LPR;
+  float gw[VPL][VEC], gb[VPL][VEC], w[VPL][VEC];
+#pragma unroll
+  for (int p = 0; p < VPL; ++p) {
+    const int f = (p * LPR + lane) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { gw[p][i] = 0.f; gb[p][i] = 0.f; w[p][i] = f < a.C ? 1.f : 0.f; }
+    if (a.w && f < a.C) Vec<T, VEC>::load((const T*)a.w + f, w[p]);
+  }
+  for (int64_t n0 = (int64_t)blockIdx.x * RG; n0 < a.N; n0 += (int64_t)gridDim.x * RG) {
+    const int64_t n = n0 + rg;
+    const bool live = n < a.N;
+    const float mean = live ? a.mean[n] : 0.f, rstd = live ? a.rstd[n] : 0.f;
+    float xh[VPL][VEC], t[VPL][VEC];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int p = 0; p < VPL; ++p) {
+      const int f = (p * LPR + lane) * VEC;
+      const bool on = live && f < a.C;
+      float g[VEC], x[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { g[i] = 0.f; x[i] = mean; }
+      if (on) {
+        Vec<T, VEC>::load((const T*)a.gy + n * a.ldg + f, g);
+        Vec<T, VEC>::load((const T*)a.x + n * a.ldx + f, x);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        xh[p][i] = (x[i] - mean) * rstd;
+        t[p][i] = g[i] * w[p][i];
+        gw[p][i] = __builtin_fmaf(g[i], xh[p][i], gw[p][i]);
+        gb[p][i] += g[i];
+        s1 += t[p][i];
+        s2 = __builtin_fmaf(t[p][i], xh[p][i], s2);
+      }
+    }
+    const float m1 = row_sum<LPR>(s1) / a.C, m2 = row_sum<LPR>(s2) / a.C;
+#pragma unroll
+    for (int p = 0; p < VPL; ++p) {
+      const int f = (p * LPR + lane) * VEC;
+      if (live && f < a.C) {
+        float o[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = rstd * (t[p][i] - m1 - xh[p][i] * m2);
+        if (a.gsum) {
+          float e[VEC];
+          Vec<T, VEC>::load((const T*)a.gsum + n * a.ldgs + f, e);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) o[i] += e[i];
+        }
+        Vec<T, VEC>::store((T*)a.gx + n * a.C + f, o);
+      }
+    }
+  }
+  if (!a.part) return;
+  float* out = a.part + (int64_t)blockIdx.x * 2 * a.C;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < VPL; ++p)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) red[rg][(p * LPR + lane) * VEC + i] = half ? gb[p][i] : gw[p][i];
+    __syncthreads();
+    for (int f = threadIdx.x; f < a.C; f += NT) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < RG; ++k) s += red[k][f];
+      out[half * a.C + f] = s;
+    }
+  }
+}
+
+// rows wider than a wave's registers: one block a row, the row read again (from cache) for each pass
+__device__ __forceinline__ float block_sum(float v, float* buf) {
+  v = row_sum<64>(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return buf[0] + buf[1] + buf[2] + buf[3];
+}
+template <typename T>
+__global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
+  __shared__ float buf[4];
+  const int64_t n = blockIdx.x;
+  const T *x = (const T*)a.x + n * a.ldx, *r = a.r ? (const T*)a.r + n * a.ldr : nullptr;
+  auto val = [&](int f) { return to_f32(x[f]) + (r ? to_f32(r[f]) : 0.f); };
+  float s = 0.f;
+  for (int f = threadIdx.x; f < a.C; f += NT) s += val(f);
+  const float mean = block_sum(s, buf) / a.C;
+  float q = 0.f;
+  for (int f = threadIdx.x; f < a.C; f += NT) { const float d = val(f) - mean; q = __builtin_fmaf(d, d, q); }
+  const float rstd = 1.0f / sqrtf(block_sum(q, buf) / a.C + a.eps);
+  if (threadIdx.x == 0 && a.mean) { a.mean[n] = mean; a.rstd[n] = rstd; }
+  for (int f = threadIdx.x; f < a.C; f += NT) {
+    const float v = val(f), w = a.w ? to_f32(((const T*)a.w)[f]) : 1.f, b = a.b ? to_f32(((const T*)a.b)[f]) : 0.f;
+    if (r) ((T*)a.s)[n * a.C + f] = from_f32<T>(v);
+    ((T*)a.y)[n * a.C + f] = from_f32<T>(__builtin_fmaf((v - mean) * rstd, w, b));
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(NT) void bwd_wide_kernel(Args a) {
+  __shared__ float buf[4];
+  const int64_t n = blockIdx.x;
+  const T *x = (const T*)a.x + n * a.ldx, *g = (const T*)a.gy + n * a.ldg;
+  const float mean = a.mean[n], rstd = a.rstd[n];
+  float s1 = 0.f, s2 = 0.f;
+  for (int f = threadIdx.x; f < a.C; f += NT) {
+    const float t = to_f32(g[f]) * (a.w ? to_f32(((const T*)a.w)[f]) : 1.f);
+    s1 += t;
+    s2 = __builtin_fmaf(t, (to_f32(x[f]) - mean) * rstd, s2);
+  }
+  const float m1 = block_sum(s1, buf) / a.C, m2 = block_sum(s2, buf) / a.C;
+  for (int f = threadIdx.x; f < a.C; f += NT) {
+    const float t = to_f32(g[f]) * (a.w ? to_f32(((const T*)a.w)[f]) : 1.f);
+    float o = rstd * (t - m1 - (to_f32(x[f]) - mean) * rstd * m2);
+    if (a.gsum) o += to_f32(((const T*)a.gsum)[n * a.ldgs + f]);
+    ((T*)a.gx)[n * a.C + f] = from_f32<T>(o);
+  }
+}
+// gw and gb of wide rows: a thread a column, rows of one of gridDim.y parts
+template <typename T>
+__global__ __launch_bounds__(NT) void bwd_wide_weights_kernel(Args a) {
+  const int f = blockIdx.x * NT + threadIdx.x;
+  if (f >= a.C) return;
+  float gw = 0.f, gb = 0.f;
+  for (int64_t n = blockIdx.y; n < a.N; n += gridDim.y) {
+    const float g = to_f32(((const T*)a.gy)[n * a.ldg + f]);
+    gw = __builtin_fmaf(g, (to_f32(((const T*)a.x)[n * a.ldx + f]) - a.mean[n]) * a.rstd[n], gw);
+    gb += g;
+  }
+  float* out = a.part + (int64_t)blockIdx.y * 2 * a.C;
+  out[f] = gw;
+  out[a.C + f] = gb;
+}
+
+// gw, gb = sums of the partial rows: 64 columns a block, 16 row groups joined in order
+template <typename T>
+__global__ __launch_bounds__(1024) void sum_kernel(const float* part, int nblk, int C, T* gw, T* gb) {
+  __shared__ float red[16][64];
+  const int c = threadIdx.x & 63, k = threadIdx.x >> 6;
+  const int f = blockIdx.x * 64 + c;
+  float s = 0.f;
+  if (f < 2 * C)
+    for (int b = k; b < nblk; b += 16) s += part[(int64_t)b * 2 * C + f];
+  red[k][c] = s;
+  __syncthreads();
+  if (k || f >= 2 * C) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += red[i][c];
+  if (f < C) { if (gw) gw[f] = from_f32<T>(s); }
+  else if (gb) gb[f - C] = from_f32<T>(s);
+}
+
+constexpr int kMaxBlocks = 1024;   // partial rows of the weight gradients
+
+// lanes and vectors of a row: the fewest vectors a lane, then the fewest lanes
+struct Shape { int vec, lpr, vpl; };
+static bool shape_of(int C, int vec, Shape* s) {
+  const int n = (C + vec - 1) / vec;
+  s->vec = vec;
+  for (s->vpl = 1; s->vpl <= 8; s->vpl *= 2)
+    for (s->lpr = 4; s->lpr <= 64; s->lpr *= 2)
+      if (s->lpr * s->vpl >= n && (s->vpl == 1 || s->lpr == 64)) return true;
+  return false;
+}
+static int64_t part_rows(int64_t N) { return N < 1 ? 1 : (N < kMaxBlocks ? N : kMaxBlocks); }
+
+template <typename T, int VEC, int LPR, int VPL>
+static void launch_shape(const Args& a, bool bwd, hipStream_t st, int* nblk) {
+  const int64_t rg = NT / LPR, n = cdiv(a.N, rg);
+  if (!bwd) { fwd_kernel<T, VEC, LPR, VPL><<<(uint32_t)n, NT, 0, st>>>(a); return; }
+  *nblk = (int)(n < kMaxBlocks ? n : kMaxBlocks);
+  bwd_kernel<T, VEC, LPR, VPL><<<(uint32_t)*nblk, NT, 0, st>>>(a);
+}
+template <typename T, int VEC>
+static void launch_vec(const Args& a, const Shape& s, bool bwd, hipStream_t st, int* nblk) {
+  if (s.vpl == 1) {
+    switch (s.lpr) {
+      case 4: return launch_shape<T, VEC, 4, 1>(a, bwd, st, nblk);
+      case 8: return launch_shape<T, VEC, 8, 1>(a, bwd, st, nblk);
+      case 16: return launch_shape<T, VEC, 16, 1>(a, bwd, st, nblk);
+      case 32: return launch_shape<T, VEC, 32, 1>(a, bwd, st, nblk);
+      default: return launch_shape<T, VEC, 64, 1>(a, bwd, st, nblk);
+    }
+  }
+  if (s.vpl == 2) return launch_shape<T, VEC, 64, 2>(a, bwd, st, nblk);
+  if (s.vpl == 4) return launch_shape<T, VEC, 64, 4>(a, bwd, st, nblk);
+  launch_shape<T, VEC, 64, 8>(a, bwd, st, nblk);
+}
+
+// 16-byte pieces where the width, every row and every vector allow them, else single values
+template <typename T>
+static int launch(const Args& a, bool bwd, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  auto al = [&](const void* p, int64_t ld) { return !p || ((uintptr_t)p % 16 == 0 && ld % V == 0); };
+  const bool vec = a.C % V == 0 && al(a.x, a.ldx) && al(a.r, a.ldr) && al(a.gy, a.ldg) && al(a.gsum, a.ldgs) && al(a.w, 0) &&
+                   al(a.b, 0) && al(a.y, 0) && al(a.s, 0) && al(a.gx, 0);
+  Shape s;
+  int nblk = 0;
+  if (a.N) {
+    if (vec && shape_of(a.C, V, &s)) launch_vec<T, V>(a, s, bwd, st, &nblk);
+    else if (shape_of(a.C, 1, &s)) launch_vec<T, 1>(a, s, bwd, st, &nblk);
+    else if (!bwd) fwd_wide_kernel<T><<<(uint32_t)a.N, NT, 0, st>>>(a);
+    else {
+      bwd_wide_kernel<T><<<(uint32_t)a.N, NT, 0, st>>>(a);
+      if (a.part) {
+        nblk = (int)(part_rows(a.N) < 128 ? part_rows(a.N) : 128);
+        bwd_wide_weights_kernel<T><<<dim3((uint32_t)cdiv(a.C, NT), (uint32_t)nblk), NT, 0, st>>>(a);
+      }
+    }
+  }
+  if (bwd && a.part) sum_kernel<T><<<(uint32_t)cdiv(2 * (int64_t)a.C, 64), 1024, 0, st>>>(a.part, nblk, a.C, (T*)a.gw, (T*)a.gb);
+  return hipGetLastError() == hipSuccess ? EGNN_OK : EGNN_ERR_HIP;
+}
+
+static bool dims_ok(const EgnnNormDims* d) {
+  return d->N >= 0 && d->N <= INT32_MAX && d->C >= 1 && d->C <= 1 << 20 && (d->dtype == EGNN_F32 || d->dtype == EGNN_BF16) &&
+         d->eps >= 0.f && d->eps - d->eps == 0.f;
+}
+
+}  // namespace norm
+}  // namespace egnn
+
+using namespace egnn::norm;
+
+extern "C" {
+
+size_t egnn_norm_bwd_workspace_bytes(const EgnnNormDims* d) {
+  return d && dims_ok(d) ? (size_t)part_rows(d->N) * 2 * d->C * 4 : 0;
+}
+
+int32_t egnn_norm_fwd(const EgnnNormDims* d, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                      const void* bias, void* y, void* sum, float* mean, float* rstd, void* stream) {
+  if (!d) return EGNN_ERR_NULL;
+  if (!dims_ok(d)) return EGNN_ERR_DIMS;
+  if (!mean != !rstd || (residual && !sum) || (d->N && (!x || !y))) return EGNN_ERR_NULL;
+  if (ldx < 0 || (residual && ldr < 0)) return EGNN_ERR_STRIDE;
+  const uintptr_t e = d->dtype == EGNN_F32 ? 4 : 2;
+  if ((uintptr_t)x % e || (uintptr_t)residual % e || (uintptr_t)weight % e || (uintptr_t)bias % e || (uintptr_t)y % e ||
+      (uintptr_t)sum % e || (uintptr_t)mean % 4 || (uintptr_t)rstd % 4)
+    return EGNN_ERR_ALIGN;
+  Args a{};
+  a.x = x; a.ldx = ldx; a.r = residual; a.ldr = ldr; a.w = weight; a.b = bias; a.y = y; a.s = residual ? sum : nullptr;
+  a.mean = mean; a.rstd = rstd; a.N = d->N; a.C = d->C; a.eps = d->eps;
+  return d->dtype == EGNN_BF16 ? launch<egnn::bf16>(a, false, (hipStream_t)stream) : launch<float>(a, false, (hipStream_t)stream);
+}
+
+int32_t egnn_norm_bwd(const EgnnNormDims* d, const void* grad_y, int64_t ldg, const void* sum, int64_t lds, const void* weight,
+                      const float* mean, const float* rstd, const void* grad_sum, int64_t ldgs, void* grad_x, void* grad_weight,
+                      void* grad_bias, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!d) return EGNN_ERR_NULL;
+  if (!dims_ok(d)) return EGNN_ERR_DIMS;
+  if (d->N && (!grad_y || !sum || !mean || !rstd || !grad_x)) return EGNN_ERR_NULL;
+  if (ldg < 0 || lds < 0 || (grad_sum && ldgs < 0)) return EGNN_ERR_STRIDE;
+  const uintptr_t e = d->dtype == EGNN_F32 ? 4 : 2;
+  if ((uintptr_t)grad_y % e || (uintptr_t)sum % e || (uintptr_t)weight % e || (uintptr_t)grad_sum % e || (uintptr_t)grad_x % e ||
+      (uintptr_t)grad_weight % e || (uintptr_t)grad_bias % e || (uintptr_t)mean % 4 || (uintptr_t)rstd % 4 || (uintptr_t)workspace % 16)
+    return EGNN_ERR_ALIGN;
+  const bool weights = grad_weight || grad_bias;
+  if (weights && (!workspace || workspace_bytes < egnn_norm_bwd_workspace_bytes(d))) return EGNN_ERR_WORKSPACE;
+  Args a{};
+  a.gy = grad_y; a.ldg = ldg; a.x = sum; a.ldx = lds; a.w = weight; a.mean = (float*)mean; a.rstd = (float*)rstd;
+  a.gsum = grad_sum; a.ldgs = ldgs; a.gx = grad_x; a.gw = grad_weight; a.gb = grad_bias;
+  a.part = weights ? (float*)workspace : nullptr; a.N = d->N; a.C = d->C; a.eps = d->eps;
+  return d->dtype == EGNN_BF16 ? launch<egnn::bf16>(a, true, (hipStream_t)stream) : launch<float>(a, true, (hipStream_t)stream);
+}
+
+}  // extern "C"
