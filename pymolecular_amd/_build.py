@@ -51,6 +51,8 @@ FILE_FLAGS = {
     "egnn_wbwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "egnn_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "egnn_f32s.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "egnn_attn_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "egnn_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -22,12 +22,25 @@
 #include "egnn_device.h"
 #include "egnn_internal.h"
 #include "egnn_split.h"
+#include <type_traits>
 
 namespace egnn {
 namespace attn {
 
-constexpr int TK = 32;                       // rows of the other axis in one step
+constexpr int TK = 32;                       // rows of the other axis that one product contracts
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+
+// n / d by a multiplication, for n < 2^31 (m = 0: d is 1)
+struct Div {
+  uint32_t m, s;
+  __host__ static Div of(uint32_t d) {
+    if (d <= 1) return Div{0, 0};
+    uint32_t s = 0;
+    while ((1u << s) < d) ++s;             // 2^(s-1) < d <= 2^s
+    return Div{(uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), s - 1};
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return m ? __umulhi(n, m) >> s : n; }
+};
 
 struct Args {
   const void *q, *k, *v, *go;
@@ -39,6 +52,7 @@ struct Args {
   const int32_t *q_ptr, *kv_ptr;
   const uint8_t* mask;                       // [Nk] or null
   int32_t Nq, Nk, B, Hq, Hkv, G, D;
+  Div by_g, by_heads, by_split;              // divisions by G, Hkv and nsplit
   float c2;                                  // |scale| log2 e
   float scale;                               // |scale|
   uint32_t flip;                             // sign bit of a negative scale: q enters negated
@@ -46,16 +60,29 @@ struct Args {
   float* part;                               // split partials
 };
 
-// How one axis is cut: slots of 16 waves rows, and the parts the other axis is walked in
-struct Plan { int64_t slots; int waves, nsplit; };
+// How one axis is cut into tiles, and the parts the other axis is walked in
+struct Plan {
+  int64_t slots;
+  int form;                                  // 0: a wave a tile of 16 rows; 1, 2: a workgroup of 4 waves, 64 or 128 rows
+  int nsplit;
+  int rows() const { return form == 0 ? 16 : 64 * form; }
+};
 inline int padded(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 int launch_fwd(const Args& a, bool is_bf16, const Plan& p, hipStream_t st);
 int launch_bwd(const Args& a, bool is_bf16, const Plan& pq, const Plan& pk, hipStream_t st);
 
 // ---- operand fragments ----------------------------------------------------------
+// Frag: 8 values a lane, a 32-deep slice of an operand.  Half: 4 values, a 16-deep slice (head widths up to 16).
+// Raw: 8 values as they lie in memory.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+struct Half3 { bf16x4 p0, p1, p2; };
 template <typename T> struct Num;
-template <> struct Num<bf16> { static constexpr int planes = 1; typedef bf16x8 Frag; typedef bf16x8 Raw; };
-template <> struct Num<float> { static constexpr int planes = 3; typedef split::Chunk3 Frag; typedef f32x8 Raw; };
+template <> struct Num<bf16> { static constexpr int planes = 1; typedef bf16x8 Frag; typedef bf16x4 Half; typedef bf16x8 Raw; };
+template <> struct Num<float> { static constexpr int planes = 3; typedef split::Chunk3 Frag; typedef Half3 Half; typedef f32x8 Raw; };
+
+__device__ __forceinline__ void mma16(f32x4& acc, const bf16x4& a, const bf16x4& b) {   // A[r][k], B[k][n]: k = 4g + s
+  acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), acc, 0, 0, 0);
+}
 
 __device__ __forceinline__ bf16x8 to_frag(const bf16x8& r) { return r; }
 __device__ __forceinline__ split::Chunk3 to_frag(const f32x8& r) { return split::split_chunk(r.lo, r.hi); }
@@ -74,19 +101,20 @@ __device__ __forceinline__ f32x8 negate(const f32x8& r, uint32_t flip) {
   return f32x8{split::flip_sign(r.lo, flip), split::flip_sign(r.hi, flip)};
 }
 
-// sum over NK 32-deep slices of a(kk) b(kk)
-template <int NK, typename FA> __device__ __forceinline__ f32x4 product(const bf16x8* b, FA a) {
-  f32x4 s = zero4();
-#pragma unroll
-  for (int kk = 0; kk < NK; ++kk) mma(s, a(kk), b[kk]);
-  return s;
+__device__ __forceinline__ void product1(f32x4& hi, f32x4&, const bf16x8& a, const bf16x8& b) { mma(hi, a, b); }
+__device__ __forceinline__ void product1(f32x4& hi, f32x4&, const bf16x4& a, const bf16x4& b) { mma16(hi, a, b); }
+__device__ __forceinline__ void product1(f32x4& hi, f32x4& lo, const split::Chunk3& a, const split::Chunk3& b) { split::mma3(hi, lo, a, b); }
+__device__ __forceinline__ void product1(f32x4& hi, f32x4& lo, const Half3& a, const Half3& b) {
+  mma16(lo, a.p2, b.p0);
+  mma16(hi, a.p0, b.p0);
+  mma16(lo, a.p0, b.p2);
+  mma16(lo, a.p1, b.p1);
+  mma16(lo, a.p1, b.p0);
+  mma16(lo, a.p0, b.p1);
 }
-template <int NK, typename FA> __device__ __forceinline__ f32x4 product(const split::Chunk3* b, FA a) {
-  f32x4 hi = zero4(), lo = zero4();
-#pragma unroll
-  for (int kk = 0; kk < NK; ++kk) split::mma3(hi, lo, a(kk), b[kk]);
-  return split::joined(hi, lo);
-}
+template <typename T> __device__ __forceinline__ f32x4 result(const f32x4& hi, const f32x4& lo);
+template <> __device__ __forceinline__ f32x4 result<bf16>(const f32x4& hi, const f32x4&) { return hi; }
+template <> __device__ __forceinline__ f32x4 result<float>(const f32x4& hi, const f32x4& lo) { return split::joined(hi, lo); }
 // acc += a b, one slice.  fp32: the slice's sum is made apart and added in fp32, so a long axis is not summed by the
 // matrix unit, which rounds to one side
 __device__ __forceinline__ void accumulate(f32x4& acc, const bf16x8& a, const bf16x8& b) { mma(acc, a, b); }
@@ -96,48 +124,119 @@ __device__ __forceinline__ void accumulate(f32x4& acc, const split::Chunk3& a, c
   acc += split::joined(hi, lo);
 }
 
-// ---- a tile of TK rows in LDS -----------------------------------------------------
-// [plane][row][KP + 8] bf16, features past D zero.  The pitch is an odd number of 16-byte units: the 16 rows that one
-// row read touches start on different banks, and so do the rows of a transposing read.
-template <typename T, int DP> struct Tile {
-  static constexpr int KP = DP < 32 ? 32 : DP, NK = KP / 32, NB = DP / 16, pitch = KP + 8, plane = TK * pitch;
-  static constexpr int elems = Num<T>::planes * plane;
+// ---- buffer loads -------------------------------------------------------------------
+// Rows 0 .. n - 1 of a tensor part (n >= 1), the last one `last` bytes wide, as a range-checked buffer: rows past them
+// read as zeros, and so do features past the head's width, which get the offset kOob.  (64 rows of at most 2^24 bytes
+// and a group's heads of at most 2^29 stay below 2^31.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* base, int n, int64_t row_bytes, int last) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)((n - 1) * row_bytes) + last, kBufFlags);
+}
+__device__ __forceinline__ bf16x8 load8(const bf16*, __amdgpu_buffer_rsrc_t b, uint32_t off) {
+  return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(b, (int)off, 0, 0));
+}
+__device__ __forceinline__ f32x8 load8(const float*, __amdgpu_buffer_rsrc_t b, uint32_t off) {
+  f32x8 r;
+  r.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(b, (int)off, 0, 0));
+  r.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(b, (int)off, 16, 0));
+  return r;
+}
 
-  // A[r][k] = tile[16 blk + r][32 kk + 8g + s]
-  static __device__ __forceinline__ typename Num<T>::Frag rows(const bf16* t, int blk, int kk, int c, int g) {
-    const bf16* p = t + (16 * blk + c) * pitch + 32 * kk + 8 * g;
-    if constexpr (Num<T>::planes == 1) return load_chunk(p);
-    else return split::Chunk3{load_chunk(p), load_chunk(p + plane), load_chunk(p + 2 * plane)};
+// ---- a tile of rows in LDS ------------------------------------------------------------
+// [plane][row][DP + 8] bf16, features past D zero.  The pitch is an odd number of 16-byte units: the 16 rows that one
+// row read touches start on different banks, and so do the rows of a transposing read.  KT: steps of TK rows.
+template <typename T, int DP, int KT = 1> struct Tile {
+  static constexpr bool half = DP == 16;
+  static constexpr int NK = half ? 1 : DP / 32, NB = DP / 16, pitch = DP + 8, plane = KT * TK * pitch;
+  static constexpr int elems = Num<T>::planes * plane;
+  typedef typename std::conditional<half, typename Num<T>::Half, typename Num<T>::Frag>::type Feat;   // over features
+
+  // A[r][k] = tile[16 blk + r][features of slice kk]
+  static __device__ __forceinline__ Feat rows(const bf16* t, int blk, int kk, int c, int g) {
+    typedef typename std::conditional<half, bf16x4, bf16x8>::type V;
+    const bf16* p = t + (16 * blk + c) * pitch + (half ? 4 * g : 32 * kk + 8 * g);
+    auto at = [](const bf16* q) { return *reinterpret_cast<const V*>(q); };
+    if constexpr (Num<T>::planes == 1) return at(p);
+    else return Feat{at(p), at(p + plane), at(p + 2 * plane)};
   }
-  // A[r][k] = tile[kappa_chain(g, s)][16 blk + r]
+  // A[r][k] = tile[32 step + kappa_chain(g, s)][16 blk + r]
   static __device__ __forceinline__ bf16x8 tr(const bf16* p) {
     const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)p);
     const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p + 16 * pitch));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  static __device__ __forceinline__ typename Num<T>::Frag cols(const bf16* t, int blk, int c, int g) {
-    const bf16* p = t + (4 * g + (c >> 2)) * pitch + 16 * blk + 4 * (c & 3);
+  static __device__ __forceinline__ typename Num<T>::Frag cols(const bf16* t, int step, int blk, int c, int g) {
+    const bf16* p = t + (TK * step + 4 * g + (c >> 2)) * pitch + 16 * blk + 4 * (c & 3);
     if constexpr (Num<T>::planes == 1) return tr(p);
     else return split::Chunk3{tr(p), tr(p + plane), tr(p + 2 * plane)};
   }
+  // the lane's B[k][n] of column n: features of one row of a tensor, from p (null: zeros), negated by flip
+  static __device__ __forceinline__ Feat column(const T* p, int kk, int g, int D, uint32_t flip) {
+    const int f = half ? 4 * g : 32 * kk + 8 * g;
+    if constexpr (half) {
+      f32x4 v = zero4();
+      if (p && f < D) v = split::flip_sign(load4_f32(p + f), flip);
+      if constexpr (Num<T>::planes == 1) {
+        bf16x4 r;
+        r[0] = (bf16)v[0]; r[1] = (bf16)v[1]; r[2] = (bf16)v[2]; r[3] = (bf16)v[3];
+        return r;
+      } else {
+        const split::Chunk3 x = split::split_chunk(v, v);
+        return Half3{__builtin_shufflevector(x.p0, x.p0, 0, 1, 2, 3), __builtin_shufflevector(x.p1, x.p1, 0, 1, 2, 3),
+                     __builtin_shufflevector(x.p2, x.p2, 0, 1, 2, 3)};
+      }
+    } else {
+      typename Num<T>::Raw r = zero_chunk<T>();
+      if (p && f < D) r = negate(load_chunk(p + f), flip);
+      return to_frag(r);
+    }
+  }
+  // the lane's part of the dot product of two rows
+  static __device__ __forceinline__ float dot(const T* p, const T* q, int kk, int g, int D) {
+    const int f = half ? 4 * g : 32 * kk + 8 * g;
+    if (f >= D) return 0.f;
+    f32x4 a = load4_f32(p + f), b = load4_f32(q + f);
+    float s = a[0] * b[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) s = __builtin_fmaf(a[i], b[i], s);
+    if constexpr (!half) {
+      a = load4_f32(p + f + 4); b = load4_f32(q + f + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = __builtin_fmaf(a[i], b[i], s);
+    }
+    return s;
+  }
+  // C[row][col] = init + sum over the features of tile[16 blk + row] b[col]
+  static __device__ __forceinline__ f32x4 product(const bf16* t, int blk, const Feat* b, int c, int g, const f32x4& init) {
+    f32x4 hi = init, lo = zero4();
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) product1(hi, lo, rows(t, blk, kk, c, g), b[kk]);
+    return result<T>(hi, lo);
+  }
 };
 
-// The rows of a tile on their way to LDS: NT threads, 8 values each and step
-template <typename T, int DP, int NT> struct Stage {
-  typedef Tile<T, DP> TL;
-  static constexpr int CH = TL::KP / 8, N = TK * CH, PER = (N + NT - 1) / NT;
+// The rows of a tile on their way to LDS: NT threads, 8 values each and piece
+template <typename T, int DP, int KT, int NT> struct Stage {
+  typedef Tile<T, DP, KT> TL;
+  static constexpr int CH = DP / 8, N = KT * TK * CH, PER = (N + NT - 1) / NT;
   typename Num<T>::Raw r[PER];
-  // row(i): address of row i of the tile, or null for a row of zeros
-  template <typename F> __device__ __forceinline__ void load(F row, int D) {
+  static __device__ __forceinline__ int row(int p) { return (p * NT + (int)threadIdx.x % NT) / CH; }
+  static __device__ __forceinline__ int feature(int p) { return 8 * ((p * NT + (int)threadIdx.x % NT) % CH); }
+  static __device__ __forceinline__ bool in(int p) { return N % NT == 0 || p * NT + (int)threadIdx.x % NT < N; }
+  // byte offsets of the lane's pieces in a buffer of rows
+  static __device__ __forceinline__ void offsets(uint32_t* off, int64_t row_bytes, int D) {
 #pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int t = p * NT + (int)threadIdx.x, i = t / CH, f = 8 * (t % CH);
-      r[p] = zero_chunk<T>();
-      if (t < N && f < D) {
-        const T* a = row(i);
-        if (a) r[p] = load_chunk(a + f);
-      }
-    }
+    for (int p = 0; p < PER; ++p)
+      off[p] = in(p) && feature(p) < D ? (uint32_t)(row(p) * (uint32_t)row_bytes + feature(p) * (uint32_t)sizeof(T)) : kOob;
+  }
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t b, const uint32_t* off) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) r[p] = load8((const T*)nullptr, b, off[p]);
+  }
+  // zeros in the rows whose bit is not set
+  __device__ __forceinline__ void keep(uint64_t bits) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (!((bits >> row(p)) & 1)) r[p] = zero_chunk<T>();
   }
   __device__ __forceinline__ void flip(uint32_t f) {
 #pragma unroll
@@ -145,15 +244,13 @@ template <typename T, int DP, int NT> struct Stage {
   }
   __device__ __forceinline__ void store(bf16* t) const {
 #pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int x = p * NT + (int)threadIdx.x;
-      if (x < N) {
-        bf16* d = t + (x / CH) * TL::pitch + 8 * (x % CH);
+    for (int p = 0; p < PER; ++p)
+      if (in(p)) {
+        bf16* d = t + row(p) * TL::pitch + feature(p);
         const auto v = to_frag(r[p]);
         if constexpr (Num<T>::planes == 1) store_chunk(d, v);
         else { store_chunk(d, v.p0); store_chunk(d + TL::plane, v.p1); store_chunk(d + 2 * TL::plane, v.p2); }
       }
-    }
   }
 };
 
@@ -167,24 +264,24 @@ __device__ __forceinline__ int edge_of(const int32_t* ptr, int e, int B, int N) 
 }
 // The extended segment of a slot and the slot's first virtual row in it (-1: an empty slot).  Every lane probes one
 // segment and step, so 64 segments take one round and 4,096 two.
-__device__ __forceinline__ int find_tile(const int32_t* ptr, int B, int N, int G, int BQ, int64_t slot, int& vq0, Seg& s) {
-  int lo = 0, hi = B + 2;
-  const int lane = lane_id();
+template <int BQ>
+__device__ __forceinline__ int find_tile(const int32_t* ptr, int B, int N, int G, uint32_t slot, int& vq0, Seg& s) {
+  uint32_t lo = 0, hi = (uint32_t)B + 2;
+  const uint32_t lane = lane_id();
   while (hi - lo > 1) {
-    const int step = (hi - lo + 63) / 64;
-    const int64_t e = lo + (int64_t)lane * step;
-    const bool le = e < hi && (int64_t)edge_of(ptr, (int)e, B, N) * G / BQ + e <= slot;
-    const int n = __builtin_popcountll(__ballot(le));
+    const uint32_t step = (hi - lo + 63) / 64, e = lo + lane * step;
+    const bool le = e < hi && (uint32_t)edge_of(ptr, (int)e, B, N) * (uint32_t)G / BQ + e <= slot;
+    const uint32_t n = __builtin_popcountll(__ballot(le));
     lo += (n > 0 ? n - 1 : 0) * step;
     hi = hi < lo + step ? hi : lo + step;
   }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  s.lo = edge_of(ptr, lo, B, N);
-  s.hi = edge_of(ptr, lo + 1, B, N);
+  const int e = __builtin_amdgcn_readfirstlane((int)lo);
+  s.lo = edge_of(ptr, e, B, N);
+  s.hi = edge_of(ptr, e + 1, B, N);
   if (s.hi < s.lo) s.hi = s.lo;
-  const int64_t v = (slot - ((int64_t)s.lo * G / BQ + lo)) * BQ;
+  const int64_t v = ((int64_t)slot - (uint32_t)s.lo * (uint32_t)G / BQ - e) * BQ;
   vq0 = v >= 0 && v < (int64_t)(s.hi - s.lo) * G ? (int)v : -1;
-  return lo;
+  return e;
 }
 // Rows of the other axis of extended segment e
 __device__ __forceinline__ Seg other_rows(const int32_t* ptr, int e, int B, int N) {
@@ -194,16 +291,37 @@ __device__ __forceinline__ Seg other_rows(const int32_t* ptr, int e, int B, int 
   return s;
 }
 // part s of n of [lo, hi), in whole steps
-__device__ __forceinline__ void split_range(int64_t lo, int64_t hi, int n, int s, int64_t& a, int64_t& b) {
-  const int64_t per = ((hi - lo + n - 1) / n + TK - 1) / TK * TK;
-  a = lo + s * per < hi ? lo + s * per : hi;
-  b = a + per < hi ? a + per : hi;
+template <int STEP>
+__device__ __forceinline__ void split_range(int lo, int hi, int n, int s, int& a, int& b) {
+  if (n == 1) { a = lo; b = hi; return; }
+  const uint32_t per = (((uint32_t)(hi - lo) + n - 1) / n + STEP - 1) / STEP * STEP;
+  const uint64_t x = (uint32_t)lo + (uint64_t)s * per;
+  a = x < (uint64_t)hi ? (int)x : hi;
+  b = (uint32_t)(hi - a) < per ? hi : a + (int)per;
 }
-// Consecutive items on one XCD (workgroups go to the 8 XCDs in turn, each has an L2 of its own): neighbouring heads of a
-// tile share the lines of its rows
-__device__ __forceinline__ int64_t item_of(int64_t bid, int64_t n) {
-  const int64_t per = n / 8, rest = n % 8, x = bid % 8, y = bid / 8;
+// Consecutive workgroups' items on one XCD (workgroups go to the 8 XCDs in turn, each has an L2 of its own):
+// neighbouring heads of a tile share the lines of its rows, and the tiles of a segment its keys
+__device__ __forceinline__ uint32_t xcd_order(uint32_t bid, uint32_t n) {
+  const uint32_t per = n / 8, rest = n % 8, x = bid % 8, y = bid / 8;
   return x * per + (x < rest ? x : rest) + y;
+}
+// One wave's (SH: one workgroup's) part of the work
+struct Item { uint32_t slot; int kvh, sp; };
+template <int W, bool SH>
+__device__ __forceinline__ bool item_of(const Args& a, uint32_t n_items, Item& it) {
+  uint32_t i = xcd_order(blockIdx.x, gridDim.x);
+  if constexpr (!SH && W > 1) i = i * W + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  if (i >= n_items) return false;
+  const uint32_t j = a.by_heads(i), k = a.by_split(j);
+  it.kvh = (int)(i - j * (uint32_t)a.Hkv);
+  it.sp = (int)(j - k * (uint32_t)a.nsplit);
+  it.slot = k;
+  return true;
+}
+// between a tile's writes and its reads
+template <bool SH> __device__ __forceinline__ void tile_sync() {
+  if constexpr (SH) __syncthreads();
+  else wave_sync();
 }
 
 // max and sum over the four lanes of a column
@@ -217,26 +335,8 @@ __device__ __forceinline__ void store4(bf16* p, const f32x4& v) {
   r[0] = (bf16)v[0]; r[1] = (bf16)v[1]; r[2] = (bf16)v[2]; r[3] = (bf16)v[3];
   *reinterpret_cast<bf16x4*>(p) = r;
 }
-__device__ __forceinline__ float dot8(const bf16x8& a, const bf16x8& b) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s = __builtin_fmaf((float)a[i], (float)b[i], s);
-  return s;
-}
-__device__ __forceinline__ float dot8(const f32x8& a, const f32x8& b) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s = __builtin_fmaf(a.hi[i], b.hi[i], __builtin_fmaf(a.lo[i], b.lo[i], s));
-  return s;
-}
-
-// 32 rows j0 .. of the key axis that exist and are not masked, as bits; the same in every wave
-__device__ __forceinline__ uint32_t key_bits(const uint8_t* mask, int j0, int hi) {
-  const int j = j0 + (lane_id() & 31);
-  bool ok = j < hi;
-  if (ok && mask) ok = mask[j] != 0;
-  return (uint32_t)__ballot(ok);
-}
+// bits of a step's first n rows
+__device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 }  // namespace attn
 }  // namespace egnn

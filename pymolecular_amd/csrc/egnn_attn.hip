@@ -13,27 +13,36 @@ bool dims_ok(const EgnnAttnDims* d) {
 }
 
 // own: (virtual) rows of the axis that is cut into tiles, other: rows of the axis a tile walks
-Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads) {
-  const int64_t segs = n_seg > 0 ? n_seg : 1;
+Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest) {
+  const int64_t segs = n_seg > 0 ? n_seg : 1, mean = own / segs;
   Plan p;
-  p.waves = own <= 48 * segs ? 1 : 4;
-  const int BQ = 16 * p.waves;
+  p.form = mean <= 48 ? 0 : mean < 256 ? 1 : 2;
+  if (widest < 0) p.form = 1;
+  else if (p.form > widest) p.form = widest;
+  const int64_t BQ = p.rows();
   p.slots = own / BQ + n_seg + 2;
-  const int64_t tiles = cdiv(own, BQ) > n_seg ? cdiv(own, BQ) : n_seg, blocks = (tiles > 0 ? tiles : 1) * heads;
+  const int64_t tiles = cdiv(own, BQ) > n_seg ? cdiv(own, BQ) : n_seg, items = (tiles > 0 ? tiles : 1) * heads;
   const int64_t len = other / segs;
   p.nsplit = 1;
-  if (blocks < 512 && len >= 512) {
-    const int64_t want = cdiv(p.waves == 1 ? 4096 : 1024, blocks), most = len / 256;
-    p.nsplit = (int)(want < most ? want : most);
+  const int64_t want = p.form == 0 ? 4096 : 1024;
+  if (items < want / 2 && len >= 512) {
+    int64_t n = cdiv(want, items);
+    if (n > len / 128) n = len / 128;
+    p.nsplit = (int)(n < 2048 ? n : 2048);
   }
   return p;
 }
-Plan plan_q(const EgnnAttnDims* d) { return make_plan(d->Nq * (d->Hq / d->Hkv), d->Nk, d->n_seg, d->Hkv); }
-Plan plan_k(const EgnnAttnDims* d) { return make_plan(d->Nk, d->Nq * (d->Hq / d->Hkv), d->n_seg, d->Hkv); }
+// The widest form whose registers hold the tile without spills; -1: form 1 alone
+int widest_q(const EgnnAttnDims* d) { return d->dtype == EGNN_F32 && d->D > 64 ? -1 : 2; }
+int widest_k(const EgnnAttnDims* d) {
+  return d->dtype == EGNN_F32 && d->D > 64 ? -1 : d->D > (d->dtype == EGNN_F32 ? 32 : 64) ? 1 : 2;
+}
+Plan plan_q(const EgnnAttnDims* d) { return make_plan(d->Nq * (d->Hq / d->Hkv), d->Nk, d->n_seg, d->Hkv, widest_q(d)); }
+Plan plan_k(const EgnnAttnDims* d) { return make_plan(d->Nk, d->Nq * (d->Hq / d->Hkv), d->n_seg, d->Hkv, widest_k(d)); }
 
 size_t fwd_bytes(const EgnnAttnDims* d) {
   const Plan p = plan_q(d);
-  return p.nsplit == 1 ? 0 : (size_t)p.nsplit * d->Nq * d->Hq * (padded(d->D) + 2) * 4;
+  return p.nsplit == 1 ? 0 : (size_t)p.nsplit * d->Nq * d->Hq * (padded(d->D) + 2) * 4;   // sums, then (m, l)
 }
 size_t delta_bytes(const EgnnAttnDims* d) { return align_up((size_t)d->Nq * d->Hq * 4); }
 size_t bwd_bytes(const EgnnAttnDims* d) {
@@ -45,11 +54,13 @@ size_t bwd_bytes(const EgnnAttnDims* d) {
 
 bool grid_ok(const EgnnAttnDims* d, const Plan& p) { return p.slots * d->Hkv * p.nsplit <= INT32_MAX; }
 
-// rows and heads 16-byte aligned, heads of a row apart from each other (inputs may overlap, outputs not)
-int check_view(const void* p, int64_t rows, int heads, int D, int64_t rs, int64_t hs, int esz, bool output) {
+// rows and heads 16-byte aligned; rows apart from each other or, of an input, all the same one (stride 0); a row at most
+// 2^24 bytes and a group's heads at most 2^29 from each other (the kernels' buffer offsets); an output's heads apart too
+int check_view(const void* p, int64_t rows, int heads, int D, int64_t rs, int64_t hs, int group, int esz, bool output) {
   if (rows == 0) return EGNN_OK;
   if (!p) return EGNN_ERR_NULL;
-  if (rs < 0 || hs < 0 || (rs * esz) % 16 || (hs * esz) % 16) return EGNN_ERR_STRIDE;
+  if (rs < 0 || hs < 0 || (rs * esz) % 16 || (hs * esz) % 16 || (rs && rs < D) || rs > (1 << 24) / esz) return EGNN_ERR_STRIDE;
+  if (group > 1 && hs > (1 << 29) / esz / (group - 1)) return EGNN_ERR_STRIDE;
   if (output && ((heads > 1 && hs < D) || (rows > 1 && rs < D))) return EGNN_ERR_STRIDE;
   return (uintptr_t)p % 16 ? EGNN_ERR_ALIGN : EGNN_OK;
 }
@@ -64,6 +75,8 @@ Args make_args(const EgnnAttnDims* d, const EgnnAttnStrides* s) {
   a.scale = d->scale < 0 ? -d->scale : d->scale;
   a.c2 = a.scale * kLog2e;
   a.flip = d->scale < 0 ? 0x80000000u : 0u;
+  a.by_g = Div::of(a.G);
+  a.by_heads = Div::of(a.Hkv);
   return a;
 }
 
@@ -87,10 +100,10 @@ int32_t egnn_attn_fwd(const EgnnAttnDims* d, const EgnnAttnStrides* s, const voi
   if (!dims_ok(d)) return EGNN_ERR_DIMS;
   const int esz = d->dtype == EGNN_F32 ? 4 : 2;
   if (!q_ptr || !kv_ptr) return EGNN_ERR_NULL;
-  EGNN_TRY(check_view(q, d->Nq, d->Hq, d->D, s->q_row, s->q_head, esz, false));
-  EGNN_TRY(check_view(k, d->Nk, d->Hkv, d->D, s->k_row, s->k_head, esz, false));
-  EGNN_TRY(check_view(v, d->Nk, d->Hkv, d->D, s->v_row, s->v_head, esz, false));
-  EGNN_TRY(check_view(out, d->Nq, d->Hq, d->D, s->out_row, s->out_head, esz, true));
+  EGNN_TRY(check_view(q, d->Nq, d->Hq, d->D, s->q_row, s->q_head, d->Hq / d->Hkv, esz, false));
+  EGNN_TRY(check_view(k, d->Nk, d->Hkv, d->D, s->k_row, s->k_head, 1, esz, false));
+  EGNN_TRY(check_view(v, d->Nk, d->Hkv, d->D, s->v_row, s->v_head, 1, esz, false));
+  EGNN_TRY(check_view(out, d->Nq, d->Hq, d->D, s->out_row, s->out_head, d->Hq / d->Hkv, esz, true));
   const Plan p = plan_q(d);
   if (!grid_ok(d, p)) return EGNN_ERR_DIMS;
   const size_t need = fwd_bytes(d);
@@ -100,6 +113,7 @@ int32_t egnn_attn_fwd(const EgnnAttnDims* d, const EgnnAttnStrides* s, const voi
   Args a = make_args(d, s);
   a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.q_ptr = q_ptr; a.kv_ptr = kv_ptr; a.mask = key_mask;
   a.nsplit = p.nsplit;
+  a.by_split = Div::of(p.nsplit);
   a.part = (float*)workspace;
   return launch_fwd(a, d->dtype == EGNN_BF16, p, (hipStream_t)stream) ? EGNN_ERR_HIP : EGNN_OK;
 }
@@ -111,14 +125,14 @@ int32_t egnn_attn_bwd(const EgnnAttnDims* d, const EgnnAttnStrides* s, const voi
   if (!dims_ok(d)) return EGNN_ERR_DIMS;
   const int esz = d->dtype == EGNN_F32 ? 4 : 2;
   if (!q_ptr || !kv_ptr || (d->Nq && !lse)) return EGNN_ERR_NULL;
-  EGNN_TRY(check_view(q, d->Nq, d->Hq, d->D, s->q_row, s->q_head, esz, false));
-  EGNN_TRY(check_view(k, d->Nk, d->Hkv, d->D, s->k_row, s->k_head, esz, false));
-  EGNN_TRY(check_view(v, d->Nk, d->Hkv, d->D, s->v_row, s->v_head, esz, false));
-  EGNN_TRY(check_view(out, d->Nq, d->Hq, d->D, s->out_row, s->out_head, esz, false));
-  EGNN_TRY(check_view(grad_out, d->Nq, d->Hq, d->D, s->grad_out_row, s->grad_out_head, esz, false));
-  EGNN_TRY(check_view(grad_q, d->Nq, d->Hq, d->D, s->grad_q_row, s->grad_q_head, esz, true));
-  EGNN_TRY(check_view(grad_k, d->Nk, d->Hkv, d->D, s->grad_k_row, s->grad_k_head, esz, true));
-  EGNN_TRY(check_view(grad_v, d->Nk, d->Hkv, d->D, s->grad_v_row, s->grad_v_head, esz, true));
+  EGNN_TRY(check_view(q, d->Nq, d->Hq, d->D, s->q_row, s->q_head, d->Hq / d->Hkv, esz, false));
+  EGNN_TRY(check_view(k, d->Nk, d->Hkv, d->D, s->k_row, s->k_head, 1, esz, false));
+  EGNN_TRY(check_view(v, d->Nk, d->Hkv, d->D, s->v_row, s->v_head, 1, esz, false));
+  EGNN_TRY(check_view(out, d->Nq, d->Hq, d->D, s->out_row, s->out_head, d->Hq / d->Hkv, esz, false));
+  EGNN_TRY(check_view(grad_out, d->Nq, d->Hq, d->D, s->grad_out_row, s->grad_out_head, d->Hq / d->Hkv, esz, false));
+  EGNN_TRY(check_view(grad_q, d->Nq, d->Hq, d->D, s->grad_q_row, s->grad_q_head, d->Hq / d->Hkv, esz, true));
+  EGNN_TRY(check_view(grad_k, d->Nk, d->Hkv, d->D, s->grad_k_row, s->grad_k_head, 1, esz, true));
+  EGNN_TRY(check_view(grad_v, d->Nk, d->Hkv, d->D, s->grad_v_row, s->grad_v_head, 1, esz, true));
   const Plan pq = plan_q(d), pk = plan_k(d);
   if (!grid_ok(d, pq) || !grid_ok(d, pk)) return EGNN_ERR_DIMS;
   const size_t need = bwd_bytes(d);

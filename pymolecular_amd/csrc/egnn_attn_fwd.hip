@@ -1,144 +1,244 @@
-// Segment attention, forward: o_i = sum_j softmax_j(scale q_i k_j) v_j over the keys of i's segment.
+// Segment attention, forward: o_i = sum_j softmax_j(scale q_i k_j) v_j over the keys of i's segment, in one pass over
+// the keys with the running maximum and sum.
+//
+// The maximum is lazy: a column keeps its reference m until a score passes it by 2^8 (in the exponent's base), so that a
+// step costs neither shuffles nor a rescaling of the output; p is then up to 2^8, which costs no precision in floating
+// point.  The sum takes the unrounded probabilities (one more product, against ones, would sum the rounded ones at less
+// cost, and put up to 2^-9 into lse).
 #include "egnn_attn.h"
 
 namespace egnn {
 namespace attn {
 
-// Workspace of a split call: per split and virtual output row [D padded to DP] sums, then (m, l)
-__device__ __forceinline__ float* part_row(const Args& a, int dp, int s, int64_t r) {
-  return a.part + ((int64_t)s * a.Nq * a.Hq + r) * (dp + 2);
+constexpr float kLazy = 8.0f, kLowest = -3.40282347e+38f;
+
+// Partial results of a split call: [split][row of q, head] sums of DP values, then (m, l)
+__device__ __forceinline__ float* part_o(const Args& a, int dp, int s, int64_t r) { return a.part + ((int64_t)s * a.Nq * a.Hq + r) * dp; }
+__device__ __forceinline__ float* part_ml(const Args& a, int dp, int s, int64_t r) {
+  return a.part + (int64_t)a.nsplit * a.Nq * a.Hq * dp + ((int64_t)s * a.Nq * a.Hq + r) * 2;
 }
 
-template <typename T, int DP, int W>
-__global__ __launch_bounds__(64 * W) void fwd_kernel(Args a, int64_t n_items) {
-  typedef Tile<T, DP> TL;
+// R: blocks of 16 columns a wave.  W waves, on one tile (SH) or each on its own.  KT: steps of 32 keys between barriers.
+template <typename T, int DP, int R, int W, bool SH, int KT>
+__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_t n_items) {
+  typedef Tile<T, DP, KT> TL;
   typedef typename Num<T>::Frag Frag;
-  constexpr int NT = 64 * W, BQ = 16 * W;
-  __shared__ __attribute__((aligned(16))) bf16 sK[TL::elems], sV[TL::elems];
-  int64_t item = item_of(blockIdx.x, n_items);
-  const int kvh = (int)(item % a.Hkv);
-  item /= a.Hkv;
-  const int sp = (int)(item % a.nsplit);
-  const int64_t slot = item / a.nsplit;
+  constexpr int NT = SH ? 64 * W : 64, BQ = 16 * R * (SH ? W : 1), KS = TK * KT;
+  __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
+  Item it;
+  if (!item_of<W, SH>(a, n_items, it)) return;
   const int l = lane_id(), c = l & 15, g = l >> 4, w = threadIdx.x >> 6;
+  bf16 *sK = lds[SH ? 0 : w][0], *sV = lds[SH ? 0 : w][1];
   int vq0;
   Seg qs;
-  const int e = find_tile(a.q_ptr, a.B, a.Nq, a.G, BQ, slot, vq0, qs);
+  const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, it.slot, vq0, qs);
   if (vq0 < 0) return;
   const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk);
-  const int nv = (qs.hi - qs.lo) * a.G, vq = vq0 + 16 * w + c;
-  const bool live = vq < nv;
-  const int row = qs.lo + (live ? vq / a.G : 0), head = kvh * a.G + (live ? vq % a.G : 0);
-  // the lane's column of Q^T
-  Frag Q[TL::NK];
-  const T* qp = (const T*)a.q + row * a.q_r + head * a.q_h;
-#pragma unroll
-  for (int kk = 0; kk < TL::NK; ++kk) {
-    const int f = 32 * kk + 8 * g;
-    typename Num<T>::Raw r = zero_chunk<T>();
-    if (live && f < a.D) r = negate(load_chunk(qp + f), a.flip);
-    Q[kk] = to_frag(r);
-  }
-  int64_t j0, j1;
-  split_range(ks.lo, ks.hi, a.nsplit, sp, j0, j1);
-  const T *kb = (const T*)a.k + kvh * a.k_h, *vb = (const T*)a.v + kvh * a.v_h;
-  f32x4 O[TL::NB];
-#pragma unroll
-  for (int b = 0; b < TL::NB; ++b) O[b] = zero4();
-  float m = -INFINITY, sum = 0.f;
+  const int nv = (qs.hi - qs.lo) * a.G, v0 = vq0 + (SH ? 16 * R * w : 0);
+  const bool act = v0 < nv;                  // a wave without rows still loads tiles for the others
+  int j, j1;
+  split_range<KS>(ks.lo, ks.hi, a.nsplit, it.sp, j, j1);
 
-  for (int64_t j = j0; j < j1; j += TK) {
-    const uint32_t bits = key_bits(a.mask, (int)j, (int)j1);
-    Stage<T, DP, NT> st;
-    st.load([&](int i) { return (bits >> i) & 1 ? kb + (j + i) * a.k_r : nullptr; }, a.D);
-    __syncthreads();   // the step before has read the tile
-    st.store(sK);
-    st.load([&](int i) { return (bits >> i) & 1 ? vb + (j + i) * a.v_r : nullptr; }, a.D);
-    st.store(sV);
-    __syncthreads();
-    f32x4 S[2];
+  Stage<T, DP, KT, NT> stK, stV;
+  uint32_t offK[stK.PER], offV[stV.PER];
+  const int64_t krb = a.k_r * (int64_t)sizeof(T), vrb = a.v_r * (int64_t)sizeof(T);
+  stK.offsets(offK, krb, a.D);
+  stV.offsets(offV, vrb, a.D);
+  const T *kb = (const T*)a.k + it.kvh * a.k_h, *vb = (const T*)a.v + it.kvh * a.v_h;
+  uint8_t mb = 1;
+  auto fetch = [&](int j) {
+    const int n = j1 - j < KS ? j1 - j : KS;
+    stK.load(rows_buffer(kb + j * a.k_r, n, krb, a.D * (int)sizeof(T)), offK);
+    stV.load(rows_buffer(vb + j * a.v_r, n, vrb, a.D * (int)sizeof(T)), offV);
+    if (a.mask) mb = l < n ? a.mask[j + l] : 0;
+  };
+  if (j < j1) fetch(j);
+
+  // the lane's columns of Q^T
+  typename TL::Feat Q[R][TL::NK];
+  int row[R], head[R];
+  bool live[R];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      S[h] = product<TL::NK>(Q, [&](int kk) { return TL::rows(sK, h, kk, c, g); });
-      if (bits != 0xffffffffu) {
+  for (int r = 0; r < R; ++r) {
+    const int v = v0 + 16 * r + c;
+    live[r] = v < nv;
+    const uint32_t i = live[r] ? a.by_g(v) : 0;
+    row[r] = qs.lo + (int)i;
+    head[r] = it.kvh * a.G + (live[r] ? v - (int)i * a.G : 0);
+    const T* qp = live[r] ? (const T*)a.q + row[r] * a.q_r + head[r] * a.q_h : nullptr;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S[h][i] = (bits >> (16 * h + 4 * g + i)) & 1 ? S[h][i] : -INFINITY;
-      }
-    }
-    float mx = fmaxf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])), fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
-    const float mn = fmaxf(m, col_max(mx) * a.c2);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - ref);
-    m = mn;
-    float ps = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        S[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[h][i], a.c2, -ref));
-        ps += S[h][i];
-      }
-    sum = __builtin_fmaf(sum, alpha, ps);
-    const Frag P = chain_frag<T>(S[0], S[1]);
-#pragma unroll
-    for (int b = 0; b < TL::NB; ++b) {
-      O[b] *= alpha;
-      accumulate(O[b], TL::cols(sV, b, c, g), P);
-    }
+    for (int kk = 0; kk < TL::NK; ++kk) Q[r][kk] = TL::column(qp, kk, g, a.D, a.flip);
   }
-  sum = col_sum(sum);
-  if (!live) return;
-  if (a.nsplit > 1) {
-    float* p = part_row(a, DP, sp, (int64_t)row * a.Hq + head);
+  f32x4 O[R][TL::NB];
+  float m[R], sum[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = kLowest;
+    sum[r] = 0.f;
+#pragma unroll
+    for (int b = 0; b < TL::NB; ++b) O[r][b] = zero4();
+  }
+
+  for (; j < j1; j += KS) {
+    uint64_t bits = first_bits(j1 - j < KS ? j1 - j : KS);
+    if (a.mask) {                            // what a masked value holds must not meet a probability of 0
+      bits &= __ballot(mb != 0);
+      stV.keep(bits);
+    }
+    tile_sync<SH>();                         // the step before has read the tile
+    stK.store(sK);
+    stV.store(sV);
+    tile_sync<SH>();
+    if (j + KS < j1) fetch(j + KS);
+    if (!act) continue;
+    f32x4 S[R][2 * KT];
+#pragma unroll
+    for (int h = 0; h < 2 * KT; ++h) {
+      f32x4 hi[R], lo[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) { hi[r] = zero4(); lo[r] = zero4(); }
+#pragma unroll
+      for (int kk = 0; kk < TL::NK; ++kk) {
+        const auto A = TL::rows(sK, h, kk, c, g);
+#pragma unroll
+        for (int r = 0; r < R; ++r) product1(hi[r], lo[r], A, Q[r][kk]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) S[r][h] = result<T>(hi[r], lo[r]);
+    }
+    if (bits != first_bits(KS)) {
+      const uint32_t b0 = (uint32_t)bits >> (4 * g), b1 = (uint32_t)(bits >> 32) >> (4 * g);
+#pragma unroll
+      for (int h = 0; h < 2 * KT; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool ok = ((h < 2 ? b0 : b1) >> (16 * (h & 1) + i)) & 1;
+#pragma unroll
+          for (int r = 0; r < R; ++r) S[r][h][i] = ok ? S[r][h][i] : -INFINITY;
+        }
+    }
+    float top[R];
+    bool over = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      top[r] = S[r][0][0];
+#pragma unroll
+      for (int h = 0; h < 2 * KT; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], S[r][h][i]);
+      over |= __builtin_fmaf(top[r], a.c2, -m[r]) > kLazy;
+    }
+    if (__ballot(over)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float mn = fmaxf(m[r], col_max(top[r]) * a.c2), alpha = __builtin_amdgcn_exp2f(m[r] - mn);
+        m[r] = mn;
+        sum[r] *= alpha;
+#pragma unroll
+        for (int b = 0; b < TL::NB; ++b) O[r][b] *= alpha;
+      }
+    }
+    Frag P[R][KT];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int h = 0; h < 2 * KT; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          S[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r][h][i], a.c2, -m[r]));
+          sum[r] += S[r][h][i];
+        }
+#pragma unroll
+      for (int t = 0; t < KT; ++t) P[r][t] = chain_frag<T>(S[r][2 * t], S[r][2 * t + 1]);
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int b = 0; b < TL::NB; ++b) {
+        const Frag A = TL::cols(sV, t, b, c, g);
+#pragma unroll
+        for (int r = 0; r < R; ++r) accumulate(O[r][b], A, P[r][t]);
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float s = col_sum(sum[r]);
+    if (!live[r]) continue;
+    if (a.nsplit > 1) {
+      const int64_t x = (int64_t)row[r] * a.Hq + head[r];
+      float* p = part_o(a, DP, it.sp, x);
+#pragma unroll
+      for (int b = 0; b < TL::NB; ++b) store4(p + 16 * b + 4 * g, O[r][b]);
+      p = part_ml(a, DP, it.sp, x);
+      if (g == 0) { p[0] = m[r]; p[1] = s; }
+      continue;
+    }
+    // no key left: the sum is 0 (a NaN is not), the output 0 and lse -inf
+    const float inv = s == 0.f ? 0.f : 1.0f / s;
+    T* op = (T*)a.out + row[r] * a.o_r + head[r] * a.o_h;
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b)
-      if (16 * b + 4 * g < a.D) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[16 * b + 4 * g + i] = O[b][i];
-      }
-    if (g == 0) { p[DP] = m; p[DP + 1] = sum; }
-    return;
+      if (16 * b + 4 * g < a.D) store4(op + 16 * b + 4 * g, O[r][b] * inv);
+    if (a.lse && g == 0) a.lse[(int64_t)head[r] * a.Nq + row[r]] = (m[r] + __builtin_amdgcn_logf(s)) * kLn2;
   }
-  // no key left: the sum is 0 (a NaN is not), the output 0
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  T* op = (T*)a.out + row * a.o_r + head * a.o_h;
-#pragma unroll
-  for (int b = 0; b < TL::NB; ++b)
-    if (16 * b + 4 * g < a.D) store4(op + 16 * b + 4 * g, O[b] * inv);
-  if (a.lse && g == 0) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// Joins the splits of one row and head: one wave each, in split order
+// Joins the splits of one row and head: their weights first, then 4 features a thread over groups of splits, whose sums
+// are added in order
+constexpr int kMaxSplit = 2048;
 template <typename T, int DP>
-__global__ __launch_bounds__(64) void fwd_join_kernel(Args a) {
-  const int64_t r = blockIdx.x;
-  const int head = (int)(r % a.Hq), l = lane_id();
-  const int64_t row = r / a.Hq;
-  float m = -INFINITY;
-  for (int s = l; s < a.nsplit; s += 64) m = fmaxf(m, part_row(a, DP, s, r)[DP]);
+__global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
+  constexpr int LF = DP / 4, GR = 256 / LF;
+  __shared__ float wt[kMaxSplit], red[4];
+  __shared__ f32x4 part[GR][LF];
+  const uint32_t r = blockIdx.x;
+  const int head = (int)(r % (uint32_t)a.Hq), t = threadIdx.x;
+  const int64_t row = r / (uint32_t)a.Hq;
+  float m = kLowest;
+  for (int s = t; s < a.nsplit; s += 256) m = fmaxf(m, part_ml(a, DP, s, r)[0]);
   for (int x = 32; x; x >>= 1) m = fmaxf(m, shfl_xor(m, x));
-  const float ref = m == -INFINITY ? 0.f : m;
-  float sum = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) {
-    const float* p = part_row(a, DP, s, r);
-    const float f = __builtin_amdgcn_exp2f(p[DP] - ref);
-    sum = __builtin_fmaf(p[DP + 1], f, sum);
-    if (l < a.D) o0 = __builtin_fmaf(p[l], f, o0);
-    if (l + 64 < a.D) o1 = __builtin_fmaf(p[l + 64], f, o1);
+  if ((t & 63) == 0) red[t >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
+  float sum = 0.f;
+  for (int s = t; s < a.nsplit; s += 256) {
+    const float* p = part_ml(a, DP, s, r);
+    wt[s] = __builtin_amdgcn_exp2f(p[0] - m);
+    sum = __builtin_fmaf(p[1], wt[s], sum);
   }
+  for (int x = 32; x; x >>= 1) sum += shfl_xor(sum, x);
+  if ((t & 63) == 0) red[t >> 6] = sum;
+  __syncthreads();
+  sum = (red[0] + red[1]) + (red[2] + red[3]);
+  const int f = 4 * (t % LF), gr = t / LF;
+  f32x4 o = zero4();
+#pragma unroll 4
+  for (int s = gr; s < a.nsplit; s += GR) o += load4_f32(part_o(a, DP, s, r) + f) * wt[s];
+  part[gr][t % LF] = o;
+  __syncthreads();
+  if (gr) return;
+#pragma unroll 4
+  for (int k = 1; k < GR; ++k) o += part[k][t];
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  T* op = (T*)a.out + row * a.o_r + head * a.o_h;
-  if (l < a.D) op[l] = from_f32<T>(o0 * inv);
-  if (l + 64 < a.D) op[l + 64] = from_f32<T>(o1 * inv);
-  if (a.lse && l == 0) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+  if (f < a.D) store4((T*)a.out + row * a.o_r + head * a.o_h + f, o * inv);
+  if (a.lse && t == 0) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
+template <typename T, int DP, int R, int W, bool SH, int KT>
+static void go(const Args& a, const Plan& p, hipStream_t st) {
+  const int64_t n = p.slots * a.Hkv * a.nsplit;
+  fwd_kernel<T, DP, R, W, SH, KT><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
+}
 template <typename T, int DP>
 static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
-  const int64_t n = p.slots * a.Hkv * a.nsplit;
-  if (p.waves == 1) fwd_kernel<T, DP, 1><<<(uint32_t)n, 64, 0, st>>>(a, n);
-  else fwd_kernel<T, DP, 4><<<(uint32_t)n, 256, 0, st>>>(a, n);
-  if (a.nsplit > 1) fwd_join_kernel<T, DP><<<(uint32_t)((int64_t)a.Nq * a.Hq), 64, 0, st>>>(a);
+  constexpr int tile = 2 * Tile<T, DP>::elems * 2, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
+  constexpr int KT = Num<T>::planes == 1 ? 2 : 1;
+  if constexpr (KT == 1 && DP == 128) go<T, DP, 1, 4, true, KT>(a, p, st);
+  else if (p.form == 0) go<T, DP, 1, W, false, 1>(a, p, st);
+  else if (p.form == 1) go<T, DP, 1, 4, true, KT>(a, p, st);
+  else go<T, DP, 2, 4, true, KT>(a, p, st);
+  if (a.nsplit > 1) fwd_join_kernel<T, DP><<<(uint32_t)((int64_t)a.Nq * a.Hq), 256, 0, st>>>(a);
   return (int)hipGetLastError();
 }
 template <typename T>

@@ -19,31 +19,36 @@ struct Args {
   float eps;
 };
 
-template <typename T, int VEC> struct Vec;
-template <> struct Vec<float, 4> {
-  static __device__ __forceinline__ void load(const float* p, float* v) {
-    const f32x4 t = load4_f32(p);
+// VEC = 16 bytes of values at a lane's column f.  Rows need no alignment but their values': the type says so, and the
+// compiler still makes one 16-byte access of it (259 fp32 values a row: 16-byte pieces with a scalar tail 24 us where
+// single values took 52, forward and backward of 40,961 rows).  The last piece of a row that is not a multiple of VEC
+// wide goes value by value.
+template <typename T> struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  static __device__ __forceinline__ void load(const T* p, int f, int C, float* v) {
+    if (f + N <= C) {
+      const type t = *reinterpret_cast<const type*>(p + f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = t[i];
-  }
-  static __device__ __forceinline__ void store(float* p, const float* v) { *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]}; }
-};
-template <> struct Vec<bf16, 8> {
-  static __device__ __forceinline__ void load(const bf16* p, float* v) {
-    const bf16x8 t = load_chunk(p);
+      for (int i = 0; i < N; ++i) v[i] = to_f32((T)t[i]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+      for (int i = 0; i < N; ++i)
+        if (f + i < C) v[i] = to_f32(p[f + i]);
+    }
   }
-  static __device__ __forceinline__ void store(bf16* p, const float* v) {
-    bf16x8 t;
+  static __device__ __forceinline__ void store(T* p, int f, int C, const float* v) {
+    if (f + N <= C) {
+      type t;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = (bf16)v[i];
-    store_chunk(p, t);
+      for (int i = 0; i < N; ++i) t[i] = from_f32<T>(v[i]);
+      *reinterpret_cast<type*>(p + f) = t;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (f + i < C) p[f + i] = from_f32<T>(v[i]);
+    }
   }
-};
-template <typename T> struct Vec<T, 1> {
-  static __device__ __forceinline__ void load(const T* p, float* v) { v[0] = to_f32(*p); }
-  static __device__ __forceinline__ void store(T* p, const float* v) { *p = from_f32<T>(v[0]); }
 };
 
 template <int LPR> __device__ __forceinline__ float row_sum(float v) {
@@ -54,38 +59,48 @@ template <int LPR> __device__ __forceinline__ float row_sum(float v) {
 
 constexpr int NT = 256;
 
-template <typename T, int VEC, int LPR, int VPL>
+template <typename T, int LPR, int VPL>
 __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
+  constexpr int VEC = Vec<T>::N;
   const int lane = threadIdx.x % LPR;
   const int64_t n = (int64_t)blockIdx.x * (NT / LPR) + threadIdx.x / LPR;
   const bool live = n < a.N;
   float v[VPL][VEC];
-  float sum = 0.f;
 #pragma unroll
   for (int p = 0; p < VPL; ++p) {
     const int f = (p * LPR + lane) * VEC;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[p][i] = 0.f;
-    if (live && f < a.C) {
-      Vec<T, VEC>::load((const T*)a.x + n * a.ldx + f, v[p]);
-      if (a.r) {
-        float r[VEC];
-        Vec<T, VEC>::load((const T*)a.r + n * a.ldr + f, r);
+    if (live && f < a.C) Vec<T>::load((const T*)a.x + n * a.ldx, f, a.C, v[p]);
+  }
+  if (a.r) {
+#pragma unroll
+    for (int p = 0; p < VPL; ++p) {
+      const int f = (p * LPR + lane) * VEC;
+      float r[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) r[i] = 0.f;
+      if (live && f < a.C) {
+        Vec<T>::load((const T*)a.r + n * a.ldr, f, a.C, r);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[p][i] += r[i];
-        Vec<T, VEC>::store((T*)a.s + n * a.C + f, v[p]);
+        Vec<T>::store((T*)a.s + n * a.C, f, a.C, v[p]);
       }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) sum += v[p][i];
     }
   }
+  float sum = 0.f;
+#pragma unroll
+  for (int p = 0; p < VPL; ++p)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum += v[p][i];
   const float mean = row_sum<LPR>(sum) / a.C;
   float sq = 0.f;
 #pragma unroll
   for (int p = 0; p < VPL; ++p)
-    if ((p * LPR + lane) * VEC < a.C) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) { const float d = v[p][i] - mean; sq = __builtin_fmaf(d, d, sq); }
+    for (int i = 0; i < VEC; ++i) {
+      const float d = v[p][i] - mean;
+      if ((p * LPR + lane) * VEC + i < a.C) sq = __builtin_fmaf(d, d, sq);
     }
   const float rstd = 1.0f / sqrtf(row_sum<LPR>(sq) / a.C + a.eps);
   if (!live) return;
@@ -97,18 +112,18 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
       float w[VEC], b[VEC], y[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) { w[i] = 1.f; b[i] = 0.f; }
-      if (a.w) Vec<T, VEC>::load((const T*)a.w + f, w);
-      if (a.b) Vec<T, VEC>::load((const T*)a.b + f, b);
+      if (a.w) Vec<T>::load((const T*)a.w, f, a.C, w);
+      if (a.b) Vec<T>::load((const T*)a.b, f, a.C, b);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) y[i] = __builtin_fmaf((v[p][i] - mean) * rstd, w[i], b[i]);
-      Vec<T, VEC>::store((T*)a.y + n * a.C + f, y);
+      Vec<T>::store((T*)a.y + n * a.C, f, a.C, y);
     }
   }
 }
 
-template <typename T, int VEC, int LPR, int VPL>
+template <typename T, int LPR, int VPL>
 __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
-  constexpr int RG = NT / LPR, W = LPR * VPL * VEC;
+  constexpr int VEC = Vec<T>::N, RG = NT / LPR, W = LPR * VPL * VEC;
   __shared__ float red[RG][W];
   const int lane = threadIdx.x % LPR, rg = threadIdx.x / LPR;
   float gw[VPL][VEC], gb[VPL][VEC], w[VPL][VEC];
@@ -116,36 +131,37 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
   for (int p = 0; p < VPL; ++p) {
     const int f = (p * LPR + lane) * VEC;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) { gw[p][i] = 0.f; gb[p][i] = 0.f; w[p][i] = f < a.C ? 1.f : 0.f; }
-    if (a.w && f < a.C) Vec<T, VEC>::load((const T*)a.w + f, w[p]);
+    for (int i = 0; i < VEC; ++i) { gw[p][i] = 0.f; gb[p][i] = 0.f; w[p][i] = f + i < a.C ? 1.f : 0.f; }
+    if (a.w && f < a.C) Vec<T>::load((const T*)a.w, f, a.C, w[p]);
   }
   for (int64_t n0 = (int64_t)blockIdx.x * RG; n0 < a.N; n0 += (int64_t)gridDim.x * RG) {
     const int64_t n = n0 + rg;
     const bool live = n < a.N;
     const float mean = live ? a.mean[n] : 0.f, rstd = live ? a.rstd[n] : 0.f;
-    float xh[VPL][VEC], t[VPL][VEC];
+    float xh[VPL][VEC], t[VPL][VEC], e[VPL][VEC];
+#pragma unroll
+    for (int p = 0; p < VPL; ++p) {   // everything the row needs, requested at once
+      const int f = (p * LPR + lane) * VEC;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { t[p][i] = 0.f; xh[p][i] = mean; e[p][i] = 0.f; }
+      if (live && f < a.C) {
+        Vec<T>::load((const T*)a.gy + n * a.ldg, f, a.C, t[p]);
+        Vec<T>::load((const T*)a.x + n * a.ldx, f, a.C, xh[p]);
+        if (a.gsum) Vec<T>::load((const T*)a.gsum + n * a.ldgs, f, a.C, e[p]);
+      }
+    }
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int p = 0; p < VPL; ++p) {
-      const int f = (p * LPR + lane) * VEC;
-      const bool on = live && f < a.C;
-      float g[VEC], x[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) { g[i] = 0.f; x[i] = mean; }
-      if (on) {
-        Vec<T, VEC>::load((const T*)a.gy + n * a.ldg + f, g);
-        Vec<T, VEC>::load((const T*)a.x + n * a.ldx + f, x);
-      }
+    for (int p = 0; p < VPL; ++p)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        xh[p][i] = (x[i] - mean) * rstd;
-        t[p][i] = g[i] * w[p][i];
-        gw[p][i] = __builtin_fmaf(g[i], xh[p][i], gw[p][i]);
-        gb[p][i] += g[i];
+        xh[p][i] = (xh[p][i] - mean) * rstd;
+        gw[p][i] = __builtin_fmaf(t[p][i], xh[p][i], gw[p][i]);
+        gb[p][i] += t[p][i];
+        t[p][i] *= w[p][i];
         s1 += t[p][i];
         s2 = __builtin_fmaf(t[p][i], xh[p][i], s2);
       }
-    }
     const float m1 = row_sum<LPR>(s1) / a.C, m2 = row_sum<LPR>(s2) / a.C;
 #pragma unroll
     for (int p = 0; p < VPL; ++p) {
@@ -153,14 +169,8 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
       if (live && f < a.C) {
         float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = rstd * (t[p][i] - m1 - xh[p][i] * m2);
-        if (a.gsum) {
-          float e[VEC];
-          Vec<T, VEC>::load((const T*)a.gsum + n * a.ldgs + f, e);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) o[i] += e[i];
-        }
-        Vec<T, VEC>::store((T*)a.gx + n * a.C + f, o);
+        for (int i = 0; i < VEC; ++i) o[i] = __builtin_fmaf(rstd, t[p][i] - m1 - xh[p][i] * m2, e[p][i]);
+        Vec<T>::store((T*)a.gx + n * a.C, f, a.C, o);
       }
     }
   }
@@ -246,73 +256,75 @@ __global__ __launch_bounds__(NT) void bwd_wide_weights_kernel(Args a) {
   out[a.C + f] = gb;
 }
 
-// gw, gb = sums of the partial rows: 64 columns a block, 16 row groups joined in order
+// gw, gb = sums of the partial rows: 16 columns a block, 64 row groups joined in order
 template <typename T>
 __global__ __launch_bounds__(1024) void sum_kernel(const float* part, int nblk, int C, T* gw, T* gb) {
-  __shared__ float red[16][64];
-  const int c = threadIdx.x & 63, k = threadIdx.x >> 6;
-  const int f = blockIdx.x * 64 + c;
+  __shared__ float red[64][17];
+  const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
+  const int f = blockIdx.x * 16 + c;
   float s = 0.f;
-  if (f < 2 * C)
-    for (int b = k; b < nblk; b += 16) s += part[(int64_t)b * 2 * C + f];
+  if (f < 2 * C) {
+#pragma unroll 8
+    for (int b = k; b < nblk; b += 64) s += part[(int64_t)b * 2 * C + f];
+  }
   red[k][c] = s;
   __syncthreads();
+  for (int h = 32; h; h >>= 1) {
+    if (k < h) red[k][c] += red[k + h][c];
+    __syncthreads();
+  }
   if (k || f >= 2 * C) return;
-#pragma unroll
-  for (int i = 1; i < 16; ++i) s += red[i][c];
+  s = red[0][c];
   if (f < C) { if (gw) gw[f] = from_f32<T>(s); }
   else if (gb) gb[f - C] = from_f32<T>(s);
 }
 
-constexpr int kMaxBlocks = 1024;   // partial rows of the weight gradients
+constexpr int kMaxBlocks = 2048;   // partial rows of the weight gradients
 
-// lanes and vectors of a row: the fewest vectors a lane, then the fewest lanes
-struct Shape { int vec, lpr, vpl; };
-static bool shape_of(int C, int vec, Shape* s) {
-  const int n = (C + vec - 1) / vec;
-  s->vec = vec;
-  for (s->vpl = 1; s->vpl <= 8; s->vpl *= 2)
-    for (s->lpr = 4; s->lpr <= 64; s->lpr *= 2)
-      if (s->lpr * s->vpl >= n && (s->vpl == 1 || s->lpr == 64)) return true;
+// lanes and pieces of a row: the fewest lane slots that hold it
+struct Shape { int lpr, vpl; };
+static bool shape_of(int pieces, Shape* s) {
+  static const Shape all[] = {{4, 1}, {8, 1}, {16, 1}, {32, 1}, {64, 1}, {32, 3}, {64, 2}, {64, 3}, {64, 4}, {64, 6}};
+  for (const Shape& x : all)
+    if (x.lpr * x.vpl >= pieces) { *s = x; return true; }
   return false;
 }
-static int64_t part_rows(int64_t N) { return N < 1 ? 1 : (N < kMaxBlocks ? N : kMaxBlocks); }
+// Partial rows of the backward: a block makes several rounds over its row groups where there are enough rows, so that
+// the sums over the partial rows stay small
+static int64_t part_rows(int64_t N) {
+  const int64_t n = cdiv(N, 32);
+  return n < 1 ? 1 : (n < kMaxBlocks ? n : kMaxBlocks);
+}
 
-template <typename T, int VEC, int LPR, int VPL>
+template <typename T, int LPR, int VPL>
 static void launch_shape(const Args& a, bool bwd, hipStream_t st, int* nblk) {
-  const int64_t rg = NT / LPR, n = cdiv(a.N, rg);
-  if (!bwd) { fwd_kernel<T, VEC, LPR, VPL><<<(uint32_t)n, NT, 0, st>>>(a); return; }
-  *nblk = (int)(n < kMaxBlocks ? n : kMaxBlocks);
-  bwd_kernel<T, VEC, LPR, VPL><<<(uint32_t)*nblk, NT, 0, st>>>(a);
+  const int64_t n = cdiv(a.N, NT / LPR);
+  if (!bwd) { fwd_kernel<T, LPR, VPL><<<(uint32_t)n, NT, 0, st>>>(a); return; }
+  *nblk = (int)(n < part_rows(a.N) ? n : part_rows(a.N));
+  bwd_kernel<T, LPR, VPL><<<(uint32_t)*nblk, NT, 0, st>>>(a);
 }
-template <typename T, int VEC>
-static void launch_vec(const Args& a, const Shape& s, bool bwd, hipStream_t st, int* nblk) {
-  if (s.vpl == 1) {
-    switch (s.lpr) {
-      case 4: return launch_shape<T, VEC, 4, 1>(a, bwd, st, nblk);
-      case 8: return launch_shape<T, VEC, 8, 1>(a, bwd, st, nblk);
-      case 16: return launch_shape<T, VEC, 16, 1>(a, bwd, st, nblk);
-      case 32: return launch_shape<T, VEC, 32, 1>(a, bwd, st, nblk);
-      default: return launch_shape<T, VEC, 64, 1>(a, bwd, st, nblk);
-    }
+template <typename T>
+static void launch_rows(const Args& a, const Shape& s, bool bwd, hipStream_t st, int* nblk) {
+  switch (s.lpr * 8 + s.vpl - 1) {
+    case 32: return launch_shape<T, 4, 1>(a, bwd, st, nblk);
+    case 64: return launch_shape<T, 8, 1>(a, bwd, st, nblk);
+    case 128: return launch_shape<T, 16, 1>(a, bwd, st, nblk);
+    case 256: return launch_shape<T, 32, 1>(a, bwd, st, nblk);
+    case 258: return launch_shape<T, 32, 3>(a, bwd, st, nblk);
+    case 512: return launch_shape<T, 64, 1>(a, bwd, st, nblk);
+    case 513: return launch_shape<T, 64, 2>(a, bwd, st, nblk);
+    case 514: return launch_shape<T, 64, 3>(a, bwd, st, nblk);
+    case 515: return launch_shape<T, 64, 4>(a, bwd, st, nblk);
+    default: return launch_shape<T, 64, 6>(a, bwd, st, nblk);
   }
-  if (s.vpl == 2) return launch_shape<T, VEC, 64, 2>(a, bwd, st, nblk);
-  if (s.vpl == 4) return launch_shape<T, VEC, 64, 4>(a, bwd, st, nblk);
-  launch_shape<T, VEC, 64, 8>(a, bwd, st, nblk);
 }
 
-// 16-byte pieces where the width, every row and every vector allow them, else single values
 template <typename T>
 static int launch(const Args& a, bool bwd, hipStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  auto al = [&](const void* p, int64_t ld) { return !p || ((uintptr_t)p % 16 == 0 && ld % V == 0); };
-  const bool vec = a.C % V == 0 && al(a.x, a.ldx) && al(a.r, a.ldr) && al(a.gy, a.ldg) && al(a.gsum, a.ldgs) && al(a.w, 0) &&
-                   al(a.b, 0) && al(a.y, 0) && al(a.s, 0) && al(a.gx, 0);
   Shape s;
   int nblk = 0;
   if (a.N) {
-    if (vec && shape_of(a.C, V, &s)) launch_vec<T, V>(a, s, bwd, st, &nblk);
-    else if (shape_of(a.C, 1, &s)) launch_vec<T, 1>(a, s, bwd, st, &nblk);
+    if (shape_of((int)cdiv(a.C, Vec<T>::N), &s)) launch_rows<T>(a, s, bwd, st, &nblk);
     else if (!bwd) fwd_wide_kernel<T><<<(uint32_t)a.N, NT, 0, st>>>(a);
     else {
       bwd_wide_kernel<T><<<(uint32_t)a.N, NT, 0, st>>>(a);
@@ -322,7 +334,7 @@ static int launch(const Args& a, bool bwd, hipStream_t st) {
       }
     }
   }
-  if (bwd && a.part) sum_kernel<T><<<(uint32_t)cdiv(2 * (int64_t)a.C, 64), 1024, 0, st>>>(a.part, nblk, a.C, (T*)a.gw, (T*)a.gb);
+  if (bwd && a.part) sum_kernel<T><<<(uint32_t)cdiv(2 * (int64_t)a.C, 16), 1024, 0, st>>>(a.part, nblk, a.C, (T*)a.gw, (T*)a.gb);
   return hipGetLastError() == hipSuccess ? EGNN_OK : EGNN_ERR_HIP;
 }
 

@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/hip/HIPStream.h>
+#include <cmath>
 #include "../../include/egnn.h"
 
 namespace {
@@ -207,6 +208,131 @@ pybind11::object gcl_layer(const Tensor& h, const Opt& x, const Opt& ef, const T
   return pybind11::cast(r[0]);
 }
 
+// ---- segment attention and layer norm ---------------------------------------------
+// The functions of segment_attention.py and layer_norm.py for tensors that need no conversion: checks, allocations and
+// the library call without returning to Python (a forward and backward over a small batch of molecules: 46 us of host
+// work in Python for 24 us of kernels).  None, before anything is allocated, for every other call: the Python path
+// converts, or reports the error.
+bool heads_ok(const Tensor& t, const Tensor& h, int64_t n, int64_t heads, int64_t d, int64_t group = 1) {
+  const int64_t e = t.element_size(), per = 16 / e;
+  return plain(t, h) && t.scalar_type() == h.scalar_type() && t.dim() == 3 && t.size(0) == n && t.size(1) == heads &&
+         t.size(2) == d && t.stride(2) == 1 && t.stride(0) % per == 0 && t.stride(1) % per == 0 && aligned16(t) &&
+         (t.stride(0) == 0 || (t.stride(0) >= d && t.stride(0) * e <= 1 << 24)) && (group - 1) * t.stride(1) * e <= 1 << 29;
+}
+bool attn_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_ptr, const Opt& kv_ptr, const Opt& mask,
+             double scale) {
+  if (torch::jit::tracer::isTracing() || q.dim() != 3 || k.dim() != 3) return false;
+  const auto dt = q.scalar_type();
+  const int64_t d = q.size(2), hk = k.size(1);
+  if ((dt != at::kFloat && dt != at::kBFloat16) || d < 8 || d > 128 || d % 8 || hk < 1 || q.size(1) < 1 || q.size(1) % hk ||
+      !std::isfinite(scale) || scale == 0.0 || (!kv_ptr && q.size(0) != k.size(0)))
+    return false;
+  if (q_ptr.dim() != 1 || q_ptr.numel() < 1 || !fits(q_ptr, q, at::kInt, {q_ptr.numel()}) ||
+      (kv_ptr && !fits(*kv_ptr, q, at::kInt, {q_ptr.numel()})))
+    return false;
+  if (mask && !fits(*mask, q, at::kBool, {k.size(0)}) && !fits(*mask, q, at::kByte, {k.size(0)})) return false;
+  return heads_ok(q, q, q.size(0), q.size(1), d, q.size(1) / hk) && heads_ok(k, q, k.size(0), hk, d) && heads_ok(v, q, k.size(0), hk, d);
+}
+EgnnAttnDims attn_dims(const Tensor& q, const Tensor& k, const Tensor& q_ptr, double scale) {
+  EgnnAttnDims d{};
+  d.Nq = q.size(0); d.Nk = k.size(0); d.n_seg = (int32_t)(q_ptr.numel() - 1);
+  d.Hq = (int32_t)q.size(1); d.Hkv = (int32_t)k.size(1); d.D = (int32_t)q.size(2);
+  d.dtype = q.scalar_type() == at::kFloat ? EGNN_F32 : EGNN_BF16;
+  d.scale = (float)scale;
+  return d;
+}
+Tensor workspace(size_t n, const Tensor& like) {
+  return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
+}
+
+pybind11::object attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_ptr, const Opt& kv_ptr,
+                              const Opt& mask, double scale, bool need_lse) {
+  if (!attn_ok(q, k, v, q_ptr, kv_ptr, mask, scale)) return pybind11::none();
+  const EgnnAttnDims d = attn_dims(q, k, q_ptr, scale);
+  Tensor out = at::empty({d.Nq, d.Hq, d.D}, q.options());
+  Tensor lse = need_lse ? at::empty({d.Hq, d.Nq}, q.options().dtype(at::kFloat)) : Tensor();
+  const size_t nb = egnn_attn_fwd_workspace_bytes(&d);
+  const Tensor ws = workspace(nb, q);
+  EgnnAttnStrides s{};
+  s.q_row = q.stride(0); s.q_head = q.stride(1); s.k_row = k.stride(0); s.k_head = k.stride(1);
+  s.v_row = v.stride(0); s.v_head = v.stride(1); s.out_row = out.stride(0); s.out_head = out.stride(1);
+  check("egnn_attn_fwd", egnn_attn_fwd(&d, &s, ptr(q), ptr(k), ptr(v), ptr<int32_t>(q_ptr), ptr<int32_t>(kv_ptr ? *kv_ptr : q_ptr),
+                                       ptr<uint8_t>(get(mask)), ptr(out), ptr<float>(lse), ptr(ws), nb, stream_of(q)));
+  return pybind11::make_tuple(out, need_lse ? pybind11::cast(lse) : pybind11::none());
+}
+
+pybind11::object attn_backward(const Tensor& go, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+                               const Tensor& lse, const Tensor& q_ptr, const Opt& kv_ptr, const Opt& mask, double scale) {
+  if (!attn_ok(q, k, v, q_ptr, kv_ptr, mask, scale) || !heads_ok(go, q, q.size(0), q.size(1), q.size(2), q.size(1) / k.size(1)) ||
+      !heads_ok(out, q, q.size(0), q.size(1), q.size(2), q.size(1) / k.size(1)) || !fits(lse, q, at::kFloat, {q.size(1), q.size(0)}))
+    return pybind11::none();
+  const EgnnAttnDims d = attn_dims(q, k, q_ptr, scale);
+  const Tensor gq = at::empty({d.Nq, d.Hq, d.D}, q.options()), gk = at::empty({d.Nk, d.Hkv, d.D}, q.options()),
+               gv = at::empty({d.Nk, d.Hkv, d.D}, q.options());
+  const size_t nb = egnn_attn_bwd_workspace_bytes(&d);
+  const Tensor ws = workspace(nb, q);
+  EgnnAttnStrides s{};
+  s.q_row = q.stride(0); s.q_head = q.stride(1); s.k_row = k.stride(0); s.k_head = k.stride(1);
+  s.v_row = v.stride(0); s.v_head = v.stride(1); s.out_row = out.stride(0); s.out_head = out.stride(1);
+  s.grad_out_row = go.stride(0); s.grad_out_head = go.stride(1); s.grad_q_row = gq.stride(0); s.grad_q_head = gq.stride(1);
+  s.grad_k_row = gk.stride(0); s.grad_k_head = gk.stride(1); s.grad_v_row = gv.stride(0); s.grad_v_head = gv.stride(1);
+  check("egnn_attn_bwd", egnn_attn_bwd(&d, &s, ptr(q), ptr(k), ptr(v), ptr(out), ptr<float>(lse), ptr(go), ptr<int32_t>(q_ptr),
+                                       ptr<int32_t>(kv_ptr ? *kv_ptr : q_ptr), ptr<uint8_t>(get(mask)), ptr(gq), ptr(gk), ptr(gv),
+                                       ptr(ws), nb, stream_of(q)));
+  return pybind11::make_tuple(gq, gk, gv);
+}
+
+// contiguous rows of one dtype; the parameters too
+bool norm_ok(const Tensor& x, const Opt& w, const Opt& b, double eps) {
+  const auto dt = x.scalar_type();
+  return !torch::jit::tracer::isTracing() && x.dim() >= 1 && x.size(-1) >= 1 && (dt == at::kFloat || dt == at::kBFloat16) &&
+         plain(x, x) && x.is_contiguous() && fits_opt(w, x, dt, x.size(-1)) && fits_opt(b, x, dt, x.size(-1)) && eps >= 0 &&
+         std::isfinite(eps);
+}
+bool same_rows(const Tensor& t, const Tensor& x) {
+  return plain(t, x) && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && t.is_contiguous();
+}
+EgnnNormDims norm_dims(const Tensor& x, double eps) {
+  EgnnNormDims d{};
+  d.C = (int32_t)x.size(-1); d.N = x.numel() / x.size(-1);
+  d.dtype = x.scalar_type() == at::kFloat ? EGNN_F32 : EGNN_BF16;
+  d.eps = (float)eps;
+  return d;
+}
+
+pybind11::object norm_forward(const Tensor& x, const Opt& w, const Opt& b, double eps, const Opt& res, bool need_stats) {
+  if (!norm_ok(x, w, b, eps) || (res && !same_rows(*res, x))) return pybind11::none();
+  const EgnnNormDims d = norm_dims(x, eps);
+  const auto f32 = x.options().dtype(at::kFloat);
+  const Tensor y = at::empty(x.sizes(), x.options()), s = res ? at::empty(x.sizes(), x.options()) : x;
+  const Tensor mean = need_stats ? at::empty({d.N}, f32) : Tensor(), rstd = need_stats ? at::empty({d.N}, f32) : Tensor();
+  check("egnn_norm_fwd", egnn_norm_fwd(&d, ptr(x), d.C, ptr(get(res)), d.C, ptr(get(w)), ptr(get(b)), ptr(y),
+                                       res ? ptr(s) : nullptr, ptr<float>(mean), ptr<float>(rstd), stream_of(x)));
+  if (!need_stats) return pybind11::make_tuple(y, s, pybind11::none(), pybind11::none());
+  return pybind11::make_tuple(y, s, mean, rstd);
+}
+
+pybind11::object norm_backward(const Tensor& gy, const Tensor& s, const Opt& w, const Tensor& mean, const Tensor& rstd,
+                               const Opt& gsum, bool need_w, bool need_b) {
+  if (!norm_ok(s, w, Opt(), 0.0) || !same_rows(gy, s) || (gsum && !same_rows(*gsum, s))) return pybind11::none();
+  const EgnnNormDims d = norm_dims(s, 0.0);
+  if (!fits(mean, s, at::kFloat, {d.N}) || !fits(rstd, s, at::kFloat, {d.N})) return pybind11::none();
+  const Tensor gx = at::empty(s.sizes(), s.options());
+  const Tensor gw = need_w ? at::empty({d.C}, s.options()) : Tensor(), gb = need_b ? at::empty({d.C}, s.options()) : Tensor();
+  const size_t nb = need_w || need_b ? egnn_norm_bwd_workspace_bytes(&d) : 0;
+  const Tensor ws = workspace(nb, s);
+  check("egnn_norm_bwd", egnn_norm_bwd(&d, ptr(gy), d.C, ptr(s), d.C, ptr(get(w)), ptr<float>(mean), ptr<float>(rstd),
+                                       ptr(get(gsum)), d.C, ptr(gx), ptr(gw), ptr(gb), ptr(ws), nb, stream_of(s)));
+  auto out = [](const Tensor& t) -> pybind11::object { return t.defined() ? pybind11::cast(t) : pybind11::none(); };
+  return pybind11::make_tuple(gx, out(gw), out(gb));
+}
+
 }  // namespace
 
-PYBIND11_MODULE(_egnn_torch, m) { m.def("gcl_layer", &gcl_layer); }
+PYBIND11_MODULE(_egnn_torch, m) {
+  m.def("gcl_layer", &gcl_layer);
+  m.def("attn_forward", &attn_forward);
+  m.def("attn_backward", &attn_backward);
+  m.def("norm_forward", &norm_forward);
+  m.def("norm_backward", &norm_backward);
+}

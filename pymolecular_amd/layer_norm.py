@@ -44,6 +44,10 @@ def _check(x, weight, bias, residual, eps):
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, need_stats=True):
     """``egnn_norm_fwd``: returns ``(y, s, mean, rstd)``; ``s`` is ``x`` itself without a residual, ``mean`` and
     ``rstd`` (rows,) float32 are what :func:`layer_norm_backward` needs (None where ``need_stats`` is false)."""
+    r = _capi.ext().norm_forward(x, weight, bias, eps, residual, need_stats)
+    if r is not None:
+        return r
+    # a tensor needs a conversion, or an argument is refused
     _check(x, weight, bias, residual, eps)
     dt, dev, shape = x.dtype, x.device, x.shape
     x2 = _rows(x)
@@ -65,6 +69,9 @@ def layer_norm_backward(gy, s, weight, mean, rstd, gsum=None, need_weight=True, 
     """``egnn_norm_bwd``: returns ``(gx, gw, gb)`` from the gradient of ``y`` and, where the sum was used too, of ``s``
     (``gsum``).  ``gx`` is the gradient of x and of the residual; ``gw`` and ``gb`` (C,) have the weight's dtype
     (``s``'s without a weight), None where they are not asked for."""
+    r = _capi.ext().norm_backward(gy, s, weight, mean, rstd, gsum, need_weight, need_bias)
+    if r is not None:
+        return r
     dt, dev, shape = s.dtype, s.device, s.shape
     if not s.is_cuda:
         raise RuntimeError("s must be a ROCm device tensor: the layer norm has no CPU path")

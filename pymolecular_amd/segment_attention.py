@@ -27,14 +27,16 @@ __all__ = ["segment_attention", "segment_attention_forward", "segment_attention_
 MAX_HEAD_DIM = 128
 
 
-def _heads(t: torch.Tensor) -> torch.Tensor:
-    """``t`` (n, heads, d) if its heads are unit-stride and 16-byte aligned, else a contiguous copy; a width that is
-    not a multiple of 8 is padded with zeros (which change neither the scores nor the output's own columns)."""
-    d = t.shape[2]
+def _heads(t: torch.Tensor, group: int = 1) -> torch.Tensor:
+    """``t`` (n, heads, d) if the kernels can read it where it lies, else a contiguous copy: unit-stride heads, 16-byte
+    aligned, rows apart (or all the same one) by at most 16 MiB, the ``group`` heads on one key head by 512 MiB.  A width
+    that is not a multiple of 8 is padded with zeros (which change neither the scores nor the output's own columns)."""
+    d, e = t.shape[2], t.element_size()
     if d % 8:
         return torch.nn.functional.pad(t, (0, 8 - d % 8))
-    per = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0:
+    rs, hs = t.stride(0), t.stride(1)
+    if (t.stride(2) == 1 and rs * e % 16 == 0 and hs * e % 16 == 0 and t.data_ptr() % 16 == 0
+            and (rs == 0 or d <= rs <= (1 << 24) // e) and (group - 1) * hs * e <= 1 << 29):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -68,10 +70,14 @@ def _check(q, k, v, q_ptr, kv_ptr, key_mask, scale):
         raise ValueError(f"scale must be finite and not 0 (got {scale})")
 
 
+def _scale(q, scale) -> float:
+    return float(q.shape[-1]) ** -0.5 if scale is None and q.dim() and q.shape[-1] else float(scale or 0.0)
+
+
 def _defaults(q, q_ptr, kv_ptr, key_mask, scale):
     if key_mask is not None and not key_mask.is_contiguous():
         key_mask = key_mask.contiguous()
-    return q_ptr if kv_ptr is None else kv_ptr, key_mask, q.shape[2] ** -0.5 if scale is None else float(scale)
+    return q_ptr if kv_ptr is None else kv_ptr, key_mask, _scale(q, scale)
 
 
 def _dims(q, k, q_ptr, scale) -> EgnnAttnDims:
@@ -86,10 +92,15 @@ def _workspace(nbytes, dev):
 def segment_attention_forward(q, k, v, q_ptr, kv_ptr=None, key_mask=None, scale=None, need_lse=True):
     """``egnn_attn_fwd``: returns ``(out, lse)``; ``lse`` (heads, Nq) float32 is what
     :func:`segment_attention_backward` needs (None where ``need_lse`` is false)."""
+    r = _capi.ext().attn_forward(q, k, v, q_ptr, kv_ptr, key_mask, _scale(q, scale), need_lse)
+    if r is not None:
+        return r
+    # a tensor needs a conversion, or an argument is refused
     kv_ptr, key_mask, scale = _defaults(q, q_ptr, kv_ptr, key_mask, scale)
     _check(q, k, v, q_ptr, kv_ptr, key_mask, scale)
     d = q.shape[2]
-    q, k, v = _heads(q), _heads(k), _heads(v)
+    group = q.shape[1] // k.shape[1]
+    q, k, v = _heads(q, group), _heads(k), _heads(v)
     dims = _dims(q, k, q_ptr, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if need_lse else None
@@ -108,6 +119,10 @@ def segment_attention_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr=None, key_
     """``egnn_attn_bwd``: returns ``(grad_q, grad_k, grad_v)`` from the forward's ``out`` and ``lse``.  ``into``: three
     tensors to write them to (parts of one buffer, say), of the inputs' shapes and dtype with 16-byte aligned
     unit-stride heads."""
+    if into is None:
+        r = _capi.ext().attn_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr, key_mask, _scale(q, scale))
+        if r is not None:
+            return r
     kv_ptr, key_mask, scale = _defaults(q, q_ptr, kv_ptr, key_mask, scale)
     _check(q, k, v, q_ptr, kv_ptr, key_mask, scale)
     if gout.shape != q.shape or out.shape != q.shape:
@@ -117,16 +132,17 @@ def segment_attention_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr=None, key_
     if any(t.device != q.device for t in (gout, out, lse)):
         raise ValueError("gout, out and lse must be on q's device")
     d = q.shape[2]
-    gout = _heads(gout if gout.dtype == q.dtype else gout.to(q.dtype))
-    out = _heads(out if out.dtype == q.dtype else out.to(q.dtype))
-    q, k, v = _heads(q), _heads(k), _heads(v)
+    group = q.shape[1] // k.shape[1]
+    gout = _heads(gout if gout.dtype == q.dtype else gout.to(q.dtype), group)
+    out = _heads(out if out.dtype == q.dtype else out.to(q.dtype), group)
+    q, k, v = _heads(q, group), _heads(k), _heads(v)
     dims = _dims(q, k, q_ptr, scale)
     if into is None:
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
     else:
         grads = list(into)
         for g, t in zip(grads, (q, k, v)):
-            if g.shape != t.shape or g.dtype != t.dtype or g.device != t.device or _heads(g) is not g:
+            if g.shape != t.shape or g.dtype != t.dtype or g.device != t.device or _heads(g) is not g or g.stride(0) < g.shape[2]:
                 raise ValueError("into must hold tensors of the inputs' shapes and dtype with 16-byte aligned heads")
     L = _capi.lib()
     nbytes = L.egnn_attn_bwd_workspace_bytes(dims)
