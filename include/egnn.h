@@ -330,7 +330,7 @@ int32_t egnn_radius_graph(const double* pos, int64_t N, const int32_t* seg_ptr, 
  * Sums, softmax statistics and lse (Hq, Nq) are fp32; bf16 rounds the
  * probabilities and their gradients once, for the second product. */
 typedef struct EgnnAttnDims {
-  int64_t Nq, Nk;        /* rows of q, and of k and v; Nq Hq and Nk below 2^31 - 1024 */
+  int64_t Nq, Nk;        /* rows of q, and of k and v; Nq Hq and Nk below 2^31 - 2^18 */
   int32_t n_seg;
   int32_t Hq, Hkv;       /* heads; Hq a multiple of Hkv */
   int32_t D;             /* head width, a multiple of 8 up to 128 */

@@ -52,7 +52,8 @@ struct Args {
   const int32_t *q_ptr, *kv_ptr;
   const uint8_t* mask;                       // [Nk] or null
   int32_t Nq, Nk, B, Hq, Hkv, G, D;
-  Div by_g, by_heads, by_split;              // divisions by G, Hkv and nsplit
+  uint32_t slots;
+  Div by_g, by_heads, by_slots;              // divisions by G, Hkv and slots
   float c2;                                  // |scale| log2 e
   float scale;                               // |scale|
   uint32_t flip;                             // sign bit of a negative scale: q enters negated
@@ -60,7 +61,9 @@ struct Args {
   float* part;                               // split partials
 };
 
-// How one axis is cut into tiles, and the parts the other axis is walked in
+// How one axis is cut into tiles; the other axis is walked in nsplit parts, part s taking every nsplit-th step from s on:
+// the parts move through memory side by side (apart, 2,048 streams at one stride fell on few memory channels: 324 us
+// where side by side takes XXX, one query over 2,000,000 keys)
 struct Plan {
   int64_t slots;
   int form;                                  // 0: a wave a tile of 16 rows; 1, 2: a workgroup of 4 waves, 64 or 128 rows
@@ -257,31 +260,34 @@ template <typename T, int DP, int KT, int NT> struct Stage {
 // ---- work items -------------------------------------------------------------------
 struct Seg { int lo, hi; };                  // rows of one axis
 __device__ __forceinline__ int edge_of(const int32_t* ptr, int e, int B, int N) {   // start of extended segment e
-  if (e <= 0) return 0;
-  if (e > B + 1) return N;
-  const int p = ptr[e - 1];
-  return p < 0 ? 0 : (p > N ? N : p);
+  const int i = e - 1 < 0 ? 0 : (e - 1 > B ? B : e - 1);
+  int p = ptr[i];
+  p = p < 0 ? 0 : (p > N ? N : p);
+  return e <= 0 ? 0 : (e > B + 1 ? N : p);
 }
 // The extended segment of a slot and the slot's first virtual row in it (-1: an empty slot).  Every lane probes one
-// segment and step, so 64 segments take one round and 4,096 two.
+// segment and step, so 63 segments take one round and 3,969 two; the last round's lanes also hold the segment's ends.
 template <int BQ>
 __device__ __forceinline__ int find_tile(const int32_t* ptr, int B, int N, int G, uint32_t slot, int& vq0, Seg& s) {
-  uint32_t lo = 0, hi = (uint32_t)B + 2;
+  uint32_t lo = 0, hi = (uint32_t)B + 2;     // the slot is at or after segment lo's first, before hi's
   const uint32_t lane = lane_id();
-  while (hi - lo > 1) {
-    const uint32_t step = (hi - lo + 63) / 64, e = lo + lane * step;
-    const bool le = e < hi && (uint32_t)edge_of(ptr, (int)e, B, N) * (uint32_t)G / BQ + e <= slot;
-    const uint32_t n = __builtin_popcountll(__ballot(le));
-    lo += (n > 0 ? n - 1 : 0) * step;
+  for (;;) {
+    const uint32_t step = (hi - lo + 62) / 63, e = lo + lane * step;
+    const int p = edge_of(ptr, (int)(e < hi ? e : hi), B, N);
+    const uint64_t le = __ballot(e < hi && (uint32_t)p * (uint32_t)G / BQ + e <= slot);
+    const int n = le ? __builtin_popcountll(le) - 1 : 0;
+    lo += n * step;
+    if (step == 1) {
+      s.lo = __builtin_amdgcn_readlane(p, n);
+      s.hi = __builtin_amdgcn_readlane(p, n + 1);
+      break;
+    }
     hi = hi < lo + step ? hi : lo + step;
   }
-  const int e = __builtin_amdgcn_readfirstlane((int)lo);
-  s.lo = edge_of(ptr, e, B, N);
-  s.hi = edge_of(ptr, e + 1, B, N);
   if (s.hi < s.lo) s.hi = s.lo;
-  const int64_t v = ((int64_t)slot - (uint32_t)s.lo * (uint32_t)G / BQ - e) * BQ;
+  const int64_t v = ((int64_t)slot - (uint32_t)s.lo * (uint32_t)G / BQ - lo) * BQ;
   vq0 = v >= 0 && v < (int64_t)(s.hi - s.lo) * G ? (int)v : -1;
-  return e;
+  return (int)lo;
 }
 // Rows of the other axis of extended segment e
 __device__ __forceinline__ Seg other_rows(const int32_t* ptr, int e, int B, int N) {
@@ -290,32 +296,26 @@ __device__ __forceinline__ Seg other_rows(const int32_t* ptr, int e, int B, int 
   if (s.hi < s.lo) s.hi = s.lo;
   return s;
 }
-// part s of n of [lo, hi), in whole steps
-template <int STEP>
-__device__ __forceinline__ void split_range(int lo, int hi, int n, int s, int& a, int& b) {
-  if (n == 1) { a = lo; b = hi; return; }
-  const uint32_t per = (((uint32_t)(hi - lo) + n - 1) / n + STEP - 1) / STEP * STEP;
-  const uint64_t x = (uint32_t)lo + (uint64_t)s * per;
-  a = x < (uint64_t)hi ? (int)x : hi;
-  b = (uint32_t)(hi - a) < per ? hi : a + (int)per;
-}
-// Consecutive workgroups' items on one XCD (workgroups go to the 8 XCDs in turn, each has an L2 of its own):
-// neighbouring heads of a tile share the lines of its rows, and the tiles of a segment its keys
+// Workgroups go to the 8 XCDs in turn, each with an L2 of its own.  Runs of 16 consecutive items stay on one XCD:
+// neighbouring heads of a tile share the lines of its rows, and the tiles of a segment its keys.  (An eighth of all items
+// each would do that too, but the work is not even along the items: of one graph's three slots two are empty.)
+constexpr uint32_t kRun = 16;
 __device__ __forceinline__ uint32_t xcd_order(uint32_t bid, uint32_t n) {
-  const uint32_t per = n / 8, rest = n % 8, x = bid % 8, y = bid / 8;
-  return x * per + (x < rest ? x : rest) + y;
+  if (bid >= n / (8 * kRun) * (8 * kRun)) return bid;
+  const uint32_t x = bid % 8, y = bid / 8;
+  return (y / kRun * 8 + x) * kRun + y % kRun;
 }
-// One wave's (SH: one workgroup's) part of the work
+// One wave's (SH: one workgroup's) part of the work: key heads of a slot side by side, then slots, then parts
 struct Item { uint32_t slot; int kvh, sp; };
 template <int W, bool SH>
 __device__ __forceinline__ bool item_of(const Args& a, uint32_t n_items, Item& it) {
   uint32_t i = xcd_order(blockIdx.x, gridDim.x);
   if constexpr (!SH && W > 1) i = i * W + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (i >= n_items) return false;
-  const uint32_t j = a.by_heads(i), k = a.by_split(j);
+  const uint32_t j = a.by_heads(i), k = a.by_slots(j);
   it.kvh = (int)(i - j * (uint32_t)a.Hkv);
-  it.sp = (int)(j - k * (uint32_t)a.nsplit);
-  it.slot = k;
+  it.slot = j - k * a.slots;
+  it.sp = (int)k;
   return true;
 }
 // between a tile's writes and its reads
@@ -335,6 +335,12 @@ __device__ __forceinline__ void store4(bf16* p, const f32x4& v) {
   r[0] = (bf16)v[0]; r[1] = (bf16)v[1]; r[2] = (bf16)v[2]; r[3] = (bf16)v[3];
   *reinterpret_cast<bf16x4*>(p) = r;
 }
+// values that a loop reads: waited for here, or every round of the loop would wait for its own prefetch as well
+__device__ __forceinline__ void landed(bf16x4& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void landed(bf16x8& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void landed(Half3& v) { landed(v.p0); landed(v.p1); landed(v.p2); }
+__device__ __forceinline__ void landed(split::Chunk3& v) { landed(v.p0); landed(v.p1); landed(v.p2); }
+
 // bits of a step's first n rows
 __device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
 

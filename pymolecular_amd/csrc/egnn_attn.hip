@@ -6,7 +6,7 @@ namespace attn {
 namespace {
 
 bool dims_ok(const EgnnAttnDims* d) {
-  const int64_t top = INT32_MAX - 1024;
+  const int64_t top = INT32_MAX - (1 << 18);   // room for a step of every split past the end
   return d && d->Nq >= 0 && d->Nk >= 0 && d->n_seg >= 0 && d->Hq >= 1 && d->Hkv >= 1 && d->Hq % d->Hkv == 0 && d->D >= 8 &&
          d->D <= 128 && d->D % 8 == 0 && (d->dtype == EGNN_F32 || d->dtype == EGNN_BF16) && d->scale - d->scale == 0.f &&
          d->scale != 0.f && d->Nk <= top && d->n_seg <= top && d->Nq <= top && d->Nq * d->Hq <= top;
@@ -113,7 +113,8 @@ int32_t egnn_attn_fwd(const EgnnAttnDims* d, const EgnnAttnStrides* s, const voi
   Args a = make_args(d, s);
   a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.q_ptr = q_ptr; a.kv_ptr = kv_ptr; a.mask = key_mask;
   a.nsplit = p.nsplit;
-  a.by_split = Div::of(p.nsplit);
+  a.slots = (uint32_t)p.slots;
+  a.by_slots = Div::of(a.slots);
   a.part = (float*)workspace;
   return launch_fwd(a, d->dtype == EGNN_BF16, p, (hipStream_t)stream) ? EGNN_ERR_HIP : EGNN_OK;
 }

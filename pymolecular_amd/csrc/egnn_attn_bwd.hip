@@ -13,15 +13,15 @@
 namespace egnn {
 namespace attn {
 
-template <typename T, int DP, int R, int W, bool SH>
+template <typename T, int DP, int R, int W, bool SH, int KT>
 __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t n_items) {
-  typedef Tile<T, DP> TL;
+  typedef Tile<T, DP, KT> TL;
   typedef typename Num<T>::Frag Frag;
-  constexpr int NT = SH ? 64 * W : 64, BQ = 16 * R * (SH ? W : 1);
+  constexpr int NT = SH ? 64 * W : 64, BQ = 16 * R * (SH ? W : 1), KS = TK * KT;
   __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
   Item it;
   if (!item_of<W, SH>(a, n_items, it)) return;
-  const int l = lane_id(), c = l & 15, g = l >> 4, w = threadIdx.x >> 6;
+  const int l = lane_id(), c = l & 15, g = l >> 4, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   bf16 *sK = lds[SH ? 0 : w][0], *sV = lds[SH ? 0 : w][1];
   int vq0;
   Seg qs;
@@ -30,11 +30,11 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
   const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk);
   const int nv = (qs.hi - qs.lo) * a.G, v0 = vq0 + (SH ? 16 * R * w : 0);
   const bool act = v0 < nv;
-  int j, j1;
-  split_range<TK>(ks.lo, ks.hi, a.nsplit, it.sp, j, j1);
-  const bool one = !SH && a.nsplit == 1 && j1 - j <= TK;   // all keys in one step
+  int j = ks.lo + it.sp * KS;
+  const int j1 = ks.hi, stride = KS * a.nsplit;
+  const bool one = !SH && a.nsplit == 1 && j1 - j <= KS;   // all keys in one step
 
-  Stage<T, DP, 1, NT> stK, stV;
+  Stage<T, DP, KT, NT> stK, stV;
   uint32_t offK[stK.PER], offV[stV.PER];
   const int64_t krb = a.k_r * (int64_t)sizeof(T), vrb = a.v_r * (int64_t)sizeof(T);
   stK.offsets(offK, krb, a.D);
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
   const T *kb = (const T*)a.k + it.kvh * a.k_h, *vb = (const T*)a.v + it.kvh * a.v_h;
   uint8_t mb = 1;
   auto fetch = [&](int j) {
-    const int n = j1 - j < TK ? j1 - j : TK;
+    const int n = j1 - j < KS ? j1 - j : KS;
     stK.load(rows_buffer(kb + j * a.k_r, n, krb, a.D * (int)sizeof(T)), offK);
     stV.load(rows_buffer(vb + j * a.v_r, n, vrb, a.D * (int)sizeof(T)), offV);
     if (a.mask) mb = l < n ? a.mask[j + l] : 0;
@@ -70,6 +70,8 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
     for (int kk = 0; kk < TL::NK; ++kk) {
       Q[r][kk] = TL::column(qp, kk, g, a.D, a.flip);
       GO[r][kk] = TL::column(gp, kk, g, a.D, 0);
+      landed(Q[r][kk]);
+      landed(GO[r][kk]);
       if (!one && live[r]) delta[r] += TL::dot(gp, op, kk, g, a.D);
     }
     if (!one) delta[r] = col_sum(delta[r]);
@@ -80,8 +82,8 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
     for (int b = 0; b < TL::NB; ++b) dQ[r][b] = zero4();
   }
 
-  for (; j < j1; j += TK) {
-    uint64_t bits = first_bits(j1 - j < TK ? j1 - j : TK);
+  for (; j < j1; j += stride) {
+    uint64_t bits = first_bits(j1 - j < KS ? j1 - j : KS);
     if (a.mask) {                            // what a masked key holds must not meet a ds of 0
       bits &= __ballot(mb != 0);
       stK.keep(bits);
@@ -90,63 +92,81 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
     stK.store(sK);
     stV.store(sV);
     tile_sync<SH>();
-    if (j + TK < j1) fetch(j + TK);
+    if (j + stride < j1) fetch(j + stride);
     if (!act) continue;
-    f32x4 P[R][2], dS[R][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 hi[R], lo[R], dhi[R], dlo[R];
+    for (int t = 0; t < KT; ++t) {
+      f32x4 P[R][2], dS[R][2];
 #pragma unroll
-      for (int r = 0; r < R; ++r) { hi[r] = zero4(); lo[r] = zero4(); dhi[r] = zero4(); dlo[r] = zero4(); }
+      for (int h = 0; h < 2; ++h) {
+        f32x4 hi[R], lo[R], dhi[R], dlo[R];
 #pragma unroll
-      for (int kk = 0; kk < TL::NK; ++kk) {
-        const auto A = TL::rows(sK, h, kk, c, g), B = TL::rows(sV, h, kk, c, g);
+        for (int r = 0; r < R; ++r) {
+          hi[r] = zero4();
+          lo[r] = zero4();
+          dhi[r] = f32x4{-delta[r], -delta[r], -delta[r], -delta[r]};   // dp - delta
+          dlo[r] = zero4();
+        }
 #pragma unroll
-        for (int r = 0; r < R; ++r) { product1(hi[r], lo[r], A, Q[r][kk]); product1(dhi[r], dlo[r], B, GO[r][kk]); }
-      }
-      const uint32_t hb = (uint32_t)bits >> (16 * h + 4 * g);
+        for (int kk = 0; kk < TL::NK; ++kk) {
+          const auto A = TL::rows(sK, 2 * t + h, kk, c, g), B = TL::rows(sV, 2 * t + h, kk, c, g);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        P[r][h] = result<T>(hi[r], lo[r]);
-        dS[r][h] = result<T>(dhi[r], dlo[r]);
+          for (int r = 0; r < R; ++r) { product1(hi[r], lo[r], A, Q[r][kk]); product1(dhi[r], dlo[r], B, GO[r][kk]); }
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) P[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r][h][i], a.c2, -ref[r]));
-        if (bits != 0xffffffffu) {
+        for (int r = 0; r < R; ++r) {
+          P[r][h] = result<T>(hi[r], lo[r]);
+          dS[r][h] = result<T>(dhi[r], dlo[r]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            P[r][h][i] = (hb >> i) & 1 ? P[r][h][i] : 0.f;
-            dS[r][h][i] = (hb >> i) & 1 ? dS[r][h][i] : 0.f;
-          }
+          for (int i = 0; i < 4; ++i) P[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r][h][i], a.c2, -ref[r]));
         }
       }
-    }
-    if (one) {
+      if (bits != first_bits(KS)) {
+        const uint32_t tb = (uint32_t)(bits >> (32 * t)) >> (4 * g);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool ok = (tb >> (16 * h + i)) & 1;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              P[r][h][i] = ok ? P[r][h][i] : 0.f;
+              dS[r][h][i] = ok ? dS[r][h][i] : 0.f;
+            }
+          }
+      }
+      if (one) {                             // delta was 0 so far
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) delta[r] = __builtin_fmaf(P[r][h][i], dS[r][h][i], delta[r]);
+          delta[r] = col_sum(delta[r]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dS[r][h][i] -= delta[r];
+        }
+      }
+      Frag F[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) delta[r] = __builtin_fmaf(P[r][h][i], dS[r][h][i], delta[r]);
-        delta[r] = col_sum(delta[r]);
+          for (int i = 0; i < 4; ++i) {
+            dS[r][h][i] *= P[r][h][i];
+            if constexpr (!SH) sum[r] += dS[r][h][i];
+          }
+        F[r] = chain_frag<T>(dS[r][0], dS[r][1]);
       }
-    }
-    Frag F[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
+      for (int b = 0; b < TL::NB; ++b) {
+        const Frag A = TL::cols(sK, t, b, c, g);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          dS[r][h][i] = P[r][h][i] * (dS[r][h][i] - delta[r]);
-          if constexpr (!SH) sum[r] += dS[r][h][i];
-        }
-      F[r] = chain_frag<T>(dS[r][0], dS[r][1]);
-    }
-#pragma unroll
-    for (int b = 0; b < TL::NB; ++b) {
-      const Frag A = TL::cols(sK, 0, b, c, g);
-#pragma unroll
-      for (int r = 0; r < R; ++r) accumulate(dQ[r][b], A, F[r]);
+        for (int r = 0; r < R; ++r) accumulate(dQ[r][b], A, F[r]);
+      }
     }
   }
   const float sc = a.flip ? -a.scale : a.scale;
@@ -168,16 +188,16 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
   }
 }
 
-template <typename T, int DP, int R, int W, bool SH>
+template <typename T, int DP, int R, int W, bool SH, int KT>
 __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_t n_items) {
-  typedef Tile<T, DP> TL;
+  typedef Tile<T, DP, KT> TL;
   typedef typename Num<T>::Frag Frag;
-  constexpr int NT = SH ? 64 * W : 64, BK = 16 * R * (SH ? W : 1);
+  constexpr int NT = SH ? 64 * W : 64, BK = 16 * R * (SH ? W : 1), KS = TK * KT;
   __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
-  __shared__ __attribute__((aligned(16))) float stat[SH ? 1 : W][2][TK];
+  __shared__ __attribute__((aligned(16))) float stat[SH ? 1 : W][2][KS];
   Item it;
   if (!item_of<W, SH>(a, n_items, it)) return;
-  const int l = lane_id(), c = l & 15, g = l >> 4, w = threadIdx.x >> 6;
+  const int l = lane_id(), c = l & 15, g = l >> 4, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   bf16 *sQ = lds[SH ? 0 : w][0], *sG = lds[SH ? 0 : w][1];
   float *sL = stat[SH ? 0 : w][0], *sD = stat[SH ? 0 : w][1];
   int k0;
@@ -187,10 +207,10 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
   const Seg qs = other_rows(a.q_ptr, e, a.B, a.Nq);
   const int key0 = ks.lo + k0 + (SH ? 16 * R * w : 0);
   const bool act = key0 < ks.hi;
-  int j, j1;                                 // virtual rows of the segment
-  split_range<TK>(0, (qs.hi - qs.lo) * a.G, a.nsplit, it.sp, j, j1);
+  int j = it.sp * KS;                        // virtual rows of the segment
+  const int j1 = (qs.hi - qs.lo) * a.G, stride = KS * a.nsplit;
 
-  Stage<T, DP, 1, NT> stQ, stG;
+  Stage<T, DP, KT, NT> stQ, stG;
   uint32_t offQ[stQ.PER], offG[stG.PER];
   const int64_t qrb = a.q_r * (int64_t)sizeof(T), grb = a.go_r * (int64_t)sizeof(T);
   stQ.offsets(offQ, qrb, a.D);
@@ -198,7 +218,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
   const T *qb = (const T*)a.q + (int64_t)it.kvh * a.G * a.q_h, *gb = (const T*)a.go + (int64_t)it.kvh * a.G * a.go_h;
   float lse = INFINITY, delta = 0.f;
   auto fetch = [&](int j) {
-    const int n = j1 - j < TK ? j1 - j : TK, r0 = (int)a.by_g(j), first = qs.lo + r0;
+    const int n = j1 - j < KS ? j1 - j : KS, r0 = (int)a.by_g(j), first = qs.lo + r0;
     int rows = n;
     if (a.G > 1) {                           // rows and heads of the step's virtual rows
       const int u0 = j - r0 * a.G;           // head of the first one
@@ -241,54 +261,60 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
     for (int kk = 0; kk < TL::NK; ++kk) {
       K[r][kk] = TL::column(kp, kk, g, a.D, a.flip);   // the scale's sign
       V[r][kk] = TL::column(vp, kk, g, a.D, 0);
+      landed(K[r][kk]);
+      landed(V[r][kk]);
     }
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b) { dK[r][b] = zero4(); dV[r][b] = zero4(); }
   }
 
-  for (; j < j1; j += TK) {
+  for (; j < j1; j += stride) {
     const float ref = lse == -INFINITY ? INFINITY : lse * kLog2e;
-    const uint64_t bits = __ballot(ref != INFINITY);   // lanes 0 .. 31
-    if (bits != 0xffffffffu) { stQ.keep(bits); stG.keep(bits); }
+    const uint64_t bits = __ballot(ref != INFINITY);   // of lanes 0 .. KS - 1
+    if (bits != first_bits(KS)) { stQ.keep(bits); stG.keep(bits); }
     tile_sync<SH>();
     stQ.store(sQ);
     stG.store(sG);
-    if ((!SH || w == 0) && l < TK) { sL[l] = ref; sD[l] = delta; }
+    if ((!SH || w == 0) && l < KS) { sL[l] = ref; sD[l] = -delta; }
     tile_sync<SH>();
-    if (j + TK < j1) fetch(j + TK);
+    if (j + stride < j1) fetch(j + stride);
     if (!act) continue;
-    f32x4 P[R][2], dS[R][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 hi[R], lo[R], dhi[R], dlo[R];
+    for (int t = 0; t < KT; ++t) {
+      f32x4 P[R][2], dS[R][2];
 #pragma unroll
-      for (int r = 0; r < R; ++r) { hi[r] = zero4(); lo[r] = zero4(); dhi[r] = zero4(); dlo[r] = zero4(); }
+      for (int h = 0; h < 2; ++h) {
+        const int b = 2 * t + h;
+        const f32x4 Lr = load4_f32(sL + 16 * b + 4 * g), nD = load4_f32(sD + 16 * b + 4 * g);
+        f32x4 hi[R], lo[R], dhi[R], dlo[R];
 #pragma unroll
-      for (int kk = 0; kk < TL::NK; ++kk) {
-        const auto A = TL::rows(sQ, h, kk, c, g), B = TL::rows(sG, h, kk, c, g);
+        for (int r = 0; r < R; ++r) { hi[r] = zero4(); lo[r] = zero4(); dhi[r] = nD; dlo[r] = zero4(); }   // dp - delta
 #pragma unroll
-        for (int r = 0; r < R; ++r) { product1(hi[r], lo[r], A, K[r][kk]); product1(dhi[r], dlo[r], B, V[r][kk]); }
-      }
-      const f32x4 Lr = load4_f32(sL + 16 * h + 4 * g), D = load4_f32(sD + 16 * h + 4 * g);
+        for (int kk = 0; kk < TL::NK; ++kk) {
+          const auto A = TL::rows(sQ, b, kk, c, g), B = TL::rows(sG, b, kk, c, g);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        P[r][h] = result<T>(hi[r], lo[r]);
-        dS[r][h] = result<T>(dhi[r], dlo[r]);
+          for (int r = 0; r < R; ++r) { product1(hi[r], lo[r], A, K[r][kk]); product1(dhi[r], dlo[r], B, V[r][kk]); }
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          P[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r][h][i], a.c2, -Lr[i]));
-          dS[r][h][i] = P[r][h][i] * (dS[r][h][i] - D[i]);
+        for (int r = 0; r < R; ++r) {
+          P[r][h] = result<T>(hi[r], lo[r]);
+          dS[r][h] = result<T>(dhi[r], dlo[r]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            P[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r][h][i], a.c2, -Lr[i]));
+            dS[r][h][i] *= P[r][h][i];
+          }
         }
       }
-    }
-    Frag FP[R], FS[R];
+      Frag FP[R], FS[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) { FP[r] = chain_frag<T>(P[r][0], P[r][1]); FS[r] = chain_frag<T>(dS[r][0], dS[r][1]); }
+      for (int r = 0; r < R; ++r) { FP[r] = chain_frag<T>(P[r][0], P[r][1]); FS[r] = chain_frag<T>(dS[r][0], dS[r][1]); }
 #pragma unroll
-    for (int b = 0; b < TL::NB; ++b) {
-      const Frag A = TL::cols(sG, 0, b, c, g), B = TL::cols(sQ, 0, b, c, g);
+      for (int b = 0; b < TL::NB; ++b) {
+        const Frag A = TL::cols(sG, t, b, c, g), B = TL::cols(sQ, t, b, c, g);
 #pragma unroll
-      for (int r = 0; r < R; ++r) { accumulate(dV[r][b], A, FP[r]); accumulate(dK[r][b], B, FS[r]); }
+        for (int r = 0; r < R; ++r) { accumulate(dV[r][b], A, FP[r]); accumulate(dK[r][b], B, FS[r]); }
+      }
     }
   }
   const float sc = a.flip ? -a.scale : a.scale;
@@ -314,66 +340,77 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
   }
 }
 
-// out[row][head][f] = mul * sum over the splits: 32 values a block, 8 groups of splits, added in order; the partial rows
-// are `width` values apart, the values from `off` on
-template <typename T>
+// out[row][head][f] = mul * sum over the splits, 4 features a thread: GR groups of splits a block, whose sums are added in
+// order.  The partial rows are `width` values apart, the values from `off` on.
+template <typename T, int GR>
 __global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int nsplit, int64_t rows, int heads, int D, int width, int off,
                                                         float mul, T* out, int64_t rs, int64_t hs) {
-  __shared__ float red[8][32];
-  const int x = threadIdx.x & 31, k = threadIdx.x >> 5;
-  const int64_t t = (int64_t)blockIdx.x * 32 + x, r = t / D, n = rows * heads;
-  const int f = (int)(t - r * D);
-  float s = 0.f;
+  constexpr int PB = 256 / GR;
+  __shared__ f32x4 red[GR][PB];
+  const int x = threadIdx.x % PB, k = threadIdx.x / PB;
+  const int64_t n = rows * heads, t = (int64_t)blockIdx.x * PB + x;
+  const int64_t r = t / (D / 4);
+  const int f = 4 * (int)(t - r * (D / 4));
+  f32x4 s = zero4();
   if (r < n) {
 #pragma unroll 4
-    for (int i = k; i < nsplit; i += 8) s += part[(i * n + r) * width + off + f];
+    for (int i = k; i < nsplit; i += GR) s += load4_f32(part + (i * n + r) * width + off + f);
   }
-  red[k][x] = s;
-  __syncthreads();
-  if (k || r >= n) return;
+  if constexpr (GR > 1) {
+    red[k][x] = s;
+    __syncthreads();
+    if (k) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s += red[i][x];
-  out[(r / heads) * rs + (r % heads) * hs + f] = from_f32<T>(s * mul);
+    for (int i = 1; i < GR; ++i) s += red[i][x];
+  }
+  if (r < n) store4(out + (r / heads) * rs + (r % heads) * hs + f, s * mul);
+}
+template <typename T>
+static void sum_parts(const float* part, int nsplit, int64_t rows, int heads, int D, int width, int off, float mul, void* out, int64_t rs,
+                      int64_t hs, hipStream_t st) {
+  const int64_t n = rows * heads * (D / 4);
+  if (nsplit <= 16) sum_parts_kernel<T, 1><<<(uint32_t)cdiv(n, 256), 256, 0, st>>>(part, nsplit, rows, heads, D, width, off, mul, (T*)out, rs, hs);
+  else sum_parts_kernel<T, 32><<<(uint32_t)cdiv(n, 8), 256, 0, st>>>(part, nsplit, rows, heads, D, width, off, mul, (T*)out, rs, hs);
 }
 
-template <typename T, int DP, int R, int W, bool SH>
+template <typename T, int DP, int R, int W, bool SH, int KT>
 static void go_q(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
-  dq_kernel<T, DP, R, W, SH><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
+  dq_kernel<T, DP, R, W, SH, KT><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
 }
-template <typename T, int DP, int R, int W, bool SH>
+template <typename T, int DP, int R, int W, bool SH, int KT>
 static void go_k(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
-  dkv_kernel<T, DP, R, W, SH><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
+  dkv_kernel<T, DP, R, W, SH, KT><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
 }
 template <typename T, int DP>
 static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
   constexpr int tile = 2 * Tile<T, DP>::elems * 2 + 256, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
   constexpr bool wide = Num<T>::planes == 3 && DP == 128;
-  auto blocks = [&](int64_t n) { return (uint32_t)cdiv(n * a.D, 32); };
+  constexpr int KT = Num<T>::planes == 1 && DP < 128 ? 2 : 1;
   a.nsplit = pq.nsplit;
-  a.by_split = Div::of(a.nsplit);
+  a.slots = (uint32_t)pq.slots;
+  a.by_slots = Div::of(a.slots);
   if (a.Nq) {
-    if constexpr (wide) go_q<T, DP, 1, 4, true>(a, pq, st);
-    else if (pq.form == 0) go_q<T, DP, 1, W, false>(a, pq, st);
-    else if (pq.form == 1) go_q<T, DP, 1, 4, true>(a, pq, st);
-    else go_q<T, DP, 2, 4, true>(a, pq, st);
+    if constexpr (wide) go_q<T, DP, 1, 4, true, KT>(a, pq, st);
+    else if (pq.form == 0) go_q<T, DP, 1, W, false, 1>(a, pq, st);
+    else if (pq.form == 1) go_q<T, DP, 1, 4, true, KT>(a, pq, st);
+    else go_q<T, DP, 2, 4, true, KT>(a, pq, st);
     if (a.nsplit > 1)
-      sum_parts_kernel<T><<<blocks((int64_t)a.Nq * a.Hq), 256, 0, st>>>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, 0,
-                                                                        a.flip ? -a.scale : a.scale, (T*)a.gq, a.gq_r, a.gq_h);
+      sum_parts<T>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, 0, a.flip ? -a.scale : a.scale, a.gq, a.gq_r, a.gq_h, st);
   }
   a.nsplit = pk.nsplit;
-  a.by_split = Div::of(a.nsplit);
+  a.slots = (uint32_t)pk.slots;
+  a.by_slots = Div::of(a.slots);
   if (a.Nk) {
-    if constexpr (wide) go_k<T, DP, 1, 4, true>(a, pk, st);
-    else if (pk.form == 0) go_k<T, DP, 1, W, false>(a, pk, st);
-    else if (pk.form == 1) go_k<T, DP, 1, 4, true>(a, pk, st);
-    else if constexpr (DP <= (Num<T>::planes == 1 ? 64 : 32)) go_k<T, DP, 2, 4, true>(a, pk, st);
+    if constexpr (wide) go_k<T, DP, 1, 4, true, KT>(a, pk, st);
+    else if (pk.form == 0) go_k<T, DP, 1, W, false, 1>(a, pk, st);
+    else if (pk.form == 1) go_k<T, DP, 1, 4, true, KT>(a, pk, st);
+    else if constexpr (DP <= (Num<T>::planes == 1 ? 64 : 32)) go_k<T, DP, 2, 4, true, KT>(a, pk, st);
     if (a.nsplit > 1) {
-      const uint32_t nb = blocks((int64_t)a.Nk * a.Hkv);
       const float sc = a.flip ? -a.scale : a.scale;
-      sum_parts_kernel<T><<<nb, 256, 0, st>>>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, 2 * DP, 0, sc, (T*)a.gk, a.gk_r, a.gk_h);
-      sum_parts_kernel<T><<<nb, 256, 0, st>>>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, 2 * DP, DP, 1.0f, (T*)a.gv, a.gv_r, a.gv_h);
+      sum_parts<T>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, 2 * DP, 0, sc, a.gk, a.gk_r, a.gk_h, st);
+      sum_parts<T>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, 2 * DP, DP, 1.0f, a.gv, a.gv_r, a.gv_h, st);
     }
   }
   return (int)hipGetLastError();

@@ -27,7 +27,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_
   __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
   Item it;
   if (!item_of<W, SH>(a, n_items, it)) return;
-  const int l = lane_id(), c = l & 15, g = l >> 4, w = threadIdx.x >> 6;
+  const int l = lane_id(), c = l & 15, g = l >> 4, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   bf16 *sK = lds[SH ? 0 : w][0], *sV = lds[SH ? 0 : w][1];
   int vq0;
   Seg qs;
@@ -36,8 +36,8 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_
   const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk);
   const int nv = (qs.hi - qs.lo) * a.G, v0 = vq0 + (SH ? 16 * R * w : 0);
   const bool act = v0 < nv;                  // a wave without rows still loads tiles for the others
-  int j, j1;
-  split_range<KS>(ks.lo, ks.hi, a.nsplit, it.sp, j, j1);
+  int j = ks.lo + it.sp * KS;
+  const int j1 = ks.hi, stride = KS * a.nsplit;
 
   Stage<T, DP, KT, NT> stK, stV;
   uint32_t offK[stK.PER], offV[stV.PER];
@@ -67,7 +67,10 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_
     head[r] = it.kvh * a.G + (live[r] ? v - (int)i * a.G : 0);
     const T* qp = live[r] ? (const T*)a.q + row[r] * a.q_r + head[r] * a.q_h : nullptr;
 #pragma unroll
-    for (int kk = 0; kk < TL::NK; ++kk) Q[r][kk] = TL::column(qp, kk, g, a.D, a.flip);
+    for (int kk = 0; kk < TL::NK; ++kk) {
+      Q[r][kk] = TL::column(qp, kk, g, a.D, a.flip);
+      landed(Q[r][kk]);
+    }
   }
   f32x4 O[R][TL::NB];
   float m[R], sum[R];
@@ -79,7 +82,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_
     for (int b = 0; b < TL::NB; ++b) O[r][b] = zero4();
   }
 
-  for (; j < j1; j += KS) {
+  for (; j < j1; j += stride) {
     uint64_t bits = first_bits(j1 - j < KS ? j1 - j : KS);
     if (a.mask) {                            // what a masked value holds must not meet a probability of 0
       bits &= __ballot(mb != 0);
@@ -89,7 +92,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_
     stK.store(sK);
     stV.store(sV);
     tile_sync<SH>();
-    if (j + KS < j1) fetch(j + KS);
+    if (j + stride < j1) fetch(j + stride);
     if (!act) continue;
     f32x4 S[R][2 * KT];
 #pragma unroll
@@ -183,14 +186,14 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_
   }
 }
 
-// Joins the splits of one row and head: their weights first, then 4 features a thread over groups of splits, whose sums
-// are added in order
+// Joins many splits of a row and head: their weights first, then 4 features a thread over 64 groups of splits, whose sums
+// are added in order.  16 features a block: with all of a row's in one, the few rows that are split this often kept few
+// CUs busy (24.8 us against XXX for 8 rows of 2,048 splits).
 constexpr int kMaxSplit = 2048;
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
-  constexpr int LF = DP / 4, GR = 256 / LF;
+__global__ __launch_bounds__(256) void fwd_join_many_kernel(Args a) {
   __shared__ float wt[kMaxSplit], red[4];
-  __shared__ f32x4 part[GR][LF];
+  __shared__ f32x4 part[64][4];
   const uint32_t r = blockIdx.x;
   const int head = (int)(r % (uint32_t)a.Hq), t = threadIdx.x;
   const int64_t row = r / (uint32_t)a.Hq;
@@ -211,18 +214,43 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
   if ((t & 63) == 0) red[t >> 6] = sum;
   __syncthreads();
   sum = (red[0] + red[1]) + (red[2] + red[3]);
-  const int f = 4 * (t % LF), gr = t / LF;
+  const int f = 16 * (int)blockIdx.y + 4 * (t & 3), gr = t >> 2;
+  f32x4 o = zero4();
+#pragma unroll 8
+  for (int s = gr; s < a.nsplit; s += 64) o += load4_f32(part_o(a, DP, s, r) + f) * wt[s];
+  part[gr][t & 3] = o;
+  __syncthreads();
+  for (int h = 32; h; h >>= 1) {
+    if (gr < h) part[gr][t & 3] += part[gr + h][t & 3];
+    __syncthreads();
+  }
+  if (gr) return;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  if (f < a.D) store4((T*)a.out + row * a.o_r + head * a.o_h + f, part[0][t & 3] * inv);
+  if (a.lse && t == 0 && blockIdx.y == 0) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+// Joins few splits: 4 features a thread
+constexpr int kFewSplits = 16;
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, r = t / (DP / 4);
+  const int f = 4 * (int)(t % (DP / 4));
+  if (r >= (int64_t)a.Nq * a.Hq) return;
+  const int head = (int)((uint32_t)r % (uint32_t)a.Hq);
+  const int64_t row = (uint32_t)r / (uint32_t)a.Hq;
+  float m = kLowest, sum = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, part_ml(a, DP, s, r)[0]);
   f32x4 o = zero4();
 #pragma unroll 4
-  for (int s = gr; s < a.nsplit; s += GR) o += load4_f32(part_o(a, DP, s, r) + f) * wt[s];
-  part[gr][t % LF] = o;
-  __syncthreads();
-  if (gr) return;
-#pragma unroll 4
-  for (int k = 1; k < GR; ++k) o += part[k][t];
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float* p = part_ml(a, DP, s, r);
+    const float x = __builtin_amdgcn_exp2f(p[0] - m);
+    sum = __builtin_fmaf(p[1], x, sum);
+    o += load4_f32(part_o(a, DP, s, r) + f) * x;
+  }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   if (f < a.D) store4((T*)a.out + row * a.o_r + head * a.o_h + f, o * inv);
-  if (a.lse && t == 0) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+  if (a.lse && f == 0) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 template <typename T, int DP, int R, int W, bool SH, int KT>
@@ -238,7 +266,9 @@ static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
   else if (p.form == 0) go<T, DP, 1, W, false, 1>(a, p, st);
   else if (p.form == 1) go<T, DP, 1, 4, true, KT>(a, p, st);
   else go<T, DP, 2, 4, true, KT>(a, p, st);
-  if (a.nsplit > 1) fwd_join_kernel<T, DP><<<(uint32_t)((int64_t)a.Nq * a.Hq), 256, 0, st>>>(a);
+  const int64_t rows = (int64_t)a.Nq * a.Hq;
+  if (a.nsplit > kFewSplits) fwd_join_many_kernel<T, DP><<<dim3((uint32_t)rows, DP / 16), 256, 0, st>>>(a);
+  else if (a.nsplit > 1) fwd_join_kernel<T, DP><<<(uint32_t)cdiv(rows * (DP / 4), 256), 256, 0, st>>>(a);
   return (int)hipGetLastError();
 }
 template <typename T>

@@ -19,24 +19,28 @@ struct Args {
   float eps;
 };
 
-// VEC = 16 bytes of values at a lane's column f.  Rows need no alignment but their values': the type says so, and the
-// compiler still makes one 16-byte access of it (259 fp32 values a row: 16-byte pieces with a scalar tail 24 us where
-// single values took 52, forward and backward of 40,961 rows).  The last piece of a row that is not a multiple of VEC
-// wide goes value by value.
+// 16 bytes of values at a lane's column f.  Rows need no alignment but their values': the type says so, and the compiler
+// still makes one 16-byte access of it (XXX).  The last piece of a row that is not a multiple of them wide goes value by
+// value.  A piece stays as it was loaded until it is used, so that the next row's can be on their way.
 template <typename T> struct Vec {
   static constexpr int N = 16 / sizeof(T);
   typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-  static __device__ __forceinline__ void load(const T* p, int f, int C, float* v) {
+  typedef T piece __attribute__((ext_vector_type(N)));
+  static __device__ __forceinline__ piece load(const T* p, int f, int C) {
+    piece t;
     if (f + N <= C) {
-      const type t = *reinterpret_cast<const type*>(p + f);
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = to_f32((T)t[i]);
+      t = *reinterpret_cast<const type*>(p + f);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (f + i < C) v[i] = to_f32(p[f + i]);
+      for (int i = 0; i < N; ++i) t[i] = f + i < C ? p[f + i] : (T)0.f;
     }
+    return t;
   }
+  static __device__ __forceinline__ void floats(const piece& t, float* v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f32((T)t[i]);
+  }
+  static __device__ __forceinline__ void load(const T* p, int f, int C, float* v) { floats(load(p, f, C), v); }
   static __device__ __forceinline__ void store(T* p, int f, int C, const float* v) {
     if (f + N <= C) {
       type t;
@@ -134,34 +138,50 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
     for (int i = 0; i < VEC; ++i) { gw[p][i] = 0.f; gb[p][i] = 0.f; w[p][i] = f + i < a.C ? 1.f : 0.f; }
     if (a.w && f < a.C) Vec<T>::load((const T*)a.w, f, a.C, w[p]);
   }
-  for (int64_t n0 = (int64_t)blockIdx.x * RG; n0 < a.N; n0 += (int64_t)gridDim.x * RG) {
-    const int64_t n = n0 + rg;
-    const bool live = n < a.N;
-    const float mean = live ? a.mean[n] : 0.f, rstd = live ? a.rstd[n] : 0.f;
-    float xh[VPL][VEC], t[VPL][VEC], e[VPL][VEC];
+  const int64_t step = (int64_t)gridDim.x * RG;
+  typename Vec<T>::piece pg[VPL], px[VPL], pe[VPL];
+  float mean = 0.f, rstd = 0.f;
+  auto fetch = [&](int64_t n) {   // everything a row needs, requested at once
+    mean = n < a.N ? a.mean[n] : 0.f;
+    rstd = n < a.N ? a.rstd[n] : 0.f;
 #pragma unroll
-    for (int p = 0; p < VPL; ++p) {   // everything the row needs, requested at once
+    for (int p = 0; p < VPL; ++p) {
       const int f = (p * LPR + lane) * VEC;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) { t[p][i] = 0.f; xh[p][i] = mean; e[p][i] = 0.f; }
-      if (live && f < a.C) {
-        Vec<T>::load((const T*)a.gy + n * a.ldg, f, a.C, t[p]);
-        Vec<T>::load((const T*)a.x + n * a.ldx, f, a.C, xh[p]);
-        if (a.gsum) Vec<T>::load((const T*)a.gsum + n * a.ldgs, f, a.C, e[p]);
+      if (n < a.N && f < a.C) {
+        pg[p] = Vec<T>::load((const T*)a.gy + n * a.ldg, f, a.C);
+        px[p] = Vec<T>::load((const T*)a.x + n * a.ldx, f, a.C);
+        if (a.gsum) pe[p] = Vec<T>::load((const T*)a.gsum + n * a.ldgs, f, a.C);
       }
     }
+  };
+  int64_t n = (int64_t)blockIdx.x * RG + rg;
+  fetch(n);
+  for (; n - rg < a.N; n += step) {
+    const bool live = n < a.N;
+    float xh[VPL][VEC], t[VPL][VEC], e[VPL][VEC];
     float s1 = 0.f, s2 = 0.f;
+    const float mu = mean, rs = rstd;
 #pragma unroll
-    for (int p = 0; p < VPL; ++p)
+    for (int p = 0; p < VPL; ++p) {
+      const int f = (p * LPR + lane) * VEC;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { t[p][i] = 0.f; xh[p][i] = mu; e[p][i] = 0.f; }
+      if (live && f < a.C) {
+        Vec<T>::floats(pg[p], t[p]);
+        Vec<T>::floats(px[p], xh[p]);
+        if (a.gsum) Vec<T>::floats(pe[p], e[p]);
+      }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        xh[p][i] = (xh[p][i] - mean) * rstd;
+        xh[p][i] = f + i < a.C ? (xh[p][i] - mu) * rs : 0.f;
         gw[p][i] = __builtin_fmaf(t[p][i], xh[p][i], gw[p][i]);
         gb[p][i] += t[p][i];
         t[p][i] *= w[p][i];
         s1 += t[p][i];
         s2 = __builtin_fmaf(t[p][i], xh[p][i], s2);
       }
+    }
+    fetch(n + step);
     const float m1 = row_sum<LPR>(s1) / a.C, m2 = row_sum<LPR>(s2) / a.C;
 #pragma unroll
     for (int p = 0; p < VPL; ++p) {
@@ -169,7 +189,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
       if (live && f < a.C) {
         float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = __builtin_fmaf(rstd, t[p][i] - m1 - xh[p][i] * m2, e[p][i]);
+        for (int i = 0; i < VEC; ++i) o[i] = __builtin_fmaf(rs, t[p][i] - m1 - xh[p][i] * m2, e[p][i]);
         Vec<T>::store((T*)a.gx + n * a.C, f, a.C, o);
       }
     }
@@ -279,7 +299,7 @@ __global__ __launch_bounds__(1024) void sum_kernel(const float* part, int nblk, 
   else if (gb) gb[f - C] = from_f32<T>(s);
 }
 
-constexpr int kMaxBlocks = 2048;   // partial rows of the weight gradients
+constexpr int kMaxBlocks = 1024;   // partial rows of the weight gradients
 
 // lanes and pieces of a row: the fewest lane slots that hold it
 struct Shape { int lpr, vpl; };
