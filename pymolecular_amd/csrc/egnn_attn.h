@@ -53,6 +53,8 @@ struct Args {
   const uint8_t* mask;                       // [Nk] or null
   int32_t Nq, Nk, B, Hq, Hkv, G, D;
   uint32_t slots;
+  float guess;                               // segments per slot
+  bool same;                                 // q_ptr is kv_ptr and there are as many queries as keys
   Div by_g, by_heads, by_slots;              // divisions by G, Hkv and slots
   float c2;                                  // |scale| log2 e
   float scale;                               // |scale|
@@ -217,38 +219,50 @@ template <typename T, int DP, int KT = 1> struct Tile {
   }
 };
 
-// The rows of a tile on their way to LDS: NT threads, 8 values each and piece
-template <typename T, int DP, int KT, int NT> struct Stage {
+// bits of a step's rows, 64 a word
+template <int KT> struct Bits {
+  static constexpr int N = (KT * TK + 63) / 64;
+  uint64_t w[N];
+  __device__ __forceinline__ uint32_t step(int t) const { return (uint32_t)(w[t / 2] >> (32 * (t & 1))); }
+  __device__ __forceinline__ bool row(int i) const {
+    uint64_t x = w[0];
+#pragma unroll
+    for (int k = 1; k < N; ++k) x = i >= 64 * k ? w[k] : x;
+    return (x >> (i & 63)) & 1;
+  }
+};
+
+// The rows of a tile on their way to LDS: NT threads, 8 values each and piece.  n: the rows there are; pieces past them
+// are left out, up to a whole number of UNIT rows, which are computed together: their zeros are written too.
+template <typename T, int DP, int KT, int NT, int UNIT = TK> struct Stage {
   typedef Tile<T, DP, KT> TL;
   static constexpr int CH = DP / 8, N = KT * TK * CH, PER = (N + NT - 1) / NT;
   typename Num<T>::Raw r[PER];
   static __device__ __forceinline__ int row(int p) { return (p * NT + (int)threadIdx.x % NT) / CH; }
   static __device__ __forceinline__ int feature(int p) { return 8 * ((p * NT + (int)threadIdx.x % NT) % CH); }
   static __device__ __forceinline__ bool in(int p) { return N % NT == 0 || p * NT + (int)threadIdx.x % NT < N; }
+  static __device__ __forceinline__ bool needed(int p, int n) { return p * NT / CH < (n + UNIT - 1) / UNIT * UNIT; }   // uniform
   // byte offsets of the lane's pieces in a buffer of rows
   static __device__ __forceinline__ void offsets(uint32_t* off, int64_t row_bytes, int D) {
 #pragma unroll
     for (int p = 0; p < PER; ++p)
       off[p] = in(p) && feature(p) < D ? (uint32_t)(row(p) * (uint32_t)row_bytes + feature(p) * (uint32_t)sizeof(T)) : kOob;
   }
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t b, const uint32_t* off) {
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t b, const uint32_t* off, int n) {
 #pragma unroll
-    for (int p = 0; p < PER; ++p) r[p] = load8((const T*)nullptr, b, off[p]);
+    for (int p = 0; p < PER; ++p)
+      if (needed(p, n)) r[p] = load8((const T*)nullptr, b, off[p]);
   }
   // zeros in the rows whose bit is not set
-  __device__ __forceinline__ void keep(uint64_t bits) {
+  __device__ __forceinline__ void keep(const Bits<KT>& bits) {
 #pragma unroll
     for (int p = 0; p < PER; ++p)
-      if (!((bits >> row(p)) & 1)) r[p] = zero_chunk<T>();
+      if (!bits.row(row(p))) r[p] = zero_chunk<T>();
   }
-  __device__ __forceinline__ void flip(uint32_t f) {
-#pragma unroll
-    for (int p = 0; p < PER; ++p) r[p] = negate(r[p], f);
-  }
-  __device__ __forceinline__ void store(bf16* t) const {
+  __device__ __forceinline__ void store(bf16* t, int n) const {
 #pragma unroll
     for (int p = 0; p < PER; ++p)
-      if (in(p)) {
+      if (needed(p, n) && in(p)) {
         bf16* d = t + row(p) * TL::pitch + feature(p);
         const auto v = to_frag(r[p]);
         if constexpr (Num<T>::planes == 1) store_chunk(d, v);
@@ -265,24 +279,39 @@ __device__ __forceinline__ int edge_of(const int32_t* ptr, int e, int B, int N) 
   p = p < 0 ? 0 : (p > N ? N : p);
   return e <= 0 ? 0 : (e > B + 1 ? N : p);
 }
-// The extended segment of a slot and the slot's first virtual row in it (-1: an empty slot).  Every lane probes one
-// segment and step, so 63 segments take one round and 3,969 two; the last round's lanes also hold the segment's ends.
+// The extended segment of a slot and the slot's first virtual row in it (-1: an empty slot).  Segments of like lengths are
+// found in one round: 64 lanes look at the segments around slot x guess (segments per slot).  Where that misses, every
+// lane probes one of 63 steps, 3,969 segments in two more rounds.  The last round's lanes also hold the segment's ends.
 template <int BQ>
-__device__ __forceinline__ int find_tile(const int32_t* ptr, int B, int N, int G, uint32_t slot, int& vq0, Seg& s) {
+__device__ __forceinline__ int find_tile(const int32_t* ptr, int B, int N, int G, float guess, uint32_t slot, int& vq0, Seg& s) {
   uint32_t lo = 0, hi = (uint32_t)B + 2;     // the slot is at or after segment lo's first, before hi's
   const uint32_t lane = lane_id();
-  for (;;) {
-    const uint32_t step = (hi - lo + 62) / 63, e = lo + lane * step;
+  uint32_t step = 1, base = (uint32_t)((float)slot * guess);
+  base = base > 31 ? base - 31 : 0;
+  base = base + 63 < hi ? base : (hi > 63 ? hi - 63 : 0);
+  for (bool first = true;; first = false) {
+    if (!first) {
+      step = (hi - lo + 62) / 63;
+      base = lo;
+    }
+    const uint32_t e = base + lane * step;
     const int p = edge_of(ptr, (int)(e < hi ? e : hi), B, N);
     const uint64_t le = __ballot(e < hi && (uint32_t)p * (uint32_t)G / BQ + e <= slot);
-    const int n = le ? __builtin_popcountll(le) - 1 : 0;
-    lo += n * step;
-    if (step == 1) {
-      s.lo = __builtin_amdgcn_readlane(p, n);
-      s.hi = __builtin_amdgcn_readlane(p, n + 1);
+    const int n = __builtin_popcountll(le);
+    if (first ? n >= 1 && n < 64 : step == 1) {   // (offsets that decrease may give n = 0 here)
+      const int i = n < 1 ? 1 : (n > 63 ? 63 : n);
+      lo = base + i - 1;
+      s.lo = __builtin_amdgcn_readlane(p, i - 1);
+      s.hi = __builtin_amdgcn_readlane(p, i);
       break;
     }
-    hi = hi < lo + step ? hi : lo + step;
+    if (first) {                             // n is 0 or 64
+      lo = n ? base + 63 : 0;
+      hi = n ? hi : base;
+    } else {
+      lo = base + (n > 0 ? n - 1 : 0) * step;
+      hi = hi < lo + step ? hi : lo + step;
+    }
   }
   if (s.hi < s.lo) s.hi = s.lo;
   const int64_t v = ((int64_t)slot - (uint32_t)s.lo * (uint32_t)G / BQ - lo) * BQ;
@@ -290,8 +319,9 @@ __device__ __forceinline__ int find_tile(const int32_t* ptr, int B, int N, int G
   return (int)lo;
 }
 // Rows of the other axis of extended segment e
-__device__ __forceinline__ Seg other_rows(const int32_t* ptr, int e, int B, int N) {
+__device__ __forceinline__ Seg other_rows(const int32_t* ptr, int e, int B, int N, bool same, const Seg& own) {
   if (e < 1 || e > B) return Seg{0, 0};
+  if (same) return own;                      // one set of offsets for both axes
   Seg s{edge_of(ptr, e, B, N), edge_of(ptr, e + 1, B, N)};
   if (s.hi < s.lo) s.hi = s.lo;
   return s;
@@ -341,8 +371,17 @@ __device__ __forceinline__ void landed(bf16x8& v) { asm volatile("" : "+v"(v)); 
 __device__ __forceinline__ void landed(Half3& v) { landed(v.p0); landed(v.p1); landed(v.p2); }
 __device__ __forceinline__ void landed(split::Chunk3& v) { landed(v.p0); landed(v.p1); landed(v.p2); }
 
-// bits of a step's first n rows
-__device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
+// the first n rows of a step, and of those the ones whose flag (of row 64 k + lane) is set
+template <int KT>
+__device__ __forceinline__ Bits<KT> step_bits(int n) {
+  Bits<KT> b;
+#pragma unroll
+  for (int k = 0; k < Bits<KT>::N; ++k) {
+    const int x = n - 64 * k;
+    b.w[k] = x >= 64 ? ~0ull : x > 0 ? (1ull << x) - 1 : 0;
+  }
+  return b;
+}
 
 }  // namespace attn
 }  // namespace egnn

@@ -112,8 +112,10 @@ int32_t egnn_attn_fwd(const EgnnAttnDims* d, const EgnnAttnStrides* s, const voi
   if (d->Nq == 0) return EGNN_OK;
   Args a = make_args(d, s);
   a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.q_ptr = q_ptr; a.kv_ptr = kv_ptr; a.mask = key_mask;
+  a.same = q_ptr == kv_ptr && a.Nq == a.Nk;
   a.nsplit = p.nsplit;
   a.slots = (uint32_t)p.slots;
+  a.guess = (float)(a.B + 2) / (float)a.slots;
   a.by_slots = Div::of(a.slots);
   a.part = (float*)workspace;
   return launch_fwd(a, d->dtype == EGNN_BF16, p, (hipStream_t)stream) ? EGNN_ERR_HIP : EGNN_OK;
@@ -143,6 +145,7 @@ int32_t egnn_attn_bwd(const EgnnAttnDims* d, const EgnnAttnStrides* s, const voi
   Args a = make_args(d, s);
   a.q = q; a.k = k; a.v = v; a.o = out; a.lse = (float*)lse; a.go = grad_out; a.gq = grad_q; a.gk = grad_k; a.gv = grad_v;
   a.q_ptr = q_ptr; a.kv_ptr = kv_ptr; a.mask = key_mask;
+  a.same = q_ptr == kv_ptr && a.Nq == a.Nk;
   a.delta = (float*)workspace;
   a.part = (float*)((char*)workspace + delta_bytes(d));
   return launch_bwd(a, d->dtype == EGNN_BF16, pq, pk, (hipStream_t)stream) ? EGNN_ERR_HIP : EGNN_OK;

@@ -25,9 +25,9 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
   bf16 *sK = lds[SH ? 0 : w][0], *sV = lds[SH ? 0 : w][1];
   int vq0;
   Seg qs;
-  const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, it.slot, vq0, qs);
+  const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, a.guess, it.slot, vq0, qs);
   if (vq0 < 0) return;
-  const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk);
+  const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk, a.same, qs);
   const int nv = (qs.hi - qs.lo) * a.G, v0 = vq0 + (SH ? 16 * R * w : 0);
   const bool act = v0 < nv;
   int j = ks.lo + it.sp * KS;
@@ -40,12 +40,16 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
   stK.offsets(offK, krb, a.D);
   stV.offsets(offV, vrb, a.D);
   const T *kb = (const T*)a.k + it.kvh * a.k_h, *vb = (const T*)a.v + it.kvh * a.v_h;
-  uint8_t mb = 1;
+  uint8_t mb[Bits<KT>::N];
+  auto rows_at = [&](int j) { return j1 - j < KS ? j1 - j : KS; };
   auto fetch = [&](int j) {
-    const int n = j1 - j < KS ? j1 - j : KS;
-    stK.load(rows_buffer(kb + j * a.k_r, n, krb, a.D * (int)sizeof(T)), offK);
-    stV.load(rows_buffer(vb + j * a.v_r, n, vrb, a.D * (int)sizeof(T)), offV);
-    if (a.mask) mb = l < n ? a.mask[j + l] : 0;
+    const int n = rows_at(j);
+    stK.load(rows_buffer(kb + j * a.k_r, n, krb, a.D * (int)sizeof(T)), offK, n);
+    stV.load(rows_buffer(vb + j * a.v_r, n, vrb, a.D * (int)sizeof(T)), offV, n);
+    if (a.mask) {
+#pragma unroll
+      for (int k = 0; k < Bits<KT>::N; ++k) mb[k] = 64 * k + l < n ? a.mask[j + 64 * k + l] : 0;
+    }
   };
   if (j < j1) fetch(j);
 
@@ -83,19 +87,22 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
   }
 
   for (; j < j1; j += stride) {
-    uint64_t bits = first_bits(j1 - j < KS ? j1 - j : KS);
+    const int n = rows_at(j);
+    Bits<KT> bits = step_bits<KT>(n);
     if (a.mask) {                            // what a masked key holds must not meet a ds of 0
-      bits &= __ballot(mb != 0);
+#pragma unroll
+      for (int k = 0; k < Bits<KT>::N; ++k) bits.w[k] &= __ballot(mb[k] != 0);
       stK.keep(bits);
     }
     tile_sync<SH>();
-    stK.store(sK);
-    stV.store(sV);
+    stK.store(sK, n);
+    stV.store(sV, n);
     tile_sync<SH>();
     if (j + stride < j1) fetch(j + stride);
     if (!act) continue;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
+      if (KT > 1 && TK * t >= n) break;
       f32x4 P[R][2], dS[R][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -121,8 +128,8 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
           for (int i = 0; i < 4; ++i) P[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r][h][i], a.c2, -ref[r]));
         }
       }
-      if (bits != first_bits(KS)) {
-        const uint32_t tb = (uint32_t)(bits >> (32 * t)) >> (4 * g);
+      if (const uint32_t b = bits.step(t); b != 0xffffffffu) {
+        const uint32_t tb = b >> (4 * g);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -202,9 +209,9 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
   float *sL = stat[SH ? 0 : w][0], *sD = stat[SH ? 0 : w][1];
   int k0;
   Seg ks;
-  const int e = find_tile<BK>(a.kv_ptr, a.B, a.Nk, 1, it.slot, k0, ks);
+  const int e = find_tile<BK>(a.kv_ptr, a.B, a.Nk, 1, a.guess, it.slot, k0, ks);
   if (k0 < 0) return;
-  const Seg qs = other_rows(a.q_ptr, e, a.B, a.Nq);
+  const Seg qs = other_rows(a.q_ptr, e, a.B, a.Nq, a.same, ks);
   const int key0 = ks.lo + k0 + (SH ? 16 * R * w : 0);
   const bool act = key0 < ks.hi;
   int j = it.sp * KS;                        // virtual rows of the segment
@@ -216,9 +223,11 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
   stQ.offsets(offQ, qrb, a.D);
   stG.offsets(offG, grb, a.D);
   const T *qb = (const T*)a.q + (int64_t)it.kvh * a.G * a.q_h, *gb = (const T*)a.go + (int64_t)it.kvh * a.G * a.go_h;
-  float lse = INFINITY, delta = 0.f;
+  constexpr int NL = Bits<KT>::N;
+  float lse[NL], delta[NL];                  // of row 64 k + lane
+  auto rows_at = [&](int j) { return j1 - j < KS ? j1 - j : KS; };
   auto fetch = [&](int j) {
-    const int n = j1 - j < KS ? j1 - j : KS, r0 = (int)a.by_g(j), first = qs.lo + r0;
+    const int n = rows_at(j), r0 = (int)a.by_g(j), first = qs.lo + r0;
     int rows = n;
     if (a.G > 1) {                           // rows and heads of the step's virtual rows
       const int u0 = j - r0 * a.G;           // head of the first one
@@ -232,16 +241,19 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
       }
     }
     const int more = a.D * (int)sizeof(T);
-    stQ.load(rows_buffer(qb + first * a.q_r, rows, qrb, more + (int)((a.G - 1) * a.q_h * (int64_t)sizeof(T))), offQ);
-    stG.load(rows_buffer(gb + first * a.go_r, rows, grb, more + (int)((a.G - 1) * a.go_h * (int64_t)sizeof(T))), offG);
+    stQ.load(rows_buffer(qb + first * a.q_r, rows, qrb, more + (int)((a.G - 1) * a.q_h * (int64_t)sizeof(T))), offQ, n);
+    stG.load(rows_buffer(gb + first * a.go_r, rows, grb, more + (int)((a.G - 1) * a.go_h * (int64_t)sizeof(T))), offG, n);
     // a row without keys, and one past the end, takes no part: its p is e^-inf
-    lse = INFINITY;
-    delta = 0.f;
-    if (l < n) {
-      const uint32_t v = j + l, i = a.by_g(v);
-      const int64_t x = (int64_t)(it.kvh * a.G + (int)(v - i * a.G)) * a.Nq + qs.lo + (int)i;
-      lse = a.lse[x];
-      delta = a.delta[x];
+#pragma unroll
+    for (int k = 0; k < NL; ++k) {
+      lse[k] = INFINITY;
+      delta[k] = 0.f;
+      if (64 * k + l < n) {
+        const uint32_t v = j + 64 * k + l, i = a.by_g(v);
+        const int64_t x = (int64_t)(it.kvh * a.G + (int)(v - i * a.G)) * a.Nq + qs.lo + (int)i;
+        lse[k] = a.lse[x];
+        delta[k] = a.delta[x];
+      }
     }
   };
   if (j < j1) fetch(j);
@@ -269,18 +281,31 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
   }
 
   for (; j < j1; j += stride) {
-    const float ref = lse == -INFINITY ? INFINITY : lse * kLog2e;
-    const uint64_t bits = __ballot(ref != INFINITY);   // of lanes 0 .. KS - 1
-    if (bits != first_bits(KS)) { stQ.keep(bits); stG.keep(bits); }
+    const int n = rows_at(j);
+    Bits<KT> bits;
+    bool all = true;
+    float ref[NL];
+#pragma unroll
+    for (int k = 0; k < NL; ++k) {
+      ref[k] = lse[k] == -INFINITY ? INFINITY : lse[k] * kLog2e;
+      bits.w[k] = __ballot(ref[k] != INFINITY);
+      all &= bits.w[k] == step_bits<KT>(KS).w[k];
+    }
+    if (!all) { stQ.keep(bits); stG.keep(bits); }
     tile_sync<SH>();
-    stQ.store(sQ);
-    stG.store(sG);
-    if ((!SH || w == 0) && l < KS) { sL[l] = ref; sD[l] = -delta; }
+    stQ.store(sQ, n);
+    stG.store(sG, n);
+    if (!SH || w == 0) {
+#pragma unroll
+      for (int k = 0; k < NL; ++k)
+        if (64 * k + l < KS) { sL[64 * k + l] = ref[k]; sD[64 * k + l] = -delta[k]; }
+    }
     tile_sync<SH>();
     if (j + stride < j1) fetch(j + stride);
     if (!act) continue;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
+      if (KT > 1 && TK * t >= n) break;
       f32x4 P[R][2], dS[R][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -387,9 +412,13 @@ template <typename T, int DP>
 static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
   constexpr int tile = 2 * Tile<T, DP>::elems * 2 + 256, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
   constexpr bool wide = Num<T>::planes == 3 && DP == 128;
-  constexpr int KT = Num<T>::planes == 1 && DP < 128 ? 2 : 1;
+#ifndef X_KTB
+#define X_KTB 2
+#endif
+  constexpr int KT = Num<T>::planes == 1 && DP < 128 ? X_KTB : 1;
   a.nsplit = pq.nsplit;
   a.slots = (uint32_t)pq.slots;
+  a.guess = (float)(a.B + 2) / (float)a.slots;
   a.by_slots = Div::of(a.slots);
   if (a.Nq) {
     if constexpr (wide) go_q<T, DP, 1, 4, true, KT>(a, pq, st);
@@ -401,6 +430,7 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
   }
   a.nsplit = pk.nsplit;
   a.slots = (uint32_t)pk.slots;
+  a.guess = (float)(a.B + 2) / (float)a.slots;
   a.by_slots = Div::of(a.slots);
   if (a.Nk) {
     if constexpr (wide) go_k<T, DP, 1, 4, true, KT>(a, pk, st);

@@ -1,16 +1,17 @@
 // Segment attention, forward: o_i = sum_j softmax_j(scale q_i k_j) v_j over the keys of i's segment, in one pass over
 // the keys with the running maximum and sum.
 //
-// The maximum is lazy: a column keeps its reference m until a score passes it by 2^8 (in the exponent's base), so that a
-// step costs neither shuffles nor a rescaling of the output; p is then up to 2^8, which costs no precision in floating
-// point.  The sum takes the unrounded probabilities (one more product, against ones, would sum the rounded ones at less
+// The maximum is lazy: a column keeps its reference m while the probabilities against it stay below 2^10, which costs no
+// precision in floating point, so that a step costs no maximum, no shuffle and no rescaling of the output.  A step whose
+// sum passes 2^10 (the first one always: m starts at the lowest float) is made again with its maximum as the reference.
+// The sum takes the unrounded probabilities (one more product, against ones, would sum the rounded ones at less
 // cost, and put up to 2^-9 into lse).
 #include "egnn_attn.h"
 
 namespace egnn {
 namespace attn {
 
-constexpr float kLazy = 8.0f, kLowest = -3.40282347e+38f;
+constexpr float kLazy = 1024.0f, kLowest = -3.40282347e+38f;
 
 // Partial results of a split call: [split][row of q, head] sums of DP values, then (m, l)
 __device__ __forceinline__ float* part_o(const Args& a, int dp, int s, int64_t r) { return a.part + ((int64_t)s * a.Nq * a.Hq + r) * dp; }
@@ -18,8 +19,9 @@ __device__ __forceinline__ float* part_ml(const Args& a, int dp, int s, int64_t 
   return a.part + (int64_t)a.nsplit * a.Nq * a.Hq * dp + ((int64_t)s * a.Nq * a.Hq + r) * 2;
 }
 
-// R: blocks of 16 columns a wave.  W waves, on one tile (SH) or each on its own.  KT: steps of 32 keys between barriers.
-template <typename T, int DP, int R, int W, bool SH, int KT>
+// R: blocks of 16 columns a wave.  W waves, on one tile (SH) or each on its own.  KT: steps of 32 keys between barriers,
+// KC of them at a time in registers.
+template <typename T, int DP, int R, int W, bool SH, int KT, int KC>
 __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_t n_items) {
   typedef Tile<T, DP, KT> TL;
   typedef typename Num<T>::Frag Frag;
@@ -31,26 +33,30 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_
   bf16 *sK = lds[SH ? 0 : w][0], *sV = lds[SH ? 0 : w][1];
   int vq0;
   Seg qs;
-  const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, it.slot, vq0, qs);
+  const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, a.guess, it.slot, vq0, qs);
   if (vq0 < 0) return;
-  const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk);
+  const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk, a.same, qs);
   const int nv = (qs.hi - qs.lo) * a.G, v0 = vq0 + (SH ? 16 * R * w : 0);
   const bool act = v0 < nv;                  // a wave without rows still loads tiles for the others
   int j = ks.lo + it.sp * KS;
   const int j1 = ks.hi, stride = KS * a.nsplit;
 
-  Stage<T, DP, KT, NT> stK, stV;
+  Stage<T, DP, KT, NT, TK * KC> stK, stV;
   uint32_t offK[stK.PER], offV[stV.PER];
   const int64_t krb = a.k_r * (int64_t)sizeof(T), vrb = a.v_r * (int64_t)sizeof(T);
   stK.offsets(offK, krb, a.D);
   stV.offsets(offV, vrb, a.D);
   const T *kb = (const T*)a.k + it.kvh * a.k_h, *vb = (const T*)a.v + it.kvh * a.v_h;
-  uint8_t mb = 1;
+  uint8_t mb[Bits<KT>::N];
+  auto rows_at = [&](int j) { return j1 - j < KS ? j1 - j : KS; };
   auto fetch = [&](int j) {
-    const int n = j1 - j < KS ? j1 - j : KS;
-    stK.load(rows_buffer(kb + j * a.k_r, n, krb, a.D * (int)sizeof(T)), offK);
-    stV.load(rows_buffer(vb + j * a.v_r, n, vrb, a.D * (int)sizeof(T)), offV);
-    if (a.mask) mb = l < n ? a.mask[j + l] : 0;
+    const int n = rows_at(j);
+    stK.load(rows_buffer(kb + j * a.k_r, n, krb, a.D * (int)sizeof(T)), offK, n);
+    stV.load(rows_buffer(vb + j * a.v_r, n, vrb, a.D * (int)sizeof(T)), offV, n);
+    if (a.mask) {
+#pragma unroll
+      for (int k = 0; k < Bits<KT>::N; ++k) mb[k] = 64 * k + l < n ? a.mask[j + 64 * k + l] : 0;
+    }
   };
   if (j < j1) fetch(j);
 
@@ -83,85 +89,100 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_
   }
 
   for (; j < j1; j += stride) {
-    uint64_t bits = first_bits(j1 - j < KS ? j1 - j : KS);
+    const int n = rows_at(j);
+    Bits<KT> bits = step_bits<KT>(n);
     if (a.mask) {                            // what a masked value holds must not meet a probability of 0
-      bits &= __ballot(mb != 0);
+#pragma unroll
+      for (int k = 0; k < Bits<KT>::N; ++k) bits.w[k] &= __ballot(mb[k] != 0);
       stV.keep(bits);
     }
     tile_sync<SH>();                         // the step before has read the tile
-    stK.store(sK);
-    stV.store(sV);
+    stK.store(sK, n);
+    stV.store(sV, n);
     tile_sync<SH>();
     if (j + stride < j1) fetch(j + stride);
     if (!act) continue;
-    f32x4 S[R][2 * KT];
 #pragma unroll
-    for (int h = 0; h < 2 * KT; ++h) {
-      f32x4 hi[R], lo[R];
+    for (int t0 = 0; t0 < KT; t0 += KC) {
+      if (KT > KC && TK * t0 >= n) break;
+      f32x4 S[R][2 * KC];
+      float ps[R];
+      for (bool again = false;; again = true) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) { hi[r] = zero4(); lo[r] = zero4(); }
+        for (int h = 0; h < 2 * KC; ++h) {
+          f32x4 hi[R], lo[R];
 #pragma unroll
-      for (int kk = 0; kk < TL::NK; ++kk) {
-        const auto A = TL::rows(sK, h, kk, c, g);
+          for (int r = 0; r < R; ++r) { hi[r] = zero4(); lo[r] = zero4(); }
 #pragma unroll
-        for (int r = 0; r < R; ++r) product1(hi[r], lo[r], A, Q[r][kk]);
-      }
+          for (int kk = 0; kk < TL::NK; ++kk) {
+            const auto A = TL::rows(sK, 2 * t0 + h, kk, c, g);
 #pragma unroll
-      for (int r = 0; r < R; ++r) S[r][h] = result<T>(hi[r], lo[r]);
-    }
-    if (bits != first_bits(KS)) {
-      const uint32_t b0 = (uint32_t)bits >> (4 * g), b1 = (uint32_t)(bits >> 32) >> (4 * g);
+            for (int r = 0; r < R; ++r) product1(hi[r], lo[r], A, Q[r][kk]);
+          }
 #pragma unroll
-      for (int h = 0; h < 2 * KT; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool ok = ((h < 2 ? b0 : b1) >> (16 * (h & 1) + i)) & 1;
-#pragma unroll
-          for (int r = 0; r < R; ++r) S[r][h][i] = ok ? S[r][h][i] : -INFINITY;
+          for (int r = 0; r < R; ++r) S[r][h] = result<T>(hi[r], lo[r]);
         }
-    }
-    float top[R];
-    bool over = false;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      top[r] = S[r][0][0];
+        for (int t = 0; t < KC; ++t) {
+          const uint32_t b = bits.step(t0 + t);
+          if (b != 0xffffffffu) {
+            const uint32_t x = b >> (4 * g);
 #pragma unroll
-      for (int h = 0; h < 2 * KT; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], S[r][h][i]);
-      over |= __builtin_fmaf(top[r], a.c2, -m[r]) > kLazy;
-    }
-    if (__ballot(over)) {
+              for (int i = 0; i < 4; ++i) {
+                const bool ok = (x >> (16 * h + i)) & 1;
+#pragma unroll
+                for (int r = 0; r < R; ++r) S[r][2 * t + h][i] = ok ? S[r][2 * t + h][i] : -INFINITY;
+              }
+          }
+        }
+        if (again) {                         // the step's maximum as the new reference
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            float top = S[r][0][0];
+#pragma unroll
+            for (int h = 0; h < 2 * KC; ++h)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) top = fmaxf(top, S[r][h][i]);
+            const float mn = fmaxf(m[r], col_max(top) * a.c2), alpha = __builtin_amdgcn_exp2f(m[r] - mn);
+            m[r] = mn;
+            sum[r] *= alpha;
+#pragma unroll
+            for (int b = 0; b < TL::NB; ++b) O[r][b] *= alpha;
+          }
+        }
+        bool over = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          ps[r] = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2 * KC; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              S[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r][h][i], a.c2, -m[r]));
+              ps[r] += S[r][h][i];
+            }
+          over |= ps[r] > kLazy;
+        }
+        if (again || !__ballot(over)) break;
+      }
+      Frag P[R][KC];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float mn = fmaxf(m[r], col_max(top[r]) * a.c2), alpha = __builtin_amdgcn_exp2f(m[r] - mn);
-        m[r] = mn;
-        sum[r] *= alpha;
+        sum[r] += ps[r];
 #pragma unroll
-        for (int b = 0; b < TL::NB; ++b) O[r][b] *= alpha;
+        for (int t = 0; t < KC; ++t) P[r][t] = chain_frag<T>(S[r][2 * t], S[r][2 * t + 1]);
       }
-    }
-    Frag P[R][KT];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
+      for (int t = 0; t < KC; ++t)
 #pragma unroll
-      for (int h = 0; h < 2 * KT; ++h)
+        for (int b = 0; b < TL::NB; ++b) {
+          const Frag A = TL::cols(sV, t0 + t, b, c, g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          S[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r][h][i], a.c2, -m[r]));
-          sum[r] += S[r][h][i];
+          for (int r = 0; r < R; ++r) accumulate(O[r][b], A, P[r][t]);
         }
-#pragma unroll
-      for (int t = 0; t < KT; ++t) P[r][t] = chain_frag<T>(S[r][2 * t], S[r][2 * t + 1]);
     }
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int b = 0; b < TL::NB; ++b) {
-        const Frag A = TL::cols(sV, t, b, c, g);
-#pragma unroll
-        for (int r = 0; r < R; ++r) accumulate(O[r][b], A, P[r][t]);
-      }
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -253,19 +274,24 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
   if (a.lse && f == 0) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-template <typename T, int DP, int R, int W, bool SH, int KT>
+template <typename T, int DP, int R, int W, bool SH, int KT, int KC>
 static void go(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
-  fwd_kernel<T, DP, R, W, SH, KT><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
+  fwd_kernel<T, DP, R, W, SH, KT, KC><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
 }
+#ifndef X_KT
+#define X_KT 2
+#define X_KC 2
+#endif
 template <typename T, int DP>
 static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
   constexpr int tile = 2 * Tile<T, DP>::elems * 2, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
-  constexpr int KT = Num<T>::planes == 1 ? 2 : 1;
-  if constexpr (KT == 1 && DP == 128) go<T, DP, 1, 4, true, KT>(a, p, st);
-  else if (p.form == 0) go<T, DP, 1, W, false, 1>(a, p, st);
-  else if (p.form == 1) go<T, DP, 1, 4, true, KT>(a, p, st);
-  else go<T, DP, 2, 4, true, KT>(a, p, st);
+  constexpr bool f32 = Num<T>::planes == 3;
+  constexpr int KT = f32 ? 1 : X_KT, KC = f32 ? 1 : X_KC;
+  if constexpr (f32 && DP == 128) go<T, DP, 1, 4, true, KT, KC>(a, p, st);
+  else if (p.form == 0) go<T, DP, 1, W, false, 1, 1>(a, p, st);
+  else if (p.form == 1) go<T, DP, 1, 4, true, KT, KC>(a, p, st);
+  else go<T, DP, 2, 4, true, KT, KC>(a, p, st);
   const int64_t rows = (int64_t)a.Nq * a.Hq;
   if (a.nsplit > kFewSplits) fwd_join_many_kernel<T, DP><<<dim3((uint32_t)rows, DP / 16), 256, 0, st>>>(a);
   else if (a.nsplit > 1) fwd_join_kernel<T, DP><<<(uint32_t)cdiv(rows * (DP / 4), 256), 256, 0, st>>>(a);
