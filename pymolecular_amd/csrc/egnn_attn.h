@@ -219,6 +219,19 @@ template <typename T, int DP, int KT = 1> struct Tile {
   }
 };
 
+__device__ __forceinline__ float dot8(const bf16x8& a, const bf16x8& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s = __builtin_fmaf((float)a[i], (float)b[i], s);
+  return s;
+}
+__device__ __forceinline__ float dot8(const f32x8& a, const f32x8& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s = __builtin_fmaf(a.hi[i], b.hi[i], __builtin_fmaf(a.lo[i], b.lo[i], s));
+  return s;
+}
+
 // bits of a step's rows, 64 a word
 template <int KT> struct Bits {
   static constexpr int N = (KT * TK + 63) / 64;

@@ -13,20 +13,18 @@
 namespace egnn {
 namespace attn {
 
+// The S and dp products of a step are made with the scale's sign in the exponent's factor.
+__device__ __forceinline__ float signed_c2(const Args& a) { return a.flip ? -a.c2 : a.c2; }
+__host__ __device__ __forceinline__ float signed_scale(const Args& a) { return a.flip ? -a.scale : a.scale; }
+
+// dq of the tile from virtual row vq0 of segment e on; sK, sV: tiles of the wave's (SH: the workgroup's) own
 template <typename T, int DP, int R, int W, bool SH, int KT>
-__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t n_items) {
+__device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, int vq0, const Seg& qs, bf16* sK, bf16* sV, int w) {
   typedef Tile<T, DP, KT> TL;
   typedef typename Num<T>::Frag Frag;
-  constexpr int NT = SH ? 64 * W : 64, BQ = 16 * R * (SH ? W : 1), KS = TK * KT;
-  __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
-  Item it;
-  if (!item_of<W, SH>(a, n_items, it)) return;
-  const int l = lane_id(), c = l & 15, g = l >> 4, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  bf16 *sK = lds[SH ? 0 : w][0], *sV = lds[SH ? 0 : w][1];
-  int vq0;
-  Seg qs;
-  const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, a.guess, it.slot, vq0, qs);
-  if (vq0 < 0) return;
+  constexpr int NT = SH ? 64 * W : 64, KS = TK * KT;
+  const int l = lane_id(), c = l & 15, g = l >> 4;
+  const float c2 = signed_c2(a);
   const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk, a.same, qs);
   const int nv = (qs.hi - qs.lo) * a.G, v0 = vq0 + (SH ? 16 * R * w : 0);
   const bool act = v0 < nv;
@@ -72,7 +70,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
     delta[r] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < TL::NK; ++kk) {
-      Q[r][kk] = TL::column(qp, kk, g, a.D, a.flip);
+      Q[r][kk] = TL::column(qp, kk, g, a.D, 0);
       GO[r][kk] = TL::column(gp, kk, g, a.D, 0);
       landed(Q[r][kk]);
       landed(GO[r][kk]);
@@ -125,7 +123,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
           P[r][h] = result<T>(hi[r], lo[r]);
           dS[r][h] = result<T>(dhi[r], dlo[r]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) P[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r][h][i], a.c2, -ref[r]));
+          for (int i = 0; i < 4; ++i) P[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r][h][i], c2, -ref[r]));
         }
       }
       if (const uint32_t b = bits.step(t); b != 0xffffffffu) {
@@ -176,12 +174,12 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
       }
     }
   }
-  const float sc = a.flip ? -a.scale : a.scale;
+  const float sc = signed_scale(a);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (!SH && !one && a.nsplit == 1) delta[r] += col_sum(sum[r]);
     if (!live[r]) continue;
-    if (it.sp == 0 && g == 0) a.delta[(int64_t)head[r] * a.Nq + row[r]] = none[r] ? 0.f : delta[r];
+    if (a.delta && it.sp == 0 && g == 0) a.delta[(int64_t)head[r] * a.Nq + row[r]] = none[r] ? 0.f : delta[r];
     if (a.nsplit > 1) {
       float* p = a.part + ((int64_t)it.sp * a.Nq * a.Hq + (int64_t)row[r] * a.Hq + head[r]) * DP;
 #pragma unroll
@@ -195,34 +193,31 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t
   }
 }
 
-template <typename T, int DP, int R, int W, bool SH, int KT>
-__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_t n_items) {
+// dk and dv of the tile from key k0 of segment e on.  OD: delta is made from o here, not read (no launch before this one
+// has written it).
+template <typename T, int DP, int R, int W, bool SH, int KT, bool OD>
+__device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, int k0, const Seg& ks, bf16* sQ, bf16* sG, float* sL,
+                                         float* sD, int w) {
   typedef Tile<T, DP, KT> TL;
   typedef typename Num<T>::Frag Frag;
-  constexpr int NT = SH ? 64 * W : 64, BK = 16 * R * (SH ? W : 1), KS = TK * KT;
-  __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
-  __shared__ __attribute__((aligned(16))) float stat[SH ? 1 : W][2][KS];
-  Item it;
-  if (!item_of<W, SH>(a, n_items, it)) return;
-  const int l = lane_id(), c = l & 15, g = l >> 4, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  bf16 *sQ = lds[SH ? 0 : w][0], *sG = lds[SH ? 0 : w][1];
-  float *sL = stat[SH ? 0 : w][0], *sD = stat[SH ? 0 : w][1];
-  int k0;
-  Seg ks;
-  const int e = find_tile<BK>(a.kv_ptr, a.B, a.Nk, 1, a.guess, it.slot, k0, ks);
-  if (k0 < 0) return;
+  constexpr int NT = SH ? 64 * W : 64, KS = TK * KT;
+  const int l = lane_id(), c = l & 15, g = l >> 4;
+  const float c2 = signed_c2(a);
   const Seg qs = other_rows(a.q_ptr, e, a.B, a.Nq, a.same, ks);
   const int key0 = ks.lo + k0 + (SH ? 16 * R * w : 0);
   const bool act = key0 < ks.hi;
   int j = it.sp * KS;                        // virtual rows of the segment
   const int j1 = (qs.hi - qs.lo) * a.G, stride = KS * a.nsplit;
 
-  Stage<T, DP, KT, NT> stQ, stG;
-  uint32_t offQ[stQ.PER], offG[stG.PER];
+  Stage<T, DP, KT, NT> stQ, stG, stO;
+  uint32_t offQ[stQ.PER], offG[stG.PER], offO[stO.PER];
   const int64_t qrb = a.q_r * (int64_t)sizeof(T), grb = a.go_r * (int64_t)sizeof(T);
   stQ.offsets(offQ, qrb, a.D);
   stG.offsets(offG, grb, a.D);
-  const T *qb = (const T*)a.q + (int64_t)it.kvh * a.G * a.q_h, *gb = (const T*)a.go + (int64_t)it.kvh * a.G * a.go_h;
+  const int64_t orb = a.o_r * (int64_t)sizeof(T);
+  if constexpr (OD) stO.offsets(offO, orb, a.D);
+  const T *qb = (const T*)a.q + (int64_t)it.kvh * a.G * a.q_h, *gb = (const T*)a.go + (int64_t)it.kvh * a.G * a.go_h,
+          *ob = (const T*)a.o + (int64_t)it.kvh * a.G * a.o_h;
   constexpr int NL = Bits<KT>::N;
   float lse[NL], delta[NL];                  // of row 64 k + lane
   auto rows_at = [&](int j) { return j1 - j < KS ? j1 - j : KS; };
@@ -238,11 +233,14 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
         const bool ok = stQ.in(p) && stQ.row(p) < n && (int)f < a.D;
         offQ[p] = ok ? (uint32_t)((i * a.q_r + h * a.q_h + f) * (int64_t)sizeof(T)) : kOob;
         offG[p] = ok ? (uint32_t)((i * a.go_r + h * a.go_h + f) * (int64_t)sizeof(T)) : kOob;
+        if constexpr (OD) offO[p] = ok ? (uint32_t)((i * a.o_r + h * a.o_h + f) * (int64_t)sizeof(T)) : kOob;
       }
     }
     const int more = a.D * (int)sizeof(T);
     stQ.load(rows_buffer(qb + first * a.q_r, rows, qrb, more + (int)((a.G - 1) * a.q_h * (int64_t)sizeof(T))), offQ, n);
     stG.load(rows_buffer(gb + first * a.go_r, rows, grb, more + (int)((a.G - 1) * a.go_h * (int64_t)sizeof(T))), offG, n);
+    if constexpr (OD)
+      stO.load(rows_buffer(ob + first * a.o_r, rows, orb, more + (int)((a.G - 1) * a.o_h * (int64_t)sizeof(T))), offO, n);
     // a row without keys, and one past the end, takes no part: its p is e^-inf
 #pragma unroll
     for (int k = 0; k < NL; ++k) {
@@ -252,7 +250,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
         const uint32_t v = j + 64 * k + l, i = a.by_g(v);
         const int64_t x = (int64_t)(it.kvh * a.G + (int)(v - i * a.G)) * a.Nq + qs.lo + (int)i;
         lse[k] = a.lse[x];
-        delta[k] = a.delta[x];
+        if constexpr (!OD) delta[k] = a.delta[x];
       }
     }
   };
@@ -271,7 +269,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
             *vp = live[r] ? (const T*)a.v + key[r] * a.v_r + it.kvh * a.v_h : nullptr;
 #pragma unroll
     for (int kk = 0; kk < TL::NK; ++kk) {
-      K[r][kk] = TL::column(kp, kk, g, a.D, a.flip);   // the scale's sign
+      K[r][kk] = TL::column(kp, kk, g, a.D, 0);
       V[r][kk] = TL::column(vp, kk, g, a.D, 0);
       landed(K[r][kk]);
       landed(V[r][kk]);
@@ -298,7 +296,19 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
     if (!SH || w == 0) {
 #pragma unroll
       for (int k = 0; k < NL; ++k)
-        if (64 * k + l < KS) { sL[64 * k + l] = ref[k]; sD[64 * k + l] = -delta[k]; }
+        if (64 * k + l < KS) {
+          sL[64 * k + l] = ref[k];
+          if constexpr (!OD) sD[64 * k + l] = -delta[k];
+        }
+    }
+    if constexpr (OD) {                      // the threads of a row are neighbours
+#pragma unroll
+      for (int p = 0; p < stG.PER; ++p) {
+        float d = dot8(stG.r[p], stO.r[p]);
+#pragma unroll
+        for (int x = 1; x < stG.CH; x <<= 1) d += shfl_xor(d, x);
+        if (stG.in(p) && stG.feature(p) == 0) sD[stG.row(p)] = -d;
+      }
     }
     tile_sync<SH>();
     if (j + stride < j1) fetch(j + stride);
@@ -326,7 +336,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
           dS[r][h] = result<T>(dhi[r], dlo[r]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            P[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r][h][i], a.c2, -Lr[i]));
+            P[r][h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r][h][i], c2, -Lr[i]));
             dS[r][h][i] *= P[r][h][i];
           }
         }
@@ -342,7 +352,7 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
       }
     }
   }
-  const float sc = a.flip ? -a.scale : a.scale;
+  const float sc = signed_scale(a);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (!in[r]) continue;
@@ -363,6 +373,237 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
         store4(gv + 16 * b + 4 * g, live[r] ? dV[r][b] : zero4());
       }
   }
+}
+
+template <typename T, int DP, int R, int W, bool SH, int KT>
+__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t n_items) {
+  typedef Tile<T, DP, KT> TL;
+  constexpr int BQ = 16 * R * (SH ? W : 1);
+  __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
+  Item it;
+  if (!item_of<W, SH>(a, n_items, it)) return;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  int vq0;
+  Seg qs;
+  const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, a.guess, it.slot, vq0, qs);
+  if (vq0 < 0) return;
+  dq_tile<T, DP, R, W, SH, KT>(a, it, e, vq0, qs, lds[SH ? 0 : w][0], lds[SH ? 0 : w][1], w);
+}
+
+template <typename T, int DP, int R, int W, bool SH, int KT>
+__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_t n_items) {
+  typedef Tile<T, DP, KT> TL;
+  constexpr int BK = 16 * R * (SH ? W : 1);
+  __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
+  __shared__ __attribute__((aligned(16))) float stat[SH ? 1 : W][2][TK * KT];
+  Item it;
+  if (!item_of<W, SH>(a, n_items, it)) return;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), x = SH ? 0 : w;
+  int k0;
+  Seg ks;
+  const int e = find_tile<BK>(a.kv_ptr, a.B, a.Nk, 1, a.guess, it.slot, k0, ks);
+  if (k0 < 0) return;
+  dkv_tile<T, DP, R, W, SH, KT, false>(a, it, e, k0, ks, lds[x][0], lds[x][1], stat[x][0], stat[x][1], w);
+}
+
+// ---- short segments: one launch -------------------------------------------------------
+// A segment with at most 32 virtual rows and 32 keys (a molecule) is one wave's: its q, k, v and do are read once, its
+// gradients written once, delta is exact, and neither o nor a statistic of another launch is read.  Both orientations of
+// the scores are made from the same LDS tiles, the second for the sums over the queries.
+template <typename T, int DP>
+__device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg& qs, const Seg& ks, bf16* lds, float* sL, float* sD) {
+  typedef Tile<T, DP> TL;
+  typedef typename Num<T>::Frag Frag;
+  const int l = lane_id(), c = l & 15, g = l >> 4;
+  const int nv = (qs.hi - qs.lo) * a.G, nk = ks.hi - ks.lo;
+  bf16 *sQ = lds, *sG = sQ + TL::elems, *sK = sG + TL::elems, *sV = sK + TL::elems;
+  const int64_t e = sizeof(T);
+  {
+    Stage<T, DP, 1, 64> stQ, stG, stK, stV;
+    uint32_t offQ[stQ.PER], offG[stQ.PER], offK[stQ.PER], offV[stQ.PER];
+    stK.offsets(offK, a.k_r * e, a.D);
+    stV.offsets(offV, a.v_r * e, a.D);
+    if (a.G == 1) {
+      stQ.offsets(offQ, a.q_r * e, a.D);
+      stG.offsets(offG, a.go_r * e, a.D);
+    } else {
+#pragma unroll
+      for (int p = 0; p < stQ.PER; ++p) {
+        const uint32_t u = stQ.row(p), i = a.by_g(u), h = u - i * a.G, f = stQ.feature(p);
+        const bool ok = stQ.in(p) && (int)u < nv && (int)f < a.D;
+        offQ[p] = ok ? (uint32_t)((i * a.q_r + h * a.q_h + f) * e) : kOob;
+        offG[p] = ok ? (uint32_t)((i * a.go_r + h * a.go_h + f) * e) : kOob;
+      }
+    }
+    const int last = a.D * (int)e, rows = qs.hi - qs.lo;
+    stQ.load(rows_buffer((const T*)a.q + qs.lo * a.q_r + (int64_t)kvh * a.G * a.q_h, rows, a.q_r * e, last + (int)((a.G - 1) * a.q_h * e)), offQ, nv);
+    stG.load(rows_buffer((const T*)a.go + qs.lo * a.go_r + (int64_t)kvh * a.G * a.go_h, rows, a.go_r * e, last + (int)((a.G - 1) * a.go_h * e)), offG, nv);
+    if (nk) {
+      stK.load(rows_buffer((const T*)a.k + ks.lo * a.k_r + kvh * a.k_h, nk, a.k_r * e, last), offK, nk);
+      stV.load(rows_buffer((const T*)a.v + ks.lo * a.v_r + kvh * a.v_h, nk, a.v_r * e, last), offV, nk);
+    }
+    float ref = INFINITY;                    // of row l
+    if (l < nv) {
+      const uint32_t i = a.by_g(l);
+      ref = a.lse[(int64_t)(kvh * a.G + (l - (int)i * a.G)) * a.Nq + qs.lo + (int)i] * kLog2e;
+      if (ref == -INFINITY) ref = INFINITY;  // a row without keys: no gradient from it or to it
+    }
+    bool key = l < nk;
+    if (key && a.mask) key = a.mask[ks.lo + l] != 0;
+    Bits<1> bits;
+    bits.w[0] = __ballot(ref != INFINITY);
+    if (bits.w[0] != (nv >= 32 ? 0xffffffffull : (1ull << nv) - 1)) { stQ.keep(bits); stG.keep(bits); }
+    if (a.mask) {
+      bits.w[0] = __ballot(key);
+      stK.keep(bits);
+      stV.keep(bits);
+    }
+    stQ.store(sQ, TK);
+    stG.store(sG, TK);
+    if (nk) {
+      stK.store(sK, nk);
+      stV.store(sV, nk);
+    }
+    if (l < TK) sL[l] = ref;
+  }
+  wave_sync();
+  const bool q2 = nv > 16, k2 = nk > 16;     // second blocks of 16 rows
+  const float c2 = signed_c2(a), sc = signed_scale(a);
+  bool live[2];                              // keys 16 b + c that exist, and are not masked
+  uint32_t kbits;
+  {
+    bool key = l < nk;
+    if (key && a.mask) key = a.mask[ks.lo + l] != 0;
+    kbits = (uint32_t)__ballot(key);
+    live[0] = (kbits >> c) & 1;
+    live[1] = (kbits >> (16 + c)) & 1;
+  }
+  // scores with the queries on the columns: delta and dq
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    if (q && !q2) break;
+    typename TL::Feat Qc[TL::NK], Gc[TL::NK];
+#pragma unroll
+    for (int kk = 0; kk < TL::NK; ++kk) { Qc[kk] = TL::rows(sQ, q, kk, c, g); Gc[kk] = TL::rows(sG, q, kk, c, g); }
+    const float ref = sL[16 * q + c];
+    f32x4 P[2] = {zero4(), zero4()}, dS[2] = {zero4(), zero4()};
+    float delta = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k ? !k2 : nk == 0) break;
+      P[k] = TL::product(sK, k, Qc, c, g, zero4());
+      dS[k] = TL::product(sV, k, Gc, c, g, zero4());
+      const uint32_t b = kbits >> (16 * k + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        P[k][i] = (b >> i) & 1 ? __builtin_amdgcn_exp2f(__builtin_fmaf(P[k][i], c2, -ref)) : 0.f;
+        delta = __builtin_fmaf(P[k][i], dS[k][i], delta);
+      }
+    }
+    delta = col_sum(delta);
+    if (g == 0) sD[16 * q + c] = -delta;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dS[k][i] = P[k][i] * (dS[k][i] - delta);
+    const Frag F = chain_frag<T>(dS[0], dS[1]);
+    const int v = 16 * q + c;
+    const uint32_t i = a.by_g(v);
+    T* out = (T*)a.gq + (qs.lo + (int)i) * a.gq_r + (kvh * a.G + (v - (int)i * a.G)) * a.gq_h;
+#pragma unroll
+    for (int b = 0; b < TL::NB; ++b) {
+      f32x4 d = zero4();
+      if (nk) accumulate(d, TL::cols(sK, 0, b, c, g), F);
+      if (v < nv && 16 * b + 4 * g < a.D) store4(out + 16 * b + 4 * g, d * sc);
+    }
+  }
+  if (nk == 0) return;
+  wave_sync();
+  // and with the keys on the columns: dk and dv
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (k && !k2) break;
+    typename TL::Feat Kc[TL::NK], Vc[TL::NK];
+#pragma unroll
+    for (int kk = 0; kk < TL::NK; ++kk) { Kc[kk] = TL::rows(sK, k, kk, c, g); Vc[kk] = TL::rows(sV, k, kk, c, g); }
+    f32x4 P[2] = {zero4(), zero4()}, dS[2] = {zero4(), zero4()};
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (q && !q2) break;
+      const f32x4 Lr = load4_f32(sL + 16 * q + 4 * g), nD = load4_f32(sD + 16 * q + 4 * g);
+      P[q] = TL::product(sQ, q, Kc, c, g, zero4());
+      dS[q] = TL::product(sG, q, Vc, c, g, nD);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        P[q][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[q][i], c2, -Lr[i]));
+        dS[q][i] *= P[q][i];
+      }
+    }
+    const Frag FP = chain_frag<T>(P[0], P[1]), FS = chain_frag<T>(dS[0], dS[1]);
+    const int key = ks.lo + 16 * k + c;
+    T *gk = (T*)a.gk + key * a.gk_r + kvh * a.gk_h, *gv = (T*)a.gv + key * a.gv_r + kvh * a.gv_h;
+#pragma unroll
+    for (int b = 0; b < TL::NB; ++b) {
+      f32x4 dK = zero4(), dV = zero4();
+      accumulate(dV, TL::cols(sG, 0, b, c, g), FP);
+      accumulate(dK, TL::cols(sQ, 0, b, c, g), FS);
+      if (16 * k + c < nk && 16 * b + 4 * g < a.D) {
+        store4(gk + 16 * b + 4 * g, live[k] ? dK * sc : zero4());
+        store4(gv + 16 * b + 4 * g, live[k] ? dV : zero4());
+      }
+    }
+  }
+}
+
+// Items 0 .. n_q - 1: a tile of 32 virtual rows and a key head: the whole segment where it is small, else its dq (and with
+// n_k = 0, where queries and keys are the same rows, the dk and dv of those).  The others: a tile of 32 keys and heads_per
+// key heads, their dk and dv where the segment is not small.
+template <typename T, int DP, int W>
+__global__ __launch_bounds__(64 * W, DP == 16 && W == 4 ? 4 : 1) void short_kernel(Args a, uint32_t n_q, uint32_t n_k, uint32_t slots_k,
+                                                                                   Div by_heads_k, int heads_per) {
+  typedef Tile<T, DP> TL;
+  __shared__ __attribute__((aligned(16))) bf16 lds[W][4][TL::elems];
+  __shared__ __attribute__((aligned(16))) float stat[W][2][TK];
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  uint32_t i = xcd_order(blockIdx.x, gridDim.x) * W + w;
+  bf16* t = lds[w][0];
+  Seg own;
+  int r0, e, h0, h1;
+  // tiles of 16 where the segment is not small: of 32 rows the registers would cost waves
+  if (i < n_q) {
+    const uint32_t slot = a.by_heads(i);
+    h0 = (int)(i - slot * (uint32_t)a.Hkv);
+    h1 = h0 + 1;
+    e = find_tile<TK>(a.q_ptr, a.B, a.Nq, a.G, a.guess, slot, r0, own);
+    if (r0 < 0) return;
+    const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk, a.same, own);
+    const int nv = (own.hi - own.lo) * a.G;
+    if (nv <= TK && ks.hi - ks.lo <= TK && (n_k || (e >= 1 && e <= a.B))) {   // (keys outside every segment: zeros, below)
+      small_segment<T, DP>(a, h0, own, ks, t, stat[w][0], stat[w][1]);
+      return;
+    }
+    for (int x = 0; x < TK && r0 + x < nv; x += 16) {
+      wave_sync();
+      dq_tile<T, DP, 1, W, false, 1>(a, Item{slot, h0, 0}, e, r0 + x, own, t, t + TL::elems, 0);
+    }
+    if (n_k) return;
+  } else {
+    i -= n_q;
+    if (i >= n_k) return;
+    const uint32_t slot = by_heads_k(i);
+    h0 = (int)(i - slot * (uint32_t)(a.Hkv / heads_per)) * heads_per;
+    h1 = h0 + heads_per;
+    e = find_tile<TK>(a.kv_ptr, a.B, a.Nk, 1, (float)(a.B + 2) / (float)slots_k, slot, r0, own);
+    if (r0 < 0) return;
+    const Seg qs = other_rows(a.q_ptr, e, a.B, a.Nq, a.same, own);
+    const int nv = (qs.hi - qs.lo) * a.G;
+    if (nv >= 1 && nv <= TK && own.hi - own.lo <= TK) return;   // a query's wave has it
+  }
+  for (int h = h0; h < h1; ++h)
+    for (int x = 0; x < TK && r0 + x < own.hi - own.lo; x += 16) {
+      wave_sync();
+      dkv_tile<T, DP, 1, W, false, 1, true>(a, Item{0, h, 0}, e, r0 + x, own, t, t + TL::elems, stat[w][0], stat[w][1], 0);
+    }
 }
 
 // out[row][head][f] = mul * sum over the splits, 4 features a thread: GR groups of splits a block, whose sums are added in
@@ -408,14 +649,33 @@ static void go_k(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
   dkv_kernel<T, DP, R, W, SH, KT><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
 }
+// One launch for both axes in short segments: both plans say waves, without splits
+template <typename T, int DP>
+static bool launch_short(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
+  constexpr bool f32 = Num<T>::planes == 3;
+  if constexpr (DP > (f32 ? 32 : 64)) return false;
+  else {
+    if (pq.form != 0 || pk.form != 0 || pq.nsplit > 1 || pk.nsplit > 1 || !a.Nq || !a.Nk) return false;
+    constexpr int tile = 4 * Tile<T, DP>::elems * 2, W = 4 * tile <= 65536 ? 4 : 2;
+    const int64_t sq = ((int64_t)a.Nq * a.G) / TK + a.B + 2, sk = a.Nk / TK + a.B + 2;
+    const int per = sk >= 1024 ? a.Hkv : 1;
+    const int64_t nq = sq * a.Hkv, nk = a.same && a.G == 1 ? 0 : sk * (a.Hkv / per);
+    if (nq + nk > INT32_MAX) return false;
+    a.delta = nullptr;
+    a.nsplit = 1;
+    a.slots = (uint32_t)sq;
+    a.guess = (float)(a.B + 2) / (float)sq;
+    short_kernel<T, DP, W><<<(uint32_t)cdiv(nq + nk, W), 64 * W, 0, st>>>(a, (uint32_t)nq, (uint32_t)nk, (uint32_t)sk, Div::of(a.Hkv / per), per);
+    return true;
+  }
+}
+
 template <typename T, int DP>
 static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
   constexpr int tile = 2 * Tile<T, DP>::elems * 2 + 256, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
+  if (launch_short<T, DP>(a, pq, pk, st)) return (int)hipGetLastError();
   constexpr bool wide = Num<T>::planes == 3 && DP == 128;
-#ifndef X_KTB
-#define X_KTB 2
-#endif
-  constexpr int KT = Num<T>::planes == 1 && DP < 128 ? X_KTB : 1;
+  constexpr int KT = Num<T>::planes == 1 && DP < 128 ? 2 : 1;
   a.nsplit = pq.nsplit;
   a.slots = (uint32_t)pq.slots;
   a.guess = (float)(a.B + 2) / (float)a.slots;
@@ -426,7 +686,7 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
     else if (pq.form == 1) go_q<T, DP, 1, 4, true, KT>(a, pq, st);
     else go_q<T, DP, 2, 4, true, KT>(a, pq, st);
     if (a.nsplit > 1)
-      sum_parts<T>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, 0, a.flip ? -a.scale : a.scale, a.gq, a.gq_r, a.gq_h, st);
+      sum_parts<T>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, 0, signed_scale(a), a.gq, a.gq_r, a.gq_h, st);
   }
   a.nsplit = pk.nsplit;
   a.slots = (uint32_t)pk.slots;
@@ -438,7 +698,7 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
     else if (pk.form == 1) go_k<T, DP, 1, 4, true, KT>(a, pk, st);
     else if constexpr (DP <= (Num<T>::planes == 1 ? 64 : 32)) go_k<T, DP, 2, 4, true, KT>(a, pk, st);
     if (a.nsplit > 1) {
-      const float sc = a.flip ? -a.scale : a.scale;
+      const float sc = signed_scale(a);
       sum_parts<T>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, 2 * DP, 0, sc, a.gk, a.gk_r, a.gk_h, st);
       sum_parts<T>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, 2 * DP, DP, 1.0f, a.gv, a.gv_r, a.gv_h, st);
     }

@@ -22,19 +22,11 @@ __device__ __forceinline__ float* part_ml(const Args& a, int dp, int s, int64_t 
 // R: blocks of 16 columns a wave.  W waves, on one tile (SH) or each on its own.  KT: steps of 32 keys between barriers,
 // KC of them at a time in registers.
 template <typename T, int DP, int R, int W, bool SH, int KT, int KC>
-__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_t n_items) {
+__device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, int vq0, const Seg& qs, bf16* sK, bf16* sV, int w) {
   typedef Tile<T, DP, KT> TL;
   typedef typename Num<T>::Frag Frag;
-  constexpr int NT = SH ? 64 * W : 64, BQ = 16 * R * (SH ? W : 1), KS = TK * KT;
-  __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
-  Item it;
-  if (!item_of<W, SH>(a, n_items, it)) return;
-  const int l = lane_id(), c = l & 15, g = l >> 4, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  bf16 *sK = lds[SH ? 0 : w][0], *sV = lds[SH ? 0 : w][1];
-  int vq0;
-  Seg qs;
-  const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, a.guess, it.slot, vq0, qs);
-  if (vq0 < 0) return;
+  constexpr int NT = SH ? 64 * W : 64, KS = TK * KT;
+  const int l = lane_id(), c = l & 15, g = l >> 4;
   const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk, a.same, qs);
   const int nv = (qs.hi - qs.lo) * a.G, v0 = vq0 + (SH ? 16 * R * w : 0);
   const bool act = v0 < nv;                  // a wave without rows still loads tiles for the others
@@ -207,6 +199,135 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_
   }
 }
 
+template <typename T, int DP, int R, int W, bool SH, int KT, int KC>
+__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_t n_items) {
+  typedef Tile<T, DP, KT> TL;
+  constexpr int BQ = 16 * R * (SH ? W : 1);
+  __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
+  Item it;
+  if (!item_of<W, SH>(a, n_items, it)) return;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  int vq0;
+  Seg qs;
+  const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, a.guess, it.slot, vq0, qs);
+  if (vq0 < 0) return;
+  fwd_tile<T, DP, R, W, SH, KT, KC>(a, it, e, vq0, qs, lds[SH ? 0 : w][0], lds[SH ? 0 : w][1], w);
+}
+
+// A segment with at most 32 virtual rows and 32 keys (a molecule): one wave, each row of q, k and v read once, in rows as
+// they lie, and one softmax over all keys.
+template <typename T, int DP>
+__device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg& qs, const Seg& ks, bf16* lds) {
+  typedef Tile<T, DP> TL;
+  typedef typename Num<T>::Frag Frag;
+  const int l = lane_id(), c = l & 15, g = l >> 4;
+  const int nv = (qs.hi - qs.lo) * a.G, nk = ks.hi - ks.lo;
+  bf16 *sQ = lds, *sK = sQ + TL::elems, *sV = sK + TL::elems;
+  const int64_t e = sizeof(T);
+  uint32_t kbits;
+  {
+    Stage<T, DP, 1, 64> stQ, stK, stV;
+    uint32_t offQ[stQ.PER], offK[stQ.PER], offV[stQ.PER];
+    stK.offsets(offK, a.k_r * e, a.D);
+    stV.offsets(offV, a.v_r * e, a.D);
+    if (a.G == 1) stQ.offsets(offQ, a.q_r * e, a.D);
+    else {
+#pragma unroll
+      for (int p = 0; p < stQ.PER; ++p) {
+        const uint32_t u = stQ.row(p), i = a.by_g(u), h = u - i * a.G, f = stQ.feature(p);
+        offQ[p] = stQ.in(p) && (int)u < nv && (int)f < a.D ? (uint32_t)((i * a.q_r + h * a.q_h + f) * e) : kOob;
+      }
+    }
+    const int last = a.D * (int)e;
+    stQ.load(rows_buffer((const T*)a.q + qs.lo * a.q_r + (int64_t)kvh * a.G * a.q_h, qs.hi - qs.lo, a.q_r * e, last + (int)((a.G - 1) * a.q_h * e)), offQ, nv);
+    if (nk) {
+      stK.load(rows_buffer((const T*)a.k + ks.lo * a.k_r + kvh * a.k_h, nk, a.k_r * e, last), offK, nk);
+      stV.load(rows_buffer((const T*)a.v + ks.lo * a.v_r + kvh * a.v_h, nk, a.v_r * e, last), offV, nk);
+    }
+    bool key = l < nk;
+    if (key && a.mask) key = a.mask[ks.lo + l] != 0;
+    kbits = (uint32_t)__ballot(key);
+    if (a.mask) {                            // what a masked value holds must not meet a probability of 0
+      Bits<1> bits;
+      bits.w[0] = kbits;
+      stV.keep(bits);
+    }
+    stQ.store(sQ, TK);
+    if (nk) {
+      stK.store(sK, nk);
+      stV.store(sV, nk);
+    }
+  }
+  wave_sync();
+  const float c2 = a.flip ? -a.c2 : a.c2;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    if (q && nv <= 16) break;
+    typename TL::Feat Qc[TL::NK];
+#pragma unroll
+    for (int kk = 0; kk < TL::NK; ++kk) Qc[kk] = TL::rows(sQ, q, kk, c, g);
+    f32x4 S[2] = {zero4(), zero4()};
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k ? nk <= 16 : nk == 0) break;
+      S[k] = TL::product(sK, k, Qc, c, g, zero4());
+      const uint32_t b = kbits >> (16 * k + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        S[k][i] = (b >> i) & 1 ? S[k][i] * c2 : -INFINITY;
+        top = fmaxf(top, S[k][i]);
+      }
+    }
+    top = col_max(top);
+    const float m = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (k ? nk > 16 : nk > 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { S[k][i] = __builtin_amdgcn_exp2f(S[k][i] - m); sum += S[k][i]; }
+      }
+    sum = col_sum(sum);
+    const Frag P = chain_frag<T>(S[0], S[1]);
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const int v = 16 * q + c;
+    const uint32_t i = a.by_g(v);
+    const int row = qs.lo + (int)i, head = kvh * a.G + (v - (int)i * a.G);
+    T* op = (T*)a.out + row * a.o_r + head * a.o_h;
+#pragma unroll
+    for (int b = 0; b < TL::NB; ++b) {
+      f32x4 O = zero4();
+      if (nk) accumulate(O, TL::cols(sV, 0, b, c, g), P);
+      if (v < nv && 16 * b + 4 * g < a.D) store4(op + 16 * b + 4 * g, O * inv);
+    }
+    if (a.lse && g == 0 && v < nv) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+  }
+}
+
+// Tiles of 32 virtual rows, a wave each: the whole segment where it is small
+template <typename T, int DP, int W>
+__global__ __launch_bounds__(64 * W) void short_kernel(Args a, uint32_t n_items) {
+  typedef Tile<T, DP> TL;
+  __shared__ __attribute__((aligned(16))) bf16 lds[W][3][TL::elems];
+  Item it;
+  if (!item_of<W, false>(a, n_items, it)) return;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  int vq0;
+  Seg qs;
+  const int e = find_tile<TK>(a.q_ptr, a.B, a.Nq, a.G, a.guess, it.slot, vq0, qs);
+  if (vq0 < 0) return;
+  const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk, a.same, qs);
+  const int nv = (qs.hi - qs.lo) * a.G;
+  if (nv <= TK && ks.hi - ks.lo <= TK) {
+    small_segment<T, DP>(a, it.kvh, qs, ks, lds[w][0]);
+    return;
+  }
+  for (int x = 0; x < TK && vq0 + x < nv; x += 16) {
+    wave_sync();
+    fwd_tile<T, DP, 1, W, false, 1, 1>(a, it, e, vq0 + x, qs, lds[w][0], lds[w][1], 0);
+  }
+}
+
 // Joins many splits of a row and head: their weights first, then 4 features a thread over 64 groups of splits, whose sums
 // are added in order.  16 features a block: with all of a row's in one, the few rows that are split this often kept few
 // CUs busy (24.8 us against XXX for 8 rows of 2,048 splits).
@@ -279,15 +400,24 @@ static void go(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
   fwd_kernel<T, DP, R, W, SH, KT, KC><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
 }
-#ifndef X_KT
-#define X_KT 2
-#define X_KC 2
-#endif
 template <typename T, int DP>
 static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
   constexpr int tile = 2 * Tile<T, DP>::elems * 2, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
   constexpr bool f32 = Num<T>::planes == 3;
-  constexpr int KT = f32 ? 1 : X_KT, KC = f32 ? 1 : X_KC;
+  constexpr int KT = f32 ? 1 : 2, KC = f32 ? 1 : 2;
+  if constexpr (DP <= (f32 ? 32 : 64)) {
+    // short segments on both axes
+    if (p.form == 0 && a.nsplit == 1 && a.Nk <= 48 * (int64_t)(a.B > 0 ? a.B : 1)) {
+      constexpr int tile3 = 3 * Tile<T, DP>::elems * 2, W3 = 4 * tile3 <= 65536 ? 4 : 2;
+      Args x = a;
+      const int64_t slots = (int64_t)a.Nq * a.G / TK + a.B + 2, n = slots * a.Hkv;
+      x.slots = (uint32_t)slots;
+      x.by_slots = Div::of(x.slots);
+      x.guess = (float)(a.B + 2) / (float)slots;
+      short_kernel<T, DP, W3><<<(uint32_t)cdiv(n, W3), 64 * W3, 0, st>>>(x, (uint32_t)n);
+      return (int)hipGetLastError();
+    }
+  }
   if constexpr (f32 && DP == 128) go<T, DP, 1, 4, true, KT, KC>(a, p, st);
   else if (p.form == 0) go<T, DP, 1, W, false, 1, 1>(a, p, st);
   else if (p.form == 1) go<T, DP, 1, 4, true, KT, KC>(a, p, st);
