@@ -14,15 +14,21 @@ bool dims_ok(const EgnnAttnDims* d) {
 
 // own: (virtual) rows of the axis that is cut into tiles, other: rows of the axis a tile walks
 Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest) {
-  const int64_t segs = n_seg > 0 ? n_seg : 1, mean = own / segs;
+  const int64_t segs = n_seg > 0 ? n_seg : 1, mean = own / segs, len = other / segs;
+  auto items_of = [&](int64_t rows) {
+    const int64_t tiles = cdiv(own, rows) > n_seg ? cdiv(own, rows) : n_seg;
+    return (tiles > 0 ? tiles : 1) * heads;
+  };
   Plan p;
-  p.form = mean <= 48 ? 0 : mean < 256 ? 1 : 2;
+  // 128 rows a workgroup where there are enough of them to fill the device, or where splits will: 37 chains of 301, fp32,
+  // 8 heads on 2 key heads: dq 52 us with 64 rows (1,406 workgroups) and 60 with 128 (740); 64 chains of 512, bf16: 27.6
+  // and 23.9 (1,024); 12,289 rows: 299 and 238, in 3 and 4 parts
+  p.form = mean <= 48 ? 0 : mean > 64 && (items_of(128) >= 1024 || len >= 2048) ? 2 : 1;
   if (widest < 0) p.form = 1;
   else if (p.form > widest) p.form = widest;
   const int64_t BQ = p.rows();
   p.slots = own / BQ + n_seg + 2;
-  const int64_t tiles = cdiv(own, BQ) > n_seg ? cdiv(own, BQ) : n_seg, items = (tiles > 0 ? tiles : 1) * heads;
-  const int64_t len = other / segs;
+  const int64_t items = items_of(BQ);
   p.nsplit = 1;
   const int64_t want = p.form == 0 ? 4096 : 1024;
   if (items < want / 2 && len >= 512) {

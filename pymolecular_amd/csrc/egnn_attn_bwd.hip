@@ -55,7 +55,7 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
   int row[R], head[R];
   bool live[R], none[R];
   float delta[R], ref[R], sum[R];
-  f32x4 dQ[R][TL::NB];
+  Sum<T> dQ[R][TL::NB];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int v = v0 + 16 * r + c;
@@ -80,8 +80,6 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
     none[r] = lse == -INFINITY;              // a row without keys: no gradient from it or to it
     ref[r] = none[r] ? INFINITY : lse;
     sum[r] = 0.f;
-#pragma unroll
-    for (int b = 0; b < TL::NB; ++b) dQ[r][b] = zero4();
   }
 
   for (; j < j1; j += stride) {
@@ -98,6 +96,12 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
     tile_sync<SH>();
     if (j + stride < j1) fetch(j + stride);
     if (!act) continue;
+    if constexpr (KT > 1) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int b = 0; b < TL::NB; ++b) dQ[r][b].begin();
+    }
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       if (KT > 1 && TK * t >= n) break;
@@ -170,8 +174,17 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
       for (int b = 0; b < TL::NB; ++b) {
         const Frag A = TL::cols(sK, t, b, c, g);
 #pragma unroll
-        for (int r = 0; r < R; ++r) accumulate(dQ[r][b], A, F[r]);
+        for (int r = 0; r < R; ++r) {
+          if constexpr (KT == 1) dQ[r][b].one(A, F[r]);
+          else dQ[r][b].add(A, F[r]);
+        }
       }
+    }
+    if constexpr (KT > 1) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int b = 0; b < TL::NB; ++b) dQ[r][b].end();
     }
   }
   const float sc = signed_scale(a);
@@ -183,13 +196,13 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
     if (a.nsplit > 1) {
       float* p = a.part + ((int64_t)it.sp * a.Nq * a.Hq + (int64_t)row[r] * a.Hq + head[r]) * DP;
 #pragma unroll
-      for (int b = 0; b < TL::NB; ++b) store4(p + 16 * b + 4 * g, none[r] ? zero4() : dQ[r][b]);
+      for (int b = 0; b < TL::NB; ++b) store4(p + 16 * b + 4 * g, none[r] ? zero4() : dQ[r][b].v);
       continue;
     }
     T* out = (T*)a.gq + row[r] * a.gq_r + head[r] * a.gq_h;
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b)
-      if (16 * b + 4 * g < a.D) store4(out + 16 * b + 4 * g, none[r] ? zero4() : dQ[r][b] * sc);
+      if (16 * b + 4 * g < a.D) store4(out + 16 * b + 4 * g, none[r] ? zero4() : dQ[r][b].v * sc);
   }
 }
 
@@ -259,7 +272,7 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
   typename TL::Feat K[R][TL::NK], V[R][TL::NK];
   int key[R];
   bool in[R], live[R];
-  f32x4 dK[R][TL::NB], dV[R][TL::NB];
+  Sum<T> dK[R][TL::NB], dV[R][TL::NB];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     key[r] = key0 + 16 * r + c;
@@ -274,8 +287,6 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
       landed(K[r][kk]);
       landed(V[r][kk]);
     }
-#pragma unroll
-    for (int b = 0; b < TL::NB; ++b) { dK[r][b] = zero4(); dV[r][b] = zero4(); }
   }
 
   for (; j < j1; j += stride) {
@@ -313,6 +324,12 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
     tile_sync<SH>();
     if (j + stride < j1) fetch(j + stride);
     if (!act) continue;
+    if constexpr (KT > 1) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int b = 0; b < TL::NB; ++b) { dK[r][b].begin(); dV[r][b].begin(); }
+    }
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       if (KT > 1 && TK * t >= n) break;
@@ -348,8 +365,17 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
       for (int b = 0; b < TL::NB; ++b) {
         const Frag A = TL::cols(sG, t, b, c, g), B = TL::cols(sQ, t, b, c, g);
 #pragma unroll
-        for (int r = 0; r < R; ++r) { accumulate(dV[r][b], A, FP[r]); accumulate(dK[r][b], B, FS[r]); }
+        for (int r = 0; r < R; ++r) {
+          if constexpr (KT == 1) { dV[r][b].one(A, FP[r]); dK[r][b].one(B, FS[r]); }
+          else { dV[r][b].add(A, FP[r]); dK[r][b].add(B, FS[r]); }
+        }
       }
+    }
+    if constexpr (KT > 1) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int b = 0; b < TL::NB; ++b) { dK[r][b].end(); dV[r][b].end(); }
     }
   }
   const float sc = signed_scale(a);
@@ -360,8 +386,8 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
       float* p = a.part + ((int64_t)it.sp * a.Nk * a.Hkv + (int64_t)key[r] * a.Hkv + it.kvh) * (2 * DP);
 #pragma unroll
       for (int b = 0; b < TL::NB; ++b) {
-        store4(p + 16 * b + 4 * g, live[r] ? dK[r][b] : zero4());
-        store4(p + DP + 16 * b + 4 * g, live[r] ? dV[r][b] : zero4());
+        store4(p + 16 * b + 4 * g, live[r] ? dK[r][b].v : zero4());
+        store4(p + DP + 16 * b + 4 * g, live[r] ? dV[r][b].v : zero4());
       }
       continue;
     }
@@ -369,8 +395,8 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b)
       if (16 * b + 4 * g < a.D) {
-        store4(gk + 16 * b + 4 * g, live[r] ? dK[r][b] * sc : zero4());
-        store4(gv + 16 * b + 4 * g, live[r] ? dV[r][b] : zero4());
+        store4(gk + 16 * b + 4 * g, live[r] ? dK[r][b].v * sc : zero4());
+        store4(gv + 16 * b + 4 * g, live[r] ? dV[r][b].v : zero4());
       }
   }
 }
@@ -512,9 +538,11 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     T* out = (T*)a.gq + (qs.lo + (int)i) * a.gq_r + (kvh * a.G + (v - (int)i * a.G)) * a.gq_h;
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b) {
-      f32x4 d = zero4();
-      if (nk) accumulate(d, TL::cols(sK, 0, b, c, g), F);
-      if (v < nv && 16 * b + 4 * g < a.D) store4(out + 16 * b + 4 * g, d * sc);
+      Sum<T> d;
+      d.begin();
+      if (nk) d.add(TL::cols(sK, 0, b, c, g), F);
+      d.end();
+      if (v < nv && 16 * b + 4 * g < a.D) store4(out + 16 * b + 4 * g, d.v * sc);
     }
   }
   if (nk == 0) return;
@@ -544,12 +572,16 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     T *gk = (T*)a.gk + key * a.gk_r + kvh * a.gk_h, *gv = (T*)a.gv + key * a.gv_r + kvh * a.gv_h;
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b) {
-      f32x4 dK = zero4(), dV = zero4();
-      accumulate(dV, TL::cols(sG, 0, b, c, g), FP);
-      accumulate(dK, TL::cols(sQ, 0, b, c, g), FS);
+      Sum<T> dK, dV;
+      dK.begin();
+      dV.begin();
+      dV.add(TL::cols(sG, 0, b, c, g), FP);
+      dK.add(TL::cols(sQ, 0, b, c, g), FS);
+      dK.end();
+      dV.end();
       if (16 * k + c < nk && 16 * b + 4 * g < a.D) {
-        store4(gk + 16 * b + 4 * g, live[k] ? dK * sc : zero4());
-        store4(gv + 16 * b + 4 * g, live[k] ? dV : zero4());
+        store4(gk + 16 * b + 4 * g, live[k] ? dK.v * sc : zero4());
+        store4(gv + 16 * b + 4 * g, live[k] ? dV.v : zero4());
       }
     }
   }
@@ -607,10 +639,13 @@ __global__ __launch_bounds__(64 * W, DP == 16 && W == 4 ? 4 : 1) void short_kern
 }
 
 // out[row][head][f] = mul * sum over the splits, 4 features a thread: GR groups of splits a block, whose sums are added in
-// order.  The partial rows are `width` values apart, the values from `off` on.
+// order.  The partial rows are `width` values apart and hold one output's DP values, or two's.
+template <typename T> struct Out { T* p; int64_t rs, hs; float mul; };
 template <typename T, int GR>
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int nsplit, int64_t rows, int heads, int D, int width, int off,
-                                                        float mul, T* out, int64_t rs, int64_t hs) {
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int nsplit, int64_t rows, int heads, int D, int DP, int width,
+                                                        Out<T> one, Out<T> two) {
+  const Out<T> o = blockIdx.y ? two : one;
+  const int off = blockIdx.y * DP;
   constexpr int PB = 256 / GR;
   __shared__ f32x4 red[GR][PB];
   const int x = threadIdx.x % PB, k = threadIdx.x / PB;
@@ -629,14 +664,14 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int n
 #pragma unroll
     for (int i = 1; i < GR; ++i) s += red[i][x];
   }
-  if (r < n) store4(out + (r / heads) * rs + (r % heads) * hs + f, s * mul);
+  if (r < n) store4(o.p + (r / heads) * o.rs + (r % heads) * o.hs + f, s * o.mul);
 }
 template <typename T>
-static void sum_parts(const float* part, int nsplit, int64_t rows, int heads, int D, int width, int off, float mul, void* out, int64_t rs,
-                      int64_t hs, hipStream_t st) {
+static void sum_parts(const float* part, int nsplit, int64_t rows, int heads, int D, int DP, Out<T> one, Out<T> two, hipStream_t st) {
   const int64_t n = rows * heads * (D / 4);
-  if (nsplit <= 16) sum_parts_kernel<T, 1><<<(uint32_t)cdiv(n, 256), 256, 0, st>>>(part, nsplit, rows, heads, D, width, off, mul, (T*)out, rs, hs);
-  else sum_parts_kernel<T, 32><<<(uint32_t)cdiv(n, 8), 256, 0, st>>>(part, nsplit, rows, heads, D, width, off, mul, (T*)out, rs, hs);
+  const int outs = two.p ? 2 : 1, width = outs * DP;
+  if (nsplit <= 16) sum_parts_kernel<T, 1><<<dim3((uint32_t)cdiv(n, 256), outs), 256, 0, st>>>(part, nsplit, rows, heads, D, DP, width, one, two);
+  else sum_parts_kernel<T, 32><<<dim3((uint32_t)cdiv(n, 8), outs), 256, 0, st>>>(part, nsplit, rows, heads, D, DP, width, one, two);
 }
 
 template <typename T, int DP, int R, int W, bool SH, int KT>
@@ -675,7 +710,7 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
   constexpr int tile = 2 * Tile<T, DP>::elems * 2 + 256, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
   if (launch_short<T, DP>(a, pq, pk, st)) return (int)hipGetLastError();
   constexpr bool wide = Num<T>::planes == 3 && DP == 128;
-  constexpr int KT = Num<T>::planes == 1 && DP < 128 ? 2 : 1;
+  constexpr int KT = Num<T>::planes == 1 ? (DP < 128 ? 2 : 1) : DP <= 32 ? 2 : 1;
   a.nsplit = pq.nsplit;
   a.slots = (uint32_t)pq.slots;
   a.guess = (float)(a.B + 2) / (float)a.slots;
@@ -686,7 +721,7 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
     else if (pq.form == 1) go_q<T, DP, 1, 4, true, KT>(a, pq, st);
     else go_q<T, DP, 2, 4, true, KT>(a, pq, st);
     if (a.nsplit > 1)
-      sum_parts<T>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, 0, signed_scale(a), a.gq, a.gq_r, a.gq_h, st);
+      sum_parts<T>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, Out<T>{(T*)a.gq, a.gq_r, a.gq_h, signed_scale(a)}, Out<T>{}, st);
   }
   a.nsplit = pk.nsplit;
   a.slots = (uint32_t)pk.slots;
@@ -697,11 +732,8 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
     else if (pk.form == 0) go_k<T, DP, 1, W, false, 1>(a, pk, st);
     else if (pk.form == 1) go_k<T, DP, 1, 4, true, KT>(a, pk, st);
     else if constexpr (DP <= (Num<T>::planes == 1 ? 64 : 32)) go_k<T, DP, 2, 4, true, KT>(a, pk, st);
-    if (a.nsplit > 1) {
-      const float sc = signed_scale(a);
-      sum_parts<T>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, 2 * DP, 0, sc, a.gk, a.gk_r, a.gk_h, st);
-      sum_parts<T>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, 2 * DP, DP, 1.0f, a.gv, a.gv_r, a.gv_h, st);
-    }
+    if (a.nsplit > 1)
+      sum_parts<T>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, DP, Out<T>{(T*)a.gk, a.gk_r, a.gk_h, signed_scale(a)}, Out<T>{(T*)a.gv, a.gv_r, a.gv_h, 1.0f}, st);
   }
   return (int)hipGetLastError();
 }

@@ -70,14 +70,12 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
       landed(Q[r][kk]);
     }
   }
-  f32x4 O[R][TL::NB];
+  Sum<T> O[R][TL::NB];
   float m[R], sum[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     m[r] = kLowest;
     sum[r] = 0.f;
-#pragma unroll
-    for (int b = 0; b < TL::NB; ++b) O[r][b] = zero4();
   }
 
   for (; j < j1; j += stride) {
@@ -94,6 +92,12 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
     tile_sync<SH>();
     if (j + stride < j1) fetch(j + stride);
     if (!act) continue;
+    if constexpr (KT > 1) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int b = 0; b < TL::NB; ++b) O[r][b].begin();
+    }
 #pragma unroll
     for (int t0 = 0; t0 < KT; t0 += KC) {
       if (KT > KC && TK * t0 >= n) break;
@@ -141,7 +145,7 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
             m[r] = mn;
             sum[r] *= alpha;
 #pragma unroll
-            for (int b = 0; b < TL::NB; ++b) O[r][b] *= alpha;
+            for (int b = 0; b < TL::NB; ++b) O[r][b].scale(alpha, KT > KC && t0 > 0);
           }
         }
         bool over = false;
@@ -172,8 +176,17 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
         for (int b = 0; b < TL::NB; ++b) {
           const Frag A = TL::cols(sV, t0 + t, b, c, g);
 #pragma unroll
-          for (int r = 0; r < R; ++r) accumulate(O[r][b], A, P[r][t]);
+          for (int r = 0; r < R; ++r) {
+            if constexpr (KT == 1) O[r][b].one(A, P[r][t]);
+            else O[r][b].add(A, P[r][t]);
+          }
         }
+    }
+    if constexpr (KT > 1) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int b = 0; b < TL::NB; ++b) O[r][b].end();
     }
   }
 #pragma unroll
@@ -184,7 +197,7 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
       const int64_t x = (int64_t)row[r] * a.Hq + head[r];
       float* p = part_o(a, DP, it.sp, x);
 #pragma unroll
-      for (int b = 0; b < TL::NB; ++b) store4(p + 16 * b + 4 * g, O[r][b]);
+      for (int b = 0; b < TL::NB; ++b) store4(p + 16 * b + 4 * g, O[r][b].v);
       p = part_ml(a, DP, it.sp, x);
       if (g == 0) { p[0] = m[r]; p[1] = s; }
       continue;
@@ -194,7 +207,7 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
     T* op = (T*)a.out + row[r] * a.o_r + head[r] * a.o_h;
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b)
-      if (16 * b + 4 * g < a.D) store4(op + 16 * b + 4 * g, O[r][b] * inv);
+      if (16 * b + 4 * g < a.D) store4(op + 16 * b + 4 * g, O[r][b].v * inv);
     if (a.lse && g == 0) a.lse[(int64_t)head[r] * a.Nq + row[r]] = (m[r] + __builtin_amdgcn_logf(s)) * kLn2;
   }
 }
@@ -296,9 +309,11 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     T* op = (T*)a.out + row * a.o_r + head * a.o_h;
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b) {
-      f32x4 O = zero4();
-      if (nk) accumulate(O, TL::cols(sV, 0, b, c, g), P);
-      if (v < nv && 16 * b + 4 * g < a.D) store4(op + 16 * b + 4 * g, O * inv);
+      Sum<T> O;
+      O.begin();
+      if (nk) O.add(TL::cols(sV, 0, b, c, g), P);
+      O.end();
+      if (v < nv && 16 * b + 4 * g < a.D) store4(op + 16 * b + 4 * g, O.v * inv);
     }
     if (a.lse && g == 0 && v < nv) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
   }
@@ -404,7 +419,7 @@ template <typename T, int DP>
 static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
   constexpr int tile = 2 * Tile<T, DP>::elems * 2, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
   constexpr bool f32 = Num<T>::planes == 3;
-  constexpr int KT = f32 ? 1 : 2, KC = f32 ? 1 : 2;
+    constexpr int KT = f32 ? (DP <= 32 ? 2 : 1) : 2, KC = f32 || DP == 128 ? 1 : 2;
   if constexpr (DP <= (f32 ? 32 : 64)) {
     // short segments on both axes
     if (p.form == 0 && a.nsplit == 1 && a.Nk <= 48 * (int64_t)(a.B > 0 ? a.B : 1)) {
