@@ -63,6 +63,8 @@ struct Args {
   float* part;                               // split partials
 };
 
+constexpr int kShortMean = 28;               // rows a segment up to which a wave takes a tile
+
 // How one axis is cut into tiles; the other axis is walked in nsplit parts, part s taking every nsplit-th step from s on:
 // the parts move through memory side by side (apart, 2,048 streams at one stride fell on few memory channels: 324 us
 // where side by side takes XXX, one query over 2,000,000 keys)
@@ -382,22 +384,54 @@ template <bool SH> __device__ __forceinline__ void tile_sync() {
   else wave_sync();
 }
 
+// Waves a SIMD that a workgroup kernel's registers have to leave room for.  The allocation is in steps that a change of a
+// register or two can cross: 169 instead of 167 (bf16, D = 64, 32 columns a wave) took the forward of 12,289 rows from 197
+// to 210 us.
+template <typename T, int DP, int R> constexpr int group_occupancy() {
+  return Num<T>::planes == 1 ? (R == 2 ? (DP <= 32 ? 4 : DP == 64 ? 3 : 2) : (DP <= 64 ? 4 : 3)) : 2;
+}
+
 // max and sum over the four lanes of a column
 __device__ __forceinline__ float col_max(float v) { v = fmaxf(v, shfl_xor(v, 16)); return fmaxf(v, shfl_xor(v, 32)); }
 __device__ __forceinline__ float col_sum(float v) { v += shfl_xor(v, 16); return v + shfl_xor(v, 32); }
 
 // four features of one row
 __device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
-__device__ __forceinline__ void store4(bf16* p, const f32x4& v) {
+__device__ __forceinline__ bf16x4 pack4(const f32x4& v) {
   bf16x4 r;
   r[0] = (bf16)v[0]; r[1] = (bf16)v[1]; r[2] = (bf16)v[2]; r[3] = (bf16)v[3];
-  *reinterpret_cast<bf16x4*>(p) = r;
+  return r;
 }
+__device__ __forceinline__ void store4(bf16* p, const f32x4& v) { *reinterpret_cast<bf16x4*>(p) = pack4(v); }
 // values that a loop reads: waited for here, or every round of the loop would wait for its own prefetch as well
 __device__ __forceinline__ void landed(bf16x4& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void landed(bf16x8& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void landed(Half3& v) { landed(v.p0); landed(v.p1); landed(v.p2); }
 __device__ __forceinline__ void landed(split::Chunk3& v) { landed(v.p0); landed(v.p1); landed(v.p2); }
+
+// Stores a column's features, NB blocks of 16: a lane has four of each block, 4g .. of it.  bf16: two blocks' four are
+// exchanged with the neighbouring lane group's, so that a lane stores 8 neighbouring values and 64 bytes of a row are
+// written at once instead of 32.
+template <int NB> __device__ __forceinline__ void store_row(float* p, const f32x4* v, int g, int D) {
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    if (16 * b + 4 * g < D) store4(p + 16 * b + 4 * g, v[b]);
+}
+template <int NB> __device__ __forceinline__ void store_row(bf16* p, const f32x4* v, int g, int D) {
+  if constexpr (NB == 1) {
+    if (4 * g < D) store4(p + 4 * g, v[0]);
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; b += 2) {
+      const u32x2 x = __builtin_bit_cast(u32x2, pack4(v[b])), y = __builtin_bit_cast(u32x2, pack4(v[b + 1]));
+      // groups 1, 3 of the first change places with groups 0, 2 of the second
+      const u32x2 s0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(x[0], y[0], false, false));
+      const u32x2 s1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(x[1], y[1], false, false));
+      const int f = 16 * (b + (g & 1)) + 4 * (g & 2);
+      if (f < D) *reinterpret_cast<u32x4*>(p + f) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+    }
+  }
+}
 
 // the first n rows of a step, and of those the ones whose flag (of row 64 k + lane) is set
 template <int KT>

@@ -20,10 +20,12 @@ Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest)
     return (tiles > 0 ? tiles : 1) * heads;
   };
   Plan p;
-  // 128 rows a workgroup where there are enough of them to fill the device, or where splits will: 37 chains of 301, fp32,
-  // 8 heads on 2 key heads: dq 52 us with 64 rows (1,406 workgroups) and 60 with 128 (740); 64 chains of 512, bf16: 27.6
-  // and 23.9 (1,024); 12,289 rows: 299 and 238, in 3 and 4 parts
-  p.form = mean <= 48 ? 0 : mean > 64 && (items_of(128) >= 1024 || len >= 2048) ? 2 : 1;
+  // Measured on both sides, forward and backward in us, bf16 unless stated.  A wave a tile, and a whole small segment
+  // (form 0), against 64 rows a workgroup (1): 15 .. 32 rows a segment, D = 64: 33.5 and 44.7; 9 .. 40, D = 16: 35 and 51;
+  // 25 .. 45, D = 64: 59 and 41; 20 .. 40, fp32, D = 32: 61 and 37.  64 rows against 128 (2): 80 rows 53 and 61, 100 .. 260
+  // 70 and 75, 256 64 and 60, 512 (D = 32) 86 and 73.  128 rows only where they fill the device, or splits will: 37
+  // chains of 301 in fp32, 8 heads on 2: 52 and 60 (1,406 and 740 workgroups), 12,289 rows 980 and 800.
+  p.form = mean <= kShortMean ? 0 : mean >= 256 && (items_of(128) >= 1024 || len >= 2048) ? 2 : 1;
   if (widest < 0) p.form = 1;
   else if (p.form > widest) p.form = widest;
   const int64_t BQ = p.rows();

@@ -200,9 +200,10 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
       continue;
     }
     T* out = (T*)a.gq + row[r] * a.gq_r + head[r] * a.gq_h;
+    f32x4 o[TL::NB];
 #pragma unroll
-    for (int b = 0; b < TL::NB; ++b)
-      if (16 * b + 4 * g < a.D) store4(out + 16 * b + 4 * g, none[r] ? zero4() : dQ[r][b].v * sc);
+    for (int b = 0; b < TL::NB; ++b) o[b] = none[r] ? zero4() : dQ[r][b].v * sc;
+    store_row<TL::NB>(out, o, g, a.D);
   }
 }
 
@@ -391,18 +392,18 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
       }
       continue;
     }
-    T *gk = (T*)a.gk + key[r] * a.gk_r + it.kvh * a.gk_h, *gv = (T*)a.gv + key[r] * a.gv_r + it.kvh * a.gv_h;
+    f32x4 o[TL::NB];
 #pragma unroll
-    for (int b = 0; b < TL::NB; ++b)
-      if (16 * b + 4 * g < a.D) {
-        store4(gk + 16 * b + 4 * g, live[r] ? dK[r][b].v * sc : zero4());
-        store4(gv + 16 * b + 4 * g, live[r] ? dV[r][b].v : zero4());
-      }
+    for (int b = 0; b < TL::NB; ++b) o[b] = live[r] ? dK[r][b].v * sc : zero4();
+    store_row<TL::NB>((T*)a.gk + key[r] * a.gk_r + it.kvh * a.gk_h, o, g, a.D);
+#pragma unroll
+    for (int b = 0; b < TL::NB; ++b) o[b] = live[r] ? dV[r][b].v : zero4();
+    store_row<TL::NB>((T*)a.gv + key[r] * a.gv_r + it.kvh * a.gv_h, o, g, a.D);
   }
 }
 
 template <typename T, int DP, int R, int W, bool SH, int KT>
-__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dq_kernel(Args a, uint32_t n_items) {
+__global__ __launch_bounds__(64 * W, (SH ? group_occupancy<T, DP, R>() : 1)) void dq_kernel(Args a, uint32_t n_items) {
   typedef Tile<T, DP, KT> TL;
   constexpr int BQ = 16 * R * (SH ? W : 1);
   __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
@@ -536,14 +537,16 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     const int v = 16 * q + c;
     const uint32_t i = a.by_g(v);
     T* out = (T*)a.gq + (qs.lo + (int)i) * a.gq_r + (kvh * a.G + (v - (int)i * a.G)) * a.gq_h;
+    f32x4 o[TL::NB];
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b) {
       Sum<T> d;
       d.begin();
       if (nk) d.add(TL::cols(sK, 0, b, c, g), F);
       d.end();
-      if (v < nv && 16 * b + 4 * g < a.D) store4(out + 16 * b + 4 * g, d.v * sc);
+      o[b] = d.v * sc;
     }
+    if (v < nv) store_row<TL::NB>(out, o, g, a.D);
   }
   if (nk == 0) return;
   wave_sync();
@@ -569,7 +572,7 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     }
     const Frag FP = chain_frag<T>(P[0], P[1]), FS = chain_frag<T>(dS[0], dS[1]);
     const int key = ks.lo + 16 * k + c;
-    T *gk = (T*)a.gk + key * a.gk_r + kvh * a.gk_h, *gv = (T*)a.gv + key * a.gv_r + kvh * a.gv_h;
+    f32x4 ok[TL::NB], ov[TL::NB];
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b) {
       Sum<T> dK, dV;
@@ -579,10 +582,12 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
       dK.add(TL::cols(sQ, 0, b, c, g), FS);
       dK.end();
       dV.end();
-      if (16 * k + c < nk && 16 * b + 4 * g < a.D) {
-        store4(gk + 16 * b + 4 * g, live[k] ? dK.v * sc : zero4());
-        store4(gv + 16 * b + 4 * g, live[k] ? dV.v : zero4());
-      }
+      ok[b] = live[k] ? dK.v * sc : zero4();
+      ov[b] = live[k] ? dV.v : zero4();
+    }
+    if (16 * k + c < nk) {
+      store_row<TL::NB>((T*)a.gk + key * a.gk_r + kvh * a.gk_h, ok, g, a.D);
+      store_row<TL::NB>((T*)a.gv + key * a.gv_r + kvh * a.gv_h, ov, g, a.D);
     }
   }
 }
@@ -710,7 +715,7 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
   constexpr int tile = 2 * Tile<T, DP>::elems * 2 + 256, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
   if (launch_short<T, DP>(a, pq, pk, st)) return (int)hipGetLastError();
   constexpr bool wide = Num<T>::planes == 3 && DP == 128;
-  constexpr int KT = Num<T>::planes == 1 ? (DP < 128 ? 2 : 1) : DP <= 32 ? 2 : 1;
+  constexpr int KT = Num<T>::planes == 1 ? (DP < 128 ? 2 : 1) : DP <= 32 ? 2 : 1, KT1 = Num<T>::planes == 1 ? 1 : KT;
   a.nsplit = pq.nsplit;
   a.slots = (uint32_t)pq.slots;
   a.guess = (float)(a.B + 2) / (float)a.slots;
@@ -718,7 +723,7 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
   if (a.Nq) {
     if constexpr (wide) go_q<T, DP, 1, 4, true, KT>(a, pq, st);
     else if (pq.form == 0) go_q<T, DP, 1, W, false, 1>(a, pq, st);
-    else if (pq.form == 1) go_q<T, DP, 1, 4, true, KT>(a, pq, st);
+    else if (pq.form == 1) go_q<T, DP, 1, 4, true, KT1>(a, pq, st);
     else go_q<T, DP, 2, 4, true, KT>(a, pq, st);
     if (a.nsplit > 1)
       sum_parts<T>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, Out<T>{(T*)a.gq, a.gq_r, a.gq_h, signed_scale(a)}, Out<T>{}, st);
@@ -730,7 +735,7 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
   if (a.Nk) {
     if constexpr (wide) go_k<T, DP, 1, 4, true, KT>(a, pk, st);
     else if (pk.form == 0) go_k<T, DP, 1, W, false, 1>(a, pk, st);
-    else if (pk.form == 1) go_k<T, DP, 1, 4, true, KT>(a, pk, st);
+    else if (pk.form == 1) go_k<T, DP, 1, 4, true, KT1>(a, pk, st);
     else if constexpr (DP <= (Num<T>::planes == 1 ? 64 : 32)) go_k<T, DP, 2, 4, true, KT>(a, pk, st);
     if (a.nsplit > 1)
       sum_parts<T>(a.part, a.nsplit, a.Nk, a.Hkv, a.D, DP, Out<T>{(T*)a.gk, a.gk_r, a.gk_h, signed_scale(a)}, Out<T>{(T*)a.gv, a.gv_r, a.gv_h, 1.0f}, st);

@@ -213,7 +213,7 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
 }
 
 template <typename T, int DP, int R, int W, bool SH, int KT, int KC>
-__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void fwd_kernel(Args a, uint32_t n_items) {
+__global__ __launch_bounds__(64 * W, (SH ? group_occupancy<T, DP, R>() : 1)) void fwd_kernel(Args a, uint32_t n_items) {
   typedef Tile<T, DP, KT> TL;
   constexpr int BQ = 16 * R * (SH ? W : 1);
   __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
@@ -307,15 +307,18 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     const uint32_t i = a.by_g(v);
     const int row = qs.lo + (int)i, head = kvh * a.G + (v - (int)i * a.G);
     T* op = (T*)a.out + row * a.o_r + head * a.o_h;
+    f32x4 o[TL::NB];
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b) {
       Sum<T> O;
       O.begin();
       if (nk) O.add(TL::cols(sV, 0, b, c, g), P);
       O.end();
-      if (v < nv && 16 * b + 4 * g < a.D) store4(op + 16 * b + 4 * g, O.v * inv);
+      o[b] = O.v * inv;
     }
-    if (a.lse && g == 0 && v < nv) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (v >= nv) continue;
+    store_row<TL::NB>(op, o, g, a.D);
+    if (a.lse && g == 0) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
   }
 }
 
@@ -422,7 +425,7 @@ static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
     constexpr int KT = f32 ? (DP <= 32 ? 2 : 1) : 2, KC = f32 || DP == 128 ? 1 : 2;
   if constexpr (DP <= (f32 ? 32 : 64)) {
     // short segments on both axes
-    if (p.form == 0 && a.nsplit == 1 && a.Nk <= 48 * (int64_t)(a.B > 0 ? a.B : 1)) {
+    if (p.form == 0 && a.nsplit == 1 && a.Nk <= kShortMean * (int64_t)(a.B > 0 ? a.B : 1)) {
       constexpr int tile3 = 3 * Tile<T, DP>::elems * 2, W3 = 4 * tile3 <= 65536 ? 4 : 2;
       Args x = a;
       const int64_t slots = (int64_t)a.Nq * a.G / TK + a.B + 2, n = slots * a.Hkv;
@@ -435,7 +438,7 @@ static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
   }
   if constexpr (f32 && DP == 128) go<T, DP, 1, 4, true, KT, KC>(a, p, st);
   else if (p.form == 0) go<T, DP, 1, W, false, 1, 1>(a, p, st);
-  else if (p.form == 1) go<T, DP, 1, 4, true, KT, KC>(a, p, st);
+  else if (p.form == 1) go<T, DP, 1, 4, true, f32 ? KT : 1, 1>(a, p, st);
   else go<T, DP, 2, 4, true, KT, KC>(a, p, st);
   const int64_t rows = (int64_t)a.Nq * a.Hq;
   if (a.nsplit > kFewSplits) fwd_join_many_kernel<T, DP><<<dim3((uint32_t)rows, DP / 16), 256, 0, st>>>(a);
