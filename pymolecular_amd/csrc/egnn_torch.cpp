@@ -262,13 +262,18 @@ pybind11::object attn_forward(const Tensor& q, const Tensor& k, const Tensor& v,
 }
 
 pybind11::object attn_backward(const Tensor& go, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
-                               const Tensor& lse, const Tensor& q_ptr, const Opt& kv_ptr, const Opt& mask, double scale) {
+                               const Tensor& lse, const Tensor& q_ptr, const Opt& kv_ptr, const Opt& mask, double scale,
+                               const std::optional<std::vector<Tensor>>& into) {
   if (!attn_ok(q, k, v, q_ptr, kv_ptr, mask, scale) || !heads_ok(go, q, q.size(0), q.size(1), q.size(2), q.size(1) / k.size(1)) ||
       !heads_ok(out, q, q.size(0), q.size(1), q.size(2), q.size(1) / k.size(1)) || !fits(lse, q, at::kFloat, {q.size(1), q.size(0)}))
     return pybind11::none();
   const EgnnAttnDims d = attn_dims(q, k, q_ptr, scale);
-  const Tensor gq = at::empty({d.Nq, d.Hq, d.D}, q.options()), gk = at::empty({d.Nk, d.Hkv, d.D}, q.options()),
-               gv = at::empty({d.Nk, d.Hkv, d.D}, q.options());
+  if (into && (into->size() != 3 || !heads_ok((*into)[0], q, d.Nq, d.Hq, d.D) || !heads_ok((*into)[1], q, d.Nk, d.Hkv, d.D) ||
+               !heads_ok((*into)[2], q, d.Nk, d.Hkv, d.D)))
+    return pybind11::none();
+  const Tensor gq = into ? (*into)[0] : at::empty({d.Nq, d.Hq, d.D}, q.options()),
+               gk = into ? (*into)[1] : at::empty({d.Nk, d.Hkv, d.D}, q.options()),
+               gv = into ? (*into)[2] : at::empty({d.Nk, d.Hkv, d.D}, q.options());
   const size_t nb = egnn_attn_bwd_workspace_bytes(&d);
   const Tensor ws = workspace(nb, q);
   EgnnAttnStrides s{};

@@ -5,3 +5,4 @@ from .forward_kernel import egnn_forward_kernel_node_parallel  # noqa: F401
 from .backward_kernel import egnn_backward_kernel_node_parallel  # noqa: F401
 from .pytorch_baseline import pytorch_egnn_baseline, swish_torch  # noqa: F401
 from .mpnn import MPNN, MPNN_GCL  # noqa: F401
+from .global_attention import EGNNGlobal, GlobalAttention, GraphReadout  # noqa: F401

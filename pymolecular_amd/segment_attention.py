@@ -22,7 +22,8 @@ from . import _capi
 from ._capi import EgnnAttnDims, EgnnAttnStrides, check
 from .fused import _dtype_code, _ptr, _stream
 
-__all__ = ["segment_attention", "segment_attention_forward", "segment_attention_backward", "SegmentAttentionFn"]
+__all__ = ["segment_attention", "segment_attention_qkv", "segment_attention_forward", "segment_attention_backward",
+           "SegmentAttentionFn", "SegmentAttentionQKVFn"]
 
 MAX_HEAD_DIM = 128
 
@@ -119,10 +120,10 @@ def segment_attention_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr=None, key_
     """``egnn_attn_bwd``: returns ``(grad_q, grad_k, grad_v)`` from the forward's ``out`` and ``lse``.  ``into``: three
     tensors to write them to (parts of one buffer, say), of the inputs' shapes and dtype with 16-byte aligned
     unit-stride heads."""
-    if into is None:
-        r = _capi.ext().attn_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr, key_mask, _scale(q, scale))
-        if r is not None:
-            return r
+    r = _capi.ext().attn_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr, key_mask, _scale(q, scale),
+                                  None if into is None else list(into))
+    if r is not None:
+        return r
     kv_ptr, key_mask, scale = _defaults(q, q_ptr, kv_ptr, key_mask, scale)
     _check(q, k, v, q_ptr, kv_ptr, key_mask, scale)
     if gout.shape != q.shape or out.shape != q.shape:
@@ -171,6 +172,47 @@ class SegmentAttentionFn(torch.autograd.Function):
         q, k, v, out, lse, q_ptr, kv_ptr, key_mask = ctx.saved_tensors
         return (*segment_attention_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr, key_mask, ctx.scale), None, None,
                 None, None)
+
+
+class SegmentAttentionQKVFn(torch.autograd.Function):
+    """``out = SegmentAttentionQKVFn.apply(qkv, heads, seg_ptr, key_mask, scale)``: queries, keys and values in the rows
+    of one projection; the three gradients are written into the rows of one buffer, the projection's gradient."""
+
+    @staticmethod
+    def forward(ctx, qkv, heads, seg_ptr, key_mask, scale):
+        out, lse = segment_attention_forward(*_parts(qkv, heads), seg_ptr, None, key_mask, scale)
+        ctx.save_for_backward(qkv, out, lse, seg_ptr, key_mask)
+        ctx.heads, ctx.scale = heads, scale
+        return out
+
+    @staticmethod
+    def backward(ctx, gout):
+        qkv, out, lse, seg_ptr, key_mask = ctx.saved_tensors
+        parts = _parts(qkv, ctx.heads)
+        if qkv.shape[2] % 8:   # widths that are padded
+            grad = torch.cat(segment_attention_backward(gout, *parts, out, lse, seg_ptr, None, key_mask, ctx.scale), dim=1)
+        else:
+            grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+            segment_attention_backward(gout, *parts, out, lse, seg_ptr, None, key_mask, ctx.scale,
+                                       into=_parts(grad, ctx.heads))
+        return grad, None, None, None, None
+
+
+def _parts(qkv, heads):
+    """(q, k, v) in the rows of one projection (N, heads + 2 kv_heads, d)."""
+    if qkv.dim() != 3 or not 0 < heads < qkv.shape[1] or (qkv.shape[1] - heads) % 2:
+        raise ValueError(f"qkv must be (N, heads + 2 kv_heads, d) with {heads} heads: got {tuple(qkv.shape)}")
+    kv = (qkv.shape[1] - heads) // 2
+    return qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
+
+
+def segment_attention_qkv(qkv: torch.Tensor, heads: int, seg_ptr: torch.Tensor, key_mask: Optional[torch.Tensor] = None,
+                          scale: Optional[float] = None) -> torch.Tensor:
+    """:func:`segment_attention` of each segment over itself, with queries, keys and values in the rows of one projection:
+    ``qkv`` (N, heads + 2 kv_heads, d) -> (N, heads, d)."""
+    if torch.is_grad_enabled() and qkv.requires_grad:
+        return SegmentAttentionQKVFn.apply(qkv, heads, seg_ptr, key_mask, scale)
+    return segment_attention_forward(*_parts(qkv, heads), seg_ptr, None, key_mask, scale, need_lse=False)[0]
 
 
 def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_ptr: torch.Tensor,
