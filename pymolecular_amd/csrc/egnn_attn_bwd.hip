@@ -5,9 +5,14 @@
 // heads of the group); each sum is made by one owner in a fixed order, so there are no atomics.  That takes seven products
 // where one kernel with atomics on dq would take five.
 //
-// delta.  o is the rounded output, so in bf16 do . o is off by up to 2^-9 |do| |o|, which shows where a row has few keys.
-// As sum_j p_ij = 1, delta is also sum_j p_ij dp_ij: where a wave has all keys of its rows in one step (molecules) it
-// takes that, and reads no o; on a longer axis it starts from do . o and adds what the ds sum to before dk's kernel reads it.
+// delta.  o is the rounded output, so in bf16 do . o is off by up to 2^-9 |do| |o|, which shows in dq and dk where a row
+// has few keys that count.  As sum_j p_ij = 1, delta is also sum_j p_ij dp_ij, and the ds made with a delta' sum to
+// delta - delta'.  Short segments (below 256 rows on average) therefore get the exact one: a wave that has all keys of
+// its rows in one step (molecules) makes it from p and dp and reads no o; the 64-row workgroups also sum p_ij k_j (one
+// product more) and take (delta - delta') sum_j p_ij k_j off dq, and dk's kernel reads the corrected delta: errors of dq
+// and dk against 64 bits 2.8e-3 -> 2.4e-3 of their norm at 80 keys (2.3e-3 is what rounding ds and the result costs), for
+// 1.4 us of 50.  Longer ones keep do . o: at 512 keys the extra product would cost 5 us of 71, at D = 64 its registers
+// would spill.
 #include "egnn_attn.h"
 
 namespace egnn {
@@ -17,8 +22,9 @@ namespace attn {
 __device__ __forceinline__ float signed_c2(const Args& a) { return a.flip ? -a.c2 : a.c2; }
 __host__ __device__ __forceinline__ float signed_scale(const Args& a) { return a.flip ? -a.scale : a.scale; }
 
-// dq of the tile from virtual row vq0 of segment e on; sK, sV: tiles of the wave's (SH: the workgroup's) own
-template <typename T, int DP, int R, int W, bool SH, int KT>
+// dq of the tile from virtual row vq0 of segment e on; sK, sV: tiles of the wave's (SH: the workgroup's) own.  EX: exact
+// delta (above)
+template <typename T, int DP, int R, int W, bool SH, int KT, bool EX>
 __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, int vq0, const Seg& qs, bf16* sK, bf16* sV, int w) {
   typedef Tile<T, DP, KT> TL;
   typedef typename Num<T>::Frag Frag;
@@ -55,7 +61,7 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
   int row[R], head[R];
   bool live[R], none[R];
   float delta[R], ref[R], sum[R];
-  Sum<T> dQ[R][TL::NB];
+  Sum<T> dQ[R][TL::NB], PK[R][EX ? TL::NB : 1];   // PK: sum_j p_j k_j
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int v = v0 + 16 * r + c;
@@ -158,15 +164,16 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
             for (int i = 0; i < 4; ++i) dS[r][h][i] -= delta[r];
         }
       }
-      Frag F[R];
+      Frag F[R], FP[EX ? R : 1];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        if constexpr (EX) FP[r] = chain_frag<T>(P[r][0], P[r][1]);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             dS[r][h][i] *= P[r][h][i];
-            if constexpr (!SH) sum[r] += dS[r][h][i];
+            if constexpr (EX || !SH) sum[r] += dS[r][h][i];
           }
         F[r] = chain_frag<T>(dS[r][0], dS[r][1]);
       }
@@ -177,6 +184,7 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
         for (int r = 0; r < R; ++r) {
           if constexpr (KT == 1) dQ[r][b].one(A, F[r]);
           else dQ[r][b].add(A, F[r]);
+          if constexpr (EX) PK[r][b].add(A, FP[r]);
         }
       }
     }
@@ -190,7 +198,14 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
   const float sc = signed_scale(a);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    if (!SH && !one && a.nsplit == 1) delta[r] += col_sum(sum[r]);
+    if ((EX || !SH) && !one && a.nsplit == 1) {
+      const float off = col_sum(sum[r]);     // delta less the one that the ds were made with
+      delta[r] += off;
+      if constexpr (EX) {
+#pragma unroll
+        for (int b = 0; b < TL::NB; ++b) dQ[r][b].v -= PK[r][b].v * off;
+      }
+    }
     if (!live[r]) continue;
     if (a.delta && it.sp == 0 && g == 0) a.delta[(int64_t)head[r] * a.Nq + row[r]] = none[r] ? 0.f : delta[r];
     if (a.nsplit > 1) {
@@ -402,7 +417,7 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
   }
 }
 
-template <typename T, int DP, int R, int W, bool SH, int KT>
+template <typename T, int DP, int R, int W, bool SH, int KT, bool EX>
 __global__ __launch_bounds__(64 * W, (SH ? group_occupancy<T, DP, R>() : 1)) void dq_kernel(Args a, uint32_t n_items) {
   typedef Tile<T, DP, KT> TL;
   constexpr int BQ = 16 * R * (SH ? W : 1);
@@ -414,7 +429,7 @@ __global__ __launch_bounds__(64 * W, (SH ? group_occupancy<T, DP, R>() : 1)) voi
   Seg qs;
   const int e = find_tile<BQ>(a.q_ptr, a.B, a.Nq, a.G, a.guess, it.slot, vq0, qs);
   if (vq0 < 0) return;
-  dq_tile<T, DP, R, W, SH, KT>(a, it, e, vq0, qs, lds[SH ? 0 : w][0], lds[SH ? 0 : w][1], w);
+  dq_tile<T, DP, R, W, SH, KT, EX>(a, it, e, vq0, qs, lds[SH ? 0 : w][0], lds[SH ? 0 : w][1], w);
 }
 
 template <typename T, int DP, int R, int W, bool SH, int KT>
@@ -621,7 +636,7 @@ __global__ __launch_bounds__(64 * W, DP == 16 && W == 4 ? 4 : 1) void short_kern
     }
     for (int x = 0; x < TK && r0 + x < nv; x += 16) {
       wave_sync();
-      dq_tile<T, DP, 1, W, false, 1>(a, Item{slot, h0, 0}, e, r0 + x, own, t, t + TL::elems, 0);
+      dq_tile<T, DP, 1, W, false, 1, false>(a, Item{slot, h0, 0}, e, r0 + x, own, t, t + TL::elems, 0);
     }
     if (n_k) return;
   } else {
@@ -682,7 +697,15 @@ static void sum_parts(const float* part, int nsplit, int64_t rows, int heads, in
 template <typename T, int DP, int R, int W, bool SH, int KT>
 static void go_q(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
-  dq_kernel<T, DP, R, W, SH, KT><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
+  const uint32_t blocks = (uint32_t)(SH ? n : cdiv(n, W));
+  constexpr bool can = SH && Num<T>::planes == 1 && R == 1;
+  if constexpr (can) {
+    if (a.nsplit == 1) {
+      dq_kernel<T, DP, R, W, SH, KT, true><<<blocks, 64 * W, 0, st>>>(a, (uint32_t)n);
+      return;
+    }
+  }
+  dq_kernel<T, DP, R, W, SH, KT, false><<<blocks, 64 * W, 0, st>>>(a, (uint32_t)n);
 }
 template <typename T, int DP, int R, int W, bool SH, int KT>
 static void go_k(const Args& a, const Plan& p, hipStream_t st) {
