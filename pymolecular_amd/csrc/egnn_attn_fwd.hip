@@ -348,7 +348,7 @@ __global__ __launch_bounds__(64 * W) void short_kernel(Args a, uint32_t n_items)
 
 // Joins many splits of a row and head: their weights first, then 4 features a thread over 64 groups of splits, whose sums
 // are added in order.  16 features a block: with all of a row's in one, the few rows that are split this often kept few
-// CUs busy (24.8 us against XXX for 8 rows of 2,048 splits).
+// CUs busy (8 rows of 2,048 splits: 24.8 us against 13.3).
 constexpr int kMaxSplit = 2048;
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void fwd_join_many_kernel(Args a) {
@@ -422,7 +422,7 @@ template <typename T, int DP>
 static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
   constexpr int tile = 2 * Tile<T, DP>::elems * 2, W = 4 * tile <= 65536 ? 4 : 2 * tile <= 65536 ? 2 : 1;
   constexpr bool f32 = Num<T>::planes == 3;
-    constexpr int KT = f32 ? (DP <= 32 ? 2 : 1) : 2, KC = f32 || DP == 128 ? 1 : 2;
+  constexpr int KT = f32 ? (DP <= 32 ? 2 : 1) : 2, KC = f32 || DP == 128 ? 1 : 2;
   if constexpr (DP <= (f32 ? 32 : 64)) {
     // short segments on both axes
     if (p.form == 0 && a.nsplit == 1 && a.Nk <= kShortMean * (int64_t)(a.B > 0 ? a.B : 1)) {

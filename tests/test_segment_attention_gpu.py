@@ -309,3 +309,57 @@ def test_refusals():
         segment_attention_backward(go, q, k, v, out, lse.t(), a)
     with pytest.raises(ValueError):
         segment_attention_backward(go, q, k, v, out, lse, a, into=(torch.empty_like(q), torch.empty_like(k), torch.empty_like(q)))
+
+
+WIDE = [
+    # 128-row tiles: enough of them, or a long segment that is split; each tile ends inside, at and past its last row
+    ([260] * 60 + [256, 384, 1, 395], None, 8, 8, 64),
+    ([2100], None, 1, 1, 64),
+    ([2100], None, 2, 1, 32),
+    ([2049, 5], None, 1, 1, 16),
+    ([2085], None, 1, 1, 128),
+    ([300, 2500], [2090, 4000], 2, 2, 32),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lq,lk,hq,hk,d", WIDE)
+def test_wide_tiles(dtype, lq, lk, hq, hk, d):
+    _compare(*_case(lq, lk, hq, hk, d, dtype, seed=len(lq)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_wide_tiles_masked(dtype):
+    q, k, v, go, a, b = _case([2100, 3], None, 2, 1, 32, dtype, seed=2, lead=2, tail=40)
+    mask = torch.rand(k.shape[0], generator=torch.Generator().manual_seed(1)).cuda() < 0.5
+    mask[100:900] = False                               # whole steps of masked keys
+    mask[-43:] = False                                  # the second graph has none
+    _compare(q, k, v, go, a, b, mask)
+
+
+SHORT = [
+    # segments of up to 32 rows among longer ones, on either axis
+    ([20, 3, 150, 32, 33, 1, 0, 7] + [11] * 40, None, 4, 2, 32),
+    ([8] * 30 + [40], [20] * 30 + [90], 4, 4, 32),
+    ([12, 0, 9, 16, 17, 31], [9, 20, 0, 16, 90, 2], 4, 2, 64),
+    ([5, 8, 9, 20], [32, 33, 7, 31], 8, 2, 16),         # 4 heads a key head: 20 to 80 rows
+    ([2, 1, 30], [30, 30, 30], 3, 1, 40),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("lq,lk,hq,hk,d", SHORT)
+def test_short_segments(dtype, masked, lq, lk, hq, hk, d):
+    q, k, v, go, a, b = _case(lq, lk, hq, hk, d, dtype, seed=len(lq), lead=4, tail=50)
+    mask = torch.rand(k.shape[0], generator=torch.Generator().manual_seed(3)).cuda() < 0.6 if masked else None
+    _compare(q, k, v, go, a, b, mask)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_equal_offsets_in_two_tensors(dtype):
+    # the same segments whether the axes share their offsets or not
+    q, k, v, go, a, _ = _case([18, 25, 70, 32], None, 4, 2, 32, dtype, seed=1)
+    want, got = _both(q, k, v, go, a, a), _both(q, k, v, go, a, a.clone())
+    for x, y in zip((want[0], want[1], *want[2]), (got[0], got[1], *got[2])):
+        assert torch.equal(x, y)
