@@ -449,97 +449,100 @@ __global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_
 }
 
 // ---- short segments: one launch -------------------------------------------------------
-// A segment with at most 32 virtual rows and 32 keys (a molecule) is one wave's: its q, k, v and do are read once, its
-// gradients written once, delta is exact, and neither o nor a statistic of another launch is read.  Both orientations of
-// the scores are made from the same LDS tiles, the second for the sums over the queries.
-template <typename T, int DP>
-__device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg& qs, const Seg& ks, bf16* lds, float* sL, float* sD) {
+// A segment with at most 32 virtual rows and 32 keys (a molecule) is one wave's, or two waves' (P): its q, k, v and do are
+// read once, its gradients written once, delta is exact, and neither o nor a statistic of another launch is read.  Both
+// orientations of the scores are made from the same LDS tiles, the second for the sums over the queries.  Two waves take
+// 16 columns each, first of the queries, then of the keys.
+template <typename T, int DP, int P>
+__device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg& qs, const Seg& ks, bf16* lds, float* sL, float* sD, int w) {
   typedef Tile<T, DP> TL;
   typedef typename Num<T>::Frag Frag;
   const int l = lane_id(), c = l & 15, g = l >> 4;
   const int nv = (qs.hi - qs.lo) * a.G, nk = ks.hi - ks.lo;
   bf16 *sQ = lds, *sG = sQ + TL::elems, *sK = sG + TL::elems, *sV = sK + TL::elems;
   const int64_t e = sizeof(T);
+  const int last = a.D * (int)e;
+  uint32_t kbits;                            // keys that exist, and are not masked
   {
+    // of two waves the first brings q, do and lse, the second k and v
+    const bool bq = P == 1 || w == 0, bk = (P == 1 || w == 1) && nk;
     Stage<T, DP, 1, 64> stQ, stG, stK, stV;
-    uint32_t offQ[stQ.PER], offG[stQ.PER], offK[stQ.PER], offV[stQ.PER];
-    stK.offsets(offK, a.k_r * e, a.D);
-    stV.offsets(offV, a.v_r * e, a.D);
-    if (a.G == 1) {
-      stQ.offsets(offQ, a.q_r * e, a.D);
-      stG.offsets(offG, a.go_r * e, a.D);
-    } else {
+    float ref = INFINITY;                    // of row l
+    if (bq) {
+      uint32_t offQ[stQ.PER], offG[stQ.PER];
+      if (a.G == 1) {
+        stQ.offsets(offQ, a.q_r * e, a.D);
+        stG.offsets(offG, a.go_r * e, a.D);
+      } else {
 #pragma unroll
-      for (int p = 0; p < stQ.PER; ++p) {
-        const uint32_t u = stQ.row(p), i = a.by_g(u), h = u - i * a.G, f = stQ.feature(p);
-        const bool ok = stQ.in(p) && (int)u < nv && (int)f < a.D;
-        offQ[p] = ok ? (uint32_t)((i * a.q_r + h * a.q_h + f) * e) : kOob;
-        offG[p] = ok ? (uint32_t)((i * a.go_r + h * a.go_h + f) * e) : kOob;
+        for (int p = 0; p < stQ.PER; ++p) {
+          const uint32_t u = stQ.row(p), i = a.by_g(u), h = u - i * a.G, f = stQ.feature(p);
+          const bool ok = stQ.in(p) && (int)u < nv && (int)f < a.D;
+          offQ[p] = ok ? (uint32_t)((i * a.q_r + h * a.q_h + f) * e) : kOob;
+          offG[p] = ok ? (uint32_t)((i * a.go_r + h * a.go_h + f) * e) : kOob;
+        }
+      }
+      const int rows = qs.hi - qs.lo;
+      stQ.load(rows_buffer((const T*)a.q + qs.lo * a.q_r + (int64_t)kvh * a.G * a.q_h, rows, a.q_r * e, last + (int)((a.G - 1) * a.q_h * e)), offQ, nv);
+      stG.load(rows_buffer((const T*)a.go + qs.lo * a.go_r + (int64_t)kvh * a.G * a.go_h, rows, a.go_r * e, last + (int)((a.G - 1) * a.go_h * e)), offG, nv);
+      if (l < nv) {
+        const uint32_t i = a.by_g(l);
+        ref = a.lse[(int64_t)(kvh * a.G + (l - (int)i * a.G)) * a.Nq + qs.lo + (int)i] * kLog2e;
+        if (ref == -INFINITY) ref = INFINITY;   // a row without keys: no gradient from it or to it
       }
     }
-    const int last = a.D * (int)e, rows = qs.hi - qs.lo;
-    stQ.load(rows_buffer((const T*)a.q + qs.lo * a.q_r + (int64_t)kvh * a.G * a.q_h, rows, a.q_r * e, last + (int)((a.G - 1) * a.q_h * e)), offQ, nv);
-    stG.load(rows_buffer((const T*)a.go + qs.lo * a.go_r + (int64_t)kvh * a.G * a.go_h, rows, a.go_r * e, last + (int)((a.G - 1) * a.go_h * e)), offG, nv);
-    if (nk) {
+    if (bk) {
+      uint32_t offK[stK.PER], offV[stV.PER];
+      stK.offsets(offK, a.k_r * e, a.D);
+      stV.offsets(offV, a.v_r * e, a.D);
       stK.load(rows_buffer((const T*)a.k + ks.lo * a.k_r + kvh * a.k_h, nk, a.k_r * e, last), offK, nk);
       stV.load(rows_buffer((const T*)a.v + ks.lo * a.v_r + kvh * a.v_h, nk, a.v_r * e, last), offV, nk);
     }
-    float ref = INFINITY;                    // of row l
-    if (l < nv) {
-      const uint32_t i = a.by_g(l);
-      ref = a.lse[(int64_t)(kvh * a.G + (l - (int)i * a.G)) * a.Nq + qs.lo + (int)i] * kLog2e;
-      if (ref == -INFINITY) ref = INFINITY;  // a row without keys: no gradient from it or to it
-    }
-    bool key = l < nk;
-    if (key && a.mask) key = a.mask[ks.lo + l] != 0;
-    Bits<1> bits;
-    bits.w[0] = __ballot(ref != INFINITY);
-    if (bits.w[0] != (nv >= 32 ? 0xffffffffull : (1ull << nv) - 1)) { stQ.keep(bits); stG.keep(bits); }
-    if (a.mask) {
-      bits.w[0] = __ballot(key);
-      stK.keep(bits);
-      stV.keep(bits);
-    }
-    stQ.store(sQ, TK);
-    stG.store(sG, TK);
-    if (nk) {
-      stK.store(sK, nk);
-      stV.store(sV, nk);
-    }
-    if (l < TK) sL[l] = ref;
-  }
-  wave_sync();
-  const bool q2 = nv > 16, k2 = nk > 16;     // second blocks of 16 rows
-  const float c2 = signed_c2(a), sc = signed_scale(a);
-  bool live[2];                              // keys 16 b + c that exist, and are not masked
-  uint32_t kbits;
-  {
     bool key = l < nk;
     if (key && a.mask) key = a.mask[ks.lo + l] != 0;
     kbits = (uint32_t)__ballot(key);
-    live[0] = (kbits >> c) & 1;
-    live[1] = (kbits >> (16 + c)) & 1;
+    Bits<1> bits;
+    if (bq) {
+      bits.w[0] = __ballot(ref != INFINITY);
+      if (bits.w[0] != (nv >= 32 ? 0xffffffffull : (1ull << nv) - 1)) { stQ.keep(bits); stG.keep(bits); }
+      stQ.store(sQ, TK);
+      stG.store(sG, TK);
+      if (l < TK) sL[l] = ref;
+    }
+    if (bk) {
+      if (a.mask) {
+        bits.w[0] = kbits;
+        stK.keep(bits);
+        stV.keep(bits);
+      }
+      stK.store(sK, nk);
+      stV.store(sV, nk);
+    }
   }
+  tile_sync<(P > 1)>();
+  const bool q2 = nv > 16, k2 = nk > 16;     // second blocks of 16 rows
+  const float c2 = signed_c2(a), sc = signed_scale(a);
   // scores with the queries on the columns: delta and dq
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    if (q && !q2) break;
+  for (int q = 0; q < 2; q += P) {
+    if (P == 2) q = w;
+    if (P == 1 ? q && nv <= 16 : 16 * q >= nv) break;
     typename TL::Feat Qc[TL::NK], Gc[TL::NK];
 #pragma unroll
     for (int kk = 0; kk < TL::NK; ++kk) { Qc[kk] = TL::rows(sQ, q, kk, c, g); Gc[kk] = TL::rows(sG, q, kk, c, g); }
     const float ref = sL[16 * q + c];
-    f32x4 P[2] = {zero4(), zero4()}, dS[2] = {zero4(), zero4()};
+    f32x4 S[2] = {zero4(), zero4()}, dS[2] = {zero4(), zero4()};
     float delta = 0.f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (k ? !k2 : nk == 0) break;
-      P[k] = TL::product(sK, k, Qc, c, g, zero4());
+      S[k] = TL::product(sK, k, Qc, c, g, zero4());
       dS[k] = TL::product(sV, k, Gc, c, g, zero4());
       const uint32_t b = kbits >> (16 * k + 4 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        P[k][i] = (b >> i) & 1 ? __builtin_amdgcn_exp2f(__builtin_fmaf(P[k][i], c2, -ref)) : 0.f;
-        delta = __builtin_fmaf(P[k][i], dS[k][i], delta);
+        S[k][i] = (b >> i) & 1 ? __builtin_amdgcn_exp2f(__builtin_fmaf(S[k][i], c2, -ref)) : 0.f;
+        delta = __builtin_fmaf(S[k][i], dS[k][i], delta);
       }
     }
     delta = col_sum(delta);
@@ -547,7 +550,7 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) dS[k][i] = P[k][i] * (dS[k][i] - delta);
+      for (int i = 0; i < 4; ++i) dS[k][i] = S[k][i] * (dS[k][i] - delta);
     const Frag F = chain_frag<T>(dS[0], dS[1]);
     const int v = 16 * q + c;
     const uint32_t i = a.by_g(v);
@@ -564,29 +567,31 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     if (v < nv) store_row<TL::NB>(out, o, g, a.D);
   }
   if (nk == 0) return;
-  wave_sync();
+  tile_sync<(P > 1)>();
   // and with the keys on the columns: dk and dv
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (k && !k2) break;
+  for (int k = 0; k < 2; k += P) {
+    if (P == 2) k = w;
+    if (P == 1 ? k && nk <= 16 : 16 * k >= nk) break;
     typename TL::Feat Kc[TL::NK], Vc[TL::NK];
 #pragma unroll
     for (int kk = 0; kk < TL::NK; ++kk) { Kc[kk] = TL::rows(sK, k, kk, c, g); Vc[kk] = TL::rows(sV, k, kk, c, g); }
-    f32x4 P[2] = {zero4(), zero4()}, dS[2] = {zero4(), zero4()};
+    f32x4 S[2] = {zero4(), zero4()}, dS[2] = {zero4(), zero4()};
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       if (q && !q2) break;
       const f32x4 Lr = load4_f32(sL + 16 * q + 4 * g), nD = load4_f32(sD + 16 * q + 4 * g);
-      P[q] = TL::product(sQ, q, Kc, c, g, zero4());
+      S[q] = TL::product(sQ, q, Kc, c, g, zero4());
       dS[q] = TL::product(sG, q, Vc, c, g, nD);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        P[q][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[q][i], c2, -Lr[i]));
-        dS[q][i] *= P[q][i];
+        S[q][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][i], c2, -Lr[i]));
+        dS[q][i] *= S[q][i];
       }
     }
-    const Frag FP = chain_frag<T>(P[0], P[1]), FS = chain_frag<T>(dS[0], dS[1]);
-    const int key = ks.lo + 16 * k + c;
+    const Frag FP = chain_frag<T>(S[0], S[1]), FS = chain_frag<T>(dS[0], dS[1]);
+    const int key0 = 16 * k + c;
+    const bool live = (kbits >> key0) & 1;
     f32x4 ok[TL::NB], ov[TL::NB];
 #pragma unroll
     for (int b = 0; b < TL::NB; ++b) {
@@ -597,28 +602,39 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
       dK.add(TL::cols(sQ, 0, b, c, g), FS);
       dK.end();
       dV.end();
-      ok[b] = live[k] ? dK.v * sc : zero4();
-      ov[b] = live[k] ? dV.v : zero4();
+      ok[b] = live ? dK.v * sc : zero4();
+      ov[b] = live ? dV.v : zero4();
     }
-    if (16 * k + c < nk) {
-      store_row<TL::NB>((T*)a.gk + key * a.gk_r + kvh * a.gk_h, ok, g, a.D);
-      store_row<TL::NB>((T*)a.gv + key * a.gv_r + kvh * a.gv_h, ov, g, a.D);
+    if (key0 < nk) {
+      store_row<TL::NB>((T*)a.gk + (ks.lo + key0) * a.gk_r + kvh * a.gk_h, ok, g, a.D);
+      store_row<TL::NB>((T*)a.gv + (ks.lo + key0) * a.gv_r + kvh * a.gv_h, ov, g, a.D);
     }
   }
 }
 
 // Items 0 .. n_q - 1: a tile of 32 virtual rows and a key head: the whole segment where it is small, else its dq (and with
 // n_k = 0, where queries and keys are the same rows, the dk and dv of those).  The others: a tile of 32 keys and heads_per
-// key heads, their dk and dv where the segment is not small.
-template <typename T, int DP, int W>
-__global__ __launch_bounds__(64 * W, DP == 16 && W == 4 ? 4 : 1) void short_kernel(Args a, uint32_t n_q, uint32_t n_k, uint32_t slots_k,
+// key heads, their dk and dv where the segment is not small.  P waves an item, W a workgroup.
+//
+// Waves a SIMD that its registers leave room for: the tiles of long segments would take those of two or three waves, where
+// the small segments, which are most, gain by four or five (left to the compiler and as here: bf16, D = 32, 4,000 segments
+// of 2 .. 10 rows 32.6 and 23.9 us; D = 16, 1,024 molecules and 8 heads 15.7 and 14.6; fp32, D = 16, 2,000 segments and 8
+// heads 58 and 52; the other widths spill in the small segments or have no room for more in LDS).
+template <typename T, int DP> constexpr int short_occupancy() {
+  return Num<T>::planes == 1 ? (DP == 16 ? 5 : DP == 32 ? 3 : 1) : DP == 16 ? 4 : 1;
+}
+template <typename T, int DP, int P, int W>
+__global__ __launch_bounds__(64 * W, (short_occupancy<T, DP>())) void short_kernel(Args a, uint32_t n_q, uint32_t n_k, uint32_t slots_k,
                                                                                    Div by_heads_k, int heads_per) {
   typedef Tile<T, DP> TL;
-  __shared__ __attribute__((aligned(16))) bf16 lds[W][4][TL::elems];
+  static_assert(P == 1 || W == P, "");
+  __shared__ __attribute__((aligned(16))) bf16 lds[W / P][4][TL::elems];
   __shared__ __attribute__((aligned(16))) float stat[W][2][TK];
-  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  uint32_t i = xcd_order(blockIdx.x, gridDim.x) * W + w;
-  bf16* t = lds[w][0];
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), x0 = P == 2 ? 16 * w : 0;
+  uint32_t i = xcd_order(blockIdx.x, gridDim.x);
+  if (P == 1) i = i * W + w;
+  bf16* t = lds[P == 1 ? w : 0][0];
+  bf16* t2 = P == 1 ? t : lds[0][2 * w];     // of a wave by itself
   Seg own;
   int r0, e, h0, h1;
   // tiles of 16 where the segment is not small: of 32 rows the registers would cost waves
@@ -631,12 +647,12 @@ __global__ __launch_bounds__(64 * W, DP == 16 && W == 4 ? 4 : 1) void short_kern
     const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk, a.same, own);
     const int nv = (own.hi - own.lo) * a.G;
     if (nv <= TK && ks.hi - ks.lo <= TK && (n_k || (e >= 1 && e <= a.B))) {   // (keys outside every segment: zeros, below)
-      small_segment<T, DP>(a, h0, own, ks, t, stat[w][0], stat[w][1]);
+      small_segment<T, DP, P>(a, h0, own, ks, t, stat[P == 1 ? w : 0][0], stat[P == 1 ? w : 0][1], w);
       return;
     }
-    for (int x = 0; x < TK && r0 + x < nv; x += 16) {
+    for (int x = x0; x < TK && r0 + x < nv; x += 16 * P) {
       wave_sync();
-      dq_tile<T, DP, 1, W, false, 1, false>(a, Item{slot, h0, 0}, e, r0 + x, own, t, t + TL::elems, 0);
+      dq_tile<T, DP, 1, W, false, 1, false>(a, Item{slot, h0, 0}, e, r0 + x, own, t2, t2 + TL::elems, 0);
     }
     if (n_k) return;
   } else {
@@ -649,12 +665,12 @@ __global__ __launch_bounds__(64 * W, DP == 16 && W == 4 ? 4 : 1) void short_kern
     if (r0 < 0) return;
     const Seg qs = other_rows(a.q_ptr, e, a.B, a.Nq, a.same, own);
     const int nv = (qs.hi - qs.lo) * a.G;
-    if (nv >= 1 && nv <= TK && own.hi - own.lo <= TK) return;   // a query's wave has it
+    if (nv >= 1 && nv <= TK && own.hi - own.lo <= TK) return;   // a query's item has it
   }
   for (int h = h0; h < h1; ++h)
-    for (int x = 0; x < TK && r0 + x < own.hi - own.lo; x += 16) {
+    for (int x = x0; x < TK && r0 + x < own.hi - own.lo; x += 16 * P) {
       wave_sync();
-      dkv_tile<T, DP, 1, W, false, 1, true>(a, Item{0, h, 0}, e, r0 + x, own, t, t + TL::elems, stat[w][0], stat[w][1], 0);
+      dkv_tile<T, DP, 1, W, false, 1, true>(a, Item{0, h, 0}, e, r0 + x, own, t2, t2 + TL::elems, stat[w][0], stat[w][1], 0);
     }
 }
 
@@ -719,7 +735,6 @@ static bool launch_short(Args a, const Plan& pq, const Plan& pk, hipStream_t st)
   if constexpr (DP > (f32 ? 32 : 64)) return false;
   else {
     if (pq.form != 0 || pk.form != 0 || pq.nsplit > 1 || pk.nsplit > 1 || !a.Nq || !a.Nk) return false;
-    constexpr int tile = 4 * Tile<T, DP>::elems * 2, W = 4 * tile <= 65536 ? 4 : 2;
     const int64_t sq = ((int64_t)a.Nq * a.G) / TK + a.B + 2, sk = a.Nk / TK + a.B + 2;
     const int per = sk >= 1024 ? a.Hkv : 1;
     const int64_t nq = sq * a.Hkv, nk = a.same && a.G == 1 ? 0 : sk * (a.Hkv / per);
@@ -728,7 +743,13 @@ static bool launch_short(Args a, const Plan& pq, const Plan& pk, hipStream_t st)
     a.nsplit = 1;
     a.slots = (uint32_t)sq;
     a.guess = (float)(a.B + 2) / (float)sq;
-    short_kernel<T, DP, W><<<(uint32_t)cdiv(nq + nk, W), 64 * W, 0, st>>>(a, (uint32_t)nq, (uint32_t)nk, (uint32_t)sk, Div::of(a.Hkv / per), per);
+    constexpr int tile = 4 * Tile<T, DP>::elems * 2, W = 4 * tile <= 65536 ? 4 : 2;
+    const Div by = Div::of(a.Hkv / per);
+    // Two waves a segment in fp32, whose products are six (one and two waves, 10 .. 30 rows a segment, D = 32, 4 heads: 27
+    // and 18 us for 512 segments, 165 and 101 for 4,000); not in bf16 (4,000 segments: 46 and 44; D = 64: 78 and 85;
+    // D = 16, 1,024 molecules and 8 heads: 15.6 and 19).
+    if constexpr (f32) short_kernel<T, DP, 2, 2><<<(uint32_t)(nq + nk), 128, 0, st>>>(a, (uint32_t)nq, (uint32_t)nk, (uint32_t)sk, by, per);
+    else short_kernel<T, DP, 1, W><<<(uint32_t)cdiv(nq + nk, W), 64 * W, 0, st>>>(a, (uint32_t)nq, (uint32_t)nk, (uint32_t)sk, by, per);
     return true;
   }
 }

@@ -227,55 +227,61 @@ __global__ __launch_bounds__(64 * W, (SH ? group_occupancy<T, DP, R>() : 1)) voi
   fwd_tile<T, DP, R, W, SH, KT, KC>(a, it, e, vq0, qs, lds[SH ? 0 : w][0], lds[SH ? 0 : w][1], w);
 }
 
-// A segment with at most 32 virtual rows and 32 keys (a molecule): one wave, each row of q, k and v read once, in rows as
-// they lie, and one softmax over all keys.
-template <typename T, int DP>
-__device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg& qs, const Seg& ks, bf16* lds) {
+// A segment with at most 32 virtual rows and 32 keys (a molecule): each row of q, k and v read once, in rows as they lie,
+// and one softmax over all keys.  One wave, or two (P) with 16 virtual rows each.
+template <typename T, int DP, int P>
+__device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg& qs, const Seg& ks, bf16* lds, int w) {
   typedef Tile<T, DP> TL;
   typedef typename Num<T>::Frag Frag;
   const int l = lane_id(), c = l & 15, g = l >> 4;
   const int nv = (qs.hi - qs.lo) * a.G, nk = ks.hi - ks.lo;
   bf16 *sQ = lds, *sK = sQ + TL::elems, *sV = sK + TL::elems;
   const int64_t e = sizeof(T);
+  const int last = a.D * (int)e;
   uint32_t kbits;
   {
+    // of two waves the first brings q, the second k and v
+    const bool bq = P == 1 || w == 0, bk = (P == 1 || w == 1) && nk;
     Stage<T, DP, 1, 64> stQ, stK, stV;
-    uint32_t offQ[stQ.PER], offK[stQ.PER], offV[stQ.PER];
-    stK.offsets(offK, a.k_r * e, a.D);
-    stV.offsets(offV, a.v_r * e, a.D);
-    if (a.G == 1) stQ.offsets(offQ, a.q_r * e, a.D);
-    else {
+    if (bq) {
+      uint32_t offQ[stQ.PER];
+      if (a.G == 1) stQ.offsets(offQ, a.q_r * e, a.D);
+      else {
 #pragma unroll
-      for (int p = 0; p < stQ.PER; ++p) {
-        const uint32_t u = stQ.row(p), i = a.by_g(u), h = u - i * a.G, f = stQ.feature(p);
-        offQ[p] = stQ.in(p) && (int)u < nv && (int)f < a.D ? (uint32_t)((i * a.q_r + h * a.q_h + f) * e) : kOob;
+        for (int p = 0; p < stQ.PER; ++p) {
+          const uint32_t u = stQ.row(p), i = a.by_g(u), h = u - i * a.G, f = stQ.feature(p);
+          offQ[p] = stQ.in(p) && (int)u < nv && (int)f < a.D ? (uint32_t)((i * a.q_r + h * a.q_h + f) * e) : kOob;
+        }
       }
+      stQ.load(rows_buffer((const T*)a.q + qs.lo * a.q_r + (int64_t)kvh * a.G * a.q_h, qs.hi - qs.lo, a.q_r * e, last + (int)((a.G - 1) * a.q_h * e)), offQ, nv);
     }
-    const int last = a.D * (int)e;
-    stQ.load(rows_buffer((const T*)a.q + qs.lo * a.q_r + (int64_t)kvh * a.G * a.q_h, qs.hi - qs.lo, a.q_r * e, last + (int)((a.G - 1) * a.q_h * e)), offQ, nv);
-    if (nk) {
+    if (bk) {
+      uint32_t offK[stK.PER], offV[stV.PER];
+      stK.offsets(offK, a.k_r * e, a.D);
+      stV.offsets(offV, a.v_r * e, a.D);
       stK.load(rows_buffer((const T*)a.k + ks.lo * a.k_r + kvh * a.k_h, nk, a.k_r * e, last), offK, nk);
       stV.load(rows_buffer((const T*)a.v + ks.lo * a.v_r + kvh * a.v_h, nk, a.v_r * e, last), offV, nk);
     }
     bool key = l < nk;
     if (key && a.mask) key = a.mask[ks.lo + l] != 0;
     kbits = (uint32_t)__ballot(key);
-    if (a.mask) {                            // what a masked value holds must not meet a probability of 0
-      Bits<1> bits;
-      bits.w[0] = kbits;
-      stV.keep(bits);
-    }
-    stQ.store(sQ, TK);
-    if (nk) {
+    if (bq) stQ.store(sQ, TK);
+    if (bk) {
+      if (a.mask) {                          // what a masked value holds must not meet a probability of 0
+        Bits<1> bits;
+        bits.w[0] = kbits;
+        stV.keep(bits);
+      }
       stK.store(sK, nk);
       stV.store(sV, nk);
     }
   }
-  wave_sync();
+  tile_sync<(P > 1)>();
   const float c2 = a.flip ? -a.c2 : a.c2;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    if (q && nv <= 16) break;
+  for (int q = 0; q < 2; q += P) {
+    if (P == 2) q = w;
+    if (P == 1 ? q && nv <= 16 : 16 * q >= nv) break;
     typename TL::Feat Qc[TL::NK];
 #pragma unroll
     for (int kk = 0; kk < TL::NK; ++kk) Qc[kk] = TL::rows(sQ, q, kk, c, g);
@@ -301,7 +307,7 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
         for (int i = 0; i < 4; ++i) { S[k][i] = __builtin_amdgcn_exp2f(S[k][i] - m); sum += S[k][i]; }
       }
     sum = col_sum(sum);
-    const Frag P = chain_frag<T>(S[0], S[1]);
+    const Frag F = chain_frag<T>(S[0], S[1]);
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     const int v = 16 * q + c;
     const uint32_t i = a.by_g(v);
@@ -312,7 +318,7 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     for (int b = 0; b < TL::NB; ++b) {
       Sum<T> O;
       O.begin();
-      if (nk) O.add(TL::cols(sV, 0, b, c, g), P);
+      if (nk) O.add(TL::cols(sV, 0, b, c, g), F);
       O.end();
       o[b] = O.v * inv;
     }
@@ -322,13 +328,14 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
   }
 }
 
-// Tiles of 32 virtual rows, a wave each: the whole segment where it is small
-template <typename T, int DP, int W>
+// Tiles of 32 virtual rows, P waves each and W a workgroup: the whole segment where it is small
+template <typename T, int DP, int P, int W>
 __global__ __launch_bounds__(64 * W) void short_kernel(Args a, uint32_t n_items) {
   typedef Tile<T, DP> TL;
-  __shared__ __attribute__((aligned(16))) bf16 lds[W][3][TL::elems];
+  static_assert(P == 1 || W == P, "");
+  __shared__ __attribute__((aligned(16))) bf16 lds[W / P][P == 1 ? 3 : 4][TL::elems];
   Item it;
-  if (!item_of<W, false>(a, n_items, it)) return;
+  if (!item_of<W, (P > 1)>(a, n_items, it)) return;
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   int vq0;
   Seg qs;
@@ -337,12 +344,13 @@ __global__ __launch_bounds__(64 * W) void short_kernel(Args a, uint32_t n_items)
   const Seg ks = other_rows(a.kv_ptr, e, a.B, a.Nk, a.same, qs);
   const int nv = (qs.hi - qs.lo) * a.G;
   if (nv <= TK && ks.hi - ks.lo <= TK) {
-    small_segment<T, DP>(a, it.kvh, qs, ks, lds[w][0]);
+    small_segment<T, DP, P>(a, it.kvh, qs, ks, lds[P == 1 ? w : 0][0], w);
     return;
   }
-  for (int x = 0; x < TK && vq0 + x < nv; x += 16) {
+  bf16* t = P == 1 ? lds[w][0] : lds[0][2 * w];   // of a wave by itself
+  for (int x = P == 2 ? 16 * w : 0; x < TK && vq0 + x < nv; x += 16 * P) {
     wave_sync();
-    fwd_tile<T, DP, 1, W, false, 1, 1>(a, it, e, vq0 + x, qs, lds[w][0], lds[w][1], 0);
+    fwd_tile<T, DP, 1, W, false, 1, 1>(a, it, e, vq0 + x, qs, t, t + TL::elems, 0);
   }
 }
 
@@ -430,9 +438,12 @@ static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
       Args x = a;
       const int64_t slots = (int64_t)a.Nq * a.G / TK + a.B + 2, n = slots * a.Hkv;
       x.slots = (uint32_t)slots;
-      x.by_slots = Div::of(x.slots);
       x.guess = (float)(a.B + 2) / (float)slots;
-      short_kernel<T, DP, W3><<<(uint32_t)cdiv(n, W3), 64 * W3, 0, st>>>(x, (uint32_t)n);
+      x.by_slots = Div::of(x.slots);
+      // Two waves a segment where its products take long (one and two waves, 10 .. 30 rows a segment, 4 heads: fp32, D = 32,
+      // 4,000 segments 59 and 51 us; bf16, D = 64 41 and 32), not where they do not (bf16, D = 32: 18.6 and 20.6)
+      if constexpr (f32 || DP == 64) short_kernel<T, DP, 2, 2><<<(uint32_t)n, 128, 0, st>>>(x, (uint32_t)n);
+      else short_kernel<T, DP, 1, W3><<<(uint32_t)cdiv(n, W3), 64 * W3, 0, st>>>(x, (uint32_t)n);
       return (int)hipGetLastError();
     }
   }
