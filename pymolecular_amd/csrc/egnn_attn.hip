@@ -13,7 +13,7 @@ bool dims_ok(const EgnnAttnDims* d) {
 }
 
 // own: (virtual) rows of the axis that is cut into tiles, other: rows of the axis a tile walks
-Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest) {
+Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest, bool f32, int D) {
   const int64_t segs = n_seg > 0 ? n_seg : 1, mean = own / segs, len = other / segs;
   auto items_of = [&](int64_t rows) {
     const int64_t tiles = cdiv(own, rows) > n_seg ? cdiv(own, rows) : n_seg;
@@ -32,12 +32,22 @@ Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest)
   p.slots = own / BQ + n_seg + 2;
   const int64_t items = items_of(BQ);
   p.nsplit = 1;
-  const int64_t want = p.form == 0 ? 4096 : 1024;
-  if (items < want / 2 && len >= 512) {
-    int64_t n = cdiv(want, items);
-    if (n > len / 128) n = len / 128;
-    p.nsplit = (int)(n < 2048 ? n : 2048);
+  if (p.form == 0) {
+    if (items < 2048 && len >= 512) p.nsplit = (int)cdiv(4096, items);
+  } else if (items < 512 && len >= 512) {
+    // Somewhat more workgroups a CU than it holds (four of heads up to 32 wide) and up to six, as evenly on the 256 CUs as
+    // may be; a part more costs its share of the joining, per tile about the time of 256 rows in bf16 and 48 in fp32.
+    // (As against 1,024 workgroups or the next number above, forward and backward: one graph of 2,500 rows, 8 heads, 164
+    // and 135 us; of 20,000, 2 heads on 1, 1,096 and 1,044.  Fewer for heads up to 32 wide: 8,000 rows, 8 heads on 2, dk
+    // and dv 182 us in 9 parts and 200 in 8.)
+    double best = 0.;
+    for (int64_t n = cdiv(D <= 32 ? 1100 : 640, items); n <= cdiv(1536, items); ++n) {
+      const double x = (double)(items * n) / 256., cost = (double)cdiv(items * n, 256) / x + (double)(n * (f32 ? 48 : 256)) / (double)len;
+      if (p.nsplit == 1 || cost < best) { best = cost; p.nsplit = (int)n; }
+    }
   }
+  if (p.nsplit > len / 128) p.nsplit = (int)(len / 128 > 0 ? len / 128 : 1);
+  if (p.nsplit > 2048) p.nsplit = 2048;
   return p;
 }
 // The widest form whose registers hold the tile without spills; -1: form 1 alone
@@ -45,8 +55,8 @@ int widest_q(const EgnnAttnDims* d) { return d->dtype == EGNN_F32 && d->D > 64 ?
 int widest_k(const EgnnAttnDims* d) {
   return d->dtype == EGNN_F32 && d->D > 64 ? -1 : d->D > (d->dtype == EGNN_F32 ? 32 : 64) ? 1 : 2;
 }
-Plan plan_q(const EgnnAttnDims* d) { return make_plan(d->Nq * (d->Hq / d->Hkv), d->Nk, d->n_seg, d->Hkv, widest_q(d)); }
-Plan plan_k(const EgnnAttnDims* d) { return make_plan(d->Nk, d->Nq * (d->Hq / d->Hkv), d->n_seg, d->Hkv, widest_k(d)); }
+Plan plan_q(const EgnnAttnDims* d) { return make_plan(d->Nq * (d->Hq / d->Hkv), d->Nk, d->n_seg, d->Hkv, widest_q(d), d->dtype == EGNN_F32, d->D); }
+Plan plan_k(const EgnnAttnDims* d) { return make_plan(d->Nk, d->Nq * (d->Hq / d->Hkv), d->n_seg, d->Hkv, widest_k(d), d->dtype == EGNN_F32, d->D); }
 
 size_t fwd_bytes(const EgnnAttnDims* d) {
   const Plan p = plan_q(d);

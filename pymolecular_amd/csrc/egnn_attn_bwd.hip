@@ -706,7 +706,10 @@ template <typename T>
 static void sum_parts(const float* part, int nsplit, int64_t rows, int heads, int D, int DP, Out<T> one, Out<T> two, hipStream_t st) {
   const int64_t n = rows * heads * (D / 4);
   const int outs = two.p ? 2 : 1, width = outs * DP;
+  // (17 .. 128 parts in 32 groups, 128 bytes of a part at a time: 44.8 us where 8 groups take
+  // 8.6, 3 graphs of 1,000 to 1,400 rows, 8 heads on 2)
   if (nsplit <= 16) sum_parts_kernel<T, 1><<<dim3((uint32_t)cdiv(n, 256), outs), 256, 0, st>>>(part, nsplit, rows, heads, D, DP, width, one, two);
+  else if (nsplit <= 128) sum_parts_kernel<T, 8><<<dim3((uint32_t)cdiv(n, 32), outs), 256, 0, st>>>(part, nsplit, rows, heads, D, DP, width, one, two);
   else sum_parts_kernel<T, 32><<<dim3((uint32_t)cdiv(n, 8), outs), 256, 0, st>>>(part, nsplit, rows, heads, D, DP, width, one, two);
 }
 

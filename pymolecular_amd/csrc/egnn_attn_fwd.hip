@@ -397,7 +397,7 @@ __global__ __launch_bounds__(256) void fwd_join_many_kernel(Args a) {
   if (f < a.D) store4((T*)a.out + row * a.o_r + head * a.o_h + f, part[0][t & 3] * inv);
   if (a.lse && t == 0 && blockIdx.y == 0) a.lse[(int64_t)head * a.Nq + row] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
-// Joins few splits: 4 features a thread
+// Joins few splits, or those of many rows: 4 features a thread
 constexpr int kFewSplits = 16;
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
@@ -452,7 +452,7 @@ static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
   else if (p.form == 1) go<T, DP, 1, 4, true, f32 ? KT : 1, 1>(a, p, st);
   else go<T, DP, 2, 4, true, KT, KC>(a, p, st);
   const int64_t rows = (int64_t)a.Nq * a.Hq;
-  if (a.nsplit > kFewSplits) fwd_join_many_kernel<T, DP><<<dim3((uint32_t)rows, DP / 16), 256, 0, st>>>(a);
+  if (a.nsplit > kFewSplits && rows * (DP / 4) < 65536) fwd_join_many_kernel<T, DP><<<dim3((uint32_t)rows, DP / 16), 256, 0, st>>>(a);
   else if (a.nsplit > 1) fwd_join_kernel<T, DP><<<(uint32_t)cdiv(rows * (DP / 4), 256), 256, 0, st>>>(a);
   return (int)hipGetLastError();
 }

@@ -363,3 +363,12 @@ def test_equal_offsets_in_two_tensors(dtype):
     want, got = _both(q, k, v, go, a, a), _both(q, k, v, go, a, a.clone())
     for x, y in zip((want[0], want[1], *want[2]), (got[0], got[1], *got[2])):
         assert torch.equal(x, y)
+
+
+MANY_PARTS = [([1100, 1300], None, 4, 1, 64), ([2000], None, 2, 1, 32), ([700], [1500], 1, 1, 24)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lq,lk,hq,hk,d", MANY_PARTS)
+def test_many_rows_in_many_parts(dtype, lq, lk, hq, hk, d):
+    _compare(*_case(lq, lk, hq, hk, d, dtype, seed=len(lq)))
