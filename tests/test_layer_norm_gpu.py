@@ -189,3 +189,16 @@ def test_refusals():
         layer_norm_backward(gy[:5], s, w, mean, rstd)
     with pytest.raises(ValueError):
         layer_norm_backward(gy, s, w, mean[:5], rstd)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,c", [(70001, 42), (66003, 91), (65601, 165), (65541, 331), (65536, 160)])
+def test_many_rows_of_odd_widths(n, c, dtype):
+    # a row's last piece overlaps the one before; many rows take three pieces a lane
+    _compare(*_inputs(n, c, dtype, n % 2 == 0, seed=c))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("c", [1, 3, 4, 7, 8, 9, 15, 31, 33, 255, 257, 511, 513])
+def test_widths_around_a_piece(c, dtype):
+    _compare(*_inputs(37, c, dtype, True, seed=c))
