@@ -376,7 +376,8 @@ typedef struct EgnnNormDims {
 } EgnnNormDims;
 
 /* Writes y (N, C) and, with a residual, s (N, C) to `sum` (both contiguous);
- * mean and rstd (N each; of the sum as it is stored) for the backward, or both NULL. */
+ * mean and rstd (N each; of the sum as it is stored where the
+ * two differ) for the backward, or both NULL. */
 int32_t egnn_norm_fwd(const EgnnNormDims* dims, const void* x, int64_t ldx, const void* residual, int64_t ldr,
                       const void* weight, const void* bias, void* y, void* sum, float* mean, float* rstd, void* stream);
 size_t egnn_norm_bwd_workspace_bytes(const EgnnNormDims* dims);

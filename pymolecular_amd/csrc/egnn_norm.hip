@@ -5,8 +5,9 @@
 // blocks walk the rows with a fixed stride; a lane keeps the sums of gw and gb of its columns in fp32 registers, a
 // block's row groups are joined in LDS and its sums leave as one partial row, which a second launch adds up in order.
 // y is made from the sum as it is, before it is rounded to the type it is stored in.  The backward reads the stored one, so
-// the statistics kept for it are those of the stored one: with the others a row whose values differ by less than their
-// rounding would get any gradient (one column of bf16: hundreds of times too large, instead of 0).
+// where the mean exceeds the deviation the statistics kept for it are those of the stored one: with the others a row whose
+// values differ by less than their rounding would get any gradient (one column of bf16: hundreds of times too large, instead
+// of 0).  Elsewhere the two agree to 2^-9 of the deviation.  (For every row: 402 us instead of 360, 2,000,000 x 128 bf16.)
 #include "egnn_device.h"
 #include "egnn_internal.h"
 #include <type_traits>
@@ -143,7 +144,13 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
   stats(std::false_type{}, mean, rstd);
   if (a.mean) {
     float m = mean, rs = rstd;
-    if (sizeof(T) == 2 && a.r) stats(std::true_type{}, m, rs);
+    if (sizeof(T) == 2 && a.r) {
+      const bool far = mean * mean * rstd * rstd > 1.f;
+      if (__ballot(far)) {
+        stats(std::true_type{}, m, rs);
+        if (!far) { m = mean; rs = rstd; }
+      }
+    }
     if (live && lane == 0) { a.mean[n] = m; a.rstd[n] = rs; }
   }
   if (!live) return;
@@ -285,7 +292,7 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
   stats(false, mean, rstd);
   if (a.mean) {
     float m = mean, rs = rstd;
-    if (sizeof(T) == 2 && r) stats(true, m, rs);
+    if (sizeof(T) == 2 && r && mean * mean * rstd * rstd > 1.f) stats(true, m, rs);
     if (threadIdx.x == 0) { a.mean[n] = m; a.rstd[n] = rs; }
   }
   for (int f = threadIdx.x; f < a.C; f += NT) {

@@ -43,7 +43,7 @@ def _check(x, weight, bias, residual, eps):
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, need_stats=True):
     """``egnn_norm_fwd``: returns ``(y, s, mean, rstd)``; ``s`` is ``x`` itself without a residual, ``mean`` and
-    ``rstd`` (rows,) float32 are those of ``s`` as it is stored, for :func:`layer_norm_backward` (None where
+    ``rstd`` (rows,) float32 are what :func:`layer_norm_backward` needs, of ``s`` as it is stored (None where
     ``need_stats`` is false)."""
     r = _capi.ext().norm_forward(x, weight, bias, eps, residual, need_stats)
     if r is not None:
