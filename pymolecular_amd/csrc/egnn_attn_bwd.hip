@@ -13,6 +13,10 @@
 // and dk against 64 bits 2.8e-3 -> 2.4e-3 of their norm at 80 keys (2.3e-3 is what rounding ds and the result costs), for
 // 1.4 us of 50.  Longer ones keep do . o: at 512 keys the extra product would cost 5 us of 71, at D = 64 its registers
 // would spill.
+//
+// Measured: 12,289 rows, 4 heads of 64, bf16, dq 240 us and dk, dv 337 us, 0.97 and 0.92 PFLOP/s of the products they make
+// (three and four), bound by vector and MFMA issue (0.43 and 0.41, 0.36 and 0.38 of the cycles) and, of dk and dv, by two
+// waves a SIMD; 128 molecules in fp32 8.2 us, bound by latency.
 #include "egnn_attn.h"
 
 namespace egnn {

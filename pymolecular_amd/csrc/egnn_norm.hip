@@ -8,6 +8,9 @@
 // where the mean exceeds the deviation the statistics kept for it are those of the stored one: with the others a row whose
 // values differ by less than their rounding would get any gradient (one column of bf16: hundreds of times too large, instead
 // of 0).  Elsewhere the two agree to 2^-9 of the deviation.  (For every row: 402 us instead of 360, 2,000,000 x 128 bf16.)
+// Bound by HBM where the tensors are large: 2,000,000 x 128 bf16 with a residual, forward 358 us and backward 341 us, 5.7 and
+// 6.0 TB/s; 40,961 x 259 fp32, rows that cross lines, 4.0 and 4.6 TB/s.  By its launches where they are small: 2,432 x 128
+// fp32, forward, 3.0 us.
 #include "egnn_device.h"
 #include "egnn_internal.h"
 #include <type_traits>
