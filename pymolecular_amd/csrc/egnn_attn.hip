@@ -40,10 +40,12 @@ Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest,
     // (As against 1,024 workgroups or the next number above, forward and backward: one graph of 2,500 rows, 8 heads, 164
     // and 135 us; of 20,000, 2 heads on 1, 1,096 and 1,044.  Fewer for heads up to 32 wide: 8,000 rows, 8 heads on 2, dk
     // and dv 182 us in 9 parts and 200 in 8.)
+    const int64_t most = len / 128, hi = cdiv(1536, items) < most ? cdiv(1536, items) : most;
+    const int64_t want = cdiv(D <= 32 ? 1100 : 640, items), lo = want < hi ? want : hi;
     double best = 0.;
-    for (int64_t n = cdiv(D <= 32 ? 1100 : 640, items); n <= cdiv(1536, items); ++n) {
+    for (int64_t n = lo; n <= hi; n += 1 + lo / 64) {   // at most some hundred
       const double x = (double)(items * n) / 256., cost = (double)cdiv(items * n, 256) / x + (double)(n * (f32 ? 48 : 256)) / (double)len;
-      if (p.nsplit == 1 || cost < best) { best = cost; p.nsplit = (int)n; }
+      if (n == lo || cost < best) { best = cost; p.nsplit = (int)n; }
     }
   }
   if (p.nsplit > len / 128) p.nsplit = (int)(len / 128 > 0 ? len / 128 : 1);
