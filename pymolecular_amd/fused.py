@@ -21,6 +21,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 from ._capi import EgnnDims, EgnnStrides, check
@@ -36,6 +37,17 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 def _stream(device: torch.device) -> int:
     """The raw handle of the device's current stream (the library's kernels are enqueued on it)."""
     return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
+
+
+def _recorded(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether something has to see a call on these tensors: autograd, a tracer (which would record the allocation of the
+    result and not the library's work) or forward-mode differentiation (whose tangents the library does not know).  Such a
+    call goes through the operator's autograd function, which a trace calls again and which refuses a tangent."""
+    if torch.jit.is_tracing():
+        return True
+    grad = torch.is_grad_enabled()
+    return any(t is not None and ((grad and t.requires_grad) or forward_ad.unpack_dual(t).tangent is not None)
+               for t in tensors)
 
 
 def _require_device(t: torch.Tensor, name: str) -> None:

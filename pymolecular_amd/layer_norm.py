@@ -15,7 +15,7 @@ import torch
 
 from . import _capi
 from ._capi import EgnnNormDims, check
-from .fused import _as, _dtype_code, _ptr, _stream
+from .fused import _as, _dtype_code, _ptr, _recorded, _stream
 
 __all__ = ["layer_norm", "layer_norm_forward", "layer_norm_backward", "LayerNormFn"]
 
@@ -130,7 +130,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5, residual: Optional[torch.Tensor] = None):
     """``y``, or ``(y, x + residual)`` with a residual (module docstring).  Differentiable in x, weight, bias and
     residual."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _recorded(x, weight, bias, residual):
         return LayerNormFn.apply(x, weight, bias, eps, residual)
     y, s, _, _ = layer_norm_forward(x, weight, bias, eps, residual, need_stats=False)
     return y if residual is None else (y, s)

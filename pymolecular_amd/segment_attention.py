@@ -20,7 +20,7 @@ import torch
 
 from . import _capi
 from ._capi import EgnnAttnDims, EgnnAttnStrides, check
-from .fused import _dtype_code, _ptr, _stream
+from .fused import _dtype_code, _ptr, _recorded, _stream
 
 __all__ = ["segment_attention", "segment_attention_qkv", "segment_attention_forward", "segment_attention_backward",
            "SegmentAttentionFn", "SegmentAttentionQKVFn"]
@@ -210,7 +210,7 @@ def segment_attention_qkv(qkv: torch.Tensor, heads: int, seg_ptr: torch.Tensor, 
                           scale: Optional[float] = None) -> torch.Tensor:
     """:func:`segment_attention` of each segment over itself, with queries, keys and values in the rows of one projection:
     ``qkv`` (N, heads + 2 kv_heads, d) -> (N, heads, d)."""
-    if torch.is_grad_enabled() and qkv.requires_grad:
+    if _recorded(qkv):
         return SegmentAttentionQKVFn.apply(qkv, heads, seg_ptr, key_mask, scale)
     return segment_attention_forward(*_parts(qkv, heads), seg_ptr, None, key_mask, scale, need_lse=False)[0]
 
@@ -220,6 +220,6 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_ptr: 
                       scale: Optional[float] = None) -> torch.Tensor:
     """Attention of each segment's queries over its keys (module docstring), (Nq, heads, d); ``scale`` defaults to
     d ** -0.5.  Differentiable in q, k and v."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _recorded(q, k, v):
         return SegmentAttentionFn.apply(q, k, v, q_ptr, kv_ptr, key_mask, scale)
     return segment_attention_forward(q, k, v, q_ptr, kv_ptr, key_mask, scale, need_lse=False)[0]
