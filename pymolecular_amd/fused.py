@@ -50,6 +50,35 @@ def _recorded(*tensors: Optional[torch.Tensor]) -> bool:
                for t in tensors)
 
 
+class _FirstOrderFn(torch.autograd.Function):
+    """``grads = _FirstOrderFn.apply(n, *grads, *sources)`` for the first n tensors: the same values, whose own gradient is
+    an error."""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tuple(t.detach() for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("this operator has no second derivative: its gradients, made by the library, cannot be "
+                           "differentiated again")
+
+
+def _first_order(grads, *sources):
+    """What the backward of an autograd function returns.  Under ``create_graph=True`` autograd would take gradients that
+    the library made for constants, and second derivatives would silently lack their part: the ones returned depend on
+    the ``sources`` they were made from, and differentiating them raises.  (``once_differentiable`` raises only where the
+    incoming gradient depends on something itself: not behind a plain sum.)"""
+    if not torch.is_grad_enabled():
+        return grads
+    sources = [t for t in sources if t is not None and t.requires_grad]
+    made = [t for t in grads if t is not None]
+    if not sources or not made:
+        return grads
+    made = iter(_FirstOrderFn.apply(len(made), *made, *sources))
+    return tuple(None if t is None else next(made) for t in grads)
+
+
 def _require_device(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a ROCm device tensor: the fused EGNN layer has no CPU path")

@@ -15,7 +15,7 @@ import torch
 
 from . import _capi
 from ._capi import EgnnNormDims, check
-from .fused import _as, _dtype_code, _ptr, _recorded, _stream
+from .fused import _as, _dtype_code, _first_order, _ptr, _recorded, _stream
 
 __all__ = ["layer_norm", "layer_norm_forward", "layer_norm_backward", "LayerNormFn"]
 
@@ -121,7 +121,8 @@ class LayerNormFn(torch.autograd.Function):
         if gy is None:   # only the sum was used
             gx, gw, gb = gsum, None, None
         else:
-            gx, gw, gb = layer_norm_backward(gy, s, weight, mean, rstd, gsum, weight is not None, ctx.has_b)
+            grads = layer_norm_backward(gy, s, weight, mean, rstd, gsum, weight is not None, ctx.has_b)
+            gx, gw, gb = _first_order(grads, gy, gsum, s, weight)
         to = lambda t, dt: t if t is None or t.dtype == dt else t.to(dt)  # noqa: E731
         return gx, gw, to(gb, ctx.bdt), None, None if ctx.rdt is None else to(gx, ctx.rdt)
 

@@ -20,7 +20,7 @@ import torch
 
 from . import _capi
 from ._capi import EgnnAttnDims, EgnnAttnStrides, check
-from .fused import _dtype_code, _ptr, _recorded, _stream
+from .fused import _dtype_code, _first_order, _ptr, _recorded, _stream
 
 __all__ = ["segment_attention", "segment_attention_qkv", "segment_attention_forward", "segment_attention_backward",
            "SegmentAttentionFn", "SegmentAttentionQKVFn"]
@@ -170,8 +170,8 @@ class SegmentAttentionFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gout):
         q, k, v, out, lse, q_ptr, kv_ptr, key_mask = ctx.saved_tensors
-        return (*segment_attention_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr, key_mask, ctx.scale), None, None,
-                None, None)
+        grads = segment_attention_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr, key_mask, ctx.scale)
+        return (*_first_order(grads, gout, q, k, v), None, None, None, None)
 
 
 class SegmentAttentionQKVFn(torch.autograd.Function):
@@ -195,7 +195,7 @@ class SegmentAttentionQKVFn(torch.autograd.Function):
             grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
             segment_attention_backward(gout, *parts, out, lse, seg_ptr, None, key_mask, ctx.scale,
                                        into=_parts(grad, ctx.heads))
-        return grad, None, None, None, None
+        return (*_first_order((grad,), gout, qkv), None, None, None, None)
 
 
 def _parts(qkv, heads):

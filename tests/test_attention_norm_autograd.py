@@ -29,7 +29,7 @@ def stand_in(monkeypatch):
         return _raw(lambda a, b, c: 2 * a + b + c, *(t.contiguous() for t in (q, k, v))), torch.zeros(q.shape[1], q.shape[0])
 
     def attention_backward(gout, q, k, v, out, lse, q_ptr, kv_ptr=None, key_mask=None, scale=None, into=None):
-        g = [t.detach() * gout for t in (k, q, v)]
+        g = [t.detach() * gout.detach() for t in (k, q, v)]
         for a, b in zip(into or (), g):
             a.copy_(b)
         return tuple(g)
@@ -39,7 +39,7 @@ def stand_in(monkeypatch):
         return _raw(lambda a: 3 * a, x), s, torch.zeros(x.shape[0]), torch.ones(x.shape[0])
 
     def norm_backward(gy, s, weight, mean, rstd, gsum=None, need_weight=True, need_bias=True, **kw):
-        return gy * s.detach(), torch.zeros(s.shape[-1]) if need_weight else None, torch.zeros(s.shape[-1]) if need_bias else None
+        return gy.detach() * s.detach(), torch.zeros(s.shape[-1]) if need_weight else None, torch.zeros(s.shape[-1]) if need_bias else None
 
     for m, name, f in ((sa, "segment_attention_forward", attention), (sa, "segment_attention_backward", attention_backward),
                        (ln, "layer_norm_forward", norm), (ln, "layer_norm_backward", norm_backward)):
@@ -78,6 +78,32 @@ def test_a_tangent_is_refused(stand_in, op, shape, grad):
             op(forward_ad.make_dual(x, torch.ones_like(x)))
 
 
+SECOND = [
+    # what meets the operator's output: nothing that depends on anything, and something that does
+    lambda y: y.sum(), lambda y: (y * y).sum()]
+
+
+def _second_order(op, x, f):
+    # another path (x^3) keeps the first gradient differentiable: without the operator's part a second one would be wrong
+    g, = torch.autograd.grad(f(op(x)) + (x ** 3).sum(), x, create_graph=True)
+    plain, = torch.autograd.grad(f(op(x)) + (x ** 3).sum(), x)
+    assert torch.equal(g, plain) and not plain.requires_grad
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.parametrize("f", SECOND)
+@pytest.mark.parametrize("op,shape", OPS)
+def test_second_order_is_refused(stand_in, op, shape, f):
+    _second_order(op, torch.randn(shape, generator=torch.Generator().manual_seed(0)).requires_grad_(), f)
+
+
+def test_second_order_of_the_sum_alone(stand_in):
+    x = torch.randn((4, 8), generator=torch.Generator().manual_seed(0)).requires_grad_()
+    g, = torch.autograd.grad((ln.layer_norm(x, residual=2 * x)[1] ** 2).sum(), x, create_graph=True)
+    assert torch.allclose(torch.autograd.grad(g.sum(), x)[0], torch.full_like(x, 18.0))
+
+
 def _device_ops():
     gen = torch.Generator().manual_seed(1)
     seg = torch.tensor([0, 7, 40, 90], dtype=torch.int32, device="cuda")
@@ -108,3 +134,10 @@ def test_a_tangent_is_refused_on_the_device(grad):
         x = torch.randn(shape, generator=torch.Generator().manual_seed(0)).cuda()
         with torch.set_grad_enabled(grad), forward_ad.dual_level(), pytest.raises(NotImplementedError):
             op(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f", SECOND)
+def test_second_order_is_refused_on_the_device(f):
+    for op, shape in _device_ops():
+        _second_order(op, torch.randn(shape, generator=torch.Generator().manual_seed(0)).cuda().requires_grad_(), f)
