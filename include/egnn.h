@@ -366,13 +366,14 @@ int32_t egnn_attn_bwd(const EgnnAttnDims* dims, const EgnnAttnStrides* strides, 
  *   s = x (+ residual),  mu = mean s,  rstd = (mean (s - mu)^2 + eps)^-1/2,
  *   y = (s - mu) rstd weight + bias
  * Any C from 1 to 2^20 and any row stride; 16-byte aligned rows and widths are
- * read and written in 16-byte pieces.  weight and bias may be NULL (1 and 0), in
- * the dtype of x.  Statistics and sums are fp32; y is made from the unrounded s. */
+ * read and written in 16-byte pieces.  weight and bias may be NULL (1 and 0).
+ * Statistics and sums are fp32; y is made from the unrounded s. */
 typedef struct EgnnNormDims {
   int64_t N;             /* below 2^31 */
   int32_t C;
-  int32_t dtype;
+  int32_t dtype;         /* EGNN_F32 or EGNN_BF16, of x, residual, y, the sum and their gradients */
   float eps;             /* >= 0 */
+  int32_t f32_params;    /* 1: weight, bias and their gradients are fp32 beside bf16 rows; 0: all of one dtype */
 } EgnnNormDims;
 
 /* Writes y (N, C) and, with a residual, s (N, C) to `sum` (both contiguous);

@@ -72,12 +72,12 @@ class EgnnAttnStrides(ctypes.Structure):
 
 
 class EgnnNormDims(ctypes.Structure):
-    _fields_ = [("N", c_int64), ("C", c_int32), ("dtype", c_int32), ("eps", c_float)]
+    _fields_ = [("N", c_int64), ("C", c_int32), ("dtype", c_int32), ("eps", c_float), ("f32_params", c_int32)]
 
 
 _lib = None
 
-ABI_VERSION = 10   # include/egnn.h egnn_abi_version()
+ABI_VERSION = 11   # include/egnn.h egnn_abi_version()
 
 
 def _check_stamp(path=None, stamp=None, digest=None, what="other sources") -> None:

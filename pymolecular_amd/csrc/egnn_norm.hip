@@ -25,6 +25,7 @@ struct Args {
   int64_t N, ldx, ldr, ldg, ldgs;
   int32_t C;
   float eps;
+  bool f32_params;                           // w, b, gw and gb are fp32 beside bf16 rows
 };
 
 // A piece: 16 bytes of values from column f on.  Rows need no alignment but their values': the type says so, and the
@@ -68,6 +69,28 @@ template <typename T, bool TAIL = true> struct Vec {
     }
   }
 };
+// a piece of the weight or the bias, which may be fp32 beside bf16 rows: rounded to bf16 they would lose what training
+// accumulates in them
+template <typename T, bool TAIL> __device__ __forceinline__ void load_params(const void* p, bool f32, int f, int C, float* v) {
+  typedef Vec<T, TAIL> V;
+  if constexpr (sizeof(T) == 2) {
+    if (f32) {
+      const float* q = (const float*)p;
+      if (!TAIL || C >= V::N) {
+        Vec<float, false>::load(q, f, C, v);
+        Vec<float, false>::load(q, f + 4, C, v + 4);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V::N; ++i) v[i] = i < C ? q[i] : 0.f;
+      }
+      return;
+    }
+  }
+  V::load((const T*)p, f, C, v);
+}
+template <typename T> __device__ __forceinline__ float param(const void* p, bool f32, int f) {
+  return sizeof(T) == 2 && f32 ? ((const float*)p)[f] : to_f32(((const T*)p)[f]);
+}
 // the lane's piece number k of a row: its first column, and how many of its columns another piece has (all of them: no
 // such piece)
 struct Piece {
@@ -163,8 +186,8 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
       float w[VEC], b[VEC], y[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) { w[i] = 1.f; b[i] = 0.f; }
-      if (a.w) V::load((const T*)a.w, c[p].f, a.C, w);
-      if (a.b) V::load((const T*)a.b, c[p].f, a.C, b);
+      if (a.w) load_params<T, TAIL>(a.w, a.f32_params, c[p].f, a.C, w);
+      if (a.b) load_params<T, TAIL>(a.b, a.f32_params, c[p].f, a.C, b);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) y[i] = __builtin_fmaf((v[p][i] - mean) * rstd, w[i], b[i]);
       V::store((T*)a.y + n * a.C, c[p].f, a.C, y);
@@ -190,7 +213,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
     c[p] = piece_of<VEC, TAIL>(p * LPR + lane, a.C);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) { gw[p][i] = 0.f; gb[p][i] = 0.f; w[p][i] = 1.f; }
-    if (a.w && c[p].in) V::load((const T*)a.w, c[p].f, a.C, w[p]);
+    if (a.w && c[p].in) load_params<T, TAIL>(a.w, a.f32_params, c[p].f, a.C, w[p]);
   }
   const int64_t step = (int64_t)gridDim.x * RG;
   typename V::piece pg[VPL], px[VPL], pe[VPL];
@@ -299,7 +322,7 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
     if (threadIdx.x == 0) { a.mean[n] = m; a.rstd[n] = rs; }
   }
   for (int f = threadIdx.x; f < a.C; f += NT) {
-    const float v = val(f), w = a.w ? to_f32(((const T*)a.w)[f]) : 1.f, b = a.b ? to_f32(((const T*)a.b)[f]) : 0.f;
+    const float v = val(f), w = a.w ? param<T>(a.w, a.f32_params, f) : 1.f, b = a.b ? param<T>(a.b, a.f32_params, f) : 0.f;
     if (r) ((T*)a.s)[n * a.C + f] = from_f32<T>(v);
     ((T*)a.y)[n * a.C + f] = from_f32<T>(__builtin_fmaf((v - mean) * rstd, w, b));
   }
@@ -312,13 +335,13 @@ __global__ __launch_bounds__(NT) void bwd_wide_kernel(Args a) {
   const float mean = a.mean[n], rstd = a.rstd[n];
   float s1 = 0.f, s2 = 0.f;
   for (int f = threadIdx.x; f < a.C; f += NT) {
-    const float t = to_f32(g[f]) * (a.w ? to_f32(((const T*)a.w)[f]) : 1.f);
+    const float t = to_f32(g[f]) * (a.w ? param<T>(a.w, a.f32_params, f) : 1.f);
     s1 += t;
     s2 = __builtin_fmaf(t, (to_f32(x[f]) - mean) * rstd, s2);
   }
   const float m1 = block_sum(s1, buf) / a.C, m2 = block_sum(s2, buf) / a.C;
   for (int f = threadIdx.x; f < a.C; f += NT) {
-    const float t = to_f32(g[f]) * (a.w ? to_f32(((const T*)a.w)[f]) : 1.f);
+    const float t = to_f32(g[f]) * (a.w ? param<T>(a.w, a.f32_params, f) : 1.f);
     float o = rstd * (t - m1 - (to_f32(x[f]) - mean) * rstd * m2);
     if (a.gsum) o += to_f32(((const T*)a.gsum)[n * a.ldgs + f]);
     ((T*)a.gx)[n * a.C + f] = from_f32<T>(o);
@@ -435,13 +458,17 @@ static int launch(const Args& a, bool bwd, hipStream_t st) {
       }
     }
   }
-  if (bwd && a.part) sum_kernel<T><<<(uint32_t)cdiv(2 * (int64_t)a.C, 16), 1024, 0, st>>>(a.part, nblk, a.C, (T*)a.gw, (T*)a.gb);
+  if (bwd && a.part) {
+    const uint32_t blocks = (uint32_t)cdiv(2 * (int64_t)a.C, 16);
+    if (a.f32_params) sum_kernel<float><<<blocks, 1024, 0, st>>>(a.part, nblk, a.C, (float*)a.gw, (float*)a.gb);
+    else sum_kernel<T><<<blocks, 1024, 0, st>>>(a.part, nblk, a.C, (T*)a.gw, (T*)a.gb);
+  }
   return hipGetLastError() == hipSuccess ? EGNN_OK : EGNN_ERR_HIP;
 }
 
 static bool dims_ok(const EgnnNormDims* d) {
   return d->N >= 0 && d->N <= INT32_MAX && d->C >= 1 && d->C <= 1 << 20 && (d->dtype == EGNN_F32 || d->dtype == EGNN_BF16) &&
-         d->eps >= 0.f && d->eps - d->eps == 0.f;
+         d->eps >= 0.f && d->eps - d->eps == 0.f && (d->f32_params == 0 || d->f32_params == 1);
 }
 
 }  // namespace norm
@@ -461,13 +488,13 @@ int32_t egnn_norm_fwd(const EgnnNormDims* d, const void* x, int64_t ldx, const v
   if (!dims_ok(d)) return EGNN_ERR_DIMS;
   if (!mean != !rstd || (residual && !sum) || (d->N && (!x || !y))) return EGNN_ERR_NULL;
   if (ldx < 0 || (residual && ldr < 0)) return EGNN_ERR_STRIDE;
-  const uintptr_t e = d->dtype == EGNN_F32 ? 4 : 2;
-  if ((uintptr_t)x % e || (uintptr_t)residual % e || (uintptr_t)weight % e || (uintptr_t)bias % e || (uintptr_t)y % e ||
+  const uintptr_t e = d->dtype == EGNN_F32 ? 4 : 2, ep = d->f32_params ? 4 : e;
+  if ((uintptr_t)x % e || (uintptr_t)residual % e || (uintptr_t)weight % ep || (uintptr_t)bias % ep || (uintptr_t)y % e ||
       (uintptr_t)sum % e || (uintptr_t)mean % 4 || (uintptr_t)rstd % 4)
     return EGNN_ERR_ALIGN;
   Args a{};
   a.x = x; a.ldx = ldx; a.r = residual; a.ldr = ldr; a.w = weight; a.b = bias; a.y = y; a.s = residual ? sum : nullptr;
-  a.mean = mean; a.rstd = rstd; a.N = d->N; a.C = d->C; a.eps = d->eps;
+  a.mean = mean; a.rstd = rstd; a.N = d->N; a.C = d->C; a.eps = d->eps; a.f32_params = d->f32_params != 0;
   return d->dtype == EGNN_BF16 ? launch<egnn::bf16>(a, false, (hipStream_t)stream) : launch<float>(a, false, (hipStream_t)stream);
 }
 
@@ -478,16 +505,16 @@ int32_t egnn_norm_bwd(const EgnnNormDims* d, const void* grad_y, int64_t ldg, co
   if (!dims_ok(d)) return EGNN_ERR_DIMS;
   if (d->N && (!grad_y || !sum || !mean || !rstd || !grad_x)) return EGNN_ERR_NULL;
   if (ldg < 0 || lds < 0 || (grad_sum && ldgs < 0)) return EGNN_ERR_STRIDE;
-  const uintptr_t e = d->dtype == EGNN_F32 ? 4 : 2;
-  if ((uintptr_t)grad_y % e || (uintptr_t)sum % e || (uintptr_t)weight % e || (uintptr_t)grad_sum % e || (uintptr_t)grad_x % e ||
-      (uintptr_t)grad_weight % e || (uintptr_t)grad_bias % e || (uintptr_t)mean % 4 || (uintptr_t)rstd % 4 || (uintptr_t)workspace % 16)
+  const uintptr_t e = d->dtype == EGNN_F32 ? 4 : 2, ep = d->f32_params ? 4 : e;
+  if ((uintptr_t)grad_y % e || (uintptr_t)sum % e || (uintptr_t)weight % ep || (uintptr_t)grad_sum % e || (uintptr_t)grad_x % e ||
+      (uintptr_t)grad_weight % ep || (uintptr_t)grad_bias % ep || (uintptr_t)mean % 4 || (uintptr_t)rstd % 4 || (uintptr_t)workspace % 16)
     return EGNN_ERR_ALIGN;
   const bool weights = grad_weight || grad_bias;
   if (weights && (!workspace || workspace_bytes < egnn_norm_bwd_workspace_bytes(d))) return EGNN_ERR_WORKSPACE;
   Args a{};
   a.gy = grad_y; a.ldg = ldg; a.x = sum; a.ldx = lds; a.w = weight; a.mean = (float*)mean; a.rstd = (float*)rstd;
   a.gsum = grad_sum; a.ldgs = ldgs; a.gx = grad_x; a.gw = grad_weight; a.gb = grad_bias;
-  a.part = weights ? (float*)workspace : nullptr; a.N = d->N; a.C = d->C; a.eps = d->eps;
+  a.part = weights ? (float*)workspace : nullptr; a.N = d->N; a.C = d->C; a.eps = d->eps; a.f32_params = d->f32_params != 0;
   return d->dtype == EGNN_BF16 ? launch<egnn::bf16>(a, true, (hipStream_t)stream) : launch<float>(a, true, (hipStream_t)stream);
 }
 

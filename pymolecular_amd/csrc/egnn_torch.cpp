@@ -287,43 +287,47 @@ pybind11::object attn_backward(const Tensor& go, const Tensor& q, const Tensor& 
   return pybind11::make_tuple(gq, gk, gv);
 }
 
-// contiguous rows of one dtype; the parameters too
-bool norm_ok(const Tensor& x, const Opt& w, const Opt& b, double eps) {
+// contiguous rows of one dtype; the parameters of that one too, or (f32) of fp32
+bool norm_ok(const Tensor& x, const Opt& w, const Opt& b, double eps, bool f32) {
   const auto dt = x.scalar_type();
   return !torch::jit::tracer::isTracing() && x.dim() >= 1 && x.size(-1) >= 1 && (dt == at::kFloat || dt == at::kBFloat16) &&
-         plain(x, x) && x.is_contiguous() && fits_opt(w, x, dt, x.size(-1)) && fits_opt(b, x, dt, x.size(-1)) && eps >= 0 &&
-         std::isfinite(eps);
+         plain(x, x) && x.is_contiguous() && fits_opt(w, x, f32 ? at::kFloat : dt, x.size(-1)) &&
+         fits_opt(b, x, f32 ? at::kFloat : dt, x.size(-1)) && eps >= 0 && std::isfinite(eps);
 }
 bool same_rows(const Tensor& t, const Tensor& x) {
   return plain(t, x) && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && t.is_contiguous();
 }
-EgnnNormDims norm_dims(const Tensor& x, double eps) {
+EgnnNormDims norm_dims(const Tensor& x, double eps, bool f32) {
   EgnnNormDims d{};
   d.C = (int32_t)x.size(-1); d.N = x.numel() / x.size(-1);
   d.dtype = x.scalar_type() == at::kFloat ? EGNN_F32 : EGNN_BF16;
   d.eps = (float)eps;
+  d.f32_params = f32 && d.dtype == EGNN_BF16;
   return d;
 }
 
 pybind11::object norm_forward(const Tensor& x, const Opt& w, const Opt& b, double eps, const Opt& res, bool need_stats) {
-  if (!norm_ok(x, w, b, eps) || (res && !same_rows(*res, x))) return pybind11::none();
-  const EgnnNormDims d = norm_dims(x, eps);
-  const auto f32 = x.options().dtype(at::kFloat);
+  const bool f32 = (w && w->scalar_type() == at::kFloat) || (b && b->scalar_type() == at::kFloat);
+  if (!norm_ok(x, w, b, eps, f32) || (res && !same_rows(*res, x))) return pybind11::none();
+  const EgnnNormDims d = norm_dims(x, eps, f32);
+  const auto stat = x.options().dtype(at::kFloat);
   const Tensor y = at::empty(x.sizes(), x.options()), s = res ? at::empty(x.sizes(), x.options()) : x;
-  const Tensor mean = need_stats ? at::empty({d.N}, f32) : Tensor(), rstd = need_stats ? at::empty({d.N}, f32) : Tensor();
+  const Tensor mean = need_stats ? at::empty({d.N}, stat) : Tensor(), rstd = need_stats ? at::empty({d.N}, stat) : Tensor();
   check("egnn_norm_fwd", egnn_norm_fwd(&d, ptr(x), d.C, ptr(get(res)), d.C, ptr(get(w)), ptr(get(b)), ptr(y),
                                        res ? ptr(s) : nullptr, ptr<float>(mean), ptr<float>(rstd), stream_of(x)));
   if (!need_stats) return pybind11::make_tuple(y, s, pybind11::none(), pybind11::none());
   return pybind11::make_tuple(y, s, mean, rstd);
 }
 
+// f32: the weight is, and the gradients of weight and bias are wanted in, fp32
 pybind11::object norm_backward(const Tensor& gy, const Tensor& s, const Opt& w, const Tensor& mean, const Tensor& rstd,
-                               const Opt& gsum, bool need_w, bool need_b) {
-  if (!norm_ok(s, w, Opt(), 0.0) || !same_rows(gy, s) || (gsum && !same_rows(*gsum, s))) return pybind11::none();
-  const EgnnNormDims d = norm_dims(s, 0.0);
+                               const Opt& gsum, bool need_w, bool need_b, bool f32) {
+  if (!norm_ok(s, w, Opt(), 0.0, f32) || !same_rows(gy, s) || (gsum && !same_rows(*gsum, s))) return pybind11::none();
+  const EgnnNormDims d = norm_dims(s, 0.0, f32);
   if (!fits(mean, s, at::kFloat, {d.N}) || !fits(rstd, s, at::kFloat, {d.N})) return pybind11::none();
   const Tensor gx = at::empty(s.sizes(), s.options());
-  const Tensor gw = need_w ? at::empty({d.C}, s.options()) : Tensor(), gb = need_b ? at::empty({d.C}, s.options()) : Tensor();
+  const auto param = s.options().dtype(f32 ? at::kFloat : s.scalar_type());
+  const Tensor gw = need_w ? at::empty({d.C}, param) : Tensor(), gb = need_b ? at::empty({d.C}, param) : Tensor();
   const size_t nb = need_w || need_b ? egnn_norm_bwd_workspace_bytes(&d) : 0;
   const Tensor ws = workspace(nb, s);
   check("egnn_norm_bwd", egnn_norm_bwd(&d, ptr(gy), d.C, ptr(s), d.C, ptr(get(w)), ptr<float>(mean), ptr<float>(rstd),
