@@ -409,10 +409,31 @@ static int64_t part_rows(int64_t N) {
   return n < 1 ? 1 : (n < kMaxBlocks ? n : kMaxBlocks);
 }
 
+// A launch may have fewer than 2^32 threads, and there may be more rows than that leaves room for (2^24 of the wide ones):
+// at most kMaxGrid blocks at a time, go(args, blocks) of the rows from one launch's first on.  A part is 1 GB of rows or
+// more, beside which its launch does not show.
+constexpr int64_t kMaxGrid = int64_t(1) << 20;
+template <typename T, typename Go>
+static void in_parts(const Args& a, int rows_per_block, Go go) {
+  const int64_t most = kMaxGrid * rows_per_block;
+  for (int64_t n = 0; n < a.N; n += most) {
+    Args x = a;
+    auto at = [&](const void* p, int64_t ld) -> const void* { return p ? (const T*)p + n * ld : nullptr; };
+    x.x = at(a.x, a.ldx); x.r = at(a.r, a.ldr); x.gy = at(a.gy, a.ldg); x.gsum = at(a.gsum, a.ldgs);
+    x.y = (void*)at(a.y, a.C); x.s = (void*)at(a.s, a.C); x.gx = (void*)at(a.gx, a.C);
+    x.mean = a.mean ? a.mean + n : nullptr; x.rstd = a.rstd ? a.rstd + n : nullptr;
+    x.N = a.N - n < most ? a.N - n : most;
+    go(x, (uint32_t)cdiv(x.N, rows_per_block));
+  }
+}
+
 template <typename T, int LPR, int VPL, bool TAIL>
 static void launch_tail(const Args& a, bool bwd, hipStream_t st, int* nblk) {
+  if (!bwd) {
+    in_parts<T>(a, NT / LPR, [&](const Args& x, uint32_t blocks) { fwd_kernel<T, LPR, VPL, TAIL><<<blocks, NT, 0, st>>>(x); });
+    return;
+  }
   const int64_t n = cdiv(a.N, NT / LPR);
-  if (!bwd) { fwd_kernel<T, LPR, VPL, TAIL><<<(uint32_t)n, NT, 0, st>>>(a); return; }
   *nblk = (int)(n < part_rows(a.N) ? n : part_rows(a.N));
   const int64_t bytes = a.N * a.C * (int64_t)sizeof(T);
   if (bytes >= kPastLoad) bwd_kernel<T, LPR, VPL, 2, TAIL><<<(uint32_t)*nblk, NT, 0, st>>>(a);
@@ -449,9 +470,9 @@ static int launch(const Args& a, bool bwd, hipStream_t st) {
   int nblk = 0;
   if (a.N) {
     if (shape_of((int)cdiv(a.C, Vec<T>::N), a.N, &s)) launch_rows<T>(a, s, bwd, st, &nblk);
-    else if (!bwd) fwd_wide_kernel<T><<<(uint32_t)a.N, NT, 0, st>>>(a);
+    else if (!bwd) in_parts<T>(a, 1, [&](const Args& x, uint32_t blocks) { fwd_wide_kernel<T><<<blocks, NT, 0, st>>>(x); });
     else {
-      bwd_wide_kernel<T><<<(uint32_t)a.N, NT, 0, st>>>(a);
+      in_parts<T>(a, 1, [&](const Args& x, uint32_t blocks) { bwd_wide_kernel<T><<<blocks, NT, 0, st>>>(x); });
       if (a.part) {
         nblk = (int)(part_rows(a.N) < 128 ? part_rows(a.N) : 128);
         bwd_wide_weights_kernel<T><<<dim3((uint32_t)cdiv(a.C, NT), (uint32_t)nblk), NT, 0, st>>>(a);

@@ -1,0 +1,66 @@
+"""Layer norm over more rows than one launch has threads for: 2^32 threads, 2^20 workgroups at a time.
+
+Every row is a row by itself, so the result at the places where launches meet and end is that of a call on a few of the
+rows, bit for bit.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def _free():
+    yield
+    torch.cuda.empty_cache()
+
+
+def _places(n, part):
+    """Ranges of rows at the start, at the end and around every boundary between parts."""
+    for at in range(0, n, part):
+        yield slice(max(0, at - 40), min(n, at + 40))
+    yield slice(n - 50, n)
+
+
+def _fill(*shape, dtype, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.empty(shape, dtype=dtype, device="cuda").normal_(generator=gen)
+
+
+# two columns: four lanes a row, 2^32 threads at 2^30 rows; rows past a wave's registers: a workgroup each
+@pytest.mark.parametrize("n,c,dtype,part", [((1 << 30) + 77, 2, BF16, 1 << 26), ((1 << 26) + 5, 3, F32, 1 << 26),
+                                            ((1 << 20) + 3, 1541, F32, 1 << 20)])
+def test_norm_forward(n, c, dtype, part):
+    from pymolecular_amd.layer_norm import layer_norm, layer_norm_forward
+    x = _fill(n, c, dtype=dtype, seed=c)
+    w, b = _fill(c, dtype=dtype, seed=1), _fill(c, dtype=dtype, seed=2)
+    y = layer_norm(x, w, b)
+    for i in _places(n, part):
+        assert torch.equal(y[i], layer_norm(x[i].contiguous(), w, b)), i
+    del y
+    if c != 2:
+        r = _fill(n, c, dtype=dtype, seed=3)
+        out = layer_norm_forward(x, w, b, residual=r)
+        for i in _places(n, part):
+            for p, q in zip(out, layer_norm_forward(x[i].contiguous(), w, b, residual=r[i].contiguous())):
+                assert torch.equal(p[i], q), i
+
+
+def test_norm_backward_of_wide_rows():
+    from pymolecular_amd.layer_norm import layer_norm_backward, layer_norm_forward
+    n, c = (1 << 20) + 3, 1541
+    x, gy = _fill(n, c, dtype=F32, seed=4), _fill(n, c, dtype=F32, seed=5)
+    w = _fill(c, dtype=F32, seed=1)
+    y, s, mean, rstd = layer_norm_forward(x, w)
+    del y
+    gx, gw, gb = layer_norm_backward(gy, s, w, mean, rstd, gsum=x)
+    for i in _places(n, 1 << 20):
+        small = layer_norm_backward(gy[i].contiguous(), s[i].contiguous(), w, mean[i].contiguous(), rstd[i].contiguous(),
+                                    gsum=x[i].contiguous())
+        assert torch.equal(gx[i], small[0]), i
+    # gb: 128 fp32 sums of 2^13 values of about 1, each addition rounding a sum of about 2^6.5: 2^-24 2^6.5 2^6.5 a sum and
+    # 2^3.5 times that for all of them; four deviations, for 1,541 columns, and a half for the addition of the 128
+    want = sum(g.double().sum(dim=0) for g in gy.split(1 << 17))
+    assert (gb.double() - want).abs().max() <= 2.0 ** -24 * 2.0 ** 16.5 * 4.5
