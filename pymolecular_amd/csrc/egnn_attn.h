@@ -60,8 +60,19 @@ struct Args {
   float scale;                               // |scale|
   uint32_t flip;                             // sign bit of a negative scale: q enters negated
   int32_t nsplit;
+  uint32_t first;                            // workgroups of the call before this launch's
   float* part;                               // split partials
 };
+
+// A launch may have fewer than 2^32 threads, a call more workgroups than that leaves room for (2^24 of 256 threads: a
+// batch of 8 million graphs with 8 key heads): at most kMaxGrid at a time, go(args, workgroups) of each part.
+constexpr uint32_t kMaxGrid = 1u << 20;
+template <typename Go> void in_parts(Args a, int64_t blocks, Go go) {
+  for (int64_t n = 0; n < blocks; n += kMaxGrid) {
+    a.first = (uint32_t)n;
+    go(a, (uint32_t)(blocks - n < kMaxGrid ? blocks - n : kMaxGrid));
+  }
+}
 
 constexpr int kShortMean = 28;               // rows a segment up to which a wave takes a tile
 
@@ -368,7 +379,7 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t bid, uint32_t n) {
 struct Item { uint32_t slot; int kvh, sp; };
 template <int W, bool SH>
 __device__ __forceinline__ bool item_of(const Args& a, uint32_t n_items, Item& it) {
-  uint32_t i = xcd_order(blockIdx.x, gridDim.x);
+  uint32_t i = a.first + xcd_order(blockIdx.x, gridDim.x);
   if constexpr (!SH && W > 1) i = i * W + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (i >= n_items) return false;
   const uint32_t j = a.by_heads(i), k = a.by_slots(j);

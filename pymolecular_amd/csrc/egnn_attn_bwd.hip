@@ -635,7 +635,7 @@ __global__ __launch_bounds__(64 * W, (short_occupancy<T, DP>())) void short_kern
   __shared__ __attribute__((aligned(16))) bf16 lds[W / P][4][TL::elems];
   __shared__ __attribute__((aligned(16))) float stat[W][2][TK];
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), x0 = P == 2 ? 16 * w : 0;
-  uint32_t i = xcd_order(blockIdx.x, gridDim.x);
+  uint32_t i = a.first + xcd_order(blockIdx.x, gridDim.x);
   if (P == 1) i = i * W + w;
   bf16* t = lds[P == 1 ? w : 0][0];
   bf16* t2 = P == 1 ? t : lds[0][2 * w];     // of a wave by itself
@@ -720,20 +720,23 @@ static void sum_parts(const float* part, int nsplit, int64_t rows, int heads, in
 template <typename T, int DP, int R, int W, bool SH, int KT>
 static void go_q(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
-  const uint32_t blocks = (uint32_t)(SH ? n : cdiv(n, W));
   constexpr bool can = SH && Num<T>::planes == 1 && R == 1;
-  if constexpr (can) {
-    if (a.nsplit == 1) {
-      dq_kernel<T, DP, R, W, SH, KT, true><<<blocks, 64 * W, 0, st>>>(a, (uint32_t)n);
-      return;
+  in_parts(a, SH ? n : cdiv(n, W), [&](const Args& x, uint32_t blocks) {
+    if constexpr (can) {
+      if (a.nsplit == 1) {
+        dq_kernel<T, DP, R, W, SH, KT, true><<<blocks, 64 * W, 0, st>>>(x, (uint32_t)n);
+        return;
+      }
     }
-  }
-  dq_kernel<T, DP, R, W, SH, KT, false><<<blocks, 64 * W, 0, st>>>(a, (uint32_t)n);
+    dq_kernel<T, DP, R, W, SH, KT, false><<<blocks, 64 * W, 0, st>>>(x, (uint32_t)n);
+  });
 }
 template <typename T, int DP, int R, int W, bool SH, int KT>
 static void go_k(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
-  dkv_kernel<T, DP, R, W, SH, KT><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
+  in_parts(a, SH ? n : cdiv(n, W), [&](const Args& x, uint32_t blocks) {
+    dkv_kernel<T, DP, R, W, SH, KT><<<blocks, 64 * W, 0, st>>>(x, (uint32_t)n);
+  });
 }
 // One launch for both axes in short segments: both plans say waves, without splits
 template <typename T, int DP>
@@ -755,8 +758,10 @@ static bool launch_short(Args a, const Plan& pq, const Plan& pk, hipStream_t st)
     // Two waves a segment in fp32, whose products are six (one and two waves, 10 .. 30 rows a segment, D = 32, 4 heads: 27
     // and 18 us for 512 segments, 165 and 101 for 4,000); not in bf16 (4,000 segments: 46 and 44; D = 64: 78 and 85;
     // D = 16, 1,024 molecules and 8 heads: 15.6 and 19).
-    if constexpr (f32) short_kernel<T, DP, 2, 2><<<(uint32_t)(nq + nk), 128, 0, st>>>(a, (uint32_t)nq, (uint32_t)nk, (uint32_t)sk, by, per);
-    else short_kernel<T, DP, 1, W><<<(uint32_t)cdiv(nq + nk, W), 64 * W, 0, st>>>(a, (uint32_t)nq, (uint32_t)nk, (uint32_t)sk, by, per);
+    constexpr int P = f32 ? 2 : 1, WS = f32 ? 2 : W;
+    in_parts(a, cdiv(nq + nk, WS / P), [&](const Args& x, uint32_t blocks) {
+      short_kernel<T, DP, P, WS><<<blocks, 64 * WS, 0, st>>>(x, (uint32_t)nq, (uint32_t)nk, (uint32_t)sk, by, per);
+    });
     return true;
   }
 }

@@ -428,7 +428,9 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
 template <typename T, int DP, int R, int W, bool SH, int KT, int KC>
 static void go(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
-  fwd_kernel<T, DP, R, W, SH, KT, KC><<<(uint32_t)(SH ? n : cdiv(n, W)), 64 * W, 0, st>>>(a, (uint32_t)n);
+  in_parts(a, SH ? n : cdiv(n, W), [&](const Args& x, uint32_t blocks) {
+    fwd_kernel<T, DP, R, W, SH, KT, KC><<<blocks, 64 * W, 0, st>>>(x, (uint32_t)n);
+  });
 }
 template <typename T, int DP>
 static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
@@ -446,8 +448,10 @@ static int launch_t(const Args& a, const Plan& p, hipStream_t st) {
       x.by_slots = Div::of(x.slots);
       // Two waves a segment where its products take long (one and two waves, 10 .. 30 rows a segment, 4 heads: fp32, D = 32,
       // 4,000 segments 59 and 51 us; bf16, D = 64 41 and 32), not where they do not (bf16, D = 32: 18.6 and 20.6)
-      if constexpr (f32 || DP == 64) short_kernel<T, DP, 2, 2><<<(uint32_t)n, 128, 0, st>>>(x, (uint32_t)n);
-      else short_kernel<T, DP, 1, W3><<<(uint32_t)cdiv(n, W3), 64 * W3, 0, st>>>(x, (uint32_t)n);
+      constexpr int P = f32 || DP == 64 ? 2 : 1, WS = P == 2 ? 2 : W3;
+      in_parts(x, cdiv(n, WS / P), [&](const Args& y, uint32_t blocks) {
+        short_kernel<T, DP, P, WS><<<blocks, 64 * WS, 0, st>>>(y, (uint32_t)n);
+      });
       return (int)hipGetLastError();
     }
   }

@@ -1,7 +1,8 @@
-"""Layer norm over more rows than one launch has threads for: 2^32 threads, 2^20 workgroups at a time.
+"""Layer norm and segment attention over more rows and segments than one launch has threads for: 2^32 threads, 2^20
+workgroups at a time.
 
-Every row is a row by itself, so the result at the places where launches meet and end is that of a call on a few of the
-rows, bit for bit.
+Every row of a norm, and every segment, is by itself, so the result at the places where launches meet and end is that of
+a call on a few of them, bit for bit.
 """
 import pytest
 import torch
@@ -64,3 +65,23 @@ def test_norm_backward_of_wide_rows():
     # 2^3.5 times that for all of them; four deviations, for 1,541 columns, and a half for the addition of the 128
     want = sum(g.double().sum(dim=0) for g in gy.split(1 << 17))
     assert (gb.double() - want).abs().max() <= 2.0 ** -24 * 2.0 ** 16.5 * 4.5
+
+
+# segments of `rows` rows.  A wave a segment and four a workgroup, 2^32 threads at 2^26 of them; two waves a segment; waves
+# with tiles of heads wider than 64; workgroups with tiles of 64 rows
+@pytest.mark.parametrize("n,rows,d,dtype,part", [((1 << 26) + 9, 2, 8, BF16, 1 << 22), ((1 << 20) + 5, 2, 8, F32, 1 << 20),
+                                                 ((1 << 21) + 7, 2, 72, BF16, 1 << 21), ((1 << 20) + 5, 2, 72, F32, 1 << 20),
+                                                 ((1 << 20) + 5, 30, 16, BF16, 1 << 20)])
+def test_attention(n, rows, d, dtype, part):
+    from pymolecular_amd.segment_attention import segment_attention_backward, segment_attention_forward
+    x = [_fill(n * rows, 1, d, dtype=dtype, seed=i) for i in range(4)]
+    ptr = torch.arange(0, n * rows + 1, rows, dtype=torch.int32, device="cuda")
+    out, lse = segment_attention_forward(*x[:3], ptr)
+    grads = segment_attention_backward(x[3], *x[:3], out, lse, ptr)
+    for i in _places(n, part):
+        j = slice(i.start * rows, i.stop * rows)
+        few = [t[j].contiguous() for t in x]
+        p = ptr[:i.stop - i.start + 1].contiguous()
+        o, l = segment_attention_forward(*few[:3], p)
+        for a, b in zip((out[j], lse[:, j], *(g[j] for g in grads)), (o, l, *segment_attention_backward(few[3], *few[:3], o, l, p))):
+            assert torch.equal(a, b), i
