@@ -225,7 +225,8 @@ bool attn_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_
   const auto dt = q.scalar_type();
   const int64_t d = q.size(2), hk = k.size(1);
   if ((dt != at::kFloat && dt != at::kBFloat16) || d < 8 || d > 128 || d % 8 || hk < 1 || q.size(1) < 1 || q.size(1) % hk ||
-      !std::isfinite(scale) || scale == 0.0 || (!kv_ptr && q.size(0) != k.size(0)))
+      q.size(1) > INT32_MAX || q_ptr.numel() - 1 > INT32_MAX || !std::isfinite(scale) || scale == 0.0 ||
+      (!kv_ptr && q.size(0) != k.size(0)))
     return false;
   if (q_ptr.dim() != 1 || q_ptr.numel() < 1 || !fits(q_ptr, q, at::kInt, {q_ptr.numel()}) ||
       (kv_ptr && !fits(*kv_ptr, q, at::kInt, {q_ptr.numel()})))
@@ -290,7 +291,7 @@ pybind11::object attn_backward(const Tensor& go, const Tensor& q, const Tensor& 
 // contiguous rows of one dtype; the parameters of that one too, or (f32) of fp32
 bool norm_ok(const Tensor& x, const Opt& w, const Opt& b, double eps, bool f32) {
   const auto dt = x.scalar_type();
-  return !torch::jit::tracer::isTracing() && x.dim() >= 1 && x.size(-1) >= 1 && (dt == at::kFloat || dt == at::kBFloat16) &&
+  return !torch::jit::tracer::isTracing() && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 1 << 20 && (dt == at::kFloat || dt == at::kBFloat16) &&
          plain(x, x) && x.is_contiguous() && fits_opt(w, x, f32 ? at::kFloat : dt, x.size(-1)) &&
          fits_opt(b, x, f32 ? at::kFloat : dt, x.size(-1)) && eps >= 0 && std::isfinite(eps);
 }

@@ -4,8 +4,8 @@
 
 ``y`` is made from the unrounded sum; with a residual the sum is returned too (what the next residual adds to).  The
 backward takes the gradients of both and makes the weight's and the bias's over all rows in a fixed order
-(``egnn_norm_fwd`` / ``egnn_norm_bwd`` in include/egnn.h).  float32 or bfloat16 with fp32 statistics, any width and row
-stride.  ``y`` and the sum have the dtype of ``x + residual``; weight and bias enter, and their gradients leave, in
+(``egnn_norm_fwd`` / ``egnn_norm_bwd`` in include/egnn.h).  float32 or bfloat16 with fp32 statistics, any width up to 2^20 and
+any row stride.  ``y`` and the sum have the dtype of ``x + residual``; weight and bias enter, and their gradients leave, in
 float32 where they have another dtype than the rows (float32 parameters beside bfloat16 activations).  There is no
 reference function for this step, and no CPU path: ROCm tensors only.
 """
@@ -21,6 +21,8 @@ from .fused import _as, _dtype_code, _first_order, _ptr, _recorded, _stream
 
 __all__ = ["layer_norm", "layer_norm_forward", "layer_norm_backward", "LayerNormFn"]
 
+MAX_WIDTH = 1 << 20
+
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as (rows, C) with unit-stride rows; a copy only where it has to be."""
@@ -32,8 +34,8 @@ def _check(x, weight, bias, residual, eps):
     if not x.is_cuda:
         raise RuntimeError("x must be a ROCm device tensor: the layer norm has no CPU path")
     _dtype_code(x.dtype)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x needs a last axis of at least 1 value (got {tuple(x.shape)})")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"x needs a last axis of 1 to {MAX_WIDTH} values (got {tuple(x.shape)})")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None and (tuple(p.shape) != (x.shape[-1],) or p.device != x.device):
             raise ValueError(f"{name} must be ({x.shape[-1]},) on {x.device} (got {tuple(p.shape)} on {p.device})")

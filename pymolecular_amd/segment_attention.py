@@ -58,6 +58,8 @@ def _check(q, k, v, q_ptr, kv_ptr, key_mask, scale):
     for name, p in (("q_ptr", q_ptr), ("kv_ptr", kv_ptr)):
         if p.dtype != torch.int32 or p.dim() != 1 or p.numel() < 1 or not p.is_contiguous():
             raise ValueError(f"{name} must hold n_seg + 1 contiguous int32 offsets")
+    if q.shape[1] >= 1 << 31 or q_ptr.numel() > 1 << 31:   # what the library counts in 32 bits
+        raise ValueError(f"{q.shape[1]} heads, {q_ptr.numel()} offsets: at most 2^31 - 1 heads and segments")
     if q_ptr.numel() != kv_ptr.numel():
         raise ValueError(f"q_ptr and kv_ptr have {q_ptr.numel()} and {kv_ptr.numel()} offsets")
     if kv_ptr is q_ptr and q.shape[0] != k.shape[0]:

@@ -85,3 +85,22 @@ def test_attention(n, rows, d, dtype, part):
         o, l = segment_attention_forward(*few[:3], p)
         for a, b in zip((out[j], lse[:, j], *(g[j] for g in grads)), (o, l, *segment_attention_backward(few[3], *few[:3], o, l, p))):
             assert torch.equal(a, b), i
+
+
+def test_counts_past_32_bits_are_refused():
+    # 2^32 + 5 columns are not 5 columns, 2^32 + 1 segments not one
+    from pymolecular_amd.layer_norm import layer_norm
+    from pymolecular_amd.segment_attention import segment_attention
+    wide = torch.zeros((1, (1 << 32) + 5), dtype=BF16, device="cuda")
+    with pytest.raises(ValueError):
+        layer_norm(wide)
+    del wide
+    ptr = torch.zeros((1 << 32) + 2, dtype=torch.int32, device="cuda")
+    ptr[-1] = 20
+    x = _fill(20, 2, 16, dtype=BF16, seed=0)
+    with pytest.raises(ValueError):
+        segment_attention(x, x, x, ptr)
+    del ptr
+    many = torch.zeros((0, (1 << 32) + 2, 16), dtype=BF16, device="cuda")
+    with pytest.raises(ValueError):
+        segment_attention(many, x[:0], x[:0], torch.zeros(2, dtype=torch.int32, device="cuda"))
