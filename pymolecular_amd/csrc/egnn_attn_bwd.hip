@@ -508,7 +508,8 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     Bits<1> bits;
     if (bq) {
       bits.w[0] = __ballot(ref != INFINITY);
-      if (bits.w[0] != (nv >= 32 ? 0xffffffffull : (1ull << nv) - 1)) { stQ.keep(bits); stG.keep(bits); }
+      // (past the last row the one row of a broadcast gradient would be read again)
+      if (bits.w[0] != (nv >= 32 ? 0xffffffffull : (1ull << nv) - 1) || a.go_r == 0) { stQ.keep(bits); stG.keep(bits); }
       stQ.store(sQ, TK);
       stG.store(sG, TK);
       if (l < TK) sL[l] = ref;

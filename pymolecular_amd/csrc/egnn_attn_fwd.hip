@@ -85,11 +85,13 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
   for (; j < j1; j += stride) {
     const int n = rows_at(j);
     Bits<KT> bits = step_bits<KT>(n);
-    if (a.mask) {                            // what a masked value holds must not meet a probability of 0
+    // what a masked value holds must not meet a probability of 0, nor what the one row of a broadcast v does past the last
+    // key (other rows there read as zeros)
+    if (a.mask) {
 #pragma unroll
       for (int k = 0; k < Bits<KT>::N; ++k) bits.w[k] &= __ballot(mb[k] != 0);
-      stV.keep(bits);
     }
+    if (a.mask || a.v_r == 0) stV.keep(bits);
     tile_sync<SH>();                         // the step before has read the tile
     stK.store(sK, n);
     stV.store(sV, n);
@@ -271,7 +273,7 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
     kbits = (uint32_t)__ballot(key);
     if (bq) stQ.store(sQ, TK);
     if (bk) {
-      if (a.mask) {                          // what a masked value holds must not meet a probability of 0
+      if (a.mask || a.v_r == 0) {            // as in fwd_tile
         Bits<1> bits;
         bits.w[0] = kbits;
         stV.keep(bits);
