@@ -106,6 +106,23 @@ template <typename T> __device__ __forceinline__ typename Num<T>::Frag chain_fra
 template <> __device__ __forceinline__ bf16x8 chain_frag<bf16>(const f32x4& lo, const f32x4& hi) { return pack_chunk_bf16(lo, hi); }
 template <> __device__ __forceinline__ split::Chunk3 chain_frag<float>(const f32x4& lo, const f32x4& hi) { return split::split_chunk(lo, hi); }
 
+// the bits of chain_frag's values whose row's bit is set: rows 0 .. 3 and 16 .. 19
+__device__ __forceinline__ u32x4 chain_rows(uint32_t b) {
+  u32x4 m;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = b >> (16 * (i / 2) + 2 * (i & 1));
+    m[i] = ((x & 1) ? 0xffffu : 0u) | ((x & 2) ? 0xffff0000u : 0u);
+  }
+  return m;
+}
+__device__ __forceinline__ bf16x8 masked(const bf16x8& r, const u32x4& m) {
+  return __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, r) & m);
+}
+__device__ __forceinline__ split::Chunk3 masked(const split::Chunk3& r, const u32x4& m) {
+  return split::Chunk3{masked(r.p0, m), masked(r.p1, m), masked(r.p2, m)};
+}
+
 __device__ __forceinline__ bf16x8 negate(const bf16x8& r, uint32_t flip) {
   u32x4 u = __builtin_bit_cast(u32x4, r);
   const uint32_t f = flip | (flip >> 16);

@@ -381,6 +381,12 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
       Frag FP[R], FS[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) { FP[r] = chain_frag<T>(P[r][0], P[r][1]); FS[r] = chain_frag<T>(dS[r][0], dS[r][1]); }
+      // rows that take no part are zeros, and 0 times an infinity of a key is NaN
+      if (const uint32_t b = bits.step(t); b != 0xffffffffu) {
+        const u32x4 m = chain_rows(b >> (4 * g));
+#pragma unroll
+        for (int r = 0; r < R; ++r) { FP[r] = masked(FP[r], m); FS[r] = masked(FS[r], m); }
+      }
 #pragma unroll
       for (int b = 0; b < TL::NB; ++b) {
         const Frag A = TL::cols(sG, t, b, c, g), B = TL::cols(sQ, t, b, c, g);
@@ -436,8 +442,9 @@ __global__ __launch_bounds__(64 * W, (SH ? group_occupancy<T, DP, R>() : 1)) voi
   dq_tile<T, DP, R, W, SH, KT, EX>(a, it, e, vq0, qs, lds[SH ? 0 : w][0], lds[SH ? 0 : w][1], w);
 }
 
+// (bf16, D = 32, 128 rows: 128 registers, four waves a SIMD; 136 took 64 chains of 512 rows from 68 to 72 us)
 template <typename T, int DP, int R, int W, bool SH, int KT>
-__global__ __launch_bounds__(64 * W, SH ? 2 : 1) void dkv_kernel(Args a, uint32_t n_items) {
+__global__ __launch_bounds__(64 * W, SH ? (Num<T>::planes == 1 && DP <= 32 ? 4 : 2) : 1) void dkv_kernel(Args a, uint32_t n_items) {
   typedef Tile<T, DP, KT> TL;
   constexpr int BK = 16 * R * (SH ? W : 1);
   __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
@@ -551,7 +558,7 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
       }
     }
     delta = col_sum(delta);
-    if (g == 0) sD[16 * q + c] = -delta;
+    if (g == 0) sD[16 * q + c] = ref == INFINITY ? 0.f : -delta;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -589,8 +596,8 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
       S[q] = TL::product(sQ, q, Kc, c, g, zero4());
       dS[q] = TL::product(sG, q, Vc, c, g, nD);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        S[q][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][i], c2, -Lr[i]));
+      for (int i = 0; i < 4; ++i) {        // rows that take no part are zeros, and 0 times an infinity of a key is NaN
+        S[q][i] = Lr[i] == INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][i], c2, -Lr[i]));
         dS[q][i] *= S[q][i];
       }
     }

@@ -58,3 +58,22 @@ def test_broadcast_rows(shape, dtype):
     q, k, v, go, a, b = _case(*shape, dtype)
     go[0, :, 2] = -INF
     _compare(q, k, v, go[:1].expand(go.shape), a, b, ["out", "dv"])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_an_infinite_key(shape, dtype):
+    # all scores of a key are -inf: no probability, no gradient of it, and the other keys' are finite; dq is 0 times an
+    # infinity in that feature
+    q, k, v, go, a, b = _case(*shape, dtype)
+    k[3, 0, 2] = -INF
+    _compare(q.abs(), k, v, go, a, b, ["out", "dq", "dk", "dv"])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_infinite_values(shape, dtype):
+    # an infinity of a value reaches the segment's outputs in its feature; dv, made without it, stays finite
+    q, k, v, go, a, b = _case(*shape, dtype)
+    v[3, 0, 5], v[2, 0, 1] = INF, -INF
+    _compare(q, k, v, go, a, b, ["out", "dv"])
