@@ -54,10 +54,12 @@ Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest,
 }
 // The widest form whose registers hold the tile without spills; -1: form 1 alone
 int widest_q(const EgnnAttnDims* d) { return d->dtype == EGNN_F32 && d->D > 64 ? -1 : 2; }
+int widest_dq(const EgnnAttnDims* d) { return d->dtype == EGNN_BF16 && d->D > 64 ? 1 : widest_q(d); }
 int widest_k(const EgnnAttnDims* d) {
   return d->dtype == EGNN_F32 && d->D > 64 ? -1 : d->D > (d->dtype == EGNN_F32 ? 32 : 64) ? 1 : 2;
 }
 Plan plan_q(const EgnnAttnDims* d) { return make_plan(d->Nq * (d->Hq / d->Hkv), d->Nk, d->n_seg, d->Hkv, widest_q(d), d->dtype == EGNN_F32, d->D); }
+Plan plan_dq(const EgnnAttnDims* d) { return make_plan(d->Nq * (d->Hq / d->Hkv), d->Nk, d->n_seg, d->Hkv, widest_dq(d), d->dtype == EGNN_F32, d->D); }
 Plan plan_k(const EgnnAttnDims* d) { return make_plan(d->Nk, d->Nq * (d->Hq / d->Hkv), d->n_seg, d->Hkv, widest_k(d), d->dtype == EGNN_F32, d->D); }
 
 size_t fwd_bytes(const EgnnAttnDims* d) {
@@ -66,8 +68,9 @@ size_t fwd_bytes(const EgnnAttnDims* d) {
 }
 size_t delta_bytes(const EgnnAttnDims* d) { return align_up((size_t)d->Nq * d->Hq * 4); }
 size_t bwd_bytes(const EgnnAttnDims* d) {
-  const Plan pq = plan_q(d), pk = plan_k(d);
-  const size_t q = pq.nsplit == 1 ? 0 : (size_t)pq.nsplit * d->Nq * d->Hq * padded(d->D) * 4;
+  const Plan pq = plan_dq(d), pk = plan_k(d);
+  // sums of ds k; of bf16 also of p k and of ds
+  const size_t q = pq.nsplit == 1 ? 0 : (size_t)pq.nsplit * d->Nq * d->Hq * (d->dtype == EGNN_BF16 ? 2 * padded(d->D) + 1 : padded(d->D)) * 4;
   const size_t k = pk.nsplit == 1 ? 0 : (size_t)pk.nsplit * d->Nk * d->Hkv * 2 * padded(d->D) * 4;
   return delta_bytes(d) + (q > k ? q : k);
 }
@@ -156,7 +159,7 @@ int32_t egnn_attn_bwd(const EgnnAttnDims* d, const EgnnAttnStrides* s, const voi
   EGNN_TRY(check_view(grad_q, d->Nq, d->Hq, d->D, s->grad_q_row, s->grad_q_head, d->Hq / d->Hkv, esz, true));
   EGNN_TRY(check_view(grad_k, d->Nk, d->Hkv, d->D, s->grad_k_row, s->grad_k_head, 1, esz, true));
   EGNN_TRY(check_view(grad_v, d->Nk, d->Hkv, d->D, s->grad_v_row, s->grad_v_head, 1, esz, true));
-  const Plan pq = plan_q(d), pk = plan_k(d);
+  const Plan pq = plan_dq(d), pk = plan_k(d);
   if (!grid_ok(d, pq) || !grid_ok(d, pk)) return EGNN_ERR_DIMS;
   const size_t need = bwd_bytes(d);
   if (need && (!workspace || workspace_bytes < need)) return EGNN_ERR_WORKSPACE;

@@ -5,14 +5,18 @@
 // heads of the group); each sum is made by one owner in a fixed order, so there are no atomics.  That takes seven products
 // where one kernel with atomics on dq would take five.
 //
-// delta.  o is the rounded output, so in bf16 do . o is off by up to 2^-9 |do| |o|, which shows in dq and dk where a row
-// has few keys that count.  As sum_j p_ij = 1, delta is also sum_j p_ij dp_ij, and the ds made with a delta' sum to
-// delta - delta'.  Short segments (below 256 rows on average) therefore get the exact one: a wave that has all keys of
-// its rows in one step (molecules) makes it from p and dp and reads no o; the 64-row workgroups also sum p_ij k_j (one
-// product more) and take (delta - delta') sum_j p_ij k_j off dq, and dk's kernel reads the corrected delta: errors of dq
-// and dk against 64 bits 2.8e-3 -> 2.4e-3 of their norm at 80 keys (2.3e-3 is what rounding ds and the result costs), for
-// 1.4 us of 50.  Longer ones keep do . o: at 512 keys the extra product would cost 5 us of 71, at D = 64 its registers
-// would spill.
+// delta.  o is the rounded output, so in bf16 do . o is off by up to 2^-9 |do| |o|, and the ds made with it sum to that
+// instead of 0.  Where keys and values have a common part (a projection's bias), o has it too and dq takes the error times
+// that of the keys: with three times the spread of the values in both, dq was off by 7 % of its norm at 512 keys and by 13 %
+// at 4,000, with ten times by as much as it is long.  As sum_j p_ij = 1, delta is also sum_j p_ij dp_ij, and the ds made with
+// a delta' sum to delta - delta'.  So in bf16 dq's kernel also sums p_ij k_j (one product more) and takes
+// (delta - delta') sum_j p_ij k_j off dq, and dk's kernel reads the corrected delta; a wave that has all keys of its rows in
+// one step (molecules) makes delta from p and dp at once and reads no o.  Left is the rounding of ds: errors of dq against
+// 64 bits with 0, 1, 3 and 10 times the spread 2.4e-3, 2.9e-3, 5.2e-3 and 1.6e-2 of its norm.  The cost, backward alone:
+// 64 x 512 rows, D = 32, 53.6 -> 59.9 us; 12,289 rows, D = 64, 600 -> 680; 80-row slabs and molecules 0 to 1 %.
+// Only segments of more than 32 rows in batches of up to 28 a segment on average keep do . o for dk, whose workgroups run
+// beside dq's in one launch (a launch more: 14.2 -> 16.6 us, 1,024 molecules); dk is off by 2^-9 |do| |o| p_ij |q_i|, without
+// the keys' common part.  fp32 keeps do . o, whose error is one of fp32.
 //
 // Measured: 12,289 rows, 4 heads of 64, bf16, dq 240 us and dk, dv 337 us, 0.97 and 0.92 PFLOP/s of the products they make
 // (three and four), bound by vector and MFMA issue (0.43 and 0.41, 0.36 and 0.38 of the cycles) and, of dk and dv, by two
@@ -171,13 +175,13 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
       Frag F[R], FP[EX ? R : 1];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        if constexpr (EX) FP[r] = chain_frag<T>(P[r][0], P[r][1]);
+        if constexpr (EX) if (!one) FP[r] = chain_frag<T>(P[r][0], P[r][1]);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             dS[r][h][i] *= P[r][h][i];
-            if constexpr (EX || !SH) sum[r] += dS[r][h][i];
+            if constexpr (EX) sum[r] += dS[r][h][i];
           }
         F[r] = chain_frag<T>(dS[r][0], dS[r][1]);
       }
@@ -188,7 +192,7 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
         for (int r = 0; r < R; ++r) {
           if constexpr (KT == 1) dQ[r][b].one(A, F[r]);
           else dQ[r][b].add(A, F[r]);
-          if constexpr (EX) PK[r][b].add(A, FP[r]);
+          if constexpr (EX) if (!one) PK[r][b].add(A, FP[r]);
         }
       }
     }
@@ -202,10 +206,11 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
   const float sc = signed_scale(a);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    if ((EX || !SH) && !one && a.nsplit == 1) {
-      const float off = col_sum(sum[r]);     // delta less the one that the ds were made with
-      delta[r] += off;
-      if constexpr (EX) {
+    float off = 0.f;                         // of these keys: delta less the one that the ds were made with
+    if constexpr (EX) {
+      if (!one) off = col_sum(sum[r]);
+      if (a.nsplit == 1) {
+        delta[r] += off;
 #pragma unroll
         for (int b = 0; b < TL::NB; ++b) dQ[r][b].v -= PK[r][b].v * off;
       }
@@ -213,9 +218,14 @@ __device__ __forceinline__ void dq_tile(const Args& a, const Item& it, int e, in
     if (!live[r]) continue;
     if (a.delta && it.sp == 0 && g == 0) a.delta[(int64_t)head[r] * a.Nq + row[r]] = none[r] ? 0.f : delta[r];
     if (a.nsplit > 1) {
-      float* p = a.part + ((int64_t)it.sp * a.Nq * a.Hq + (int64_t)row[r] * a.Hq + head[r]) * DP;
+      const int64_t rows = (int64_t)a.Nq * a.Hq, x = (int64_t)it.sp * rows + (int64_t)row[r] * a.Hq + head[r];
+      float* p = a.part + x * ((EX ? 2 : 1) * DP);
 #pragma unroll
-      for (int b = 0; b < TL::NB; ++b) store4(p + 16 * b + 4 * g, none[r] ? zero4() : dQ[r][b].v);
+      for (int b = 0; b < TL::NB; ++b) {
+        store4(p + 16 * b + 4 * g, none[r] ? zero4() : dQ[r][b].v);
+        if constexpr (EX) store4(p + DP + 16 * b + 4 * g, none[r] ? zero4() : PK[r][b].v);
+      }
+      if constexpr (EX) if (g == 0) a.part[a.nsplit * rows * (2 * DP) + x] = none[r] ? 0.f : off;
       continue;
     }
     T* out = (T*)a.gq + row[r] * a.gq_r + head[r] * a.gq_h;
@@ -427,8 +437,11 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
   }
 }
 
+template <typename T, int DP, int R> constexpr int dq_occupancy() {
+  return Num<T>::planes == 1 ? (R == 2 ? (DP <= 16 ? 4 : DP == 32 ? 3 : 2) : DP <= 64 ? 4 : 3) : 2;
+}
 template <typename T, int DP, int R, int W, bool SH, int KT, bool EX>
-__global__ __launch_bounds__(64 * W, (SH ? group_occupancy<T, DP, R>() : 1)) void dq_kernel(Args a, uint32_t n_items) {
+__global__ __launch_bounds__(64 * W, (SH ? dq_occupancy<T, DP, R>() : 1)) void dq_kernel(Args a, uint32_t n_items) {
   typedef Tile<T, DP, KT> TL;
   constexpr int BQ = 16 * R * (SH ? W : 1);
   __shared__ __attribute__((aligned(16))) bf16 lds[SH ? 1 : W][2][TL::elems];
@@ -664,7 +677,7 @@ __global__ __launch_bounds__(64 * W, (short_occupancy<T, DP>())) void short_kern
     }
     for (int x = x0; x < TK && r0 + x < nv; x += 16 * P) {
       wave_sync();
-      dq_tile<T, DP, 1, W, false, 1, false>(a, Item{slot, h0, 0}, e, r0 + x, own, t2, t2 + TL::elems, 0);
+      dq_tile<T, DP, 1, W, false, 1, Num<T>::planes == 1>(a, Item{slot, h0, 0}, e, r0 + x, own, t2, t2 + TL::elems, 0);
     }
     if (n_k) return;
   } else {
@@ -714,6 +727,44 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int n
   }
   if (r < n) store4(o.p + (r / heads) * o.rs + (r % heads) * o.hs + f, s * o.mul);
 }
+// dq of the splits whose rows hold sum_j ds_j k_j and sum_j p_j k_j, DP values each, and behind all rows sum_j ds_j: the last
+// is what delta lacked, over all splits.  It is added to the row's delta, which dk's kernel reads.
+template <typename T, int GR>
+__global__ __launch_bounds__(256) void join_dq_kernel(const float* part, int nsplit, int64_t rows, int heads, int D, int DP, Out<T> o,
+                                                      float* delta) {
+  constexpr int PB = 256 / GR;
+  __shared__ f32x4 red[2][GR][PB];
+  __shared__ float reds[GR][PB];
+  const int x = threadIdx.x % PB, k = threadIdx.x / PB;
+  const int64_t n = rows * heads, t = (int64_t)blockIdx.x * PB + x;
+  const int64_t r = t / (D / 4);
+  const int f = 4 * (int)(t - r * (D / 4));
+  const float* offs = part + nsplit * n * (2 * DP);
+  f32x4 s = zero4(), pk = zero4();
+  float off = 0.f;
+  if (r < n) {
+#pragma unroll 4
+    for (int i = k; i < nsplit; i += GR) {
+      const float* p = part + (i * n + r) * (2 * DP) + f;
+      s += load4_f32(p);
+      pk += load4_f32(p + DP);
+      off += offs[i * n + r];
+    }
+  }
+  if constexpr (GR > 1) {
+    red[0][k][x] = s;
+    red[1][k][x] = pk;
+    reds[k][x] = off;
+    __syncthreads();
+    if (k) return;
+#pragma unroll 4
+    for (int i = 1; i < GR; ++i) { s += red[0][i][x]; pk += red[1][i][x]; off += reds[i][x]; }
+  }
+  if (r >= n) return;
+  const int64_t row = r / heads, head = r % heads;
+  store4(o.p + row * o.rs + head * o.hs + f, (s - pk * off) * o.mul);
+  if (f == 0) delta[head * rows + row] += off;
+}
 template <typename T>
 static void sum_parts(const float* part, int nsplit, int64_t rows, int heads, int D, int DP, Out<T> one, Out<T> two, hipStream_t st) {
   const int64_t n = rows * heads * (D / 4);
@@ -725,18 +776,19 @@ static void sum_parts(const float* part, int nsplit, int64_t rows, int heads, in
   else sum_parts_kernel<T, 32><<<dim3((uint32_t)cdiv(n, 8), outs), 256, 0, st>>>(part, nsplit, rows, heads, D, DP, width, one, two);
 }
 
+template <typename T>
+static void join_dq(const Args& a, int DP, Out<T> o, hipStream_t st) {
+  const int64_t n = (int64_t)a.Nq * a.Hq * (a.D / 4);
+  if (a.nsplit <= 16) join_dq_kernel<T, 1><<<(uint32_t)cdiv(n, 256), 256, 0, st>>>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, o, a.delta);
+  else if (a.nsplit <= 128) join_dq_kernel<T, 8><<<(uint32_t)cdiv(n, 32), 256, 0, st>>>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, o, a.delta);
+  else join_dq_kernel<T, 32><<<(uint32_t)cdiv(n, 8), 256, 0, st>>>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, o, a.delta);
+}
+
 template <typename T, int DP, int R, int W, bool SH, int KT>
 static void go_q(const Args& a, const Plan& p, hipStream_t st) {
   const int64_t n = p.slots * a.Hkv * a.nsplit;
-  constexpr bool can = SH && Num<T>::planes == 1 && R == 1;
   in_parts(a, SH ? n : cdiv(n, W), [&](const Args& x, uint32_t blocks) {
-    if constexpr (can) {
-      if (a.nsplit == 1) {
-        dq_kernel<T, DP, R, W, SH, KT, true><<<blocks, 64 * W, 0, st>>>(x, (uint32_t)n);
-        return;
-      }
-    }
-    dq_kernel<T, DP, R, W, SH, KT, false><<<blocks, 64 * W, 0, st>>>(x, (uint32_t)n);
+    dq_kernel<T, DP, R, W, SH, KT, Num<T>::planes == 1><<<blocks, 64 * W, 0, st>>>(x, (uint32_t)n);
   });
 }
 template <typename T, int DP, int R, int W, bool SH, int KT>
@@ -788,9 +840,12 @@ static int launch_t(Args a, const Plan& pq, const Plan& pk, hipStream_t st) {
     if constexpr (wide) go_q<T, DP, 1, 4, true, KT>(a, pq, st);
     else if (pq.form == 0) go_q<T, DP, 1, W, false, 1>(a, pq, st);
     else if (pq.form == 1) go_q<T, DP, 1, 4, true, KT1>(a, pq, st);
-    else go_q<T, DP, 2, 4, true, KT>(a, pq, st);
-    if (a.nsplit > 1)
-      sum_parts<T>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, Out<T>{(T*)a.gq, a.gq_r, a.gq_h, signed_scale(a)}, Out<T>{}, st);
+    else if constexpr (Num<T>::planes == 3 || DP <= 64) go_q<T, DP, 2, 4, true, KT>(a, pq, st);
+    if (a.nsplit > 1) {
+      const Out<T> gq{(T*)a.gq, a.gq_r, a.gq_h, signed_scale(a)};
+      if constexpr (Num<T>::planes == 1) join_dq<T>(a, DP, gq, st);
+      else sum_parts<T>(a.part, a.nsplit, a.Nq, a.Hq, a.D, DP, gq, Out<T>{}, st);
+    }
   }
   a.nsplit = pk.nsplit;
   a.slots = (uint32_t)pk.slots;
