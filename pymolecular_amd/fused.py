@@ -40,14 +40,10 @@ def _stream(device: torch.device) -> int:
 
 
 def _recorded(*tensors: Optional[torch.Tensor]) -> bool:
-    """Whether something has to see a call on these tensors: autograd, a tracer (which would record the allocation of the
-    result and not the library's work) or forward-mode differentiation (whose tangents the library does not know).  Such a
-    call goes through the operator's autograd function, which a trace calls again and which refuses a tangent."""
-    if torch.jit.is_tracing():
-        return True
-    grad = torch.is_grad_enabled()
-    return any(t is not None and ((grad and t.requires_grad) or forward_ad.unpack_dual(t).tangent is not None)
-               for t in tensors)
+    """Whether something has to see a call on these tensors: a tracer (which would record the allocation of the result and
+    not the library's work) or forward-mode differentiation (whose tangents the library does not know).  Such a call goes
+    through the operator's autograd function, which a trace calls again and which refuses a tangent."""
+    return torch.jit.is_tracing() or any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _FirstOrderFn(torch.autograd.Function):

@@ -149,7 +149,11 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5, residual: Optional[torch.Tensor] = None):
     """``y``, or ``(y, x + residual)`` with a residual (module docstring).  Differentiable in x, weight, bias and
     residual."""
-    if _recorded(x, weight, bias, residual):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return LayerNormFn.apply(x, weight, bias, eps, residual)
-    y, s, _, _ = layer_norm_forward(x, weight, bias, eps, residual, need_stats=False)
-    return y if residual is None else (y, s)
+    r = _capi.ext().norm_forward(x, weight, bias, eps, residual, False)
+    if r is None:   # a tensor needs a conversion, or the call has to be recorded
+        if _recorded(x, weight, bias, residual):
+            return LayerNormFn.apply(x, weight, bias, eps, residual)
+        r = layer_norm_forward(x, weight, bias, eps, residual, need_stats=False)
+    return r[0] if residual is None else (r[0], r[1])

@@ -208,13 +208,25 @@ def _parts(qkv, heads):
     return qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
 
 
+def _inference(q, k, v, q_ptr, kv_ptr, key_mask, scale):
+    """The output alone, or None where the call has to be recorded (the native entry refuses such tensors by itself)."""
+    r = _capi.ext().attn_forward(q, k, v, q_ptr, kv_ptr, key_mask, _scale(q, scale), False)
+    if r is not None:
+        return r[0]
+    if _recorded(q, k, v):
+        return None
+    return segment_attention_forward(q, k, v, q_ptr, kv_ptr, key_mask, scale, need_lse=False)[0]
+
+
 def segment_attention_qkv(qkv: torch.Tensor, heads: int, seg_ptr: torch.Tensor, key_mask: Optional[torch.Tensor] = None,
                           scale: Optional[float] = None) -> torch.Tensor:
     """:func:`segment_attention` of each segment over itself, with queries, keys and values in the rows of one projection:
     ``qkv`` (N, heads + 2 kv_heads, d) -> (N, heads, d)."""
-    if _recorded(qkv):
-        return SegmentAttentionQKVFn.apply(qkv, heads, seg_ptr, key_mask, scale)
-    return segment_attention_forward(*_parts(qkv, heads), seg_ptr, None, key_mask, scale, need_lse=False)[0]
+    if not (torch.is_grad_enabled() and qkv.requires_grad):
+        r = _inference(*_parts(qkv, heads), seg_ptr, None, key_mask, scale)
+        if r is not None:
+            return r
+    return SegmentAttentionQKVFn.apply(qkv, heads, seg_ptr, key_mask, scale)
 
 
 def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_ptr: torch.Tensor,
@@ -222,6 +234,8 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_ptr: 
                       scale: Optional[float] = None) -> torch.Tensor:
     """Attention of each segment's queries over its keys (module docstring), (Nq, heads, d); ``scale`` defaults to
     d ** -0.5.  Differentiable in q, k and v."""
-    if _recorded(q, k, v):
-        return SegmentAttentionFn.apply(q, k, v, q_ptr, kv_ptr, key_mask, scale)
-    return segment_attention_forward(q, k, v, q_ptr, kv_ptr, key_mask, scale, need_lse=False)[0]
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        r = _inference(q, k, v, q_ptr, kv_ptr, key_mask, scale)
+        if r is not None:
+            return r
+    return SegmentAttentionFn.apply(q, k, v, q_ptr, kv_ptr, key_mask, scale)
