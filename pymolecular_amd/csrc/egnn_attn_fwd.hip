@@ -44,6 +44,7 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
   stV.offsets(offV, vrb, a.D);
   const T *kb = (const T*)a.k + it.kvh * a.k_h, *vb = (const T*)a.v + it.kvh * a.v_h;
   uint8_t mb[Bits<KT>::N];
+  const bool masked = a.mask || a.v_r == 0;
   auto rows_at = [&](int j) { return j1 - j < KS ? j1 - j : KS; };
   auto fetch = [&](int j) {
     const int n = rows_at(j);
@@ -87,11 +88,13 @@ __device__ __forceinline__ void fwd_tile(const Args& a, const Item& it, int e, i
     Bits<KT> bits = step_bits<KT>(n);
     // what a masked value holds must not meet a probability of 0, nor what the one row of a broadcast v does past the last
     // key (other rows there read as zeros)
-    if (a.mask) {
+    if (masked) {
+      if (a.mask) {
 #pragma unroll
-      for (int k = 0; k < Bits<KT>::N; ++k) bits.w[k] &= __ballot(mb[k] != 0);
+        for (int k = 0; k < Bits<KT>::N; ++k) bits.w[k] &= __ballot(mb[k] != 0);
+      }
+      stV.keep(bits);
     }
-    if (a.mask || a.v_r == 0) stV.keep(bits);
     tile_sync<SH>();                         // the step before has read the tile
     stK.store(sK, n);
     stV.store(sV, n);
