@@ -69,28 +69,23 @@ template <typename T, bool TAIL = true> struct Vec {
     }
   }
 };
-// a piece of the weight or the bias, which may be fp32 beside bf16 rows: rounded to bf16 they would lose what training
-// accumulates in them
-template <typename T, bool TAIL> __device__ __forceinline__ void load_params(const void* p, bool f32, int f, int C, float* v) {
-  typedef Vec<T, TAIL> V;
-  if constexpr (sizeof(T) == 2) {
-    if (f32) {
-      const float* q = (const float*)p;
-      if (!TAIL || C >= V::N) {
-        Vec<float, false>::load(q, f, C, v);
-        Vec<float, false>::load(q, f + 4, C, v + 4);
-      } else {
+// A piece of the weight or the bias, of type P: T, or float beside bf16 rows (rounded to bf16 they would lose what training
+// accumulates in them).
+template <typename T, typename P, bool TAIL> __device__ __forceinline__ void load_params(const void* p, int f, int C, float* v) {
+  constexpr int N = Vec<T, TAIL>::N;
+  if constexpr (std::is_same<T, P>::value) Vec<T, TAIL>::load((const T*)p, f, C, v);
+  else {
+    const P* q = (const P*)p;
+    if (!TAIL || C >= N) {
+      Vec<P, false>::load(q, f, C, v);
+      Vec<P, false>::load(q, f + N / 2, C, v + N / 2);
+    } else {
 #pragma unroll
-        for (int i = 0; i < V::N; ++i) v[i] = i < C ? q[i] : 0.f;
-      }
-      return;
+      for (int i = 0; i < N; ++i) v[i] = i < C ? q[i] : 0.f;
     }
   }
-  V::load((const T*)p, f, C, v);
 }
-template <typename T> __device__ __forceinline__ float param(const void* p, bool f32, int f) {
-  return sizeof(T) == 2 && f32 ? ((const float*)p)[f] : to_f32(((const T*)p)[f]);
-}
+template <typename P> __device__ __forceinline__ float param(const void* p, int f) { return to_f32(((const P*)p)[f]); }
 // the lane's piece number k of a row: its first column, and how many of its columns another piece has (all of them: no
 // such piece)
 struct Piece {
@@ -115,7 +110,7 @@ template <int LPR> __device__ __forceinline__ float row_sum(float v) {
 
 constexpr int NT = 256;
 
-template <typename T, int LPR, int VPL, bool TAIL>
+template <typename T, typename P, int LPR, int VPL, bool TAIL>
 __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
   typedef Vec<T, TAIL> V;
   constexpr int VEC = V::N;
@@ -186,8 +181,8 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
       float w[VEC], b[VEC], y[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) { w[i] = 1.f; b[i] = 0.f; }
-      if (a.w) load_params<T, TAIL>(a.w, a.f32_params, c[p].f, a.C, w);
-      if (a.b) load_params<T, TAIL>(a.b, a.f32_params, c[p].f, a.C, b);
+      if (a.w) load_params<T, P, TAIL>(a.w, c[p].f, a.C, w);
+      if (a.b) load_params<T, P, TAIL>(a.b, c[p].f, a.C, b);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) y[i] = __builtin_fmaf((v[p][i] - mean) * rstd, w[i], b[i]);
       V::store((T*)a.y + n * a.C, c[p].f, a.C, y);
@@ -213,7 +208,10 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
     c[p] = piece_of<VEC, TAIL>(p * LPR + lane, a.C);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) { gw[p][i] = 0.f; gb[p][i] = 0.f; w[p][i] = 1.f; }
-    if (a.w && c[p].in) load_params<T, TAIL>(a.w, a.f32_params, c[p].f, a.C, w[p]);
+    if (a.w && c[p].in) {                    // (once a block: no kernel of its own for fp32 parameters)
+      if (sizeof(T) == 2 && a.f32_params) load_params<T, float, TAIL>(a.w, c[p].f, a.C, w[p]);
+      else load_params<T, T, TAIL>(a.w, c[p].f, a.C, w[p]);
+    }
   }
   const int64_t step = (int64_t)gridDim.x * RG;
   typename V::piece pg[VPL], px[VPL], pe[VPL];
@@ -299,7 +297,7 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
   __syncthreads();
   return buf[0] + buf[1] + buf[2] + buf[3];
 }
-template <typename T>
+template <typename T, typename P>
 __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
   __shared__ float buf[4];
   const int64_t n = blockIdx.x;
@@ -322,12 +320,12 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
     if (threadIdx.x == 0) { a.mean[n] = m; a.rstd[n] = rs; }
   }
   for (int f = threadIdx.x; f < a.C; f += NT) {
-    const float v = val(f), w = a.w ? param<T>(a.w, a.f32_params, f) : 1.f, b = a.b ? param<T>(a.b, a.f32_params, f) : 0.f;
+    const float v = val(f), w = a.w ? param<P>(a.w, f) : 1.f, b = a.b ? param<P>(a.b, f) : 0.f;
     if (r) ((T*)a.s)[n * a.C + f] = from_f32<T>(v);
     ((T*)a.y)[n * a.C + f] = from_f32<T>(__builtin_fmaf((v - mean) * rstd, w, b));
   }
 }
-template <typename T>
+template <typename T, typename P>
 __global__ __launch_bounds__(NT) void bwd_wide_kernel(Args a) {
   __shared__ float buf[4];
   const int64_t n = blockIdx.x;
@@ -335,13 +333,13 @@ __global__ __launch_bounds__(NT) void bwd_wide_kernel(Args a) {
   const float mean = a.mean[n], rstd = a.rstd[n];
   float s1 = 0.f, s2 = 0.f;
   for (int f = threadIdx.x; f < a.C; f += NT) {
-    const float t = to_f32(g[f]) * (a.w ? param<T>(a.w, a.f32_params, f) : 1.f);
+    const float t = to_f32(g[f]) * (a.w ? param<P>(a.w, f) : 1.f);
     s1 += t;
     s2 = __builtin_fmaf(t, (to_f32(x[f]) - mean) * rstd, s2);
   }
   const float m1 = block_sum(s1, buf) / a.C, m2 = block_sum(s2, buf) / a.C;
   for (int f = threadIdx.x; f < a.C; f += NT) {
-    const float t = to_f32(g[f]) * (a.w ? param<T>(a.w, a.f32_params, f) : 1.f);
+    const float t = to_f32(g[f]) * (a.w ? param<P>(a.w, f) : 1.f);
     float o = rstd * (t - m1 - (to_f32(x[f]) - mean) * rstd * m2);
     if (a.gsum) o += to_f32(((const T*)a.gsum)[n * a.ldgs + f]);
     ((T*)a.gx)[n * a.C + f] = from_f32<T>(o);
@@ -430,7 +428,10 @@ static void in_parts(const Args& a, int rows_per_block, Go go) {
 template <typename T, int LPR, int VPL, bool TAIL>
 static void launch_tail(const Args& a, bool bwd, hipStream_t st, int* nblk) {
   if (!bwd) {
-    in_parts<T>(a, NT / LPR, [&](const Args& x, uint32_t blocks) { fwd_kernel<T, LPR, VPL, TAIL><<<blocks, NT, 0, st>>>(x); });
+    in_parts<T>(a, NT / LPR, [&](const Args& x, uint32_t blocks) {
+      if (sizeof(T) == 2 && a.f32_params) fwd_kernel<T, float, LPR, VPL, TAIL><<<blocks, NT, 0, st>>>(x);
+      else fwd_kernel<T, T, LPR, VPL, TAIL><<<blocks, NT, 0, st>>>(x);
+    });
     return;
   }
   const int64_t n = cdiv(a.N, NT / LPR);
@@ -464,19 +465,25 @@ static void launch_rows(const Args& a, const Shape& s, bool bwd, hipStream_t st,
   }
 }
 
+template <typename T, typename P>
+static void launch_wide(const Args& a, bool bwd, hipStream_t st) {
+  in_parts<T>(a, 1, [&](const Args& x, uint32_t blocks) {
+    if (bwd) bwd_wide_kernel<T, P><<<blocks, NT, 0, st>>>(x);
+    else fwd_wide_kernel<T, P><<<blocks, NT, 0, st>>>(x);
+  });
+}
 template <typename T>
 static int launch(const Args& a, bool bwd, hipStream_t st) {
   Shape s;
   int nblk = 0;
   if (a.N) {
-    if (shape_of((int)cdiv(a.C, Vec<T>::N), a.N, &s)) launch_rows<T>(a, s, bwd, st, &nblk);
-    else if (!bwd) in_parts<T>(a, 1, [&](const Args& x, uint32_t blocks) { fwd_wide_kernel<T><<<blocks, NT, 0, st>>>(x); });
-    else {
-      in_parts<T>(a, 1, [&](const Args& x, uint32_t blocks) { bwd_wide_kernel<T><<<blocks, NT, 0, st>>>(x); });
-      if (a.part) {
-        nblk = (int)(part_rows(a.N) < 128 ? part_rows(a.N) : 128);
-        bwd_wide_weights_kernel<T><<<dim3((uint32_t)cdiv(a.C, NT), (uint32_t)nblk), NT, 0, st>>>(a);
-      }
+    const bool narrow = shape_of((int)cdiv(a.C, Vec<T>::N), a.N, &s);
+    if (narrow) launch_rows<T>(a, s, bwd, st, &nblk);
+    else if (a.f32_params) launch_wide<T, float>(a, bwd, st);
+    else launch_wide<T, T>(a, bwd, st);
+    if (!narrow && bwd && a.part) {
+      nblk = (int)(part_rows(a.N) < 128 ? part_rows(a.N) : 128);
+      bwd_wide_weights_kernel<T><<<dim3((uint32_t)cdiv(a.C, NT), (uint32_t)nblk), NT, 0, st>>>(a);
     }
   }
   if (bwd && a.part) {
