@@ -328,9 +328,11 @@ int32_t egnn_radius_graph(const double* pos, int64_t N, const int32_t* seg_ptr, 
  * clamped to the rows there are, so no access leaves the tensors whatever they
  * hold; offsets that decrease give unspecified results.
  * Sums, softmax statistics and lse (Hq, Nq) are fp32; bf16 rounds the
- * probabilities and their gradients once, for the second product. */
+ * probabilities and their gradients once, for the second product.  A part that
+ * all keys have in common reaches grad_q by those roundings alone. */
 typedef struct EgnnAttnDims {
-  int64_t Nq, Nk;        /* rows of q, and of k and v; Nq Hq and Nk below 2^31 - 2^18 */
+  int64_t Nq, Nk;        /* rows of q, and of k and v; Nq Hq, Nk and n_seg at most 2^31 - 2^18 - 1, and
+                            (n_seg + 2) Hkv with a sixteenth of Nq Hq, and of Nk Hkv, below 2^31 */
   int32_t n_seg;
   int32_t Hq, Hkv;       /* heads; Hq a multiple of Hkv */
   int32_t D;             /* head width, a multiple of 8 up to 128 */

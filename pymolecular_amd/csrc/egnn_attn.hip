@@ -22,9 +22,9 @@ Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest,
   Plan p;
   // Measured on both sides, forward and backward in us, bf16 unless stated.  A wave a tile, and a whole small segment
   // (form 0), against 64 rows a workgroup (1): 15 .. 32 rows a segment, D = 64: 33.5 and 44.7; 9 .. 40, D = 16: 35 and 51;
-  // 25 .. 45, D = 64: 59 and 41; 20 .. 40, fp32, D = 32: 61 and 37.  64 rows against 128 (2): 80 rows 53 and 61, 100 .. 260
-  // 70 and 75, 256 64 and 60, 512 (D = 32) 86 and 73.  128 rows only where they fill the device, or splits will: 37
-  // chains of 301 in fp32, 8 heads on 2: 52 and 60 (1,406 and 740 workgroups), 12,289 rows 980 and 800.
+  // 25 .. 45, D = 64: 59 and 41; 20 .. 40, fp32, D = 32: 61 and 37.  64 rows against 128 (2), 4 heads: 80 rows, D = 64, 54 and
+  // 61; 100 .. 260, D = 32, 45 and 46; 256 61 and 56 at D = 32, 87 and 86 at 64; 512 94 and 75, 135 and 120.  128 rows only
+  // where they fill the device, or splits will: 37 chains of 301 in fp32, 8 heads on 2, 135 and 156; 12,289 rows 1,252 and 881.
   p.form = mean <= kShortMean ? 0 : mean >= 256 && (items_of(128) >= 1024 || len >= 2048) ? 2 : 1;
   if (widest < 0) p.form = 1;
   else if (p.form > widest) p.form = widest;
@@ -37,7 +37,7 @@ Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest,
   } else if (items < 512 && len >= 512) {
     // Somewhat more workgroups a CU than it holds (four of heads up to 32 wide) and up to six, as evenly on the 256 CUs as
     // may be; a part more costs its share of the joining, per tile about the time of 256 rows in bf16 and 48 in fp32.
-    // (As against 1,024 workgroups or the next number above, forward and backward: one graph of 2,500 rows, 8 heads, 164
+    // (Measured with parts of dq half as wide as bf16 has them now.  As against 1,024 workgroups or the next number above, forward and backward: one graph of 2,500 rows, 8 heads, 164
     // and 135 us; of 20,000, 2 heads on 1, 1,096 and 1,044.  Fewer for heads up to 32 wide: 8,000 rows, 8 heads on 2, dk
     // and dv 182 us in 9 parts and 200 in 8.)
     const int64_t most = len / 128, hi = cdiv(1536, items) < most ? cdiv(1536, items) : most;
@@ -52,7 +52,9 @@ Plan make_plan(int64_t own, int64_t other, int64_t n_seg, int heads, int widest,
   if (p.nsplit > 2048) p.nsplit = 2048;
   return p;
 }
-// The widest form whose registers hold the tile without spills; -1: form 1 alone
+// The widest form whose registers hold the tile; -1: form 1 alone.  (Spills are left where the next smaller form is slower
+// or there is none: of dk and dv, 2 registers at bf16 D = 32 and 3 at fp32 D = 32 with 128 rows, 19 at fp32 above 64.)  dq in
+// bf16 above 64 with 128 rows would spill 95.
 int widest_q(const EgnnAttnDims* d) { return d->dtype == EGNN_F32 && d->D > 64 ? -1 : 2; }
 int widest_dq(const EgnnAttnDims* d) { return d->dtype == EGNN_BF16 && d->D > 64 ? 1 : widest_q(d); }
 int widest_k(const EgnnAttnDims* d) {

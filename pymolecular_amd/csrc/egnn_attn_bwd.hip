@@ -3,7 +3,7 @@
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i.
 // dq's kernel owns tiles of queries and walks the keys, dk and dv's owns tiles of keys and walks the queries (of all
 // heads of the group); each sum is made by one owner in a fixed order, so there are no atomics.  That takes seven products
-// where one kernel with atomics on dq would take five.
+// (eight in bf16, below) where one kernel with atomics on dq would take five.
 //
 // delta.  o is the rounded output, so in bf16 do . o is off by up to 2^-9 |do| |o|, and the ds made with it sum to that
 // instead of 0.  Where keys and values have a common part (a projection's bias), o has it too and dq takes the error times
@@ -14,13 +14,13 @@
 // one step (molecules) makes delta from p and dp at once and reads no o.  Left is the rounding of ds: errors of dq against
 // 64 bits with 0, 1, 3 and 10 times the spread 2.4e-3, 2.9e-3, 5.2e-3 and 1.6e-2 of its norm.  The cost, backward alone:
 // 64 x 512 rows, D = 32, 53.6 -> 59.9 us; 12,289 rows, D = 64, 600 -> 680; 80-row slabs and molecules 0 to 1 %.
-// Only segments of more than 32 rows in batches of up to 28 a segment on average keep do . o for dk, whose workgroups run
-// beside dq's in one launch (a launch more: 14.2 -> 16.6 us, 1,024 molecules); dk is off by 2^-9 |do| |o| p_ij |q_i|, without
-// the keys' common part.  fp32 keeps do . o, whose error is one of fp32.
+// One case keeps do . o for dk: segments of more than 32 rows or keys in batches of short ones (launch_short), where dk's
+// workgroups run beside dq's in one launch (a launch more: 14.2 -> 16.6 us, 1,024 molecules).  There dk takes the error times
+// p_ij q_i: 2.6e-3 instead of 2.3e-3, and 6.7e-3 with three times the spread.  fp32 keeps do . o, whose error is one of fp32.
 //
-// Measured: 12,289 rows, 4 heads of 64, bf16, dq 240 us and dk, dv 337 us, 0.97 and 0.92 PFLOP/s of the products they make
-// (three and four), bound by vector and MFMA issue (0.43 and 0.41, 0.36 and 0.38 of the cycles) and, of dk and dv, by two
-// waves a SIMD; 128 molecules in fp32 8.2 us, bound by latency.
+// Measured (each kernel alone, called back to back): 12,289 rows, 4 heads of 64, bf16, dq 315 us and dk, dv 338 us, 0.98 and
+// 0.91 PFLOP/s of the four products each makes, bound by vector and MFMA issue (0.42 and 0.41, 0.36 and 0.38 of the cycles)
+// and by two waves a SIMD; 128 molecules in fp32 8.2 us, bound by latency.
 #include "egnn_attn.h"
 
 namespace egnn {
@@ -437,6 +437,9 @@ __device__ __forceinline__ void dkv_tile(const Args& a, const Item& it, int e, i
   }
 }
 
+// Waves a SIMD that dq's registers leave room for: the sums of p k take its 128-row tiles to 143 registers at D = 32 and 219
+// at D = 64.  (D = 64 held to three waves spills 50.  The backward of 12,289 rows: as here 680 us, in steps of 32 keys 691, in
+// 64-row tiles 772.)
 template <typename T, int DP, int R> constexpr int dq_occupancy() {
   return Num<T>::planes == 1 ? (R == 2 ? (DP <= 16 ? 4 : DP == 32 ? 3 : 2) : DP <= 64 ? 4 : 3) : 2;
 }
@@ -644,7 +647,8 @@ __device__ __forceinline__ void small_segment(const Args& a, int kvh, const Seg&
 // Waves a SIMD that its registers leave room for: the tiles of long segments would take those of two or three waves, where
 // the small segments, which are most, gain by four or five (left to the compiler and as here: bf16, D = 32, 4,000 segments
 // of 2 .. 10 rows 32.6 and 23.9 us; D = 16, 1,024 molecules and 8 heads 15.7 and 14.6; fp32, D = 16, 2,000 segments and 8
-// heads 58 and 52; the other widths spill in the small segments or have no room for more in LDS).
+// heads 58 and 52), although at D = 16 that spills 18 registers in bf16 and 9 in fp32.  The other widths would spill more, or
+// have no room for more waves in LDS.
 template <typename T, int DP> constexpr int short_occupancy() {
   return Num<T>::planes == 1 ? (DP == 16 ? 5 : DP == 32 ? 3 : 1) : DP == 16 ? 4 : 1;
 }

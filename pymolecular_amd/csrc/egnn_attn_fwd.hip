@@ -7,9 +7,9 @@
 // The sum takes the unrounded probabilities (one more product, against ones, would sum the rounded ones at less
 // cost, and put up to 2^-9 into lse).
 //
-// Measured: 12,289 rows, 4 heads of 64, bf16, 197 us, 0.79 PFLOP/s, bound by vector and MFMA issue, which do not overlap
-// (0.50 and 0.32 of the cycles); one query of 8 heads on 2 over 2,000,000 keys 183 us, 5.6 TB/s, bound by HBM; 128 molecules
-// in fp32 5.2 us, bound by three round trips to memory.
+// Measured (the kernel alone, called back to back): 12,289 rows, 4 heads of 64, bf16, 196 us, 0.79 PFLOP/s, bound by vector
+// and MFMA issue, which do not overlap (0.50 and 0.32 of the cycles); one query of 8 heads on 2 over 2,000,000 keys 183 us,
+// 5.6 TB/s, bound by HBM; 128 molecules in fp32 4.9 us, bound by three round trips to memory.
 #include "egnn_attn.h"
 
 namespace egnn {

@@ -8,9 +8,10 @@
 // where the mean exceeds the deviation the statistics kept for it are those of the stored one: with the others a row whose
 // values differ by less than their rounding would get any gradient (one column of bf16: hundreds of times too large, instead
 // of 0).  Elsewhere the two agree to 2^-9 of the deviation.  (For every row: 402 us instead of 360, 2,000,000 x 128 bf16.)
-// Bound by HBM where the tensors are large: 2,000,000 x 128 bf16 with a residual, forward 358 us and backward 341 us, 5.7 and
-// 6.0 TB/s; 40,961 x 259 fp32, rows that cross lines, 4.0 and 4.6 TB/s.  By its launches where they are small: 2,432 x 128
-// fp32, forward, 3.0 us.
+// Bound by HBM where the tensors are large: 2,000,000 x 128 bf16 with a residual, forward 337 us and backward 323 us, 6.1 and
+// 6.3 TB/s (each kernel alone, called back to back); 40,961 x 259 fp32, rows that cross lines, 18.4 and 23.6 us, 4.6 and 5.4
+// TB/s.  By its launches where they are small: 2,432 x 128 fp32, forward, 2.8 us.  Rows wider than a wave's registers are read
+// value by value, twice or three times: 20,000 x 4,096 bf16, forward and backward, 265 and 395 us, floors 64 and 95.
 #include "egnn_device.h"
 #include "egnn_internal.h"
 #include <type_traits>
