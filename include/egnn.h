@@ -392,6 +392,37 @@ int32_t egnn_norm_bwd(const EgnnNormDims* dims, const void* grad_y, int64_t ldg,
                       const void* weight, const float* mean, const float* rstd, const void* grad_sum, int64_t ldgs,
                       void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- dropout --------------------------------------------------------------------
+ * No counterpart in the reference.  Value (row n, column f) stays where its 16
+ * random bits u are not below cut = round(65536 p), times 65536 / (65536 - cut);
+ * where it does not stay it becomes 0, whatever it was.  u is halfword f % 8
+ * (lower half of a word first) of the four words that the counter-based generator
+ * Philox4x32 with seven rounds makes of the counter (f / 8, n, offset low, offset
+ * high) and the key (seed low, seed high): no mask is stored, the backward makes it
+ * again, and it depends on neither dtype nor strides nor launch. */
+typedef struct EgnnDropout {
+  const int64_t* rng;    /* device memory, read when the call runs: seed, offset */
+  int64_t site;          /* added to the offset: a mask of its own for each dropout of a pass that shares rng */
+  double p;              /* 0 to 1 */
+} EgnnDropout;
+
+/* y (N, C) contiguous = (residual +) dropout(x); residual may be NULL.  On the
+ * gradient of y, without a residual, the same call is the backward.  N below 2^31,
+ * C up to 2^20, any row strides. */
+int32_t egnn_dropout(const EgnnDropout* drop, int32_t dtype, int64_t N, int32_t C, const void* x, int64_t ldx,
+                     const void* residual, int64_t ldr, void* y, void* stream);
+
+/* egnn_norm_fwd of s = residual + dropout(x), and its backward: grad_residual (N, C)
+ * is the gradient of s, grad_x (N, C) its dropout.  The residual and the sum are
+ * not optional here; workspace: egnn_norm_bwd_workspace_bytes. */
+int32_t egnn_norm_drop_fwd(const EgnnNormDims* dims, const EgnnDropout* drop, const void* x, int64_t ldx, const void* residual,
+                           int64_t ldr, const void* weight, const void* bias, void* y, void* sum, float* mean, float* rstd,
+                           void* stream);
+int32_t egnn_norm_drop_bwd(const EgnnNormDims* dims, const EgnnDropout* drop, const void* grad_y, int64_t ldg, const void* sum,
+                           int64_t lds, const void* weight, const float* mean, const float* rstd, const void* grad_sum,
+                           int64_t ldgs, void* grad_x, void* grad_residual, void* grad_weight, void* grad_bias,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,6 +30,7 @@ EXPORTED = (
     "egnn_graph_tmp_bytes", "egnn_knn_graph", "egnn_radius_graph",
     "egnn_attn_fwd_workspace_bytes", "egnn_attn_bwd_workspace_bytes", "egnn_attn_fwd", "egnn_attn_bwd",
     "egnn_norm_fwd", "egnn_norm_bwd_workspace_bytes", "egnn_norm_bwd",
+    "egnn_dropout", "egnn_norm_drop_fwd", "egnn_norm_drop_bwd",
 )
 
 # kernel classes of the instrumentation hook
@@ -75,9 +76,13 @@ class EgnnNormDims(ctypes.Structure):
     _fields_ = [("N", c_int64), ("C", c_int32), ("dtype", c_int32), ("eps", c_float), ("f32_params", c_int32)]
 
 
+class EgnnDropout(ctypes.Structure):
+    _fields_ = [("rng", c_void_p), ("site", c_int64), ("p", ctypes.c_double)]
+
+
 _lib = None
 
-ABI_VERSION = 11   # include/egnn.h egnn_abi_version()
+ABI_VERSION = 12   # include/egnn.h egnn_abi_version()
 
 
 def _check_stamp(path=None, stamp=None, digest=None, what="other sources") -> None:
@@ -184,6 +189,13 @@ def lib() -> ctypes.CDLL:
     L.egnn_norm_bwd_workspace_bytes.argtypes = [MD]
     L.egnn_norm_bwd.restype = c_int32
     L.egnn_norm_bwd.argtypes = [MD, P, c_int64, P, c_int64, P, P, P, P, c_int64, P, P, P, P, c_size_t, P]
+    DR = ctypes.POINTER(EgnnDropout)
+    L.egnn_dropout.restype = c_int32
+    L.egnn_dropout.argtypes = [DR, c_int32, c_int64, c_int32, P, c_int64, P, c_int64, P, P]
+    L.egnn_norm_drop_fwd.restype = c_int32
+    L.egnn_norm_drop_fwd.argtypes = [MD, DR, P, c_int64, P, c_int64] + [P] * 7
+    L.egnn_norm_drop_bwd.restype = c_int32
+    L.egnn_norm_drop_bwd.argtypes = [MD, DR, P, c_int64, P, c_int64, P, P, P, P, c_int64] + [P] * 5 + [c_size_t, P]
     _lib = L
     return L
 

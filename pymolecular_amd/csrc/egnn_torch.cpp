@@ -337,6 +337,52 @@ pybind11::object norm_backward(const Tensor& gy, const Tensor& s, const Opt& w, 
   return pybind11::make_tuple(gx, out(gw), out(gb));
 }
 
+// ---- dropout ------------------------------------------------------------------------
+bool drop_ok(const Tensor& x, double p, const Tensor& rng) { return p >= 0.0 && p <= 1.0 && fits(rng, x, at::kLong, {2}); }
+
+pybind11::object dropout(const Tensor& x, double p, const Tensor& rng, int64_t site, const Opt& res) {
+  if (!norm_ok(x, Opt(), Opt(), 0.0, false) || !drop_ok(x, p, rng) || (res && !same_rows(*res, x))) return pybind11::none();
+  const Tensor y = at::empty(x.sizes(), x.options());
+  const int64_t C = x.size(-1);
+  const EgnnDropout d{ptr<const int64_t>(rng), site, p};
+  check("egnn_dropout", egnn_dropout(&d, x.scalar_type() == at::kFloat ? EGNN_F32 : EGNN_BF16, x.numel() / C, (int32_t)C, ptr(x), C,
+                                     ptr(get(res)), C, ptr(y), stream_of(x)));
+  return pybind11::cast(y);
+}
+
+pybind11::object norm_drop_forward(const Tensor& x, const Opt& res, double p, const Tensor& rng, int64_t site, const Opt& w,
+                                   const Opt& b, double eps, bool need_stats) {
+  const bool f32 = (w && w->scalar_type() == at::kFloat) || (b && b->scalar_type() == at::kFloat);
+  if (!norm_ok(x, w, b, eps, f32) || !res || !same_rows(*res, x) || !drop_ok(x, p, rng)) return pybind11::none();
+  const EgnnNormDims d = norm_dims(x, eps, f32);
+  const EgnnDropout dr{ptr<const int64_t>(rng), site, p};
+  const auto stat = x.options().dtype(at::kFloat);
+  const Tensor y = at::empty(x.sizes(), x.options()), s = at::empty(x.sizes(), x.options());
+  const Tensor mean = need_stats ? at::empty({d.N}, stat) : Tensor(), rstd = need_stats ? at::empty({d.N}, stat) : Tensor();
+  check("egnn_norm_drop_fwd", egnn_norm_drop_fwd(&d, &dr, ptr(x), d.C, ptr(*res), d.C, ptr(get(w)), ptr(get(b)), ptr(y), ptr(s),
+                                                 ptr<float>(mean), ptr<float>(rstd), stream_of(x)));
+  if (!need_stats) return pybind11::make_tuple(y, s, pybind11::none(), pybind11::none());
+  return pybind11::make_tuple(y, s, mean, rstd);
+}
+
+pybind11::object norm_drop_backward(const Tensor& gy, const Tensor& s, double p, const Tensor& rng, int64_t site, const Opt& w,
+                                    const Tensor& mean, const Tensor& rstd, const Opt& gsum, bool need_w, bool need_b, bool f32) {
+  if (!norm_ok(s, w, Opt(), 0.0, f32) || !same_rows(gy, s) || (gsum && !same_rows(*gsum, s)) || !drop_ok(s, p, rng))
+    return pybind11::none();
+  const EgnnNormDims d = norm_dims(s, 0.0, f32);
+  if (!fits(mean, s, at::kFloat, {d.N}) || !fits(rstd, s, at::kFloat, {d.N})) return pybind11::none();
+  const EgnnDropout dr{ptr<const int64_t>(rng), site, p};
+  const Tensor gx = at::empty(s.sizes(), s.options()), gr = at::empty(s.sizes(), s.options());
+  const auto param = s.options().dtype(f32 ? at::kFloat : s.scalar_type());
+  const Tensor gw = need_w ? at::empty({d.C}, param) : Tensor(), gb = need_b ? at::empty({d.C}, param) : Tensor();
+  const size_t nb = need_w || need_b ? egnn_norm_bwd_workspace_bytes(&d) : 0;
+  const Tensor ws = workspace(nb, s);
+  check("egnn_norm_drop_bwd", egnn_norm_drop_bwd(&d, &dr, ptr(gy), d.C, ptr(s), d.C, ptr(get(w)), ptr<float>(mean), ptr<float>(rstd),
+                                                 ptr(get(gsum)), d.C, ptr(gx), ptr(gr), ptr(gw), ptr(gb), ptr(ws), nb, stream_of(s)));
+  auto out = [](const Tensor& t) -> pybind11::object { return t.defined() ? pybind11::cast(t) : pybind11::none(); };
+  return pybind11::make_tuple(gx, gr, out(gw), out(gb));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_egnn_torch, m) {
@@ -345,4 +391,7 @@ PYBIND11_MODULE(_egnn_torch, m) {
   m.def("attn_backward", &attn_backward);
   m.def("norm_forward", &norm_forward);
   m.def("norm_backward", &norm_backward);
+  m.def("dropout", &dropout);
+  m.def("norm_drop_forward", &norm_drop_forward);
+  m.def("norm_drop_backward", &norm_drop_backward);
 }
