@@ -423,6 +423,27 @@ int32_t egnn_norm_drop_bwd(const EgnnNormDims* dims, const EgnnDropout* drop, co
                            int64_t ldgs, void* grad_x, void* grad_residual, void* grad_weight, void* grad_bias,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- rows of a table ------------------------------------------------------------
+ * No counterpart in the reference.  out_i = scale W[t_i] for N tokens, and
+ * grad W[v] = scale sum of grad_out_i over the i with t_i = v.  A token outside
+ * [0, V) has a row of zeros and no gradient. */
+typedef struct EgnnEmbedDims {
+  int64_t N;             /* tokens, below 2^31 */
+  int32_t V;             /* rows of the table, 1 to 2^31 - 1; V C below 2^40 */
+  int32_t C;             /* 1 to 2^20 */
+  int32_t dtype;         /* EGNN_F32 or EGNN_BF16, of out and its gradient */
+  int32_t f32_table;     /* 1: the table and its gradient are fp32 beside bf16 rows; 0: all of one dtype */
+  int32_t index64;       /* 1: int64 tokens, 0: int32 */
+  float scale;           /* finite */
+} EgnnEmbedDims;
+
+int32_t egnn_embed_fwd(const EgnnEmbedDims* dims, const void* tokens, const void* weight, int64_t ldw, void* out, void* stream);
+size_t egnn_embed_bwd_workspace_bytes(const EgnnEmbedDims* dims);
+/* Writes grad_weight (V, C), contiguous; the row of `padding` (-1: none) becomes 0.
+ * fp32 sums in a fixed order, no atomics on values. */
+int32_t egnn_embed_bwd(const EgnnEmbedDims* dims, int64_t padding, const void* grad_out, int64_t ldg, const void* tokens,
+                       void* grad_weight, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -31,6 +31,7 @@ EXPORTED = (
     "egnn_attn_fwd_workspace_bytes", "egnn_attn_bwd_workspace_bytes", "egnn_attn_fwd", "egnn_attn_bwd",
     "egnn_norm_fwd", "egnn_norm_bwd_workspace_bytes", "egnn_norm_bwd",
     "egnn_dropout", "egnn_norm_drop_fwd", "egnn_norm_drop_bwd",
+    "egnn_embed_fwd", "egnn_embed_bwd_workspace_bytes", "egnn_embed_bwd",
 )
 
 # kernel classes of the instrumentation hook
@@ -78,6 +79,11 @@ class EgnnNormDims(ctypes.Structure):
 
 class EgnnDropout(ctypes.Structure):
     _fields_ = [("rng", c_void_p), ("site", c_int64), ("p", ctypes.c_double)]
+
+
+class EgnnEmbedDims(ctypes.Structure):
+    _fields_ = [("N", c_int64), ("V", c_int32), ("C", c_int32), ("dtype", c_int32), ("f32_table", c_int32),
+                ("index64", c_int32), ("scale", c_float)]
 
 
 _lib = None
@@ -196,6 +202,13 @@ def lib() -> ctypes.CDLL:
     L.egnn_norm_drop_fwd.argtypes = [MD, DR, P, c_int64, P, c_int64] + [P] * 7
     L.egnn_norm_drop_bwd.restype = c_int32
     L.egnn_norm_drop_bwd.argtypes = [MD, DR, P, c_int64, P, c_int64, P, P, P, P, c_int64] + [P] * 5 + [c_size_t, P]
+    ED = ctypes.POINTER(EgnnEmbedDims)
+    L.egnn_embed_fwd.restype = c_int32
+    L.egnn_embed_fwd.argtypes = [ED, P, P, c_int64, P, P]
+    L.egnn_embed_bwd_workspace_bytes.restype = c_size_t
+    L.egnn_embed_bwd_workspace_bytes.argtypes = [ED]
+    L.egnn_embed_bwd.restype = c_int32
+    L.egnn_embed_bwd.argtypes = [ED, c_int64, P, c_int64, P, P, P, c_size_t, P]
     _lib = L
     return L
 

@@ -383,6 +383,49 @@ pybind11::object norm_drop_backward(const Tensor& gy, const Tensor& s, double p,
   return pybind11::make_tuple(gx, gr, out(gw), out(gb));
 }
 
+// ---- rows of a table -------------------------------------------------------------------
+// tokens of any shape, contiguous; rows of dtype dt and a table of that one, or of fp32 beside bf16 rows
+bool embed_ok(const Tensor& tokens, int64_t V, int64_t C, at::ScalarType dt, at::ScalarType table) {
+  const auto it = tokens.scalar_type();
+  return !torch::jit::tracer::isTracing() && plain(tokens, tokens) && tokens.is_contiguous() && (it == at::kInt || it == at::kLong) &&
+         (dt == at::kFloat || dt == at::kBFloat16) && (table == dt || table == at::kFloat) && V >= 1 && V <= INT32_MAX && C >= 1 &&
+         C <= 1 << 20 && tokens.numel() <= INT32_MAX;
+}
+EgnnEmbedDims embed_dims(const Tensor& tokens, int64_t V, int64_t C, double scale, at::ScalarType dt, at::ScalarType table) {
+  EgnnEmbedDims d{};
+  d.N = tokens.numel(); d.V = (int32_t)V; d.C = (int32_t)C;
+  d.dtype = dt == at::kFloat ? EGNN_F32 : EGNN_BF16;
+  d.f32_table = table != dt;
+  d.index64 = tokens.scalar_type() == at::kLong;
+  d.scale = (float)scale;
+  return d;
+}
+
+pybind11::object embed_forward(const Tensor& tokens, const Tensor& w, double scale, at::ScalarType dt) {
+  if (w.dim() != 2 || !plain(w, tokens) || w.stride(1) != 1 || w.stride(0) < w.size(1) || !std::isfinite(scale) ||
+      !embed_ok(tokens, w.size(0), w.size(1), dt, w.scalar_type()))
+    return pybind11::none();
+  const EgnnEmbedDims d = embed_dims(tokens, w.size(0), w.size(1), scale, dt, w.scalar_type());
+  auto shape = tokens.sizes().vec();
+  shape.push_back(d.C);
+  const Tensor out = at::empty(shape, w.options().dtype(dt));
+  check("egnn_embed_fwd", egnn_embed_fwd(&d, ptr(tokens), ptr(w), w.stride(0), ptr(out), stream_of(w)));
+  return pybind11::cast(out);
+}
+
+pybind11::object embed_backward(const Tensor& go, const Tensor& tokens, int64_t V, double scale, int64_t padding, at::ScalarType table) {
+  const auto dt = go.scalar_type();
+  if (go.dim() != tokens.dim() + 1 || !plain(go, tokens) || !go.is_contiguous() || !std::isfinite(scale) ||
+      !embed_ok(tokens, V, go.size(-1), dt, table) || go.sizes().slice(0, tokens.dim()) != tokens.sizes() || padding < -1 || padding >= V)
+    return pybind11::none();
+  const EgnnEmbedDims d = embed_dims(tokens, V, go.size(-1), scale, dt, table);
+  const Tensor gw = at::empty({V, d.C}, go.options().dtype(table));
+  const size_t nb = egnn_embed_bwd_workspace_bytes(&d);
+  const Tensor ws = workspace(nb, go);
+  check("egnn_embed_bwd", egnn_embed_bwd(&d, padding, ptr(go), d.C, ptr(tokens), ptr(gw), ptr(ws), nb, stream_of(go)));
+  return pybind11::cast(gw);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_egnn_torch, m) {
@@ -394,4 +437,6 @@ PYBIND11_MODULE(_egnn_torch, m) {
   m.def("dropout", &dropout);
   m.def("norm_drop_forward", &norm_drop_forward);
   m.def("norm_drop_backward", &norm_drop_backward);
+  m.def("embed_forward", &embed_forward);
+  m.def("embed_backward", &embed_backward);
 }
