@@ -444,6 +444,47 @@ size_t egnn_embed_bwd_workspace_bytes(const EgnnEmbedDims* dims);
 int32_t egnn_embed_bwd(const EgnnEmbedDims* dims, int64_t padding, const void* grad_out, int64_t ldg, const void* tokens,
                        void* grad_weight, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- norm and rotation of queries and keys -----------------------------------------
+ * No counterpart in the reference.  For every head x (D values) of the Hq query
+ * heads, with weight q_weight, and of the Hk key heads, with k_weight:
+ *   y = x w / sqrt(mean x^2 + eps),
+ * then the pairs (a, b) of its first `rotary` values are turned by the angle
+ * position base^(-2 i / rotary), i the pair's number: (a cos - b sin, b cos + a sin).
+ * Pairs are (y_i, y_{i + rotary / 2}), or neighbours (y_2i, y_2i+1) if interleaved.
+ * The angle is position times frequency to 2^-30 turns for positions up to 2^32 in
+ * magnitude: their product is made in 64-bit fixed point.  The weights may be NULL
+ * (1), and the positions where nothing is turned. */
+typedef struct EgnnQkDims {
+  int64_t N;             /* rows, below 2^31 */
+  int32_t Hq, Hk;        /* heads, 1 to 4096 each */
+  int32_t D;             /* head width, even, 2 to 128 */
+  int32_t rotary;        /* even, 0 to D */
+  int32_t interleaved;   /* 0 or 1 */
+  int32_t dtype;         /* EGNN_F32 or EGNN_BF16 */
+  int32_t f32_params;    /* 1: the weights and their gradients are fp32 beside bf16 rows; 0: all of one dtype */
+  int32_t index64;       /* 1: int64 positions, 0: int32 */
+  float eps;             /* >= 0 */
+  double base;           /* 1 or more, finite */
+} EgnnQkDims;
+
+/* Strides in elements of q, k, the outputs, their gradients and the gradients of q
+ * and k; a head's D values are contiguous.  The forward reads the first eight.
+ * Outputs must not overlap themselves or the inputs. */
+typedef struct EgnnQkStrides {
+  int64_t q_row, q_head, k_row, k_head, q_out_row, q_out_head, k_out_row, k_out_head;
+  int64_t grad_q_out_row, grad_q_out_head, grad_k_out_row, grad_k_out_head, grad_q_row, grad_q_head, grad_k_row, grad_k_head;
+} EgnnQkStrides;
+
+int32_t egnn_qk_fwd(const EgnnQkDims* dims, const EgnnQkStrides* strides, const void* q, const void* k, const void* q_weight,
+                    const void* k_weight, const void* positions, void* q_out, void* k_out, void* stream);
+size_t egnn_qk_bwd_workspace_bytes(const EgnnQkDims* dims);
+/* Backward from the inputs.  grad_q_weight and grad_k_weight (D) may be NULL, and
+ * need the workspace otherwise; fixed-order sums, no atomics. */
+int32_t egnn_qk_bwd(const EgnnQkDims* dims, const EgnnQkStrides* strides, const void* grad_q_out, const void* grad_k_out,
+                    const void* q, const void* k, const void* q_weight, const void* k_weight, const void* positions,
+                    void* grad_q, void* grad_k, void* grad_q_weight, void* grad_k_weight, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

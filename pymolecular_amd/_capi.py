@@ -32,6 +32,7 @@ EXPORTED = (
     "egnn_norm_fwd", "egnn_norm_bwd_workspace_bytes", "egnn_norm_bwd",
     "egnn_dropout", "egnn_norm_drop_fwd", "egnn_norm_drop_bwd",
     "egnn_embed_fwd", "egnn_embed_bwd_workspace_bytes", "egnn_embed_bwd",
+    "egnn_qk_fwd", "egnn_qk_bwd_workspace_bytes", "egnn_qk_bwd",
 )
 
 # kernel classes of the instrumentation hook
@@ -84,6 +85,17 @@ class EgnnDropout(ctypes.Structure):
 class EgnnEmbedDims(ctypes.Structure):
     _fields_ = [("N", c_int64), ("V", c_int32), ("C", c_int32), ("dtype", c_int32), ("f32_table", c_int32),
                 ("index64", c_int32), ("scale", c_float)]
+
+
+class EgnnQkDims(ctypes.Structure):
+    _fields_ = [("N", c_int64), ("Hq", c_int32), ("Hk", c_int32), ("D", c_int32), ("rotary", c_int32),
+                ("interleaved", c_int32), ("dtype", c_int32), ("f32_params", c_int32), ("index64", c_int32),
+                ("eps", c_float), ("base", ctypes.c_double)]
+
+
+class EgnnQkStrides(ctypes.Structure):
+    _fields_ = [(n + x, c_int64) for n in ("q", "k", "q_out", "k_out", "grad_q_out", "grad_k_out", "grad_q", "grad_k")
+                for x in ("_row", "_head")]
 
 
 _lib = None
@@ -209,6 +221,13 @@ def lib() -> ctypes.CDLL:
     L.egnn_embed_bwd_workspace_bytes.argtypes = [ED]
     L.egnn_embed_bwd.restype = c_int32
     L.egnn_embed_bwd.argtypes = [ED, c_int64, P, c_int64, P, P, P, c_size_t, P]
+    QD, QS = ctypes.POINTER(EgnnQkDims), ctypes.POINTER(EgnnQkStrides)
+    L.egnn_qk_fwd.restype = c_int32
+    L.egnn_qk_fwd.argtypes = [QD, QS] + [P] * 8
+    L.egnn_qk_bwd_workspace_bytes.restype = c_size_t
+    L.egnn_qk_bwd_workspace_bytes.argtypes = [QD]
+    L.egnn_qk_bwd.restype = c_int32
+    L.egnn_qk_bwd.argtypes = [QD, QS] + [P] * 12 + [c_size_t, P]
     _lib = L
     return L
 

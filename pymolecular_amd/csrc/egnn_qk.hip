@@ -1,0 +1,407 @@
+// Norm of every head of queries and keys and their rotation by position, and the backward.
+//   r = (mean x^2 + eps)^-1/2, xh = x r, y = xh w, out = turn(y): pairs (a, b) -> (a cos - b sin, b cos + a sin)
+//   backward: gn = turn^-1(g), gw = sum over rows and heads of gn xh, t = gn w, gx = r (t - xh mean(t xh))
+// One pass: a head lives in the registers of a few lanes, each of which holds both values of its pairs, so that nothing but
+// the two row sums crosses lanes.  The angles depend on the row alone: a workgroup makes cos and sin of its rows once, in LDS,
+// for all its heads.  An angle is position times frequency in turns, as a 64-bit fixed-point product whose overflow is the
+// whole turns: exact for any position, with no large argument to reduce.  cos and sin come from their series on an eighth of a
+// turn to either side.  Queries and keys are different workgroups of one launch.
+#include "egnn_internal.h"
+#include "egnn_rows.h"
+#include <cmath>
+
+namespace egnn {
+namespace qk {
+
+constexpr int NT = 256, U = 2;               // threads; heads that a group of lanes loads at once
+constexpr int kPairs = 64;                   // pairs of a head at most
+constexpr int kTable = 2048;                 // cos and sin of a tile at most: 16 KB, two tiles' worth
+constexpr int kHeads = 4096;
+constexpr int64_t kMaxGrid = int64_t(1) << 20;
+
+struct Side {
+  const void *x, *w, *g;
+  void* y;                                   // the output, or the gradient of x
+  void* gw;
+  float* part;                               // [blocks][D] sums of gw
+  int64_t xr, xh, gr, gh, yr, yh;            // strides of rows and heads
+  int32_t H, TB, blocks;                     // heads, rows of a tile, workgroups
+  uint32_t magic;                            // u / H = the high word of u magic (H > 1)
+};
+struct Args {
+  Side s[2];
+  const void* pos;
+  int64_t N;
+  int32_t D, rot, lanes, act;                // lanes of a head (a power of two), and those of them with values
+  uint32_t pair_magic;                       // i / (D / 2)
+  float eps;
+  bool il, f32, i64;
+  uint64_t freq[kPairs];                     // turns a position, in units of 2^-64
+};
+
+// cos and sin of t 2^-32 turns
+__device__ __forceinline__ float2 cos_sin(uint32_t t) {
+  const uint32_t q = (t + (1u << 29)) >> 30; // quarter turns, rounded
+  const float x = (float)(int32_t)(t - (q << 30)) * (float)(6.283185307179586 / 4294967296.0);
+  const float z = x * x;
+  const float s = __builtin_fmaf(x * z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), x);
+  const float c = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
+  const float u = q & 1 ? s : c, v = q & 1 ? c : s;
+  return float2{(q + 1) & 2 ? -u : u, q & 2 ? -v : v};
+}
+
+template <typename T, int VEC> struct Piece {
+  typedef T type __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+  typedef T vals __attribute__((ext_vector_type(VEC)));
+  static __device__ __forceinline__ vals load(const T* p) { return *reinterpret_cast<const type*>(p); }
+  static __device__ __forceinline__ void store(T* p, const float* v) {
+    type t;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<type*>(p) = t;
+  }
+};
+template <typename T> struct Piece<T, 1> {
+  struct vals { T x; __device__ __forceinline__ T operator[](int) const { return x; } };
+  static __device__ __forceinline__ vals load(const T* p) { return vals{*p}; }
+  static __device__ __forceinline__ void store(T* p, const float* v) { *p = from_f32<T>(v[0]); }
+};
+
+// The two pieces a lane holds of a head, as values a[i] and b[i] of its pairs
+template <int VEC, bool IL, typename V> __device__ __forceinline__ void to_pairs(const V& p0, const V& p1, float* a, float* b) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    if (IL) {
+      a[i] = to_f32(2 * i < VEC ? p0[(2 * i) % VEC] : p1[(2 * i) % VEC]);
+      b[i] = to_f32(2 * i + 1 < VEC ? p0[(2 * i + 1) % VEC] : p1[(2 * i + 1) % VEC]);
+    } else {
+      a[i] = to_f32(p0[i]);
+      b[i] = to_f32(p1[i]);
+    }
+  }
+}
+template <int VEC, bool IL> __device__ __forceinline__ void from_pairs(const float* a, const float* b, float* p0, float* p1) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    p0[i] = !IL ? a[i] : i & 1 ? b[i / 2] : a[i / 2];
+    p1[i] = !IL ? b[i] : (VEC + i) & 1 ? b[(VEC + i) / 2] : a[(VEC + i) / 2];
+  }
+}
+
+template <typename T, int VEC, bool IL, bool BWD>
+__global__ __launch_bounds__(NT) void qk_kernel(Args a) {
+  typedef Piece<T, VEC> P;
+  __shared__ float2 table[2][kTable];
+  const int half = a.D / 2;
+  const bool key = (int)blockIdx.x >= a.s[0].blocks;
+  const Side s = a.s[key];
+  const int block = key ? blockIdx.x - a.s[0].blocks : blockIdx.x;
+  const int lanes = a.lanes, groups = NT / lanes, group = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
+  const bool lives = lane < a.act;
+  const int j0 = lives ? lane * VEC : 0;     // the lane's first pair
+  int f0, f1;                                // the columns of its two pieces
+  if (IL) { f0 = 2 * j0; f1 = f0 + VEC; }
+  else if (j0 < a.rot / 2) { f0 = j0; f1 = j0 + a.rot / 2; }
+  else { f0 = a.rot + j0 - a.rot / 2; f1 = f0 + (a.D - a.rot) / 2; }
+  float wa[VEC], wb[VEC], ga[VEC], gb[VEC];
+  {
+    float p0[VEC], p1[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      p0[i] = !s.w ? 1.f : a.f32 ? ((const float*)s.w)[f0 + i] : to_f32(((const T*)s.w)[f0 + i]);
+      p1[i] = !s.w ? 1.f : a.f32 ? ((const float*)s.w)[f1 + i] : to_f32(((const T*)s.w)[f1 + i]);
+      ga[i] = gb[i] = 0.f;
+    }
+    struct Arr { const float* p; __device__ float operator[](int i) const { return p[i]; } };
+    to_pairs<VEC, IL>(Arr{p0}, Arr{p1}, wa, wb);
+  }
+  const int64_t tiles = (a.N + s.TB - 1) / s.TB;
+  int buf = 0;
+  for (int64_t tile = block; tile < tiles; tile += s.blocks, buf ^= 1) {
+    const int64_t n0 = tile * s.TB;
+    const int rows = (int)(a.N - n0 < s.TB ? a.N - n0 : s.TB), units = rows * s.H;
+    typename P::vals x0[U], x1[U], g0[U], g1[U];
+    auto fetch = [&](int base) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = min(base + u * groups + group, units - 1);
+        const int row = s.H > 1 ? (int)__umulhi(k, s.magic) : k;
+        const T* x = (const T*)s.x + (n0 + row) * s.xr + (k - row * s.H) * s.xh;
+        x0[u] = P::load(x + f0);
+        x1[u] = P::load(x + f1);
+        if (BWD) {
+          const T* g = (const T*)s.g + (n0 + row) * s.gr + (k - row * s.H) * s.gh;
+          g0[u] = P::load(g + f0);
+          g1[u] = P::load(g + f1);
+        }
+      }
+    };
+    fetch(0);
+    for (int i = threadIdx.x; i < rows * half; i += NT) {
+      const int row = half > 1 ? (int)__umulhi(i, a.pair_magic) : i, j = i - row * half;
+      float2 cs{1.f, 0.f};
+      if (j < a.rot / 2) {
+        const int64_t p = a.i64 ? ((const int64_t*)a.pos)[n0 + row] : ((const int32_t*)a.pos)[n0 + row];
+        cs = cos_sin((uint32_t)(((uint64_t)p * a.freq[j]) >> 32));
+      }
+      table[buf][i] = cs;
+    }
+    __syncthreads();                         // (the table before last is free again: all threads have passed the last barrier)
+    for (int base = 0; base < units; base += U * groups) {
+      if (base) fetch(base);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = base + u * groups + group;
+        const bool in = k < units && lives;
+        const int row = s.H > 1 ? (int)__umulhi(min(k, units - 1), s.magic) : min(k, units - 1);
+        const int head = min(k, units - 1) - row * s.H;
+        float va[VEC], vb[VEC], ca[VEC], sa[VEC];
+        to_pairs<VEC, IL>(x0[u], x1[u], va, vb);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          sum = __builtin_fmaf(va[i], va[i], sum);
+          sum = __builtin_fmaf(vb[i], vb[i], sum);
+          const float2 cs = table[buf][row * half + j0 + i];
+          ca[i] = cs.x;
+          sa[i] = cs.y;
+        }
+        sum = lives ? sum : 0.f;
+        for (int m = lanes / 2; m; m >>= 1) sum += shfl_xor(sum, m);
+        const float r = 1.0f / sqrtf(sum / a.D + a.eps);
+        float oa[VEC], ob[VEC];
+        if constexpr (!BWD) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float ya = va[i] * r * wa[i], yb = vb[i] * r * wb[i];
+            oa[i] = ya * ca[i] - yb * sa[i];
+            ob[i] = yb * ca[i] + ya * sa[i];
+          }
+        } else {
+          float ta[VEC], tb[VEC], dot = 0.f;
+          to_pairs<VEC, IL>(g0[u], g1[u], ta, tb);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float na = ta[i] * ca[i] + tb[i] * sa[i], nb = tb[i] * ca[i] - ta[i] * sa[i];
+            va[i] *= r;
+            vb[i] *= r;
+            if (in) {
+              ga[i] = __builtin_fmaf(na, va[i], ga[i]);
+              gb[i] = __builtin_fmaf(nb, vb[i], gb[i]);
+            }
+            ta[i] = na * wa[i];
+            tb[i] = nb * wb[i];
+            dot = __builtin_fmaf(ta[i], va[i], dot);
+            dot = __builtin_fmaf(tb[i], vb[i], dot);
+          }
+          dot = lives ? dot : 0.f;
+          for (int m = lanes / 2; m; m >>= 1) dot += shfl_xor(dot, m);
+          dot /= a.D;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            oa[i] = r * (ta[i] - va[i] * dot);
+            ob[i] = r * (tb[i] - vb[i] * dot);
+          }
+        }
+        if (in) {
+          float p0[VEC], p1[VEC];
+          from_pairs<VEC, IL>(oa, ob, p0, p1);
+          T* y = (T*)s.y + (n0 + row) * s.yr + head * s.yh;
+          P::store(y + f0, p0);
+          P::store(y + f1, p1);
+        }
+      }
+    }
+  }
+  if (!BWD || !s.part) return;
+  // the groups' sums of a column, in order: [group][D] in the tables' place
+  float* red = (float*)table;
+  float p0[VEC], p1[VEC];
+  from_pairs<VEC, IL>(ga, gb, p0, p1);
+  __syncthreads();
+  if (lives)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      red[group * a.D + f0 + i] = p0[i];
+      red[group * a.D + f1 + i] = p1[i];
+    }
+  __syncthreads();
+  for (int f = threadIdx.x; f < a.D; f += NT) {
+    float t = 0.f;
+    for (int g = 0; g < groups; ++g) t += red[g * a.D + f];
+    s.part[(int64_t)block * a.D + f] = t;
+  }
+}
+
+// gw = the sums over the workgroups: 16 columns of one side a workgroup, 64 groups joined in order
+template <typename P> __global__ __launch_bounds__(1024) void sum_kernel(Args a) {
+  __shared__ float red[64][17];
+  const Side s = a.s[blockIdx.y];
+  const int c = threadIdx.x & 15, k = threadIdx.x >> 4, f = blockIdx.x * 16 + c;
+  float t = 0.f;
+  if (f < a.D && s.gw) {
+#pragma unroll 8
+    for (int b = k; b < s.blocks; b += 64) t += s.part[(int64_t)b * a.D + f];
+  }
+  red[k][c] = t;
+  __syncthreads();
+  for (int h = 32; h; h >>= 1) {
+    if (k < h) red[k][c] += red[k + h][c];
+    __syncthreads();
+  }
+  if (!k && f < a.D && s.gw) ((P*)s.gw)[f] = from_f32<P>(red[0][c]);
+}
+
+// Widest piece that fits 16 bytes and never lies across the rotated part's middle or end
+static int piece_of(const EgnnQkDims* d) {
+  int v = d->dtype == EGNN_F32 ? 4 : 8;
+  const int half = d->D / 2, r = d->rotary / 2;
+  while (v > 1 && (half % v || (!d->interleaved && r % v))) v /= 2;
+  return v;
+}
+static int lanes_of(const EgnnQkDims* d) {
+  int l = 1;
+  while (l * piece_of(d) < d->D / 2) l *= 2;
+  return l;
+}
+// Rows of a tile, and tiles
+static int tile_rows(const EgnnQkDims* d, int H, int lanes) {
+  int tb = NT / lanes * U / H;
+  if (tb > kTable / (d->D / 2)) tb = kTable / (d->D / 2);
+  return tb < 1 ? 1 : tb;
+}
+// Workgroups of the backward, and partial rows of the weight gradients, of the two sides
+constexpr int kBlocks = 1024;
+static void bwd_blocks(const EgnnQkDims* d, int32_t* q, int32_t* k) {
+  const int lanes = lanes_of(d);
+  const int64_t qt = cdiv(d->N, tile_rows(d, d->Hq, lanes)), kt = cdiv(d->N, tile_rows(d, d->Hk, lanes));
+  int64_t qb = (int64_t)kBlocks * d->Hq / (d->Hq + d->Hk), kb = kBlocks - qb;
+  if (qb < 1) qb = 1;
+  if (kb < 1) kb = 1;
+  *q = (int32_t)(qt < qb ? qt : qb);
+  *k = (int32_t)(kt < kb ? kt : kb);
+}
+
+template <typename T, int VEC>
+static void launch(const Args& a, bool bwd, hipStream_t st) {
+  const uint32_t grid = (uint32_t)(a.s[0].blocks + a.s[1].blocks);
+  if (!grid) return;
+  if (a.il) {
+    if (bwd) qk_kernel<T, VEC, true, true><<<grid, NT, 0, st>>>(a);
+    else qk_kernel<T, VEC, true, false><<<grid, NT, 0, st>>>(a);
+  } else {
+    if (bwd) qk_kernel<T, VEC, false, true><<<grid, NT, 0, st>>>(a);
+    else qk_kernel<T, VEC, false, false><<<grid, NT, 0, st>>>(a);
+  }
+}
+static int run(const EgnnQkDims* d, Args& a, bool bwd, hipStream_t st) {
+  const int vec = piece_of(d), half = d->D / 2;
+  a.N = d->N; a.D = d->D; a.rot = d->rotary; a.lanes = lanes_of(d); a.act = half / vec; a.eps = d->eps;
+  a.il = d->interleaved; a.f32 = d->f32_params; a.i64 = d->index64;
+  a.pair_magic = half > 1 ? (uint32_t)(((uint64_t(1) << 32) + half - 1) / half) : 0;
+  // base^(-2 i / rotary) / 2 pi in units of 2^-64, by repeated multiplication in extended precision
+  const long double step = d->rotary ? powl((long double)d->base, -2.0L / d->rotary) : 1.0L;
+  long double f = 18446744073709551616.0L / 6.283185307179586476925286766559L;
+  for (int i = 0; i < d->rotary / 2; ++i, f *= step) a.freq[i] = (uint64_t)(f + 0.5L);
+  for (int i = 0; i < 2; ++i) {
+    Side& s = a.s[i];
+    s.H = i ? d->Hk : d->Hq;
+    s.magic = s.H > 1 ? (uint32_t)(((uint64_t(1) << 32) + s.H - 1) / s.H) : 0;
+    s.TB = tile_rows(d, s.H, a.lanes);
+    const int64_t tiles = cdiv(d->N, s.TB);
+    s.blocks = (int32_t)(tiles < kMaxGrid ? tiles : kMaxGrid);
+  }
+  if (bwd) bwd_blocks(d, &a.s[0].blocks, &a.s[1].blocks);
+  if (d->dtype == EGNN_F32) {
+    if (vec == 4) launch<float, 4>(a, bwd, st);
+    else if (vec == 2) launch<float, 2>(a, bwd, st);
+    else launch<float, 1>(a, bwd, st);
+  } else {
+    if (vec == 8) launch<bf16, 8>(a, bwd, st);
+    else if (vec == 4) launch<bf16, 4>(a, bwd, st);
+    else if (vec == 2) launch<bf16, 2>(a, bwd, st);
+    else launch<bf16, 1>(a, bwd, st);
+  }
+  if (bwd && (a.s[0].gw || a.s[1].gw)) {  // (without rows: sums of nothing)
+    const dim3 grid((uint32_t)cdiv(d->D, 16), 2);
+    if (d->dtype == EGNN_F32 || d->f32_params) sum_kernel<float><<<grid, 1024, 0, st>>>(a);
+    else sum_kernel<bf16><<<grid, 1024, 0, st>>>(a);
+  }
+  return hipGetLastError() == hipSuccess ? EGNN_OK : EGNN_ERR_HIP;
+}
+
+static bool dims_ok(const EgnnQkDims* d) {
+  return d->N >= 0 && d->N <= INT32_MAX && d->Hq >= 1 && d->Hq <= kHeads && d->Hk >= 1 && d->Hk <= kHeads && d->D >= 2 &&
+         d->D <= 2 * kPairs && d->D % 2 == 0 && d->rotary >= 0 && d->rotary <= d->D && d->rotary % 2 == 0 &&
+         (d->interleaved == 0 || d->interleaved == 1) && (d->dtype == EGNN_F32 || d->dtype == EGNN_BF16) &&
+         (d->f32_params == 0 || d->f32_params == 1) && (d->index64 == 0 || d->index64 == 1) && d->eps >= 0.f &&
+         d->eps - d->eps == 0.f && d->base >= 1.0 && d->base - d->base == 0.0;
+}
+
+}  // namespace qk
+}  // namespace egnn
+
+using namespace egnn::qk;
+
+extern "C" {
+
+int32_t egnn_qk_fwd(const EgnnQkDims* d, const EgnnQkStrides* st, const void* q, const void* k, const void* q_weight,
+                    const void* k_weight, const void* positions, void* q_out, void* k_out, void* stream) {
+  if (!d || !st) return EGNN_ERR_NULL;
+  if (!dims_ok(d)) return EGNN_ERR_DIMS;
+  if (d->N && (!q || !k || !q_out || !k_out || (d->rotary && !positions))) return EGNN_ERR_NULL;
+  if (st->q_row < 0 || st->q_head < 0 || st->k_row < 0 || st->k_head < 0 || st->q_out_head < d->D || st->k_out_head < d->D ||
+      st->q_out_row < d->Hq * (int64_t)d->D || st->k_out_row < d->Hk * (int64_t)d->D)
+    return EGNN_ERR_STRIDE;
+  const uintptr_t e = d->dtype == EGNN_F32 ? 4 : 2, ep = d->f32_params ? 4 : e, ei = d->index64 ? 8 : 4;
+  if ((uintptr_t)q % e || (uintptr_t)k % e || (uintptr_t)q_out % e || (uintptr_t)k_out % e || (uintptr_t)q_weight % ep ||
+      (uintptr_t)k_weight % ep || (uintptr_t)positions % ei)
+    return EGNN_ERR_ALIGN;
+  Args a{};
+  a.pos = positions;
+  Side &x = a.s[0], &y = a.s[1];
+  x.x = q; x.w = q_weight; x.y = q_out; x.xr = st->q_row; x.xh = st->q_head; x.yr = st->q_out_row; x.yh = st->q_out_head;
+  y.x = k; y.w = k_weight; y.y = k_out; y.xr = st->k_row; y.xh = st->k_head; y.yr = st->k_out_row; y.yh = st->k_out_head;
+  return run(d, a, false, (hipStream_t)stream);
+}
+
+size_t egnn_qk_bwd_workspace_bytes(const EgnnQkDims* d) {
+  if (!d || !dims_ok(d)) return 0;
+  int32_t q, k;
+  bwd_blocks(d, &q, &k);
+  return ((size_t)q + k) * d->D * 4;
+}
+
+int32_t egnn_qk_bwd(const EgnnQkDims* d, const EgnnQkStrides* st, const void* grad_q_out, const void* grad_k_out,
+                    const void* q, const void* k, const void* q_weight, const void* k_weight, const void* positions,
+                    void* grad_q, void* grad_k, void* grad_q_weight, void* grad_k_weight, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  if (!d || !st) return EGNN_ERR_NULL;
+  if (!dims_ok(d)) return EGNN_ERR_DIMS;
+  if (d->N && (!grad_q_out || !grad_k_out || !q || !k || !grad_q || !grad_k || (d->rotary && !positions))) return EGNN_ERR_NULL;
+  if (st->q_row < 0 || st->q_head < 0 || st->k_row < 0 || st->k_head < 0 || st->grad_q_out_row < 0 || st->grad_q_out_head < 0 ||
+      st->grad_k_out_row < 0 || st->grad_k_out_head < 0 || st->grad_q_head < d->D || st->grad_k_head < d->D ||
+      st->grad_q_row < d->Hq * (int64_t)d->D || st->grad_k_row < d->Hk * (int64_t)d->D)
+    return EGNN_ERR_STRIDE;
+  const uintptr_t e = d->dtype == EGNN_F32 ? 4 : 2, ep = d->f32_params ? 4 : e, ei = d->index64 ? 8 : 4;
+  if ((uintptr_t)grad_q_out % e || (uintptr_t)grad_k_out % e || (uintptr_t)q % e || (uintptr_t)k % e || (uintptr_t)grad_q % e ||
+      (uintptr_t)grad_k % e || (uintptr_t)q_weight % ep || (uintptr_t)k_weight % ep || (uintptr_t)grad_q_weight % ep ||
+      (uintptr_t)grad_k_weight % ep || (uintptr_t)positions % ei || (uintptr_t)workspace % 16)
+    return EGNN_ERR_ALIGN;
+  const size_t need = egnn_qk_bwd_workspace_bytes(d);
+  if ((grad_q_weight || grad_k_weight) && need && (!workspace || workspace_bytes < need)) return EGNN_ERR_WORKSPACE;
+  Args a{};
+  a.pos = positions;
+  Side &x = a.s[0], &y = a.s[1];
+  x.x = q; x.w = q_weight; x.g = grad_q_out; x.y = grad_q; x.gw = grad_q_weight;
+  x.xr = st->q_row; x.xh = st->q_head; x.gr = st->grad_q_out_row; x.gh = st->grad_q_out_head; x.yr = st->grad_q_row; x.yh = st->grad_q_head;
+  y.x = k; y.w = k_weight; y.g = grad_k_out; y.y = grad_k; y.gw = grad_k_weight;
+  y.xr = st->k_row; y.xh = st->k_head; y.gr = st->grad_k_out_row; y.gh = st->grad_k_out_head; y.yr = st->grad_k_row; y.yh = st->grad_k_head;
+  int32_t qb, kb;
+  bwd_blocks(d, &qb, &kb);
+  x.part = grad_q_weight ? (float*)workspace : nullptr;
+  y.part = grad_k_weight ? (float*)workspace + (int64_t)qb * d->D : nullptr;
+  return run(d, a, true, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -426,6 +426,78 @@ pybind11::object embed_backward(const Tensor& go, const Tensor& tokens, int64_t 
   return pybind11::cast(gw);
 }
 
+// ---- norm and rotation of queries and keys ---------------------------------------------
+bool heads_of(const Tensor& t, const Tensor& q, int64_t n, int64_t heads, int64_t d) {
+  return plain(t, q) && t.scalar_type() == q.scalar_type() && t.dim() == 3 && t.size(0) == n && t.size(1) == heads && t.size(2) == d &&
+         t.stride(2) == 1;
+}
+// a gradient's buffer: rows apart, heads apart
+bool room_of(const Tensor& t, const Tensor& q, int64_t n, int64_t heads, int64_t d) {
+  return heads_of(t, q, n, heads, d) && t.stride(1) >= d && t.stride(0) >= heads * d;
+}
+struct Qk {
+  bool ok;
+  EgnnQkDims d;
+};
+Qk qk_of(const Tensor& q, const Tensor& k, const Opt& qw, const Opt& kw, const Opt& pos, double base, int64_t rotary, bool il,
+         double eps) {
+  Qk r{};
+  if (torch::jit::tracer::isTracing() || q.dim() != 3 || k.dim() != 3) return r;
+  const auto dt = q.scalar_type();
+  const int64_t n = q.size(0), D = q.size(2);
+  if ((dt != at::kFloat && dt != at::kBFloat16) || D < 2 || D > 128 || D % 2 || q.size(1) < 1 || q.size(1) > 4096 || k.size(1) < 1 ||
+      k.size(1) > 4096 || n > INT32_MAX || rotary < 0 || rotary > D || rotary % 2 || !(base >= 1.0) || !std::isfinite(base) ||
+      !(eps >= 0.0) || !std::isfinite(eps) || !heads_of(q, q, n, q.size(1), D) || !heads_of(k, q, n, k.size(1), D))
+    return r;
+  const bool f32 = (qw && qw->scalar_type() == at::kFloat) || (kw && kw->scalar_type() == at::kFloat);
+  const auto pt = f32 ? at::kFloat : dt;
+  if (!fits_opt(qw, q, pt, D) || !fits_opt(kw, q, pt, D)) return r;
+  if (!pos ? rotary != 0 : !fits(*pos, q, at::kInt, {n}) && !fits(*pos, q, at::kLong, {n})) return r;
+  EgnnQkDims& d = r.d;
+  d.N = n; d.Hq = (int32_t)q.size(1); d.Hk = (int32_t)k.size(1); d.D = (int32_t)D; d.rotary = (int32_t)rotary; d.interleaved = il;
+  d.dtype = dt == at::kFloat ? EGNN_F32 : EGNN_BF16;
+  d.f32_params = f32 && d.dtype == EGNN_BF16;
+  d.index64 = pos && pos->scalar_type() == at::kLong;
+  d.eps = (float)eps; d.base = base;
+  r.ok = true;
+  return r;
+}
+
+pybind11::object qk_forward(const Tensor& q, const Tensor& k, const Opt& qw, const Opt& kw, const Opt& pos, double base, int64_t rotary,
+                            bool il, double eps) {
+  const Qk r = qk_of(q, k, qw, kw, pos, base, rotary, il, eps);
+  if (!r.ok) return pybind11::none();
+  const Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), q.options());
+  EgnnQkStrides s{};
+  s.q_row = q.stride(0); s.q_head = q.stride(1); s.k_row = k.stride(0); s.k_head = k.stride(1);
+  s.q_out_row = qo.stride(0); s.q_out_head = qo.stride(1); s.k_out_row = ko.stride(0); s.k_out_head = ko.stride(1);
+  check("egnn_qk_fwd", egnn_qk_fwd(&r.d, &s, ptr(q), ptr(k), ptr(get(qw)), ptr(get(kw)), ptr(get(pos)), ptr(qo), ptr(ko), stream_of(q)));
+  return pybind11::make_tuple(qo, ko);
+}
+
+pybind11::object qk_backward(const Tensor& gqo, const Tensor& gko, const Tensor& q, const Tensor& k, const Opt& qw, const Opt& kw,
+                             const Opt& pos, double base, int64_t rotary, bool il, double eps,
+                             const std::optional<std::vector<Tensor>>& into) {
+  const Qk r = qk_of(q, k, qw, kw, pos, base, rotary, il, eps);
+  const EgnnQkDims& d = r.d;
+  if (!r.ok || !heads_of(gqo, q, d.N, d.Hq, d.D) || !heads_of(gko, q, d.N, d.Hk, d.D)) return pybind11::none();
+  if (into && (into->size() != 2 || !room_of((*into)[0], q, d.N, d.Hq, d.D) || !room_of((*into)[1], q, d.N, d.Hk, d.D)))
+    return pybind11::none();
+  const Tensor gq = into ? (*into)[0] : at::empty(q.sizes(), q.options()), gk = into ? (*into)[1] : at::empty(k.sizes(), q.options());
+  const auto param = q.options().dtype(d.f32_params ? at::kFloat : q.scalar_type());
+  const Tensor gqw = qw ? at::empty({d.D}, param) : Tensor(), gkw = kw ? at::empty({d.D}, param) : Tensor();
+  const size_t nb = qw || kw ? egnn_qk_bwd_workspace_bytes(&d) : 0;
+  const Tensor ws = workspace(nb, q);
+  EgnnQkStrides s{};
+  s.q_row = q.stride(0); s.q_head = q.stride(1); s.k_row = k.stride(0); s.k_head = k.stride(1);
+  s.grad_q_out_row = gqo.stride(0); s.grad_q_out_head = gqo.stride(1); s.grad_k_out_row = gko.stride(0); s.grad_k_out_head = gko.stride(1);
+  s.grad_q_row = gq.stride(0); s.grad_q_head = gq.stride(1); s.grad_k_row = gk.stride(0); s.grad_k_head = gk.stride(1);
+  check("egnn_qk_bwd", egnn_qk_bwd(&d, &s, ptr(gqo), ptr(gko), ptr(q), ptr(k), ptr(get(qw)), ptr(get(kw)), ptr(get(pos)), ptr(gq), ptr(gk),
+                                   ptr(gqw), ptr(gkw), ptr(ws), nb, stream_of(q)));
+  auto out = [](const Tensor& t) -> pybind11::object { return t.defined() ? pybind11::cast(t) : pybind11::none(); };
+  return pybind11::make_tuple(gq, gk, out(gqw), out(gkw));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_egnn_torch, m) {
@@ -439,4 +511,6 @@ PYBIND11_MODULE(_egnn_torch, m) {
   m.def("norm_drop_backward", &norm_drop_backward);
   m.def("embed_forward", &embed_forward);
   m.def("embed_backward", &embed_backward);
+  m.def("qk_forward", &qk_forward);
+  m.def("qk_backward", &qk_backward);
 }
