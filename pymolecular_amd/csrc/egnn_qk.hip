@@ -3,9 +3,9 @@
 //   backward: gn = turn^-1(g), gw = sum over rows and heads of gn xh, t = gn w, gx = r (t - xh mean(t xh))
 // One pass: a head lives in the registers of a few lanes, each of which holds both values of its pairs, so that nothing but
 // the two row sums crosses lanes.  The angles depend on the row alone: a workgroup makes cos and sin of its rows once, in LDS,
-// for all its heads.  An angle is position times frequency in turns, as a 64-bit fixed-point product whose overflow is the
+// for all its heads, queries' and keys'.  An angle is position times frequency in turns, as a 64-bit fixed-point product whose overflow is the
 // whole turns: exact for any position, with no large argument to reduce.  cos and sin come from their series on an eighth of a
-// turn to either side.  Queries and keys are different workgroups of one launch.
+// turn to either side.
 #include "egnn_internal.h"
 #include "egnn_rows.h"
 #include <cmath>
@@ -13,9 +13,9 @@
 namespace egnn {
 namespace qk {
 
-constexpr int NT = 256, U = 2;               // threads; heads that a group of lanes loads at once
+constexpr int NT = 256;
 constexpr int kPairs = 64;                   // pairs of a head at most
-constexpr int kTable = 2048;                 // cos and sin of a tile at most: 16 KB, two tiles' worth
+constexpr int kTable = 2304;                 // cos and sin of a tile at most: 18 KB
 constexpr int kHeads = 4096;
 constexpr int64_t kMaxGrid = int64_t(1) << 20;
 
@@ -25,16 +25,17 @@ struct Side {
   void* gw;
   float* part;                               // [blocks][D] sums of gw
   int64_t xr, xh, gr, gh, yr, yh;            // strides of rows and heads
-  int32_t H, TB, blocks;                     // heads, rows of a tile, workgroups
+  int32_t H;                                 // heads
   uint32_t magic;                            // u / H = the high word of u magic (H > 1)
 };
 struct Args {
   Side s[2];
   const void* pos;
   int64_t N;
+  int32_t TB, blocks;                        // rows of a tile, workgroups
   int32_t D, rot, lanes, act;                // lanes of a head (a power of two), and those of them with values
   uint32_t pair_magic;                       // i / (D / 2)
-  float eps;
+  float eps, inv;                            // inv = 1 / D
   bool il, f32, i64;
   uint64_t freq[kPairs];                     // turns a position, in units of 2^-64
 };
@@ -60,6 +61,33 @@ template <typename T, int VEC> struct Piece {
     for (int i = 0; i < VEC; ++i) t[i] = from_f32<T>(v[i]);
     *reinterpret_cast<type*>(p) = t;
   }
+};
+// (pairs of bf16 stay words until they are used: vectors of bf16 that live across the loop take a register a value)
+template <int VEC> struct Piece<bf16, VEC> {
+  typedef bf16 type __attribute__((ext_vector_type(VEC), aligned(2)));
+  typedef uint32_t words __attribute__((ext_vector_type(VEC / 2), aligned(2)));
+  struct vals {
+    uint32_t w[VEC / 2];
+    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
+  };
+  static __device__ __forceinline__ vals load(const bf16* p) {
+    vals v;
+    const words t = *reinterpret_cast<const words*>(p);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) v.w[i] = t[i];
+    return v;
+  }
+  static __device__ __forceinline__ void store(bf16* p, const float* v) {
+    type t;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t[i] = (bf16)v[i];
+    *reinterpret_cast<type*>(p) = t;
+  }
+};
+template <> struct Piece<bf16, 1> {
+  struct vals { bf16 x; __device__ __forceinline__ float operator[](int) const { return (float)x; } };
+  static __device__ __forceinline__ vals load(const bf16* p) { return vals{*p}; }
+  static __device__ __forceinline__ void store(bf16* p, const float* v) { *p = (bf16)v[0]; }
 };
 template <typename T> struct Piece<T, 1> {
   struct vals { T x; __device__ __forceinline__ T operator[](int) const { return x; } };
@@ -88,14 +116,30 @@ template <int VEC, bool IL> __device__ __forceinline__ void from_pairs(const flo
   }
 }
 
+// What a lane has of a side: the weights of its pairs and, in the backward, their gradient
+template <int VEC> struct Weights {
+  float a[VEC], b[VEC], ga[VEC], gb[VEC];
+};
+// the pairs' cos and sin: rows of the table are an even number of pairs apart where VEC is even
+template <int VEC> __device__ __forceinline__ void angles(const float2* t, float* c, float* s) {
+  if constexpr (VEC == 1) {
+    c[0] = t->x;
+    s[0] = t->y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const float4 v = *reinterpret_cast<const float4*>(t + i);
+      c[i] = v.x; s[i] = v.y; c[i + 1] = v.z; s[i + 1] = v.w;
+    }
+  }
+}
+
 template <typename T, int VEC, bool IL, bool BWD>
 __global__ __launch_bounds__(NT) void qk_kernel(Args a) {
   typedef Piece<T, VEC> P;
-  __shared__ float2 table[2][kTable];
-  const int half = a.D / 2;
-  const bool key = (int)blockIdx.x >= a.s[0].blocks;
-  const Side s = a.s[key];
-  const int block = key ? blockIdx.x - a.s[0].blocks : blockIdx.x;
+  constexpr int U = BWD ? 1 : 2;             // heads that a group of lanes loads at once
+  __shared__ __align__(16) float2 table[kTable];
+  const int half = a.D / 2, apart = half + 2;   // (rows of the table 16 bytes further apart: fewer of them in one bank)
   const int lanes = a.lanes, groups = NT / lanes, group = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
   const bool lives = lane < a.act;
   const int j0 = lives ? lane * VEC : 0;     // the lane's first pair
@@ -103,40 +147,112 @@ __global__ __launch_bounds__(NT) void qk_kernel(Args a) {
   if (IL) { f0 = 2 * j0; f1 = f0 + VEC; }
   else if (j0 < a.rot / 2) { f0 = j0; f1 = j0 + a.rot / 2; }
   else { f0 = a.rot + j0 - a.rot / 2; f1 = f0 + (a.D - a.rot) / 2; }
-  float wa[VEC], wb[VEC], ga[VEC], gb[VEC];
-  {
-    float p0[VEC], p1[VEC];
+  Weights<VEC> ws[2];
+  const int64_t tiles = (a.N + a.TB - 1) / a.TB;
+  struct Raw { typename P::vals x0, x1, g0, g1; };
+  auto fetch = [&](const Side& s, int64_t n0, int units, int base, Raw* raw) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      p0[i] = !s.w ? 1.f : a.f32 ? ((const float*)s.w)[f0 + i] : to_f32(((const T*)s.w)[f0 + i]);
-      p1[i] = !s.w ? 1.f : a.f32 ? ((const float*)s.w)[f1 + i] : to_f32(((const T*)s.w)[f1 + i]);
-      ga[i] = gb[i] = 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int k = min(base + u * groups + group, units - 1);
+      const int row = s.H > 1 ? (int)__umulhi(k, s.magic) : k;
+      const T* x = (const T*)s.x + (n0 + row) * s.xr + (k - row * s.H) * s.xh;
+      raw[u].x0 = P::load(x + f0);
+      raw[u].x1 = P::load(x + f1);
+      if (BWD) {
+        const T* g = (const T*)s.g + (n0 + row) * s.gr + (k - row * s.H) * s.gh;
+        raw[u].g0 = P::load(g + f0);
+        raw[u].g1 = P::load(g + f1);
+      }
     }
-    struct Arr { const float* p; __device__ float operator[](int i) const { return p[i]; } };
-    to_pairs<VEC, IL>(Arr{p0}, Arr{p1}, wa, wb);
-  }
-  const int64_t tiles = (a.N + s.TB - 1) / s.TB;
-  int buf = 0;
-  for (int64_t tile = block; tile < tiles; tile += s.blocks, buf ^= 1) {
-    const int64_t n0 = tile * s.TB;
-    const int rows = (int)(a.N - n0 < s.TB ? a.N - n0 : s.TB), units = rows * s.H;
-    typename P::vals x0[U], x1[U], g0[U], g1[U];
-    auto fetch = [&](int base) {
+  };
+  auto compute = [&](const Side& s, Weights<VEC>& w, int64_t n0, int units, int base, const Raw* raw) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = min(base + u * groups + group, units - 1);
-        const int row = s.H > 1 ? (int)__umulhi(k, s.magic) : k;
-        const T* x = (const T*)s.x + (n0 + row) * s.xr + (k - row * s.H) * s.xh;
-        x0[u] = P::load(x + f0);
-        x1[u] = P::load(x + f1);
-        if (BWD) {
-          const T* g = (const T*)s.g + (n0 + row) * s.gr + (k - row * s.H) * s.gh;
-          g0[u] = P::load(g + f0);
-          g1[u] = P::load(g + f1);
+    for (int u = 0; u < U; ++u) {
+      const int k = base + u * groups + group, kk = min(k, units - 1);
+      const bool in = k < units && lives;
+      const int row = s.H > 1 ? (int)__umulhi(kk, s.magic) : kk, head = kk - row * s.H;
+      float va[VEC], vb[VEC], c[VEC], sn[VEC];
+      to_pairs<VEC, IL>(raw[u].x0, raw[u].x1, va, vb);
+      angles<VEC>(table + row * apart + j0, c, sn);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        sum = __builtin_fmaf(va[i], va[i], sum);
+        sum = __builtin_fmaf(vb[i], vb[i], sum);
+      }
+      sum = lives ? sum : 0.f;
+      for (int m = lanes / 2; m; m >>= 1) sum += shfl_xor(sum, m);
+      const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(sum, a.inv, a.eps));   // (to one unit of 2^-23)
+      float oa[VEC], ob[VEC];
+      if constexpr (!BWD) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float ya = va[i] * r * w.a[i], yb = vb[i] * r * w.b[i];
+          oa[i] = ya * c[i] - yb * sn[i];
+          ob[i] = yb * c[i] + ya * sn[i];
+        }
+      } else {
+        float ta[VEC], tb[VEC], dot = 0.f;
+        to_pairs<VEC, IL>(raw[u].g0, raw[u].g1, ta, tb);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float na = ta[i] * c[i] + tb[i] * sn[i], nb = tb[i] * c[i] - ta[i] * sn[i];
+          va[i] *= r;
+          vb[i] *= r;
+          if (in) {
+            w.ga[i] = __builtin_fmaf(na, va[i], w.ga[i]);
+            w.gb[i] = __builtin_fmaf(nb, vb[i], w.gb[i]);
+          }
+          ta[i] = na * w.a[i];
+          tb[i] = nb * w.b[i];
+          dot = __builtin_fmaf(ta[i], va[i], dot);
+          dot = __builtin_fmaf(tb[i], vb[i], dot);
+        }
+        dot = lives ? dot : 0.f;
+        for (int m = lanes / 2; m; m >>= 1) dot += shfl_xor(dot, m);
+        dot *= a.inv;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          oa[i] = r * (ta[i] - va[i] * dot);
+          ob[i] = r * (tb[i] - vb[i] * dot);
         }
       }
-    };
-    fetch(0);
+      if (in) {
+        float p0[VEC], p1[VEC];
+        from_pairs<VEC, IL>(oa, ob, p0, p1);
+        T* y = (T*)s.y + (n0 + row) * s.yr + head * s.yh;
+        P::store(y + f0, p0);
+        P::store(y + f1, p1);
+      }
+    }
+  };
+  bool first = true;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += a.blocks) {
+    const int64_t n0 = tile * a.TB;
+    const int rows = (int)(a.N - n0 < a.TB ? a.N - n0 : a.TB);
+    Raw raw[U];
+    fetch(a.s[0], n0, rows * a.s[0].H, 0, raw);
+    if (first) {                             // (behind the first rows' loads, which take longest)
+      first = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const void* w = a.s[i].w;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          ws[i].a[v] = ws[i].b[v] = 1.f;
+          ws[i].ga[v] = ws[i].gb[v] = 0.f;
+        }
+        if (!w) continue;
+        if (sizeof(T) == 2 && a.f32) {
+          typedef Piece<float, VEC> F;
+          to_pairs<VEC, IL>(F::load((const float*)w + f0), F::load((const float*)w + f1), ws[i].a, ws[i].b);
+        } else {
+          to_pairs<VEC, IL>(P::load((const T*)w + f0), P::load((const T*)w + f1), ws[i].a, ws[i].b);
+        }
+      }
+    } else {
+      __syncthreads();                       // the table is read no more
+    }
     for (int i = threadIdx.x; i < rows * half; i += NT) {
       const int row = half > 1 ? (int)__umulhi(i, a.pair_magic) : i, j = i - row * half;
       float2 cs{1.f, 0.f};
@@ -144,92 +260,47 @@ __global__ __launch_bounds__(NT) void qk_kernel(Args a) {
         const int64_t p = a.i64 ? ((const int64_t*)a.pos)[n0 + row] : ((const int32_t*)a.pos)[n0 + row];
         cs = cos_sin((uint32_t)(((uint64_t)p * a.freq[j]) >> 32));
       }
-      table[buf][i] = cs;
+      table[row * apart + j] = cs;
     }
-    __syncthreads();                         // (the table before last is free again: all threads have passed the last barrier)
-    for (int base = 0; base < units; base += U * groups) {
-      if (base) fetch(base);
+    __syncthreads();
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = base + u * groups + group;
-        const bool in = k < units && lives;
-        const int row = s.H > 1 ? (int)__umulhi(min(k, units - 1), s.magic) : min(k, units - 1);
-        const int head = min(k, units - 1) - row * s.H;
-        float va[VEC], vb[VEC], ca[VEC], sa[VEC];
-        to_pairs<VEC, IL>(x0[u], x1[u], va, vb);
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          sum = __builtin_fmaf(va[i], va[i], sum);
-          sum = __builtin_fmaf(vb[i], vb[i], sum);
-          const float2 cs = table[buf][row * half + j0 + i];
-          ca[i] = cs.x;
-          sa[i] = cs.y;
-        }
-        sum = lives ? sum : 0.f;
-        for (int m = lanes / 2; m; m >>= 1) sum += shfl_xor(sum, m);
-        const float r = 1.0f / sqrtf(sum / a.D + a.eps);
-        float oa[VEC], ob[VEC];
-        if constexpr (!BWD) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float ya = va[i] * r * wa[i], yb = vb[i] * r * wb[i];
-            oa[i] = ya * ca[i] - yb * sa[i];
-            ob[i] = yb * ca[i] + ya * sa[i];
-          }
-        } else {
-          float ta[VEC], tb[VEC], dot = 0.f;
-          to_pairs<VEC, IL>(g0[u], g1[u], ta, tb);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float na = ta[i] * ca[i] + tb[i] * sa[i], nb = tb[i] * ca[i] - ta[i] * sa[i];
-            va[i] *= r;
-            vb[i] *= r;
-            if (in) {
-              ga[i] = __builtin_fmaf(na, va[i], ga[i]);
-              gb[i] = __builtin_fmaf(nb, vb[i], gb[i]);
-            }
-            ta[i] = na * wa[i];
-            tb[i] = nb * wb[i];
-            dot = __builtin_fmaf(ta[i], va[i], dot);
-            dot = __builtin_fmaf(tb[i], vb[i], dot);
-          }
-          dot = lives ? dot : 0.f;
-          for (int m = lanes / 2; m; m >>= 1) dot += shfl_xor(dot, m);
-          dot /= a.D;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            oa[i] = r * (ta[i] - va[i] * dot);
-            ob[i] = r * (tb[i] - vb[i] * dot);
-          }
-        }
-        if (in) {
-          float p0[VEC], p1[VEC];
-          from_pairs<VEC, IL>(oa, ob, p0, p1);
-          T* y = (T*)s.y + (n0 + row) * s.yr + head * s.yh;
-          P::store(y + f0, p0);
-          P::store(y + f1, p1);
-        }
+    for (int i = 0; i < 2; ++i) {
+      const int units = rows * a.s[i].H;
+      for (int base = 0; base < units; base += U * groups) {
+        if (i || base) fetch(a.s[i], n0, units, base, raw);
+        compute(a.s[i], ws[i], n0, units, base, raw);
       }
     }
   }
-  if (!BWD || !s.part) return;
-  // the groups' sums of a column, in order: [group][D] in the tables' place
+  if (!BWD) return;
+  // the groups' sums of a column, in order, by all threads: parts of the groups first, [group][D] in the table's place
   float* red = (float*)table;
-  float p0[VEC], p1[VEC];
-  from_pairs<VEC, IL>(ga, gb, p0, p1);
-  __syncthreads();
-  if (lives)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      red[group * a.D + f0 + i] = p0[i];
-      red[group * a.D + f1 + i] = p1[i];
-    }
-  __syncthreads();
-  for (int f = threadIdx.x; f < a.D; f += NT) {
+  for (int i = 0; i < 2; ++i) {
+    if (!a.s[i].part) continue;
+    float p0[VEC], p1[VEC];
+    from_pairs<VEC, IL>(ws[i].ga, ws[i].gb, p0, p1);
+    __syncthreads();
+    if (lives)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        red[group * a.D + f0 + v] = p0[v];
+        red[group * a.D + f1 + v] = p1[v];
+      }
+    __syncthreads();
+    const int parts = NT / a.D, part = threadIdx.x / a.D, f = threadIdx.x - part * a.D;
     float t = 0.f;
-    for (int g = 0; g < groups; ++g) t += red[g * a.D + f];
-    s.part[(int64_t)block * a.D + f] = t;
+    if (part < parts) {
+#pragma unroll 8
+      for (int g = part; g < groups; g += parts) t += red[g * a.D + f];
+    }
+    __syncthreads();
+    red[threadIdx.x] = t;
+    __syncthreads();
+    if (part == 0) {
+      for (int k = 1; k < parts; ++k) t += red[k * a.D + f];
+      a.s[i].part[(int64_t)blockIdx.x * a.D + f] = t;
+    }
   }
 }
 
@@ -241,7 +312,7 @@ template <typename P> __global__ __launch_bounds__(1024) void sum_kernel(Args a)
   float t = 0.f;
   if (f < a.D && s.gw) {
 #pragma unroll 8
-    for (int b = k; b < s.blocks; b += 64) t += s.part[(int64_t)b * a.D + f];
+    for (int b = k; b < a.blocks; b += 64) t += s.part[(int64_t)b * a.D + f];
   }
   red[k][c] = t;
   __syncthreads();
@@ -264,27 +335,25 @@ static int lanes_of(const EgnnQkDims* d) {
   while (l * piece_of(d) < d->D / 2) l *= 2;
   return l;
 }
-// Rows of a tile, and tiles
-static int tile_rows(const EgnnQkDims* d, int H, int lanes) {
-  int tb = NT / lanes * U / H;
-  if (tb > kTable / (d->D / 2)) tb = kTable / (d->D / 2);
-  return tb < 1 ? 1 : tb;
+// Rows of a tile: enough heads of the side with fewer of them for two of each group of lanes, but a tile for each of 1,024
+// workgroups first
+static int tile_rows(const EgnnQkDims* d) {
+  const int H = d->Hq < d->Hk ? d->Hq : d->Hk;
+  int64_t tb = NT / lanes_of(d) * 2 / H;
+  if (tb > kTable / (d->D / 2 + 2)) tb = kTable / (d->D / 2 + 2);
+  if (tb > cdiv(d->N, 1024)) tb = cdiv(d->N, 1024);
+  return tb < 1 ? 1 : (int)tb;
 }
-// Workgroups of the backward, and partial rows of the weight gradients, of the two sides
+// Workgroups of the backward at most, and partial rows of the weight gradients
 constexpr int kBlocks = 1024;
-static void bwd_blocks(const EgnnQkDims* d, int32_t* q, int32_t* k) {
-  const int lanes = lanes_of(d);
-  const int64_t qt = cdiv(d->N, tile_rows(d, d->Hq, lanes)), kt = cdiv(d->N, tile_rows(d, d->Hk, lanes));
-  int64_t qb = (int64_t)kBlocks * d->Hq / (d->Hq + d->Hk), kb = kBlocks - qb;
-  if (qb < 1) qb = 1;
-  if (kb < 1) kb = 1;
-  *q = (int32_t)(qt < qb ? qt : qb);
-  *k = (int32_t)(kt < kb ? kt : kb);
+static int32_t blocks_of(const EgnnQkDims* d, int64_t most) {
+  const int64_t tiles = cdiv(d->N, tile_rows(d));
+  return (int32_t)(tiles < most ? tiles : most);
 }
 
 template <typename T, int VEC>
 static void launch(const Args& a, bool bwd, hipStream_t st) {
-  const uint32_t grid = (uint32_t)(a.s[0].blocks + a.s[1].blocks);
+  const uint32_t grid = (uint32_t)a.blocks;
   if (!grid) return;
   if (a.il) {
     if (bwd) qk_kernel<T, VEC, true, true><<<grid, NT, 0, st>>>(a);
@@ -307,11 +376,10 @@ static int run(const EgnnQkDims* d, Args& a, bool bwd, hipStream_t st) {
     Side& s = a.s[i];
     s.H = i ? d->Hk : d->Hq;
     s.magic = s.H > 1 ? (uint32_t)(((uint64_t(1) << 32) + s.H - 1) / s.H) : 0;
-    s.TB = tile_rows(d, s.H, a.lanes);
-    const int64_t tiles = cdiv(d->N, s.TB);
-    s.blocks = (int32_t)(tiles < kMaxGrid ? tiles : kMaxGrid);
   }
-  if (bwd) bwd_blocks(d, &a.s[0].blocks, &a.s[1].blocks);
+  a.inv = 1.f / d->D;
+  a.TB = tile_rows(d);
+  a.blocks = blocks_of(d, bwd ? kBlocks : kMaxGrid);
   if (d->dtype == EGNN_F32) {
     if (vec == 4) launch<float, 4>(a, bwd, st);
     else if (vec == 2) launch<float, 2>(a, bwd, st);
@@ -367,9 +435,7 @@ int32_t egnn_qk_fwd(const EgnnQkDims* d, const EgnnQkStrides* st, const void* q,
 
 size_t egnn_qk_bwd_workspace_bytes(const EgnnQkDims* d) {
   if (!d || !dims_ok(d)) return 0;
-  int32_t q, k;
-  bwd_blocks(d, &q, &k);
-  return ((size_t)q + k) * d->D * 4;
+  return (size_t)blocks_of(d, kBlocks) * 2 * d->D * 4;
 }
 
 int32_t egnn_qk_bwd(const EgnnQkDims* d, const EgnnQkStrides* st, const void* grad_q_out, const void* grad_k_out,
@@ -397,10 +463,8 @@ int32_t egnn_qk_bwd(const EgnnQkDims* d, const EgnnQkStrides* st, const void* gr
   x.xr = st->q_row; x.xh = st->q_head; x.gr = st->grad_q_out_row; x.gh = st->grad_q_out_head; x.yr = st->grad_q_row; x.yh = st->grad_q_head;
   y.x = k; y.w = k_weight; y.g = grad_k_out; y.y = grad_k; y.gw = grad_k_weight;
   y.xr = st->k_row; y.xh = st->k_head; y.gr = st->grad_k_out_row; y.gh = st->grad_k_out_head; y.yr = st->grad_k_row; y.yh = st->grad_k_head;
-  int32_t qb, kb;
-  bwd_blocks(d, &qb, &kb);
   x.part = grad_q_weight ? (float*)workspace : nullptr;
-  y.part = grad_k_weight ? (float*)workspace + (int64_t)qb * d->D : nullptr;
+  y.part = grad_k_weight ? (float*)workspace + (int64_t)blocks_of(d, kBlocks) * d->D : nullptr;
   return run(d, a, true, (hipStream_t)stream);
 }
 
