@@ -34,7 +34,6 @@ struct Args {
   int64_t N;
   int32_t TB, blocks;                        // rows of a tile, workgroups
   int32_t D, rot, lanes, act;                // lanes of a head (a power of two), and those of them with values
-  uint32_t pair_magic;                       // i / (D / 2)
   float eps, inv;                            // inv = 1 / D
   bool il, f32, i64;
   uint64_t freq[kPairs];                     // turns a position, in units of 2^-64
@@ -147,6 +146,9 @@ __global__ __launch_bounds__(NT) void qk_kernel(Args a) {
   if (IL) { f0 = 2 * j0; f1 = f0 + VEC; }
   else if (j0 < a.rot / 2) { f0 = j0; f1 = j0 + a.rot / 2; }
   else { f0 = a.rot + j0 - a.rot / 2; f1 = f0 + (a.D - a.rot) / 2; }
+  // a thread makes cos and sin of one pair (past the turned ones: of angle 0), for every per-th row
+  const int per = NT / half, tr = (int)threadIdx.x < per * half ? threadIdx.x / half : 1 << 30, tj = threadIdx.x % half;
+  const uint64_t freq = tj < a.rot / 2 ? a.freq[tj] : 0;
   Weights<VEC> ws[2];
   const int64_t tiles = (a.N + a.TB - 1) / a.TB;
   struct Raw { typename P::vals x0, x1, g0, g1; };
@@ -253,14 +255,16 @@ __global__ __launch_bounds__(NT) void qk_kernel(Args a) {
     } else {
       __syncthreads();                       // the table is read no more
     }
-    for (int i = threadIdx.x; i < rows * half; i += NT) {
-      const int row = half > 1 ? (int)__umulhi(i, a.pair_magic) : i, j = i - row * half;
-      float2 cs{1.f, 0.f};
-      if (j < a.rot / 2) {
-        const int64_t p = a.i64 ? ((const int64_t*)a.pos)[n0 + row] : ((const int32_t*)a.pos)[n0 + row];
-        cs = cos_sin((uint32_t)(((uint64_t)p * a.freq[j]) >> 32));
+    for (int row0 = tr; row0 < rows; row0 += 4 * per) {
+      int64_t p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t n = n0 + min(row0 + u * per, rows - 1);
+        p[u] = !a.rot ? 0 : a.i64 ? ((const int64_t*)a.pos)[n] : ((const int32_t*)a.pos)[n];
       }
-      table[row * apart + j] = cs;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (row0 + u * per < rows) table[(row0 + u * per) * apart + tj] = cos_sin((uint32_t)(((uint64_t)p[u] * freq) >> 32));
     }
     __syncthreads();
 #pragma unroll
@@ -323,31 +327,38 @@ template <typename P> __global__ __launch_bounds__(1024) void sum_kernel(Args a)
   if (!k && f < a.D && s.gw) ((P*)s.gw)[f] = from_f32<P>(red[0][c]);
 }
 
-// Widest piece that fits 16 bytes and never lies across the rotated part's middle or end
-static int piece_of(const EgnnQkDims* d) {
-  int v = d->dtype == EGNN_F32 ? 4 : 8;
+// Widest piece that fits 16 bytes (8 in the backward) and never lies across the rotated part's middle or end.  The backward
+// with pieces of 8 bf16 holds 184 registers, two waves a SIMD, with 4 it holds 113: 32,768 x 8 heads of 32, 24.5 and 16.3 us;
+// 1,048,576 x 3 heads of 128, 757 and 613; only the largest tensors of narrow heads lose, 2,000,000 x 8 heads of 32, 660 and 712.
+static int piece_of(const EgnnQkDims* d, bool bwd) {
+  int v = d->dtype == EGNN_F32 || bwd ? 4 : 8;
   const int half = d->D / 2, r = d->rotary / 2;
   while (v > 1 && (half % v || (!d->interleaved && r % v))) v /= 2;
   return v;
 }
-static int lanes_of(const EgnnQkDims* d) {
+static int lanes_of(const EgnnQkDims* d, bool bwd) {
   int l = 1;
-  while (l * piece_of(d) < d->D / 2) l *= 2;
+  while (l * piece_of(d, bwd) < d->D / 2) l *= 2;
   return l;
 }
 // Rows of a tile: enough heads of the side with fewer of them for two of each group of lanes, but a tile for each of 1,024
 // workgroups first
-static int tile_rows(const EgnnQkDims* d) {
+static int tile_rows(const EgnnQkDims* d, bool bwd) {
   const int H = d->Hq < d->Hk ? d->Hq : d->Hk;
-  int64_t tb = NT / lanes_of(d) * 2 / H;
+  const int groups = NT / lanes_of(d, bwd);
+  int64_t tb = groups * 2 / H;
   if (tb > kTable / (d->D / 2 + 2)) tb = kTable / (d->D / 2 + 2);
   if (tb > cdiv(d->N, 1024)) tb = cdiv(d->N, 1024);
+  int m = groups;                            // whole rounds of the groups over the heads
+  for (int h = H; h % 2 == 0 && m > 1; h /= 2) m /= 2;
+  if (tb > m) tb = tb / m * m;
   return tb < 1 ? 1 : (int)tb;
 }
 // Workgroups of the backward at most, and partial rows of the weight gradients
 constexpr int kBlocks = 1024;
-static int32_t blocks_of(const EgnnQkDims* d, int64_t most) {
-  const int64_t tiles = cdiv(d->N, tile_rows(d));
+static int32_t blocks_of(const EgnnQkDims* d, bool bwd) {
+  const int64_t most = bwd ? kBlocks : kMaxGrid;
+  const int64_t tiles = cdiv(d->N, tile_rows(d, bwd));
   return (int32_t)(tiles < most ? tiles : most);
 }
 
@@ -355,19 +366,20 @@ template <typename T, int VEC>
 static void launch(const Args& a, bool bwd, hipStream_t st) {
   const uint32_t grid = (uint32_t)a.blocks;
   if (!grid) return;
-  if (a.il) {
-    if (bwd) qk_kernel<T, VEC, true, true><<<grid, NT, 0, st>>>(a);
-    else qk_kernel<T, VEC, true, false><<<grid, NT, 0, st>>>(a);
-  } else {
-    if (bwd) qk_kernel<T, VEC, false, true><<<grid, NT, 0, st>>>(a);
-    else qk_kernel<T, VEC, false, false><<<grid, NT, 0, st>>>(a);
+  if constexpr (VEC <= 4) {
+    if (bwd) {
+      if (a.il) qk_kernel<T, VEC, true, true><<<grid, NT, 0, st>>>(a);
+      else qk_kernel<T, VEC, false, true><<<grid, NT, 0, st>>>(a);
+      return;
+    }
   }
+  if (a.il) qk_kernel<T, VEC, true, false><<<grid, NT, 0, st>>>(a);
+  else qk_kernel<T, VEC, false, false><<<grid, NT, 0, st>>>(a);
 }
 static int run(const EgnnQkDims* d, Args& a, bool bwd, hipStream_t st) {
-  const int vec = piece_of(d), half = d->D / 2;
-  a.N = d->N; a.D = d->D; a.rot = d->rotary; a.lanes = lanes_of(d); a.act = half / vec; a.eps = d->eps;
+  const int vec = piece_of(d, bwd), half = d->D / 2;
+  a.N = d->N; a.D = d->D; a.rot = d->rotary; a.lanes = lanes_of(d, bwd); a.act = half / vec; a.eps = d->eps;
   a.il = d->interleaved; a.f32 = d->f32_params; a.i64 = d->index64;
-  a.pair_magic = half > 1 ? (uint32_t)(((uint64_t(1) << 32) + half - 1) / half) : 0;
   // base^(-2 i / rotary) / 2 pi in units of 2^-64, by repeated multiplication in extended precision
   const long double step = d->rotary ? powl((long double)d->base, -2.0L / d->rotary) : 1.0L;
   long double f = 18446744073709551616.0L / 6.283185307179586476925286766559L;
@@ -378,8 +390,8 @@ static int run(const EgnnQkDims* d, Args& a, bool bwd, hipStream_t st) {
     s.magic = s.H > 1 ? (uint32_t)(((uint64_t(1) << 32) + s.H - 1) / s.H) : 0;
   }
   a.inv = 1.f / d->D;
-  a.TB = tile_rows(d);
-  a.blocks = blocks_of(d, bwd ? kBlocks : kMaxGrid);
+  a.TB = tile_rows(d, bwd);
+  a.blocks = blocks_of(d, bwd);
   if (d->dtype == EGNN_F32) {
     if (vec == 4) launch<float, 4>(a, bwd, st);
     else if (vec == 2) launch<float, 2>(a, bwd, st);
@@ -435,7 +447,7 @@ int32_t egnn_qk_fwd(const EgnnQkDims* d, const EgnnQkStrides* st, const void* q,
 
 size_t egnn_qk_bwd_workspace_bytes(const EgnnQkDims* d) {
   if (!d || !dims_ok(d)) return 0;
-  return (size_t)blocks_of(d, kBlocks) * 2 * d->D * 4;
+  return (size_t)blocks_of(d, true) * 2 * d->D * 4;
 }
 
 int32_t egnn_qk_bwd(const EgnnQkDims* d, const EgnnQkStrides* st, const void* grad_q_out, const void* grad_k_out,
@@ -464,7 +476,7 @@ int32_t egnn_qk_bwd(const EgnnQkDims* d, const EgnnQkStrides* st, const void* gr
   y.x = k; y.w = k_weight; y.g = grad_k_out; y.y = grad_k; y.gw = grad_k_weight;
   y.xr = st->k_row; y.xh = st->k_head; y.gr = st->grad_k_out_row; y.gh = st->grad_k_out_head; y.yr = st->grad_k_row; y.yh = st->grad_k_head;
   x.part = grad_q_weight ? (float*)workspace : nullptr;
-  y.part = grad_k_weight ? (float*)workspace + (int64_t)blocks_of(d, kBlocks) * d->D : nullptr;
+  y.part = grad_k_weight ? (float*)workspace + (int64_t)blocks_of(d, true) * d->D : nullptr;
   return run(d, a, true, (hipStream_t)stream);
 }
 
