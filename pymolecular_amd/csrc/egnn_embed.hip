@@ -101,9 +101,9 @@ static void launch_fwd(FwdArgs a, hipStream_t st) {
 }
 
 // ---- backward: sorting inside a workgroup --------------------------------------------------
-constexpr int BT = 512, NW = BT / 64;        // threads and waves of a workgroup
-constexpr int kBins = 1024;                  // values of a digit at most: two a thread
-constexpr int kChunk = 6144;                 // tokens of a workgroup at most (LDS: 24 KB of entries, 4 of offsets, 32 of counts)
+constexpr int BT = 256, NW = BT / 64;        // threads and waves of a workgroup
+constexpr int kBins = 1024, BPT = kBins / BT;   // values of a digit at most, and of them a thread's
+constexpr int kChunk = 8192;                 // tokens of a workgroup at most (LDS: 32 KB of entries, 4 of offsets, 16 of counts)
 
 // A stable counting sort of len values: bin_of(i) in [0, bins), or negative for none; put(i, bin, position).  cnt: NW * bins
 // words, off: bins + 1 (off[b]: where bin b begins).  The waves take consecutive parts, so a bin's values of a wave come
@@ -128,14 +128,12 @@ __device__ __forceinline__ void sort_block(int len, int bins, uint32_t* cnt, uin
       if (b[u] >= 0) atomicAdd(&mine[b[u]], 1u);
   }
   __syncthreads();
-  uint32_t tot[2], s = 0;
+  uint32_t s = 0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int b = 2 * threadIdx.x + j;
-    tot[j] = 0;
+  for (int j = 0; j < BPT; ++j) {
+    const int b = BPT * threadIdx.x + j;
     if (b < bins)
-      for (int k = 0; k < NW; ++k) tot[j] += cnt[k * bins + b];
-    s += tot[j];
+      for (int k = 0; k < NW; ++k) s += cnt[k * bins + b];
   }
   uint32_t inc = s;
 #pragma unroll
@@ -148,8 +146,8 @@ __device__ __forceinline__ void sort_block(int len, int bins, uint32_t* cnt, uin
   uint32_t base = inc - s;
   for (int k = 0; k < w; ++k) base += wave_sum[k];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int b = 2 * threadIdx.x + j;
+  for (int j = 0; j < BPT; ++j) {
+    const int b = BPT * threadIdx.x + j;
     if (b < bins) {
       off[b] = base;
       uint32_t at = base;
@@ -290,8 +288,9 @@ template <typename T, typename P, typename I, bool TAIL>
 __global__ __launch_bounds__(BT) void local_kernel(BwdArgs a) {
   extern __shared__ __align__(16) uint32_t lds[];
   constexpr int VEC = Vec<T>::N;
-  const int64_t r = blockIdx.x / a.chunks, chunk = blockIdx.x - r * a.chunks;
-  const int64_t n0 = chunk * a.chunk, v0 = r * a.range;
+  const uint32_t r = blockIdx.x / (uint32_t)a.chunks;
+  const int64_t chunk = blockIdx.x - r * (uint32_t)a.chunks;
+  const int64_t n0 = chunk * a.chunk, v0 = (int64_t)r * a.range;
   const int len = (int)(a.N - n0 < a.chunk ? a.N - n0 : a.chunk), bins = (int)(a.V - v0 < a.range ? a.V - v0 : a.range);
   uint32_t *ent = lds, *off = ent + a.chunk, *cnt = off + ((a.range + 4) & ~3);
   const I* tokens = (const I*)a.tokens + n0;
@@ -358,7 +357,7 @@ __global__ __launch_bounds__(1024) void reduce_kernel(const float* part, int chu
 }
 
 // ---- backward: the whole order sorted -------------------------------------------------------
-constexpr int kSortTile = 4096;              // values of a workgroup in a pass
+constexpr int kSortTile = 4096;              // values of a workgroup in a pass at most
 
 // A value is token << 32 | row; tokens outside the table get V and come last.
 struct SortArgs {
@@ -367,7 +366,7 @@ struct SortArgs {
   uint64_t* to;
   uint32_t *hist, *total;                    // [tile][digits], [digits]
   int64_t N, V;
-  int32_t shift, digits, tiles;
+  int32_t shift, digits, tile, tiles;
 };
 template <typename I, bool FIRST> __device__ __forceinline__ uint64_t sort_value(const SortArgs& a, int64_t n) {
   if (!FIRST) return a.from[n];
@@ -379,7 +378,7 @@ __global__ __launch_bounds__(BT) void hist_kernel(SortArgs a) {
   __shared__ uint32_t h[kBins];
   for (int d = threadIdx.x; d < a.digits; d += BT) h[d] = 0;
   __syncthreads();
-  const int64_t n0 = (int64_t)blockIdx.x * kSortTile, n1 = a.N - n0 < kSortTile ? a.N : n0 + kSortTile;
+  const int64_t n0 = (int64_t)blockIdx.x * a.tile, n1 = a.N - n0 < a.tile ? a.N : n0 + a.tile;
   for (int64_t n = n0 + threadIdx.x; n < n1; n += BT)
     atomicAdd(&h[(uint32_t)(sort_value<I, FIRST>(a, n) >> (32 + a.shift)) & (uint32_t)(a.digits - 1)], 1u);
   __syncthreads();
@@ -413,10 +412,10 @@ __global__ __launch_bounds__(BT) void scatter_kernel(SortArgs a) {
   __shared__ uint32_t cnt[NW * kBins], off[kBins + 1], base[kBins], sums[NW];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   // where a digit's values of this tile begin: all values of smaller digits, then those of the tiles before
-  uint32_t t[2], s = 0;
+  uint32_t t[BPT], s = 0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int d = 2 * threadIdx.x + j;
+  for (int j = 0; j < BPT; ++j) {
+    const int d = BPT * threadIdx.x + j;
     t[j] = d < a.digits ? a.total[d] : 0;
     s += t[j];
   }
@@ -431,13 +430,13 @@ __global__ __launch_bounds__(BT) void scatter_kernel(SortArgs a) {
   uint32_t at = inc - s;
   for (int k = 0; k < w; ++k) at += sums[k];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int d = 2 * threadIdx.x + j;
+  for (int j = 0; j < BPT; ++j) {
+    const int d = BPT * threadIdx.x + j;
     if (d < a.digits) base[d] = at + a.hist[(int64_t)blockIdx.x * a.digits + d];
     at += t[j];
   }
-  const int64_t n0 = (int64_t)blockIdx.x * kSortTile;
-  const int len = (int)(a.N - n0 < kSortTile ? a.N - n0 : kSortTile);
+  const int64_t n0 = (int64_t)blockIdx.x * a.tile;
+  const int len = (int)(a.N - n0 < a.tile ? a.N - n0 : a.tile);
   sort_block(len, a.digits, cnt, off,
              [&](int i) { return (int)((uint32_t)(sort_value<I, FIRST>(a, n0 + i) >> (32 + a.shift)) & (uint32_t)(a.digits - 1)); },
              [&](int i, int d, int pos) { a.to[base[d] + (uint32_t)pos - off[d]] = sort_value<I, FIRST>(a, n0 + i); });
@@ -484,66 +483,94 @@ __global__ __launch_bounds__(BT) void sorted_kernel(BwdArgs a) {
 }
 
 // Table rows whose run crosses tiles, or that no token names
-constexpr int FT = 256, kFixRows = 64, kLight = 16;
+constexpr int FT = 256, kFixRows = 64, kLight = 16, kFew = 4096;
+// The first position with a token of `want` or above, by a wave: 64 places of the rest at a time
+__device__ __forceinline__ int64_t first_of(const uint64_t* sorted, int64_t N, uint64_t want) {
+  int64_t lo = 0, n = N;                     // it is in [lo, lo + n]
+  while (n > 0) {
+    const int64_t step = (n + 63) / 64;
+    const int64_t p = lo + lane_id() * step;
+    const bool below = p < lo + n && sorted[p] >> 32 < want;
+    const int k = (int)__popcll(__ballot(below));   // the places below it come first
+    if (k == 0) return lo;
+    const int64_t end = lo + n;
+    lo += (k - 1) * step + 1;
+    n = lo + step - 1 < end ? step - 1 : end - lo;
+  }
+  return lo;
+}
 template <typename T, typename P, bool TAIL>
 __global__ __launch_bounds__(FT) void fix_kernel(BwdArgs a) {
   constexpr int VEC = Vec<T>::N;
-  __shared__ int64_t at[kFixRows + 1];
+  __shared__ int32_t at[kFixRows + 1], t0[kFixRows], t1[kFixRows], ends[2];
   __shared__ float join[FT * VEC];
   const int lpr = a.lpr, groups = FT / lpr, g = threadIdx.x / lpr, lane = threadIdx.x - g * lpr;
   const int k = blockIdx.y * lpr + lane;
   const bool lives = g < groups && k < a.pieces;
   const int f = lives ? first_column<VEC>(k, a.C) : 0;
   const int64_t blocks = (a.V + kFixRows - 1) / kFixRows;
+  auto part = [&](int t, int which) { return a.part + ((int64_t)t * 2 + which) * a.C; };
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     const int64_t v0 = b * kFixRows;
     const int nv = (int)(a.V - v0 < kFixRows ? a.V - v0 : kFixRows);
+    auto write = [&](int i, const float* acc) {
+      float o[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) o[j] = v0 + i == a.padding ? 0.f : acc[j] * a.scale;
+      store_params<T, P, TAIL>((P*)a.gw + (v0 + i) * a.C, f, a.C, o);
+    };
+    // where the rows' tokens begin
+    if (threadIdx.x < 128) {
+      const int32_t p = (int32_t)first_of(a.sorted, a.N, (uint64_t)(v0 + (threadIdx.x < 64 ? 0 : nv)));
+      if (lane_id() == 0) ends[threadIdx.x / 64] = p;
+    }
     __syncthreads();
-    if ((int)threadIdx.x <= nv) {            // the first position with a token of v0 + i or above
-      int64_t lo = 0, hi = a.N;
+    const int32_t s0 = ends[0], s1 = ends[1];
+    if (s1 - s0 <= kFew) {                   // few tokens: each looks whether it begins the next rows
+      for (int32_t p = s0 + threadIdx.x; p <= s1; p += FT) {
+        const int v = p < s1 ? (int)((int64_t)(a.sorted[p] >> 32) - v0) : nv;
+        for (int u = p > s0 ? (int)((int64_t)(a.sorted[p - 1] >> 32) - v0) + 1 : 0; u <= v; ++u) at[u] = p;
+      }
+    } else if ((int)threadIdx.x <= nv) {     // many: by halving
+      int32_t lo = s0, hi = s1;
       const uint64_t want = (uint64_t)(v0 + threadIdx.x);
       while (lo < hi) {
-        const int64_t mid = (lo + hi) / 2;
+        const int32_t mid = lo + (hi - lo) / 2;
         if (a.sorted[mid] >> 32 >= want) hi = mid;
         else lo = mid + 1;
       }
       at[threadIdx.x] = lo;
     }
     __syncthreads();
-    auto part = [&](int64_t t, int which) { return a.part + (t * 2 + which) * a.C; };
-    auto write = [&](int64_t v, const float* acc) {
-      float o[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) o[i] = v == a.padding ? 0.f : acc[i] * a.scale;
-      store_params<T, P, TAIL>((P*)a.gw + v * a.C, f, a.C, o);
-    };
+    // the tiles of a run; t0 = t1: it is written already.  No run: one less.
+    if ((int)threadIdx.x < nv) {
+      const uint32_t s = at[threadIdx.x], e = at[threadIdx.x + 1];
+      t0[threadIdx.x] = (int32_t)(s / (uint32_t)a.tile);
+      t1[threadIdx.x] = s < e ? (int32_t)((e - 1) / (uint32_t)a.tile) : (int32_t)(s / (uint32_t)a.tile) - 1;
+    }
+    __syncthreads();
     for (int i = g; i < nv && lives; i += groups) {
-      const int64_t s = at[i], e = at[i + 1];
+      const int b0 = t0[i], b1 = t1[i];
+      if (b0 == b1 || b1 - b0 > kLight) continue;
       float acc[VEC] = {};
-      if (s < e) {
-        const int64_t t0 = s / a.tile, t1 = (e - 1) / a.tile;
-        if (t0 == t1 || t1 - t0 > kLight) continue;
-        load_params<T, float, TAIL>(part(t0, 1), f, a.C, acc);
-        for (int64_t t = t0 + 1; t <= t1; ++t) {
-          float x[VEC];
-          load_params<T, float, TAIL>(part(t, 0), f, a.C, x);
+      for (int t = b0; t <= b1; ++t) {
+        float x[VEC];
+        load_params<T, float, TAIL>(part(t, t == b0 ? 1 : 0), f, a.C, x);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[j] += x[j];
-        }
+        for (int j = 0; j < VEC; ++j) acc[j] += x[j];
       }
-      write(v0 + i, acc);
+      write(i, acc);
     }
     // long runs: the groups take their tiles in turn
     for (int i = 0; i < nv; ++i) {
-      const int64_t s = at[i], e = at[i + 1];
-      if (s >= e || (e - 1) / a.tile - s / a.tile <= kLight) continue;   // (the same for all threads)
-      const int64_t t0 = s / a.tile, t1 = (e - 1) / a.tile;
+      const int b0 = t0[i], b1 = t1[i];
+      if (b1 - b0 <= kLight) continue;       // (the same for all threads)
       float acc[VEC] = {};
       if (lives) {
 #pragma unroll 4
-        for (int64_t t = t0 + g; t <= t1; t += groups) {
+        for (int t = b0 + g; t <= b1; t += groups) {
           float x[VEC];
-          load_params<T, float, TAIL>(part(t, t == t0 ? 1 : 0), f, a.C, x);
+          load_params<T, float, TAIL>(part(t, t == b0 ? 1 : 0), f, a.C, x);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) acc[j] += x[j];
         }
@@ -556,9 +583,10 @@ __global__ __launch_bounds__(FT) void fix_kernel(BwdArgs a) {
         for (int h = 1; h < groups; ++h)
 #pragma unroll
           for (int j = 0; j < VEC; ++j) acc[j] += join[(h * lpr + lane) * VEC + j];
-        write(v0 + i, acc);
+        write(i, acc);
       }
     }
+    __syncthreads();
   }
 }
 
@@ -568,25 +596,26 @@ struct Plan {
   int lpr, pieces, tiles;                    // lanes of a row in a column tile, pieces of a row, column tiles
   int chunk, chunks, range, ranges;          // local
   int span, tile, blocks;                    // sorted: positions of a group, of a workgroup, workgroups
-  int passes, bits, sort_tiles;
+  int passes, bits, sort_tile, sort_tiles;
   size_t part, sorted, hist, bytes;          // offsets of sorted and hist behind part; bytes altogether
 };
 static Plan plan_of(const EgnnEmbedDims* d) {
   Plan p{};
   const int64_t N = d->N, V = d->V;
   p.pieces = (int)cdiv(d->C, d->dtype == EGNN_F32 ? 4 : 8);
-  p.tiles = (int)cdiv(p.pieces, 128);
-  p.lpr = (int)cdiv(p.pieces, p.tiles);
   const int64_t least = N ? cdiv(N, kChunk) : 1;
   p.local = least == 1 || (V <= 4096 && least * V <= N / 2);
   if (p.local) {
-    int64_t most = N / (2 * V);              // partial tables: at most half as many rows as there are tokens
-    if (most > cdiv(N, 256)) most = cdiv(N, 256);
-    if (most > cdiv(1024, p.tiles)) most = cdiv(1024, p.tiles);
-    int64_t K = N <= 4096 ? 1 : most;
+    int64_t K = N <= 4096 ? 1 : N / (2 * V);   // partial tables: at most half as many rows as there are tokens
+    if (K > cdiv(N, 256)) K = cdiv(N, 256);
+    if (K > 1024) K = 1024;
     if (K < least) K = least;
     p.chunk = (int)cdiv(cdiv(N ? N : 1, K), 64) * 64;
     p.chunks = (int)cdiv(N ? N : 1, p.chunk);
+    // too few of them: column tiles, down to 128 bytes of a row, then ranges of the table
+    p.tiles = (int)cdiv(p.pieces, 64);
+    while (p.chunks * p.tiles < 512 && cdiv(p.pieces, 2 * p.tiles) >= 8) p.tiles *= 2;
+    p.lpr = (int)cdiv(p.pieces, p.tiles);
     int64_t R = cdiv(512, (int64_t)p.chunks * p.tiles);
     if (R > V) R = V;
     if (R < cdiv(V, kBins)) R = cdiv(V, kBins);
@@ -595,11 +624,14 @@ static Plan plan_of(const EgnnEmbedDims* d) {
     p.bytes = p.chunks > 1 ? (size_t)p.chunks * V * d->C * 4 : 0;
     return p;
   }
+  p.tiles = (int)cdiv(p.pieces, 64);
+  p.lpr = (int)cdiv(p.pieces, p.tiles);
   int width = 0;                             // bits of a key: 0 .. V
   while (V >> width) ++width;
   p.passes = (int)cdiv(width, 10);
   p.bits = (int)cdiv(width, p.passes);
-  p.sort_tiles = (int)cdiv(N, kSortTile);
+  p.sort_tile = (int)(N < 256 * 512 ? 512 : N > 256 * (int64_t)kSortTile ? kSortTile : cdiv(N, 256 * 512) * 512);
+  p.sort_tiles = (int)cdiv(N, p.sort_tile);
   const int groups = BT / p.lpr;
   int64_t span = N / ((int64_t)groups * 1024) / 8 * 8;
   span = span < 8 ? 8 : span > 32 ? 32 : span;
@@ -639,7 +671,7 @@ static int launch_bwd(BwdArgs a, const Plan& p, void* ws, hipStream_t st) {
   a.part = (float*)at;
   uint64_t *one = (uint64_t*)(at + p.part), *two = (uint64_t*)(at + p.part + p.sorted);
   SortArgs s{};
-  s.tokens = a.tokens; s.N = a.N; s.V = a.V; s.digits = 1 << p.bits; s.tiles = p.sort_tiles;
+  s.tokens = a.tokens; s.N = a.N; s.V = a.V; s.digits = 1 << p.bits; s.tile = p.sort_tile; s.tiles = p.sort_tiles;
   s.total = (uint32_t*)(at + p.part + 2 * p.sorted);
   s.hist = s.total + s.digits;
   for (int k = 0; k < p.passes; ++k) {
