@@ -49,7 +49,7 @@ struct FwdArgs {
   float scale;
 };
 
-template <typename T, typename P, typename I, bool TAIL>
+template <typename T, typename P, typename I, bool TAIL, bool PAST>
 __global__ __launch_bounds__(NT) void fwd_kernel(FwdArgs a) {
   typedef Vec<T, TAIL> V;
   constexpr int VEC = V::N;
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(FwdArgs a) {
   }
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (in[u]) V::store((T*)a.out + n[u] * a.C, f[u], a.C, v[u]);
+    if (in[u]) V::template store<PAST>((T*)a.out + n[u] * a.C, f[u], a.C, v[u]);
 }
 
 template <typename T, typename P, typename I>
@@ -95,21 +95,27 @@ static void launch_fwd(FwdArgs a, hipStream_t st) {
     a.out = (T*)all.out + n * a.C;
     a.N = N - n < most ? N - n : most;
     const dim3 grid((uint32_t)cdiv(a.N, a.R), (uint32_t)tiles);
-    if (a.C % VEC) fwd_kernel<T, P, I, true><<<grid, NT, 0, st>>>(a);
-    else fwd_kernel<T, P, I, false><<<grid, NT, 0, st>>>(a);
+    if (N * a.C * (int64_t)sizeof(T) >= kPastStore) {
+      if (a.C % VEC) fwd_kernel<T, P, I, true, true><<<grid, NT, 0, st>>>(a);
+      else fwd_kernel<T, P, I, false, true><<<grid, NT, 0, st>>>(a);
+    } else {
+      if (a.C % VEC) fwd_kernel<T, P, I, true, false><<<grid, NT, 0, st>>>(a);
+      else fwd_kernel<T, P, I, false, false><<<grid, NT, 0, st>>>(a);
+    }
   }
 }
 
 // ---- backward: sorting inside a workgroup --------------------------------------------------
 constexpr int BT = 256, NW = BT / 64;        // threads and waves of a workgroup
-constexpr int kBins = 1024, BPT = kBins / BT;   // values of a digit at most, and of them a thread's
-constexpr int kChunk = 8192;                 // tokens of a workgroup at most (LDS: 32 KB of entries, 4 of offsets, 16 of counts)
+constexpr int kBins = 2048;                  // values of a digit at most
+constexpr int kChunk = 6144, kRange = 1024;  // local: tokens and table rows of a workgroup at most
 
 // A stable counting sort of len values: bin_of(i) in [0, bins), or negative for none; put(i, bin, position).  cnt: NW * bins
-// words, off: bins + 1 (off[b]: where bin b begins).  The waves take consecutive parts, so a bin's values of a wave come
-// after those of the waves before it; within 64 values the lanes of one bin find each other by votes on its bits.
+// words, off: bins + 1 (off[b]: where bin b begins), memo: len halfwords.  The waves take consecutive parts, so a bin's values
+// of a wave come after those of the waves before it; within 64 values the lanes of one bin find each other by votes on its
+// bits.
 template <typename Bin, typename Put>
-__device__ __forceinline__ void sort_block(int len, int bins, uint32_t* cnt, uint32_t* off, Bin bin_of, Put put) {
+__device__ __forceinline__ void sort_block(int len, int bins, uint32_t* cnt, uint32_t* off, uint16_t* memo, Bin bin_of, Put put) {
   __shared__ uint32_t wave_sum[NW];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int per = (len + BT - 1) / BT * 64, lo = w * per;
@@ -124,17 +130,18 @@ __device__ __forceinline__ void sort_block(int len, int bins, uint32_t* cnt, uin
       b[u] = r + 64 * u < per && i < len ? bin_of(i) : -1;
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 4; ++u) {
+      const int i = lo + r + 64 * u + lane;
+      if (r + 64 * u < per && i < len) memo[i] = (uint16_t)b[u];
       if (b[u] >= 0) atomicAdd(&mine[b[u]], 1u);
+    }
   }
   __syncthreads();
+  const int own = (bins + BT - 1) / BT, own0 = own * threadIdx.x, own1 = min(bins, own0 + own);   // a thread's bins
   uint32_t s = 0;
+  for (int b = own0; b < own1; ++b)
 #pragma unroll
-  for (int j = 0; j < BPT; ++j) {
-    const int b = BPT * threadIdx.x + j;
-    if (b < bins)
-      for (int k = 0; k < NW; ++k) s += cnt[k * bins + b];
-  }
+    for (int k = 0; k < NW; ++k) s += cnt[k * bins + b];
   uint32_t inc = s;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -145,20 +152,15 @@ __device__ __forceinline__ void sort_block(int len, int bins, uint32_t* cnt, uin
   __syncthreads();
   uint32_t base = inc - s;
   for (int k = 0; k < w; ++k) base += wave_sum[k];
+  for (int b = own0; b < own1; ++b) {
+    off[b] = base;
 #pragma unroll
-  for (int j = 0; j < BPT; ++j) {
-    const int b = BPT * threadIdx.x + j;
-    if (b < bins) {
-      off[b] = base;
-      uint32_t at = base;
-      for (int k = 0; k < NW; ++k) {
-        const uint32_t c = cnt[k * bins + b];
-        cnt[k * bins + b] = at;
-        at += c;
-      }
-      base = at;
-      if (b == bins - 1) off[bins] = base;
+    for (int k = 0; k < NW; ++k) {
+      const uint32_t c = cnt[k * bins + b];
+      cnt[k * bins + b] = base;
+      base += c;
     }
+    if (b == bins - 1) off[bins] = base;
   }
   __syncthreads();
   const int bits = 32 - __clz(bins - 1);
@@ -168,7 +170,7 @@ __device__ __forceinline__ void sort_block(int len, int bins, uint32_t* cnt, uin
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int i = lo + r + 64 * u + lane;
-      bin[u] = r + 64 * u < per && i < len ? bin_of(i) : -1;
+      bin[u] = r + 64 * u < per && i < len ? (int)(int16_t)memo[i] : -1;
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -205,11 +207,12 @@ struct BwdArgs {
 };
 
 // Positions [0, S) of a tile: key(p) and row(p) (a row of the gradient).  before / after: the first / last run goes on outside
-// the tile.  A group of lpr lanes sums `span` positions; emit(key, kind, v) gets each run's sum: kind 0 the whole run, 1 its
-// part if it began before the tile, 2 its part if it goes on behind it.
-template <typename T, bool TAIL, typename Key, typename Row, typename Emit>
+// the tile.  A group of lpr lanes sums `span` positions; end(key, p): where the run of this key ends that holds position
+// p - 1.  emit(key, kind, v) gets each run's sum: kind 0 the whole run, 1 its part if it began before the tile, 2 its part if it
+// goes on behind it.
+template <typename T, bool TAIL, bool PAST, typename Key, typename Row, typename End, typename Emit>
 __device__ __forceinline__ void sum_tile(const BwdArgs& a, int S, int span, bool before, bool after, float* carry, Key key,
-                                         Row row, Emit emit) {
+                                         Row row, End end, Emit emit) {
   typedef Vec<T, TAIL> V;
   constexpr int VEC = V::N, UR = 8;
   const int lpr = a.lpr, groups = BT / lpr, g = threadIdx.x / lpr, lane = threadIdx.x - g * lpr;
@@ -234,7 +237,7 @@ __device__ __forceinline__ void sum_tile(const BwdArgs& a, int S, int span, bool
     for (int p = p0; p < p1; p += UR) {
       typename V::piece x[UR];
 #pragma unroll
-      for (int u = 0; u < UR; ++u) x[u] = V::load((const T*)a.g + row(min(p + u, p1 - 1)) * a.ldg, f, a.C);
+      for (int u = 0; u < UR; ++u) x[u] = V::template load<PAST>((const T*)a.g + row(min(p + u, p1 - 1)) * a.ldg, f, a.C);
       if (p + UR <= p1 && key(p + UR - 1) == cur) {   // one run: eight rows are added up by themselves first
         float e[UR][VEC];
 #pragma unroll
@@ -270,11 +273,11 @@ __device__ __forceinline__ void sum_tile(const BwdArgs& a, int S, int span, bool
   auto join = [&](uint32_t cur, int which) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = slot(g, which)[i];
-    int h = g + 1;
-    for (; h * span < S && key(h * span) == cur; ++h) {
+    const int h = (min(end(cur, p1), S) - 1) / span + 1;   // the groups up to that of its last position
+#pragma unroll 4
+    for (int q = g + 1; q < h; ++q)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] += slot(h, 0)[i];
-    }
+      for (int i = 0; i < VEC; ++i) acc[i] += slot(q, 0)[i];
     const bool ends = !after || key(S - 1) != cur;
     emit(cur, which == 0 ? 1 : ends ? 0 : 2, f, acc);
   };
@@ -284,7 +287,7 @@ __device__ __forceinline__ void sum_tile(const BwdArgs& a, int S, int span, bool
   if (!last_began && goes_on) join(last, 1);
 }
 
-template <typename T, typename P, typename I, bool TAIL>
+template <typename T, typename P, typename I, bool TAIL, bool PAST>
 __global__ __launch_bounds__(BT) void local_kernel(BwdArgs a) {
   extern __shared__ __align__(16) uint32_t lds[];
   constexpr int VEC = Vec<T>::N;
@@ -292,9 +295,10 @@ __global__ __launch_bounds__(BT) void local_kernel(BwdArgs a) {
   const int64_t chunk = blockIdx.x - r * (uint32_t)a.chunks;
   const int64_t n0 = chunk * a.chunk, v0 = (int64_t)r * a.range;
   const int len = (int)(a.N - n0 < a.chunk ? a.N - n0 : a.chunk), bins = (int)(a.V - v0 < a.range ? a.V - v0 : a.range);
-  uint32_t *ent = lds, *off = ent + a.chunk, *cnt = off + ((a.range + 4) & ~3);
+  uint32_t *ent = lds, *off = ent + a.chunk, *cnt = off + ((a.range + 4) & ~3);   // (cnt: at least the carries of sum_tile)
+  uint16_t* memo = (uint16_t*)(cnt + max(NW * a.range, BT * 2 * VEC));
   const I* tokens = (const I*)a.tokens + n0;
-  sort_block(len, bins, cnt, off,
+  sort_block(len, bins, cnt, off, memo,
              [&](int i) {
                const uint64_t b = (uint64_t)((int64_t)tokens[i] - v0);
                return b < (uint64_t)bins ? (int)b : -1;
@@ -312,8 +316,8 @@ __global__ __launch_bounds__(BT) void local_kernel(BwdArgs a) {
       store_params<T, P, TAIL>((P*)a.gw + v * a.C, f, a.C, o);
     }
   };
-  sum_tile<T, TAIL>(a, S, (S + groups - 1) / groups, false, false, (float*)cnt, [&](int p) { return ent[p] >> 16; },
-                    [&](int p) { return n0 + (int64_t)(ent[p] & 0xffff); },
+  sum_tile<T, TAIL, PAST>(a, S, (S + groups - 1) / groups, false, false, (float*)cnt, [&](int p) { return ent[p] >> 16; },
+                    [&](int p) { return n0 + (int64_t)(ent[p] & 0xffff); }, [&](uint32_t b, int) { return (int)off[b + 1]; },
                     [&](uint32_t b, int, int f, const float* acc) { write(v0 + b, f, acc); });
   const int g = threadIdx.x / a.lpr, k = blockIdx.y * a.lpr + threadIdx.x - g * a.lpr;
   if (g >= groups || k >= a.pieces) return;
@@ -358,6 +362,7 @@ __global__ __launch_bounds__(1024) void reduce_kernel(const float* part, int chu
 
 // ---- backward: the whole order sorted -------------------------------------------------------
 constexpr int kSortTile = 4096;              // values of a workgroup in a pass at most
+constexpr int kFewTiles = 64;                // up to so many a workgroup adds up their counts by itself
 
 // A value is token << 32 | row; tokens outside the table get V and come last.
 struct SortArgs {
@@ -407,18 +412,33 @@ __global__ __launch_bounds__(1024) void scan_kernel(SortArgs a) {
   }
   if (k == 63) a.total[d] = at;
 }
-template <typename I, bool FIRST>
+// FEW: no scan_kernel ran; the workgroup adds up the tiles' counts by itself (and the first one leaves the totals)
+template <typename I, bool FIRST, bool FEW>
 __global__ __launch_bounds__(BT) void scatter_kernel(SortArgs a) {
-  __shared__ uint32_t cnt[NW * kBins], off[kBins + 1], base[kBins], sums[NW];
+  extern __shared__ __align__(16) uint32_t lds[];
+  __shared__ uint32_t sums[NW];
+  uint32_t *base = lds, *off = base + a.digits, *cnt = off + a.digits + 4;
+  uint16_t* memo = (uint16_t*)(cnt + NW * a.digits);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   // where a digit's values of this tile begin: all values of smaller digits, then those of the tiles before
-  uint32_t t[BPT], s = 0;
-#pragma unroll
-  for (int j = 0; j < BPT; ++j) {
-    const int d = BPT * threadIdx.x + j;
-    t[j] = d < a.digits ? a.total[d] : 0;
-    s += t[j];
+  if (FEW) {
+    for (int d = threadIdx.x; d < a.digits; d += BT) {
+      uint32_t all = 0, mine = 0;
+#pragma unroll 16
+      for (int b = 0; b < a.tiles; ++b) {
+        const uint32_t x = a.hist[(int64_t)b * a.digits + d];
+        all += x;
+        mine += b < (int)blockIdx.x ? x : 0;
+      }
+      base[d] = mine;
+      cnt[d] = all;
+      if (!blockIdx.x) a.total[d] = all;
+    }
+    __syncthreads();
   }
+  const int own = (a.digits + BT - 1) / BT, own0 = own * threadIdx.x, own1 = min(a.digits, own0 + own);   // a thread's digits
+  uint32_t s = 0;
+  for (int d = own0; d < own1; ++d) s += FEW ? cnt[d] : a.total[d];
   uint32_t inc = s;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -429,20 +449,19 @@ __global__ __launch_bounds__(BT) void scatter_kernel(SortArgs a) {
   __syncthreads();
   uint32_t at = inc - s;
   for (int k = 0; k < w; ++k) at += sums[k];
-#pragma unroll
-  for (int j = 0; j < BPT; ++j) {
-    const int d = BPT * threadIdx.x + j;
-    if (d < a.digits) base[d] = at + a.hist[(int64_t)blockIdx.x * a.digits + d];
-    at += t[j];
+  for (int d = own0; d < own1; ++d) {
+    base[d] = at + (FEW ? base[d] : a.hist[(int64_t)blockIdx.x * a.digits + d]);
+    at += FEW ? cnt[d] : a.total[d];
   }
+  __syncthreads();
   const int64_t n0 = (int64_t)blockIdx.x * a.tile;
   const int len = (int)(a.N - n0 < a.tile ? a.N - n0 : a.tile);
-  sort_block(len, a.digits, cnt, off,
+  sort_block(len, a.digits, cnt, off, memo,
              [&](int i) { return (int)((uint32_t)(sort_value<I, FIRST>(a, n0 + i) >> (32 + a.shift)) & (uint32_t)(a.digits - 1)); },
              [&](int i, int d, int pos) { a.to[base[d] + (uint32_t)pos - off[d]] = sort_value<I, FIRST>(a, n0 + i); });
 }
 
-template <typename T, typename P, bool TAIL>
+template <typename T, typename P, bool TAIL, bool PAST>
 __global__ __launch_bounds__(BT) void sorted_kernel(BwdArgs a) {
   extern __shared__ __align__(16) uint32_t lds[];
   constexpr int VEC = Vec<T>::N;
@@ -469,7 +488,13 @@ __global__ __launch_bounds__(BT) void sorted_kernel(BwdArgs a) {
     S = lo;
   }
   const bool before = S > 0 && key[0] == key[1], after = S == len && key[len] == key[len + 1];
-  sum_tile<T, TAIL>(a, S, a.span, before, after, carry, [&](int p) { return key[p + 1]; }, [&](int p) { return (int64_t)row[p]; },
+  auto end = [&](uint32_t v, int p) {
+    for (int step = a.tile; step; step >>= 1)
+      while (p + step <= S && key[p + step] == v) p += step;
+    return p;
+  };
+  sum_tile<T, TAIL, PAST>(a, S, a.span, before, after, carry, [&](int p) { return key[p + 1]; },
+                          [&](int p) { return (int64_t)row[p]; }, end,
                     [&](uint32_t v, int kind, int f, const float* acc) {
                       if (kind) {
                         store_params<T, float, TAIL>(a.part + ((int64_t)blockIdx.x * 2 + kind - 1) * a.C, f, a.C, acc);
@@ -483,10 +508,9 @@ __global__ __launch_bounds__(BT) void sorted_kernel(BwdArgs a) {
 }
 
 // Table rows whose run crosses tiles, or that no token names
-constexpr int FT = 256, kFixRows = 64, kLight = 16, kFew = 4096;
-// The first position with a token of `want` or above, by a wave: 64 places of the rest at a time
-__device__ __forceinline__ int64_t first_of(const uint64_t* sorted, int64_t N, uint64_t want) {
-  int64_t lo = 0, n = N;                     // it is in [lo, lo + n]
+constexpr int FT = 256, kFixRows = 64, kLight = 16, kFew = 1024;
+// The first position with a token of `want` or above, which is in [lo, lo + n], by a wave: 64 places of the rest at a time
+__device__ __forceinline__ int64_t first_of(const uint64_t* sorted, int64_t lo, int64_t n, uint64_t want) {
   while (n > 0) {
     const int64_t step = (n + 63) / 64;
     const int64_t p = lo + lane_id() * step;
@@ -499,37 +523,59 @@ __device__ __forceinline__ int64_t first_of(const uint64_t* sorted, int64_t N, u
   }
   return lo;
 }
+// The last digit's totals say between which positions the tokens of 2^shift rows lie; a workgroup takes some of those rows.
 template <typename T, typename P, bool TAIL>
-__global__ __launch_bounds__(FT) void fix_kernel(BwdArgs a) {
+__global__ __launch_bounds__(FT) void fix_kernel(BwdArgs a, const uint32_t* total, int shift, int rows) {
   constexpr int VEC = Vec<T>::N;
-  __shared__ int32_t at[kFixRows + 1], t0[kFixRows], t1[kFixRows], ends[2];
+  __shared__ int32_t at[kFixRows + 1], t0[kFixRows], t1[kFixRows], ends[2], part_sum[FT / 64];
   __shared__ float join[FT * VEC];
   const int lpr = a.lpr, groups = FT / lpr, g = threadIdx.x / lpr, lane = threadIdx.x - g * lpr;
   const int k = blockIdx.y * lpr + lane;
   const bool lives = g < groups && k < a.pieces;
   const int f = lives ? first_column<VEC>(k, a.C) : 0;
-  const int64_t blocks = (a.V + kFixRows - 1) / kFixRows;
+  const int64_t blocks = (a.V + rows - 1) / rows;
   auto part = [&](int t, int which) { return a.part + ((int64_t)t * 2 + which) * a.C; };
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const int64_t v0 = b * kFixRows;
-    const int nv = (int)(a.V - v0 < kFixRows ? a.V - v0 : kFixRows);
+    const int64_t v0 = b * rows;             // (rows divides 2^shift, or shift is 0)
+    const int nv = (int)(a.V - v0 < rows ? a.V - v0 : rows);
     auto write = [&](int i, const float* acc) {
       float o[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) o[j] = v0 + i == a.padding ? 0.f : acc[j] * a.scale;
       store_params<T, P, TAIL>((P*)a.gw + (v0 + i) * a.C, f, a.C, o);
     };
-    // where the rows' tokens begin
-    if (threadIdx.x < 128) {
-      const int32_t p = (int32_t)first_of(a.sorted, a.N, (uint64_t)(v0 + (threadIdx.x < 64 ? 0 : nv)));
-      if (lane_id() == 0) ends[threadIdx.x / 64] = p;
-    }
+    // where the rows' tokens begin: behind those of all smaller last digits
+    const int digit = (int)(v0 >> shift);
+    uint32_t before = 0;
+    for (int d = threadIdx.x; d < digit; d += FT) before += total[d];
+#pragma unroll
+    for (int m = 32; m; m >>= 1) before += __shfl_xor(before, m, 64);
+    if (lane_id() == 0) part_sum[threadIdx.x / 64] = (int32_t)before;
     __syncthreads();
-    const int32_t s0 = ends[0], s1 = ends[1];
-    if (s1 - s0 <= kFew) {                   // few tokens: each looks whether it begins the next rows
+    int32_t s0 = part_sum[0] + part_sum[1] + part_sum[2] + part_sum[3], s1 = s0;
+    if (shift) {
+      s1 += (int32_t)total[digit];
+      if (s1 - s0 > FT) {                    // among many: the part of these rows
+        if (threadIdx.x < 128) {
+          const int32_t p = (int32_t)first_of(a.sorted, s0, s1 - s0, (uint64_t)(v0 + (threadIdx.x < 64 ? 0 : nv)));
+          if (lane_id() == 0) ends[threadIdx.x / 64] = p;
+        }
+        __syncthreads();
+        s0 = ends[0];
+        s1 = ends[1];
+      }
+    }
+    if (!shift) {                            // a digit is a row
+      if (threadIdx.x == 0) {
+        at[0] = s0;
+        for (int i = 0; i < nv; ++i) at[i + 1] = at[i] + (int32_t)total[v0 + i];
+      }
+    } else if (s1 - s0 <= kFew) {            // few tokens: each looks whether it begins the next rows
       for (int32_t p = s0 + threadIdx.x; p <= s1; p += FT) {
-        const int v = p < s1 ? (int)((int64_t)(a.sorted[p] >> 32) - v0) : nv;
-        for (int u = p > s0 ? (int)((int64_t)(a.sorted[p - 1] >> 32) - v0) + 1 : 0; u <= v; ++u) at[u] = p;
+        // (tokens of the digit's rows before and behind these count as one row there)
+        const int64_t v = p < s1 ? (int64_t)(a.sorted[p] >> 32) - v0 : nv;
+        const int64_t u = p > s0 ? (int64_t)(a.sorted[p - 1] >> 32) - v0 + 1 : 0;
+        for (int r = (int)(u > 0 ? u : 0); r <= (v < nv ? v : nv); ++r) at[r] = p;
       }
     } else if ((int)threadIdx.x <= nv) {     // many: by halving
       int32_t lo = s0, hi = s1;
@@ -604,7 +650,7 @@ static Plan plan_of(const EgnnEmbedDims* d) {
   const int64_t N = d->N, V = d->V;
   p.pieces = (int)cdiv(d->C, d->dtype == EGNN_F32 ? 4 : 8);
   const int64_t least = N ? cdiv(N, kChunk) : 1;
-  p.local = least == 1 || (V <= 4096 && least * V <= N / 2);
+  p.local = least == 1 || (V <= kRange && least * V <= N / 2);
   if (p.local) {
     int64_t K = N <= 4096 ? 1 : N / (2 * V);   // partial tables: at most half as many rows as there are tokens
     if (K > cdiv(N, 256)) K = cdiv(N, 256);
@@ -618,7 +664,7 @@ static Plan plan_of(const EgnnEmbedDims* d) {
     p.lpr = (int)cdiv(p.pieces, p.tiles);
     int64_t R = cdiv(512, (int64_t)p.chunks * p.tiles);
     if (R > V) R = V;
-    if (R < cdiv(V, kBins)) R = cdiv(V, kBins);
+    if (R < cdiv(V, kRange)) R = cdiv(V, kRange);
     p.range = (int)cdiv(V, R);
     p.ranges = (int)cdiv(V, p.range);
     p.bytes = p.chunks > 1 ? (size_t)p.chunks * V * d->C * 4 : 0;
@@ -628,9 +674,9 @@ static Plan plan_of(const EgnnEmbedDims* d) {
   p.lpr = (int)cdiv(p.pieces, p.tiles);
   int width = 0;                             // bits of a key: 0 .. V
   while (V >> width) ++width;
-  p.passes = (int)cdiv(width, 10);
+  p.passes = (int)cdiv(width, 11);
   p.bits = (int)cdiv(width, p.passes);
-  p.sort_tile = (int)(N < 256 * 512 ? 512 : N > 256 * (int64_t)kSortTile ? kSortTile : cdiv(N, 256 * 512) * 512);
+  p.sort_tile = N <= kFewTiles * 1024 ? 1024 : (int)(N > 256 * (int64_t)kSortTile ? kSortTile : cdiv(N, 256 * 512) * 512);
   p.sort_tiles = (int)cdiv(N, p.sort_tile);
   const int groups = BT / p.lpr;
   int64_t span = N / ((int64_t)groups * 1024) / 8 * 8;
@@ -646,20 +692,18 @@ static Plan plan_of(const EgnnEmbedDims* d) {
   return p;
 }
 
-template <typename T, typename P, typename I>
+template <typename T, typename P, typename I, bool TAIL, bool PAST>
 static int launch_bwd(BwdArgs a, const Plan& p, void* ws, hipStream_t st) {
   constexpr int VEC = Vec<T>::N;
-  const bool tail = a.C % VEC;
   const size_t carry = (size_t)BT * 2 * VEC * 4;
   a.lpr = p.lpr; a.pieces = p.pieces;
   if (p.local) {
     a.chunk = p.chunk; a.chunks = p.chunks; a.range = p.range;
     a.part = p.chunks > 1 ? (float*)ws : nullptr;
     const size_t cnt = (size_t)NW * p.range * 4;
-    const size_t lds = ((size_t)p.chunk + ((p.range + 4) & ~3)) * 4 + (cnt > carry ? cnt : carry);
+    const size_t lds = ((size_t)p.chunk + ((p.range + 4) & ~3)) * 4 + (cnt > carry ? cnt : carry) + (size_t)p.chunk * 2;
     const dim3 grid((uint32_t)(p.chunks * (int64_t)p.ranges), (uint32_t)p.tiles);
-    if (tail) local_kernel<T, P, I, true><<<grid, BT, lds, st>>>(a);
-    else local_kernel<T, P, I, false><<<grid, BT, lds, st>>>(a);
+    local_kernel<T, P, I, TAIL, PAST><<<grid, BT, lds, st>>>(a);
     if (p.chunks > 1) {
       const int64_t M = a.V * a.C, pad = a.padding * a.C;
       reduce_kernel<P><<<(uint32_t)cdiv(M, 64), 1024, 0, st>>>(a.part, p.chunks, M, a.padding < 0 ? 0 : pad,
@@ -678,25 +722,28 @@ static int launch_bwd(BwdArgs a, const Plan& p, void* ws, hipStream_t st) {
     s.shift = k * p.bits;
     s.from = k & 1 ? one : two;
     s.to = k & 1 ? two : one;
+    const size_t lds = ((size_t)(2 + NW) * s.digits + 4) * 4 + (size_t)s.tile * 2;
+    const bool few = s.tiles <= kFewTiles;
     if (!k) hist_kernel<I, true><<<(uint32_t)s.tiles, BT, 0, st>>>(s);
     else hist_kernel<I, false><<<(uint32_t)s.tiles, BT, 0, st>>>(s);
-    scan_kernel<<<(uint32_t)cdiv(s.digits, 16), 1024, 0, st>>>(s);
-    if (!k) scatter_kernel<I, true><<<(uint32_t)s.tiles, BT, 0, st>>>(s);
-    else scatter_kernel<I, false><<<(uint32_t)s.tiles, BT, 0, st>>>(s);
+    if (!few) scan_kernel<<<(uint32_t)cdiv(s.digits, 16), 1024, 0, st>>>(s);
+    if (!k && few) scatter_kernel<I, true, true><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
+    else if (!k) scatter_kernel<I, true, false><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
+    else if (few) scatter_kernel<I, false, true><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
+    else scatter_kernel<I, false, false><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
   }
   a.sorted = s.to;
   a.span = p.span; a.tile = p.tile;
   const size_t lds = ((size_t)((p.tile + 5) & ~3) + ((p.tile + 3) & ~3)) * 4 + carry;
   const dim3 grid((uint32_t)p.blocks, (uint32_t)p.tiles);
-  const int64_t fix = cdiv(a.V, kFixRows);
-  const dim3 fgrid((uint32_t)(fix < kMaxGrid / p.tiles ? fix : kMaxGrid / p.tiles), (uint32_t)p.tiles);
-  if (tail) {
-    sorted_kernel<T, P, true><<<grid, BT, lds, st>>>(a);
-    fix_kernel<T, P, true><<<fgrid, FT, 0, st>>>(a);
-  } else {
-    sorted_kernel<T, P, false><<<grid, BT, lds, st>>>(a);
-    fix_kernel<T, P, false><<<fgrid, FT, 0, st>>>(a);
-  }
+  sorted_kernel<T, P, TAIL, PAST><<<grid, BT, lds, st>>>(a);
+  int rows = kFixRows;                       // (a power of two: divides 2^shift; fewer where the table is short)
+  while (rows > 1 && (rows > 1 << s.shift && s.shift || cdiv(a.V, rows) < 512)) rows /= 2;
+  const int64_t fix = cdiv(a.V, rows);
+  const int tiles = (int)cdiv(p.pieces, FT);   // wider column tiles than those of the sums: every one looks for the rows again
+  a.lpr = (int)cdiv(p.pieces, tiles);
+  const dim3 fgrid((uint32_t)(fix < kMaxGrid / tiles ? fix : kMaxGrid / tiles), (uint32_t)tiles);
+  fix_kernel<T, P, TAIL><<<fgrid, FT, 0, st>>>(a, s.total, s.shift, rows);
   return hipGetLastError() == hipSuccess ? EGNN_OK : EGNN_ERR_HIP;
 }
 
@@ -719,7 +766,11 @@ template <typename T, typename P, typename I> struct Fwd {
   }
 };
 template <typename T, typename P, typename I> struct Bwd {
-  static int go(const BwdArgs& a, const Plan* p, void* ws, hipStream_t st) { return launch_bwd<T, P, I>(a, *p, ws, st); }
+  static int go(const BwdArgs& a, const Plan* p, void* ws, hipStream_t st) {
+    if (a.N * a.C * (int64_t)sizeof(T) >= kPastLoad)
+      return a.C % Vec<T>::N ? launch_bwd<T, P, I, true, true>(a, *p, ws, st) : launch_bwd<T, P, I, false, true>(a, *p, ws, st);
+    return a.C % Vec<T>::N ? launch_bwd<T, P, I, true, false>(a, *p, ws, st) : launch_bwd<T, P, I, false, false>(a, *p, ws, st);
+  }
 };
 
 }  // namespace embed

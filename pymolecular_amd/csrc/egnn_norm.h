@@ -138,11 +138,8 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
   }
 }
 
-// PAST: 1: the result is stored past the cache, 2: the operands are read past it too.  By the size of one tensor (the
-// cache holds 256 MB): from 64 MB on storing past it is the faster (60,000 x 512 fp32, 123 MB: 71 -> 58 us; 40,961 x 259,
-// 42 MB: 32.0 -> 33.3), from 256 MB on reading too (2,000,000 x 128 bf16: 347 -> 325 us; the 123 MB: 58 -> 67).
-constexpr int64_t kPastStore = int64_t(64) << 20, kPastLoad = int64_t(256) << 20;
-
+// PAST: 1: the result is stored past the cache, 2: the operands are read past it too (egnn_rows.h).  60,000 x 512 fp32, 123 MB:
+// 71, 58 and 67 us at 0, 1 and 2; 40,961 x 259, 42 MB: 32.0 and 33.3 at 0 and 1; 2,000,000 x 128 bf16: 347 and 325 at 1 and 2.
 template <typename T, int LPR, int VPL, int PAST, bool TAIL, bool DROP>
 __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
   typedef Vec<T, TAIL> V;

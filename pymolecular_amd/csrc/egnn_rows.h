@@ -5,6 +5,11 @@
 
 namespace egnn {
 
+// From which size of one tensor on it is written, and read, past the cache (which holds 256 MB) where the next kernel reads it,
+// or this one reads it once.  The norm's backward and the table rows were measured on both sides, see there.
+constexpr int64_t kPastStore = int64_t(64) << 20, kPastLoad = int64_t(256) << 20;
+
+
 // A piece: 16 bytes of values from column f on.  Rows need no alignment but their values': the type says so, and the
 // compiler still makes one 16-byte access of it.  The last piece of a row that is not a multiple of them wide ends with the
 // row and overlaps the one before: its first `skip` columns enter no sum and are stored twice, with the same bits (value by
