@@ -362,7 +362,6 @@ __global__ __launch_bounds__(1024) void reduce_kernel(const float* part, int chu
 
 // ---- backward: the whole order sorted -------------------------------------------------------
 constexpr int kSortTile = 4096;              // values of a workgroup in a pass at most
-constexpr int kFewTiles = 64;                // up to so many a workgroup adds up their counts by itself
 
 // A value is token << 32 | row; tokens outside the table get V and come last.
 struct SortArgs {
@@ -412,8 +411,7 @@ __global__ __launch_bounds__(1024) void scan_kernel(SortArgs a) {
   }
   if (k == 63) a.total[d] = at;
 }
-// FEW: no scan_kernel ran; the workgroup adds up the tiles' counts by itself (and the first one leaves the totals)
-template <typename I, bool FIRST, bool FEW>
+template <typename I, bool FIRST>
 __global__ __launch_bounds__(BT) void scatter_kernel(SortArgs a) {
   extern __shared__ __align__(16) uint32_t lds[];
   __shared__ uint32_t sums[NW];
@@ -421,24 +419,9 @@ __global__ __launch_bounds__(BT) void scatter_kernel(SortArgs a) {
   uint16_t* memo = (uint16_t*)(cnt + NW * a.digits);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   // where a digit's values of this tile begin: all values of smaller digits, then those of the tiles before
-  if (FEW) {
-    for (int d = threadIdx.x; d < a.digits; d += BT) {
-      uint32_t all = 0, mine = 0;
-#pragma unroll 16
-      for (int b = 0; b < a.tiles; ++b) {
-        const uint32_t x = a.hist[(int64_t)b * a.digits + d];
-        all += x;
-        mine += b < (int)blockIdx.x ? x : 0;
-      }
-      base[d] = mine;
-      cnt[d] = all;
-      if (!blockIdx.x) a.total[d] = all;
-    }
-    __syncthreads();
-  }
   const int own = (a.digits + BT - 1) / BT, own0 = own * threadIdx.x, own1 = min(a.digits, own0 + own);   // a thread's digits
   uint32_t s = 0;
-  for (int d = own0; d < own1; ++d) s += FEW ? cnt[d] : a.total[d];
+  for (int d = own0; d < own1; ++d) s += a.total[d];
   uint32_t inc = s;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -450,8 +433,8 @@ __global__ __launch_bounds__(BT) void scatter_kernel(SortArgs a) {
   uint32_t at = inc - s;
   for (int k = 0; k < w; ++k) at += sums[k];
   for (int d = own0; d < own1; ++d) {
-    base[d] = at + (FEW ? base[d] : a.hist[(int64_t)blockIdx.x * a.digits + d]);
-    at += FEW ? cnt[d] : a.total[d];
+    base[d] = at + a.hist[(int64_t)blockIdx.x * a.digits + d];
+    at += a.total[d];
   }
   __syncthreads();
   const int64_t n0 = (int64_t)blockIdx.x * a.tile;
@@ -676,7 +659,7 @@ static Plan plan_of(const EgnnEmbedDims* d) {
   while (V >> width) ++width;
   p.passes = (int)cdiv(width, 11);
   p.bits = (int)cdiv(width, p.passes);
-  p.sort_tile = N <= kFewTiles * 1024 ? 1024 : (int)(N > 256 * (int64_t)kSortTile ? kSortTile : cdiv(N, 256 * 512) * 512);
+  p.sort_tile = (int)(N > 256 * (int64_t)kSortTile ? kSortTile : cdiv(N, 256 * 512) * 512);
   p.sort_tiles = (int)cdiv(N, p.sort_tile);
   const int groups = BT / p.lpr;
   int64_t span = N / ((int64_t)groups * 1024) / 8 * 8;
@@ -723,25 +706,25 @@ static int launch_bwd(BwdArgs a, const Plan& p, void* ws, hipStream_t st) {
     s.from = k & 1 ? one : two;
     s.to = k & 1 ? two : one;
     const size_t lds = ((size_t)(2 + NW) * s.digits + 4) * 4 + (size_t)s.tile * 2;
-    const bool few = s.tiles <= kFewTiles;
     if (!k) hist_kernel<I, true><<<(uint32_t)s.tiles, BT, 0, st>>>(s);
     else hist_kernel<I, false><<<(uint32_t)s.tiles, BT, 0, st>>>(s);
-    if (!few) scan_kernel<<<(uint32_t)cdiv(s.digits, 16), 1024, 0, st>>>(s);
-    if (!k && few) scatter_kernel<I, true, true><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
-    else if (!k) scatter_kernel<I, true, false><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
-    else if (few) scatter_kernel<I, false, true><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
-    else scatter_kernel<I, false, false><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
+    scan_kernel<<<(uint32_t)cdiv(s.digits, 16), 1024, 0, st>>>(s);
+    if (!k) scatter_kernel<I, true><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
+    else scatter_kernel<I, false><<<(uint32_t)s.tiles, BT, lds, st>>>(s);
   }
   a.sorted = s.to;
   a.span = p.span; a.tile = p.tile;
   const size_t lds = ((size_t)((p.tile + 5) & ~3) + ((p.tile + 3) & ~3)) * 4 + carry;
   const dim3 grid((uint32_t)p.blocks, (uint32_t)p.tiles);
   sorted_kernel<T, P, TAIL, PAST><<<grid, BT, lds, st>>>(a);
-  int rows = kFixRows;                       // (a power of two: divides 2^shift; fewer where the table is short)
-  while (rows > 1 && (rows > 1 << s.shift && s.shift || cdiv(a.V, rows) < 512)) rows /= 2;
-  const int64_t fix = cdiv(a.V, rows);
   const int tiles = (int)cdiv(p.pieces, FT);   // wider column tiles than those of the sums: every one looks for the rows again
   a.lpr = (int)cdiv(p.pieces, tiles);
+  // about four rows a group of lanes (40,961 x 259 fp32 over 50,021 rows, three groups: 66, 59, 56 and 61 us at 64, 32, 16 and 8
+  // rows; 1,000,000 x 32 over 131,072, 32 groups: 112, 112, 119 and 132), fewer where the table is short; a power of two
+  int rows = 8;
+  while (rows < kFixRows && rows < 4 * (FT / a.lpr)) rows *= 2;
+  while (rows > 1 && ((s.shift && rows > 1 << s.shift) || cdiv(a.V, rows) < 512)) rows /= 2;
+  const int64_t fix = cdiv(a.V, rows);
   const dim3 fgrid((uint32_t)(fix < kMaxGrid / tiles ? fix : kMaxGrid / tiles), (uint32_t)tiles);
   fix_kernel<T, P, TAIL><<<fgrid, FT, 0, st>>>(a, s.total, s.shift, rows);
   return hipGetLastError() == hipSuccess ? EGNN_OK : EGNN_ERR_HIP;
