@@ -4,12 +4,12 @@
 // are on their way while the bits are made.
 #include "egnn_internal.h"
 #include "egnn_random.h"
+#include "egnn_rows.h"
 
 namespace egnn {
 namespace dropout {
 
 constexpr int NT = 256;
-constexpr int U = 4;                         // groups of eight columns a thread
 
 struct Args {
   const void *x, *r;
@@ -23,20 +23,23 @@ struct Args {
 template <typename T> struct Group {
   typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
   typedef T vals __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ vals load(const T* p, int n) {
+  template <bool PAST> static __device__ __forceinline__ vals load(const T* p, int n) {
     vals v;
-    if (n >= 8) v = *reinterpret_cast<const type*>(p);
-    else
+    if (n >= 8) {
+      if constexpr (PAST) v = __builtin_nontemporal_load(reinterpret_cast<const type*>(p));
+      else v = *reinterpret_cast<const type*>(p);
+    } else
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.f;
     return v;
   }
-  static __device__ __forceinline__ void store(T* p, int n, const float* v) {
+  template <bool PAST> static __device__ __forceinline__ void store(T* p, int n, const float* v) {
     if (n >= 8) {
       type t;
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(v[i]);
-      *reinterpret_cast<type*>(p) = t;
+      if constexpr (PAST) __builtin_nontemporal_store(t, reinterpret_cast<type*>(p));
+      else *reinterpret_cast<type*>(p) = t;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -45,7 +48,8 @@ template <typename T> struct Group {
   }
 };
 
-template <typename T, bool RES>
+// U: groups of eight columns a thread; PAST: 1: the result is stored past the cache, 2: the operands are read past it too
+template <typename T, bool RES, int U, int PAST>
 __global__ __launch_bounds__(NT) void drop_kernel(Args a) {
   typedef Group<T> V;
   const Mask m = mask_of(a.d);
@@ -61,8 +65,8 @@ __global__ __launch_bounds__(NT) void drop_kernel(Args a) {
     g[u] = (int)(l - k * a.GT) + blockIdx.y * a.GT;
     in[u] = (int)k < a.R && n[u] < a.N && g[u] < a.G;
     if (in[u]) {
-      x[u] = V::load((const T*)a.x + n[u] * a.ldx + 8 * g[u], a.C - 8 * g[u]);
-      if (RES) r[u] = V::load((const T*)a.r + n[u] * a.ldr + 8 * g[u], a.C - 8 * g[u]);
+      x[u] = V::template load<PAST == 2>((const T*)a.x + n[u] * a.ldx + 8 * g[u], a.C - 8 * g[u]);
+      if (RES) r[u] = V::template load<PAST == 2>((const T*)a.r + n[u] * a.ldr + 8 * g[u], a.C - 8 * g[u]);
     }
   }
 #pragma unroll
@@ -76,15 +80,18 @@ __global__ __launch_bounds__(NT) void drop_kernel(Args a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += to_f32((T)r[u][i]);
     }
-    V::store((T*)a.y + n[u] * a.C + 8 * g[u], a.C - 8 * g[u], v);
+    V::template store<(PAST > 0)>((T*)a.y + n[u] * a.C + 8 * g[u], a.C - 8 * g[u], v);
   }
 }
 
+// Up to so many groups a thread takes one: more workgroups come before more loads in flight (2,432 x 128 fp32: 3.5 us, and 4.1
+// with four; 32,768 x 128 bf16: 4.2 and 5.1; at 1,048,576 groups the same)
+constexpr int64_t kFewGroups = 1024 * 1024;
 // A launch may have fewer than 2^32 threads: at most this many blocks at a time
 constexpr int64_t kMaxGrid = int64_t(1) << 20;
 
-template <typename T>
-static void launch(Args a, hipStream_t st) {
+template <typename T, int U, int PAST>
+static void launch_parts(Args a, hipStream_t st) {
   a.G = (int32_t)cdiv(a.C, 8);
   const int tiles = (int)cdiv(a.G, NT * U);
   a.GT = (int32_t)cdiv(a.G, tiles);
@@ -99,9 +106,20 @@ static void launch(Args a, hipStream_t st) {
     a.row0 = n;
     a.N = N - n < most ? N - n : most;
     const dim3 grid((uint32_t)cdiv(a.N, a.R), (uint32_t)tiles);
-    if (a.r) drop_kernel<T, true><<<grid, NT, 0, st>>>(a);
-    else drop_kernel<T, false><<<grid, NT, 0, st>>>(a);
+    if (a.r) drop_kernel<T, true, U, PAST><<<grid, NT, 0, st>>>(a);
+    else drop_kernel<T, false, U, PAST><<<grid, NT, 0, st>>>(a);
   }
+}
+// Past the cache: 600,000 x 128 bf16, with a residual, 84.4 us at 0 and 70.7 at 1; 2,000,000 x 128 271 at 0, 249 at 2.  A
+// group of fp32 is two loads of half a line each, which are slower past the cache where it holds nothing anyway: 1,000,000 x
+// 128, 271, 277 and 288 at 0, 1 and 2; 150,000 x 259, 96 and 89 at 0 and 1.
+template <typename T>
+static void launch(const Args& a, hipStream_t st) {
+  const int64_t bytes = a.N * a.C * (int64_t)sizeof(T);
+  if (a.N * cdiv(a.C, 8) < kFewGroups) launch_parts<T, 1, 0>(a, st);
+  else if (bytes < kPastStore) launch_parts<T, 4, 0>(a, st);
+  else if (bytes < kPastLoad) launch_parts<T, 4, 1>(a, st);
+  else launch_parts<T, 4, sizeof(T) == 2 ? 2 : 0>(a, st);
 }
 
 }  // namespace dropout
