@@ -331,33 +331,36 @@ template <typename P>
 __global__ __launch_bounds__(1024) void reduce_kernel(const float* part, int chunks, int64_t M, int64_t pad0, int64_t pad1,
                                                       float scale, P* gw) {
   __shared__ float red[64][16][5];
+  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
   const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
-  const int64_t f = ((int64_t)blockIdx.x * 16 + c) * 4;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  const int m = f + 4 <= M ? 4 : f < M ? (int)(M - f) : 0;
+  for (int64_t f0 = (int64_t)blockIdx.x * 64; f0 < M; f0 += (int64_t)gridDim.x * 64) {
+    const int64_t f = f0 + 4 * c;
+    const int m = f + 4 <= M ? 4 : f < M ? (int)(M - f) : 0;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int b = k; b < chunks; b += 64) {
-    const float* p = part + b * M + f;
-    if (m == 4) {
-      typedef float type __attribute__((ext_vector_type(4), aligned(4)));
-      const type t = *(const type*)p;
+    for (int b = k; b < chunks; b += 64) {
+      const float* p = part + b * M + f;
+      if (m == 4) {
+        const type t = *(const type*)p;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] += t[i];
-    } else {
-      for (int i = 0; i < m; ++i) s[i] += p[i];
+        for (int i = 0; i < 4; ++i) s[i] += t[i];
+      } else {
+        for (int i = 0; i < m; ++i) s[i] += p[i];
+      }
     }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) red[k][c][i] = s[i];
-  __syncthreads();
-  for (int h = 32; h; h >>= 1) {
-    if (k < h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) red[k][c][i] += red[k + h][c][i];
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[k][c][i] = s[i];
+    __syncthreads();
+    for (int h = 32; h; h >>= 1) {
+      if (k < h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[k][c][i] += red[k + h][c][i];
+      __syncthreads();
+    }
+    if (k == 0)
+      for (int i = 0; i < m; ++i) gw[f + i] = from_f32<P>(f + i >= pad0 && f + i < pad1 ? 0.f : red[0][c][i] * scale);
   }
-  if (k) return;
-  for (int i = 0; i < m; ++i) gw[f + i] = from_f32<P>(f + i >= pad0 && f + i < pad1 ? 0.f : red[0][c][i] * scale);
 }
 
 // ---- backward: the whole order sorted -------------------------------------------------------
@@ -665,6 +668,7 @@ static Plan plan_of(const EgnnEmbedDims* d) {
   int64_t span = N / ((int64_t)groups * 1024) / 8 * 8;
   span = span < 8 ? 8 : span > 32 ? 32 : span;
   while (span > 4 && span * groups > 2048) span /= 2;
+  while (cdiv(N, span * groups) > kMaxGrid && span * groups <= 1024) span *= 2;
   p.span = (int)span;
   p.tile = (int)span * groups;
   p.blocks = (int)cdiv(N, p.tile);
@@ -689,7 +693,7 @@ static int launch_bwd(BwdArgs a, const Plan& p, void* ws, hipStream_t st) {
     local_kernel<T, P, I, TAIL, PAST><<<grid, BT, lds, st>>>(a);
     if (p.chunks > 1) {
       const int64_t M = a.V * a.C, pad = a.padding * a.C;
-      reduce_kernel<P><<<(uint32_t)cdiv(M, 64), 1024, 0, st>>>(a.part, p.chunks, M, a.padding < 0 ? 0 : pad,
+      reduce_kernel<P><<<(uint32_t)(cdiv(M, 64) < kMaxGrid ? cdiv(M, 64) : kMaxGrid), 1024, 0, st>>>(a.part, p.chunks, M, a.padding < 0 ? 0 : pad,
                                                                 a.padding < 0 ? 0 : pad + a.C, a.scale, (P*)a.gw);
     }
     return hipGetLastError() == hipSuccess ? EGNN_OK : EGNN_ERR_HIP;

@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/core/DeviceGuard.h>
 #include <cmath>
 #include "../../include/egnn.h"
 
@@ -342,6 +343,7 @@ bool drop_ok(const Tensor& x, double p, const Tensor& rng) { return p >= 0.0 && 
 
 pybind11::object dropout(const Tensor& x, double p, const Tensor& rng, int64_t site, const Opt& res) {
   if (!norm_ok(x, Opt(), Opt(), 0.0, false) || !drop_ok(x, p, rng) || (res && !same_rows(*res, x))) return pybind11::none();
+  const c10::DeviceGuard device(x.device());
   const Tensor y = at::empty(x.sizes(), x.options());
   const int64_t C = x.size(-1);
   const EgnnDropout d{ptr<const int64_t>(rng), site, p};
@@ -357,6 +359,7 @@ pybind11::object norm_drop_forward(const Tensor& x, const Opt& res, double p, co
   const EgnnNormDims d = norm_dims(x, eps, f32);
   const EgnnDropout dr{ptr<const int64_t>(rng), site, p};
   const auto stat = x.options().dtype(at::kFloat);
+  const c10::DeviceGuard device(x.device());
   const Tensor y = at::empty(x.sizes(), x.options()), s = at::empty(x.sizes(), x.options());
   const Tensor mean = need_stats ? at::empty({d.N}, stat) : Tensor(), rstd = need_stats ? at::empty({d.N}, stat) : Tensor();
   check("egnn_norm_drop_fwd", egnn_norm_drop_fwd(&d, &dr, ptr(x), d.C, ptr(*res), d.C, ptr(get(w)), ptr(get(b)), ptr(y), ptr(s),
@@ -372,6 +375,7 @@ pybind11::object norm_drop_backward(const Tensor& gy, const Tensor& s, double p,
   const EgnnNormDims d = norm_dims(s, 0.0, f32);
   if (!fits(mean, s, at::kFloat, {d.N}) || !fits(rstd, s, at::kFloat, {d.N})) return pybind11::none();
   const EgnnDropout dr{ptr<const int64_t>(rng), site, p};
+  const c10::DeviceGuard device(s.device());
   const Tensor gx = at::empty(s.sizes(), s.options()), gr = at::empty(s.sizes(), s.options());
   const auto param = s.options().dtype(f32 ? at::kFloat : s.scalar_type());
   const Tensor gw = need_w ? at::empty({d.C}, param) : Tensor(), gb = need_b ? at::empty({d.C}, param) : Tensor();
@@ -408,6 +412,7 @@ pybind11::object embed_forward(const Tensor& tokens, const Tensor& w, double sca
   const EgnnEmbedDims d = embed_dims(tokens, w.size(0), w.size(1), scale, dt, w.scalar_type());
   auto shape = tokens.sizes().vec();
   shape.push_back(d.C);
+  const c10::DeviceGuard device(w.device());
   const Tensor out = at::empty(shape, w.options().dtype(dt));
   check("egnn_embed_fwd", egnn_embed_fwd(&d, ptr(tokens), ptr(w), w.stride(0), ptr(out), stream_of(w)));
   return pybind11::cast(out);
@@ -419,6 +424,7 @@ pybind11::object embed_backward(const Tensor& go, const Tensor& tokens, int64_t 
       !embed_ok(tokens, V, go.size(-1), dt, table) || go.sizes().slice(0, tokens.dim()) != tokens.sizes() || padding < -1 || padding >= V)
     return pybind11::none();
   const EgnnEmbedDims d = embed_dims(tokens, V, go.size(-1), scale, dt, table);
+  const c10::DeviceGuard device(go.device());
   const Tensor gw = at::empty({V, d.C}, go.options().dtype(table));
   const size_t nb = egnn_embed_bwd_workspace_bytes(&d);
   const Tensor ws = workspace(nb, go);
@@ -467,6 +473,7 @@ pybind11::object qk_forward(const Tensor& q, const Tensor& k, const Opt& qw, con
                             bool il, double eps) {
   const Qk r = qk_of(q, k, qw, kw, pos, base, rotary, il, eps);
   if (!r.ok) return pybind11::none();
+  const c10::DeviceGuard device(q.device());
   const Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), q.options());
   EgnnQkStrides s{};
   s.q_row = q.stride(0); s.q_head = q.stride(1); s.k_row = k.stride(0); s.k_head = k.stride(1);
@@ -483,6 +490,7 @@ pybind11::object qk_backward(const Tensor& gqo, const Tensor& gko, const Tensor&
   if (!r.ok || !heads_of(gqo, q, d.N, d.Hq, d.D) || !heads_of(gko, q, d.N, d.Hk, d.D)) return pybind11::none();
   if (into && (into->size() != 2 || !room_of((*into)[0], q, d.N, d.Hq, d.D) || !room_of((*into)[1], q, d.N, d.Hk, d.D)))
     return pybind11::none();
+  const c10::DeviceGuard device(q.device());
   const Tensor gq = into ? (*into)[0] : at::empty(q.sizes(), q.options()), gk = into ? (*into)[1] : at::empty(k.sizes(), q.options());
   const auto param = q.options().dtype(d.f32_params ? at::kFloat : q.scalar_type());
   const Tensor gqw = qw ? at::empty({d.D}, param) : Tensor(), gkw = kw ? at::empty({d.D}, param) : Tensor();

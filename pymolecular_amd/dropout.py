@@ -65,9 +65,10 @@ def dropout_forward(x, p, rng, residual=None, site=0):
         x, residual = x.to(dt), residual.to(dt)
     x2, r2 = _rows(x), None if residual is None else _rows(residual)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    check("egnn_dropout",
-          _capi.lib().egnn_dropout(drop, _dtype_code(x.dtype), x2.shape[0], x2.shape[1], x2.data_ptr(), x2.stride(0),
-                                   _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), _stream(x.device)))
+    with torch.cuda.device(x.device):   # (its stream may not be of the current one)
+        check("egnn_dropout",
+              _capi.lib().egnn_dropout(drop, _dtype_code(x.dtype), x2.shape[0], x2.shape[1], x2.data_ptr(), x2.stride(0),
+                                       _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), _stream(x.device)))
     return y
 
 

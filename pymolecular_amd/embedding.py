@@ -62,9 +62,10 @@ def embedding_forward(tokens, weight, scale=1.0, dtype=None):
     w = _rows(w)
     t = tokens.contiguous()
     out = torch.empty((*tokens.shape, weight.shape[1]), dtype=dtype, device=tokens.device)
-    check("egnn_embed_fwd",
-          _capi.lib().egnn_embed_fwd(_dims(t, *weight.shape, dtype, w.dtype, scale), t.data_ptr(), w.data_ptr(), w.stride(0),
-                                     out.data_ptr(), _stream(t.device)))
+    with torch.cuda.device(t.device):   # (its stream may not be of the current one)
+        check("egnn_embed_fwd",
+              _capi.lib().egnn_embed_fwd(_dims(t, *weight.shape, dtype, w.dtype, scale), t.data_ptr(), w.data_ptr(), w.stride(0),
+                                         out.data_ptr(), _stream(t.device)))
     return out
 
 
@@ -87,9 +88,10 @@ def embedding_backward(grad_out, tokens, vocab, scale=1.0, padding=None, dtype=N
     L = _capi.lib()
     nbytes = L.egnn_embed_bwd_workspace_bytes(d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
-    check("egnn_embed_bwd",
-          L.egnn_embed_bwd(d, -1 if padding is None else padding, g.data_ptr(), g.stride(0), t.data_ptr(), gw.data_ptr(),
-                           _ptr(ws), nbytes, _stream(t.device)))
+    with torch.cuda.device(t.device):   # (its stream may not be of the current one)
+        check("egnn_embed_bwd",
+              L.egnn_embed_bwd(d, -1 if padding is None else padding, g.data_ptr(), g.stride(0), t.data_ptr(), gw.data_ptr(),
+                               _ptr(ws), nbytes, _stream(t.device)))
     return gw if gw.dtype == dtype else gw.to(dtype)
 
 

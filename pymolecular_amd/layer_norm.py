@@ -184,11 +184,13 @@ def layer_norm_dropout_forward(x, residual, drop, weight=None, bias=None, eps=1e
     w, b = _as(weight, pdt), _as(bias, pdt)
     n, c = x2.shape
     y, s = (torch.empty(shape, dtype=dt, device=dev) for _ in range(2))
-    mean, rstd = torch.empty((2, n), dtype=torch.float32, device=dev) if need_stats else (None, None)
-    check("egnn_norm_drop_fwd",
-          _capi.lib().egnn_norm_drop_fwd(EgnnNormDims(n, c, _dtype_code(dt), eps, pdt != dt), d, x2.data_ptr(), x2.stride(0),
-                                         r2.data_ptr(), r2.stride(0), _ptr(w), _ptr(b), y.data_ptr(), s.data_ptr(),
-                                         _ptr(mean), _ptr(rstd), _stream(dev)))
+    stats = torch.empty((2, n), dtype=torch.float32, device=dev) if need_stats else None
+    mean, rstd = (stats[0], stats[1]) if need_stats else (None, None)
+    with torch.cuda.device(dev):
+        check("egnn_norm_drop_fwd",
+              _capi.lib().egnn_norm_drop_fwd(EgnnNormDims(n, c, _dtype_code(dt), eps, pdt != dt), d, x2.data_ptr(), x2.stride(0),
+                                             r2.data_ptr(), r2.stride(0), _ptr(w), _ptr(b), y.data_ptr(), s.data_ptr(),
+                                             _ptr(mean), _ptr(rstd), _stream(dev)))
     return y, s, mean, rstd
 
 
@@ -222,10 +224,11 @@ def layer_norm_dropout_backward(gy, s, drop, weight, mean, rstd, gsum=None, need
     L = _capi.lib()
     nbytes = L.egnn_norm_bwd_workspace_bytes(nd) if need_weight or need_bias else 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    check("egnn_norm_drop_bwd",
-          L.egnn_norm_drop_bwd(nd, d, g2.data_ptr(), g2.stride(0), s2.data_ptr(), s2.stride(0), _ptr(w), mean.data_ptr(),
-                               rstd.data_ptr(), _ptr(e2), 0 if e2 is None else e2.stride(0), gx.data_ptr(), gr.data_ptr(),
-                               _ptr(gw), _ptr(gb), _ptr(ws), nbytes, _stream(dev)))
+    with torch.cuda.device(dev):
+        check("egnn_norm_drop_bwd",
+              L.egnn_norm_drop_bwd(nd, d, g2.data_ptr(), g2.stride(0), s2.data_ptr(), s2.stride(0), _ptr(w), mean.data_ptr(),
+                                   rstd.data_ptr(), _ptr(e2), 0 if e2 is None else e2.stride(0), gx.data_ptr(), gr.data_ptr(),
+                                   _ptr(gw), _ptr(gb), _ptr(ws), nbytes, _stream(dev)))
     return gx, gr, _as(gw, wdt), _as(gb, bdt)
 
 

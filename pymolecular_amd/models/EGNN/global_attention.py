@@ -104,8 +104,9 @@ class EGNNGlobal(nn.Module):
     the dtype of their vectors (None: the parameters').  ``qk_norm``, ``rotary_base``: see :class:`GlobalAttention`;
     ``forward`` takes ``positions`` then.  ``dropout``: the probability, in training, with which a value of the embedding
     and of each update is dropped in front of its residual sum.  Its masks come from the buffer ``dropout_state`` (seed and
-    offset), whose offset each such pass advances on the device, so a captured pass draws anew on every replay; replicas of
-    a network want a seed each (:meth:`seed_dropout`)."""
+    offset), whose offset each such pass advances on the device, so a captured pass draws anew on every replay.  Replicas of
+    a network want a seed each (:meth:`seed_dropout`; and no broadcast of buffers), and a pass that is made again for its
+    backward has to start from the same state."""
 
     def __init__(self, in_node_nf, hidden_nf, out_nf, in_edge_nf=0, device='cpu', act_fn=nn.SiLU(), n_layers=4, heads=4,
                  kv_heads=None, eps=1e-5, n_types=None, node_dtype=None, qk_norm=False, rotary_base=10000.0, dropout=0.0):

@@ -87,8 +87,9 @@ def qk_norm_rotary_forward(q, k, q_weight=None, k_weight=None, positions=None, b
     q, k, qw, kw, pos, d = _call(q, k, q_weight, k_weight, positions, base, rotary_dim, interleaved, eps)
     out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
     s = EgnnQkStrides(*(x for t in (q, k, *out) for x in t.stride()[:2]))
-    check("egnn_qk_fwd", _capi.lib().egnn_qk_fwd(d, s, q.data_ptr(), k.data_ptr(), _ptr(qw), _ptr(kw), _ptr(pos),
-                                                 out[0].data_ptr(), out[1].data_ptr(), _stream(q.device)))
+    with torch.cuda.device(q.device):   # (its stream may not be of the current one)
+        check("egnn_qk_fwd", _capi.lib().egnn_qk_fwd(d, s, q.data_ptr(), k.data_ptr(), _ptr(qw), _ptr(kw), _ptr(pos),
+                                                     out[0].data_ptr(), out[1].data_ptr(), _stream(q.device)))
     return tuple(out)
 
 
@@ -123,10 +124,11 @@ def qk_norm_rotary_backward(gq_out, gk_out, q, k, q_weight=None, k_weight=None, 
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     out = [g.stride()[:2] for g in (gq_out, gk_out, *grads)]
     s = EgnnQkStrides(*q.stride()[:2], *k.stride()[:2], 0, 0, 0, 0, *(x for t in out for x in t))
-    check("egnn_qk_bwd",
-          L.egnn_qk_bwd(d, s, gq_out.data_ptr(), gk_out.data_ptr(), q.data_ptr(), k.data_ptr(), _ptr(qw), _ptr(kw),
-                        _ptr(pos), grads[0].data_ptr(), grads[1].data_ptr(), _ptr(gw[0]), _ptr(gw[1]), _ptr(ws), nbytes,
-                        _stream(q.device)))
+    with torch.cuda.device(q.device):   # (its stream may not be of the current one)
+        check("egnn_qk_bwd",
+              L.egnn_qk_bwd(d, s, gq_out.data_ptr(), gk_out.data_ptr(), q.data_ptr(), k.data_ptr(), _ptr(qw), _ptr(kw),
+                            _ptr(pos), grads[0].data_ptr(), grads[1].data_ptr(), _ptr(gw[0]), _ptr(gw[1]), _ptr(ws), nbytes,
+                            _stream(q.device)))
     return (*grads, *(_as(g, t) for g, t in zip(gw, wdt)))
 
 
