@@ -211,9 +211,9 @@ def lib() -> ctypes.CDLL:
     L.egnn_dropout.restype = c_int32
     L.egnn_dropout.argtypes = [DR, c_int32, c_int64, c_int32, P, c_int64, P, c_int64, P, P]
     L.egnn_norm_drop_fwd.restype = c_int32
-    L.egnn_norm_drop_fwd.argtypes = [MD, DR, P, c_int64, P, c_int64] + [P] * 7
+    L.egnn_norm_drop_fwd.argtypes = [MD, DR, P, c_int64, P, c_int64] + [P] * 8
     L.egnn_norm_drop_bwd.restype = c_int32
-    L.egnn_norm_drop_bwd.argtypes = [MD, DR, P, c_int64, P, c_int64, P, P, P, P, c_int64] + [P] * 5 + [c_size_t, P]
+    L.egnn_norm_drop_bwd.argtypes = [MD, DR, P, c_int64, P, c_int64, P, P, P, P, P, c_int64] + [P] * 5 + [c_size_t, P]
     ED = ctypes.POINTER(EgnnEmbedDims)
     L.egnn_embed_fwd.restype = c_int32
     L.egnn_embed_fwd.argtypes = [ED, P, P, c_int64, P, P]

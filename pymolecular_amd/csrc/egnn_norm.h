@@ -32,15 +32,55 @@ struct Args {
   float eps;
   bool f32_params;                           // w, b, gw and gb are fp32 beside bf16 rows
   void* gr;                                  // DROP: the residual's gradient, gs
+  int16_t* low;                              // DROP: what the stored sum's rounding lost (Low), or NULL
   int64_t row0;                              // DROP: the first row's number
   DropArgs d;
 };
 
 constexpr int NT = 256;
 
-template <typename T, typename P, int LPR, int VPL, bool TAIL, bool DROP>
+// What a bf16 sum's rounding lost, in 16 bits: the fp32 value's bits less those of the rounded one, so that the two make it
+// again (but for one unit of 2^-24 at ties).  The gradients of fp32 parameters are sums over all rows, whose own roundings are
+// 2^-24; from the rounded sum they would carry 2^-9.
+template <bool TAIL> struct Low {
+  typedef int16_t type __attribute__((ext_vector_type(8), aligned(2)));
+  typedef int16_t piece __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ int16_t of(float v) {
+    const int32_t d = (int32_t)(__float_as_uint(v) - __float_as_uint((float)(bf16)v));
+    return (int16_t)min(max(d, -32768), 32767);
+  }
+  static __device__ __forceinline__ float with(float rounded, int16_t d) { return __uint_as_float(__float_as_uint(rounded) + (uint32_t)(int32_t)d); }
+  template <bool PAST> static __device__ __forceinline__ piece load(const int16_t* p, int f, int C) {
+    piece t;
+    if (!TAIL || C >= 8) {
+      if constexpr (PAST) t = __builtin_nontemporal_load(reinterpret_cast<const type*>(p + f));
+      else t = *reinterpret_cast<const type*>(p + f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = i < C ? p[i] : (int16_t)0;
+    }
+    return t;
+  }
+  static __device__ __forceinline__ void store(int16_t* p, int f, int C, const float* v) {
+    if (!TAIL || C >= 8) {
+      type t;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = of(v[i]);
+      *reinterpret_cast<type*>(p + f) = t;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < C) p[i] = of(v[i]);
+    }
+  }
+};
+// With dropout or without, and with what the sum's rounding lost
+enum { kPlain, kDrop, kDropLow };
+
+template <typename T, typename P, int LPR, int VPL, bool TAIL, int D>
 __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
   typedef Vec<T, TAIL> V;
+  constexpr bool DROP = D != kPlain, LOW = D == kDropLow;
   constexpr int VEC = V::N;
   const int lane = threadIdx.x % LPR;
   const int64_t n = (int64_t)blockIdx.x * (NT / LPR) + threadIdx.x / LPR;
@@ -73,6 +113,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[p][i] += e[i];
         V::store((T*)a.s + n * a.C, c[p].f, a.C, v[p]);
+        if constexpr (LOW) Low<TAIL>::store(a.low + n * a.C, c[p].f, a.C, v[p]);
       }
   } else if (a.r) {
     typename V::piece r[VPL];
@@ -113,7 +154,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
   stats(std::false_type{}, mean, rstd);
   if (a.mean) {
     float m = mean, rs = rstd;
-    if (sizeof(T) == 2 && a.r) {
+    if (sizeof(T) == 2 && !LOW && a.r) {
       const bool far = mean * mean * rstd * rstd > 1.f;
       if (__ballot(far)) {
         stats(std::true_type{}, m, rs);
@@ -140,9 +181,10 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
 
 // PAST: 1: the result is stored past the cache, 2: the operands are read past it too (egnn_rows.h).  60,000 x 512 fp32, 123 MB:
 // 71, 58 and 67 us at 0, 1 and 2; 40,961 x 259, 42 MB: 32.0 and 33.3 at 0 and 1; 2,000,000 x 128 bf16: 347 and 325 at 1 and 2.
-template <typename T, int LPR, int VPL, int PAST, bool TAIL, bool DROP>
+template <typename T, int LPR, int VPL, int PAST, bool TAIL, int D>
 __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
   typedef Vec<T, TAIL> V;
+  constexpr bool DROP = D != kPlain, LOW = D == kDropLow;
   constexpr int VEC = V::N, RG = NT / LPR, W = LPR * VPL * VEC;
   __shared__ float red[RG][W];
   const int lane = threadIdx.x % LPR, rg = threadIdx.x / LPR;
@@ -161,6 +203,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
   const Mask m = DROP ? mask_of(a.d) : Mask{};
   const int64_t step = (int64_t)gridDim.x * RG;
   typename V::piece pg[VPL], px[VPL], pe[VPL];
+  typename Low<TAIL>::piece pl[LOW ? VPL : 1];
   float mean = 0.f, rstd = 0.f;
   // everything a row needs, requested at once; without branches, which would make the loop wait for the loads they join
   // (2,000,000 x 128 bf16: 409 us, and 326 without).  Past the rows, and in lanes without a piece, what is there is read
@@ -174,6 +217,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
       pg[p] = V::template load<PAST == 2>((const T*)a.gy + n * a.ldg, c[p].f, a.C);
       px[p] = V::template load<PAST == 2>((const T*)a.x + n * a.ldx, c[p].f, a.C);
       if (a.gsum) pe[p] = V::template load<PAST == 2>((const T*)a.gsum + n * a.ldgs, c[p].f, a.C);
+      if constexpr (LOW) pl[p] = Low<TAIL>::template load<PAST == 2>(a.low + n * a.C, c[p].f, a.C);
     }
   };
   int64_t n = (int64_t)blockIdx.x * RG + rg;
@@ -190,6 +234,9 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
       if (live && c[p].in) {
         V::floats(pg[p], t[p]);
         V::floats(px[p], xh[p]);
+        if constexpr (LOW)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) xh[p][i] = Low<TAIL>::with(xh[p][i], pl[p][i]);
         if (a.gsum) V::floats(pe[p], e[p]);
       }
 #pragma unroll
@@ -251,9 +298,10 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
 template <int S, typename F> __device__ __forceinline__ void columns(int C, F go) {
   for (int f = S * threadIdx.x; f < C; f += S * NT) go(f);
 }
-template <typename T, typename P, bool DROP>
+template <typename T, typename P, int D>
 __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
   __shared__ float buf[4];
+  constexpr bool DROP = D != kPlain, LOW = D == kDropLow;
   constexpr int S = DROP ? 4 : 1;
   const int64_t n = blockIdx.x;
   const T *x = (const T*)a.x + n * a.ldx, *r = a.r ? (const T*)a.r + n * a.ldr : nullptr;
@@ -293,7 +341,7 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
   stats(false, mean, rstd);
   if (a.mean) {
     float m = mean, rs = rstd;
-    if (sizeof(T) == 2 && r && mean * mean * rstd * rstd > 1.f) stats(true, m, rs);
+    if (sizeof(T) == 2 && !LOW && r && mean * mean * rstd * rstd > 1.f) stats(true, m, rs);
     if (threadIdx.x == 0) { a.mean[n] = m; a.rstd[n] = rs; }
   }
   columns<S>(a.C, [&](int f) {
@@ -304,21 +352,24 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
       if (i >= k) break;
       const float w = a.w ? param<P>(a.w, f + i) : 1.f, b = a.b ? param<P>(a.b, f + i) : 0.f;
       if (r) ((T*)a.s)[n * a.C + f + i] = from_f32<T>(v[i]);
+      if (LOW) a.low[n * a.C + f + i] = Low<true>::of(v[i]);
       ((T*)a.y)[n * a.C + f + i] = from_f32<T>(__builtin_fmaf((v[i] - mean) * rstd, w, b));
     }
   });
 }
-template <typename T, typename P, bool DROP>
+template <typename T, typename P, int D>
 __global__ __launch_bounds__(NT) void bwd_wide_kernel(Args a) {
   __shared__ float buf[4];
+  constexpr bool DROP = D != kPlain, LOW = D == kDropLow;
   const int64_t n = blockIdx.x;
   const T *x = (const T*)a.x + n * a.ldx, *g = (const T*)a.gy + n * a.ldg;
   const float mean = a.mean[n], rstd = a.rstd[n];
+  auto sum_at = [&](int f) { return LOW ? Low<true>::with(to_f32(x[f]), a.low[n * a.C + f]) : to_f32(x[f]); };
   float s1 = 0.f, s2 = 0.f;
   for (int f = threadIdx.x; f < a.C; f += NT) {
     const float t = to_f32(g[f]) * (a.w ? param<P>(a.w, f) : 1.f);
     s1 += t;
-    s2 = __builtin_fmaf(t, (to_f32(x[f]) - mean) * rstd, s2);
+    s2 = __builtin_fmaf(t, (sum_at(f) - mean) * rstd, s2);
   }
   const float m1 = block_sum(s1, buf) / a.C, m2 = block_sum(s2, buf) / a.C;
   constexpr int S = DROP ? 4 : 1;
@@ -331,7 +382,7 @@ __global__ __launch_bounds__(NT) void bwd_wide_kernel(Args a) {
       o[i] = 0.f;
       if (i >= k) break;
       const float t = to_f32(g[f + i]) * (a.w ? param<P>(a.w, f + i) : 1.f);
-      o[i] = rstd * (t - m1 - (to_f32(x[f + i]) - mean) * rstd * m2);
+      o[i] = rstd * (t - m1 - (sum_at(f + i) - mean) * rstd * m2);
       if (a.gsum) o[i] += to_f32(((const T*)a.gsum)[n * a.ldgs + f + i]);
       if (DROP) ((T*)a.gr)[n * a.C + f + i] = from_f32<T>(o[i]);
     }
@@ -342,14 +393,16 @@ __global__ __launch_bounds__(NT) void bwd_wide_kernel(Args a) {
   });
 }
 // gw and gb of wide rows: a thread a column, rows of one of gridDim.y parts
-template <typename T>
+template <typename T, int D>
 __global__ __launch_bounds__(NT) void bwd_wide_weights_kernel(Args a) {
   const int f = blockIdx.x * NT + threadIdx.x;
   if (f >= a.C) return;
   float gw = 0.f, gb = 0.f;
   for (int64_t n = blockIdx.y; n < a.N; n += gridDim.y) {
     const float g = to_f32(((const T*)a.gy)[n * a.ldg + f]);
-    gw = __builtin_fmaf(g, (to_f32(((const T*)a.x)[n * a.ldx + f]) - a.mean[n]) * a.rstd[n], gw);
+    float v = to_f32(((const T*)a.x)[n * a.ldx + f]);
+    if (D == kDropLow) v = Low<true>::with(v, a.low[n * a.C + f]);
+    gw = __builtin_fmaf(g, (v - a.mean[n]) * a.rstd[n], gw);
     gb += g;
   }
   float* out = a.part + (int64_t)blockIdx.y * 2 * a.C;
@@ -415,6 +468,7 @@ static void in_parts(const Args& a, int rows_per_block, Go go) {
     auto at = [&](const void* p, int64_t ld) -> const void* { return p ? (const T*)p + n * ld : nullptr; };
     x.x = at(a.x, a.ldx); x.r = at(a.r, a.ldr); x.gy = at(a.gy, a.ldg); x.gsum = at(a.gsum, a.ldgs);
     x.y = (void*)at(a.y, a.C); x.s = (void*)at(a.s, a.C); x.gx = (void*)at(a.gx, a.C); x.gr = (void*)at(a.gr, a.C);
+    x.low = a.low ? a.low + n * a.C : nullptr;
     x.row0 = n;
     x.mean = a.mean ? a.mean + n : nullptr; x.rstd = a.rstd ? a.rstd + n : nullptr;
     x.N = a.N - n < most ? a.N - n : most;
@@ -422,65 +476,65 @@ static void in_parts(const Args& a, int rows_per_block, Go go) {
   }
 }
 
-template <typename T, int LPR, int VPL, bool TAIL, bool DROP>
+template <typename T, int LPR, int VPL, bool TAIL, int D>
 static void launch_tail(const Args& a, bool bwd, hipStream_t st, int* nblk) {
   if (!bwd) {
     in_parts<T>(a, NT / LPR, [&](const Args& x, uint32_t blocks) {
-      if (sizeof(T) == 2 && a.f32_params) fwd_kernel<T, float, LPR, VPL, TAIL, DROP><<<blocks, NT, 0, st>>>(x);
-      else fwd_kernel<T, T, LPR, VPL, TAIL, DROP><<<blocks, NT, 0, st>>>(x);
+      if (sizeof(T) == 2 && a.f32_params) fwd_kernel<T, float, LPR, VPL, TAIL, D><<<blocks, NT, 0, st>>>(x);
+      else fwd_kernel<T, T, LPR, VPL, TAIL, D><<<blocks, NT, 0, st>>>(x);
     });
     return;
   }
   const int64_t n = cdiv(a.N, NT / LPR);
   *nblk = (int)(n < part_rows(a.N) ? n : part_rows(a.N));
   const int64_t bytes = a.N * a.C * (int64_t)sizeof(T);
-  if (bytes >= kPastLoad) bwd_kernel<T, LPR, VPL, 2, TAIL, DROP><<<(uint32_t)*nblk, NT, 0, st>>>(a);
-  else if (bytes >= kPastStore) bwd_kernel<T, LPR, VPL, 1, TAIL, DROP><<<(uint32_t)*nblk, NT, 0, st>>>(a);
-  else bwd_kernel<T, LPR, VPL, 0, TAIL, DROP><<<(uint32_t)*nblk, NT, 0, st>>>(a);
+  if (bytes >= kPastLoad) bwd_kernel<T, LPR, VPL, 2, TAIL, D><<<(uint32_t)*nblk, NT, 0, st>>>(a);
+  else if (bytes >= kPastStore) bwd_kernel<T, LPR, VPL, 1, TAIL, D><<<(uint32_t)*nblk, NT, 0, st>>>(a);
+  else bwd_kernel<T, LPR, VPL, 0, TAIL, D><<<(uint32_t)*nblk, NT, 0, st>>>(a);
 }
-template <typename T, int LPR, int VPL, bool DROP>
+template <typename T, int LPR, int VPL, int D>
 static void launch_shape(const Args& a, bool bwd, hipStream_t st, int* nblk) {
-  if (a.C % Vec<T>::N) launch_tail<T, LPR, VPL, true, DROP>(a, bwd, st, nblk);
-  else launch_tail<T, LPR, VPL, false, DROP>(a, bwd, st, nblk);
+  if (a.C % Vec<T>::N) launch_tail<T, LPR, VPL, true, D>(a, bwd, st, nblk);
+  else launch_tail<T, LPR, VPL, false, D>(a, bwd, st, nblk);
 }
-template <typename T, bool DROP>
+template <typename T, int D>
 static void launch_rows(const Args& a, const Shape& s, bool bwd, hipStream_t st, int* nblk) {
   switch (s.lpr * 8 + s.vpl - 1) {
-    case 32: return launch_shape<T, 4, 1, DROP>(a, bwd, st, nblk);
-    case 34: return launch_shape<T, 4, 3, DROP>(a, bwd, st, nblk);
-    case 64: return launch_shape<T, 8, 1, DROP>(a, bwd, st, nblk);
-    case 128: return launch_shape<T, 16, 1, DROP>(a, bwd, st, nblk);
-    case 256: return launch_shape<T, 32, 1, DROP>(a, bwd, st, nblk);
-    case 66: return launch_shape<T, 8, 3, DROP>(a, bwd, st, nblk);
-    case 130: return launch_shape<T, 16, 3, DROP>(a, bwd, st, nblk);
-    case 258: return launch_shape<T, 32, 3, DROP>(a, bwd, st, nblk);
-    case 512: return launch_shape<T, 64, 1, DROP>(a, bwd, st, nblk);
-    case 513: return launch_shape<T, 64, 2, DROP>(a, bwd, st, nblk);
-    case 514: return launch_shape<T, 64, 3, DROP>(a, bwd, st, nblk);
-    case 515: return launch_shape<T, 64, 4, DROP>(a, bwd, st, nblk);
-    default: return launch_shape<T, 64, 6, DROP>(a, bwd, st, nblk);
+    case 32: return launch_shape<T, 4, 1, D>(a, bwd, st, nblk);
+    case 34: return launch_shape<T, 4, 3, D>(a, bwd, st, nblk);
+    case 64: return launch_shape<T, 8, 1, D>(a, bwd, st, nblk);
+    case 128: return launch_shape<T, 16, 1, D>(a, bwd, st, nblk);
+    case 256: return launch_shape<T, 32, 1, D>(a, bwd, st, nblk);
+    case 66: return launch_shape<T, 8, 3, D>(a, bwd, st, nblk);
+    case 130: return launch_shape<T, 16, 3, D>(a, bwd, st, nblk);
+    case 258: return launch_shape<T, 32, 3, D>(a, bwd, st, nblk);
+    case 512: return launch_shape<T, 64, 1, D>(a, bwd, st, nblk);
+    case 513: return launch_shape<T, 64, 2, D>(a, bwd, st, nblk);
+    case 514: return launch_shape<T, 64, 3, D>(a, bwd, st, nblk);
+    case 515: return launch_shape<T, 64, 4, D>(a, bwd, st, nblk);
+    default: return launch_shape<T, 64, 6, D>(a, bwd, st, nblk);
   }
 }
 
-template <typename T, typename P, bool DROP>
+template <typename T, typename P, int D>
 static void launch_wide(const Args& a, bool bwd, hipStream_t st) {
   in_parts<T>(a, 1, [&](const Args& x, uint32_t blocks) {
-    if (bwd) bwd_wide_kernel<T, P, DROP><<<blocks, NT, 0, st>>>(x);
-    else fwd_wide_kernel<T, P, DROP><<<blocks, NT, 0, st>>>(x);
+    if (bwd) bwd_wide_kernel<T, P, D><<<blocks, NT, 0, st>>>(x);
+    else fwd_wide_kernel<T, P, D><<<blocks, NT, 0, st>>>(x);
   });
 }
-template <typename T, bool DROP>
+template <typename T, int D>
 static int launch(const Args& a, bool bwd, hipStream_t st) {
   Shape s;
   int nblk = 0;
   if (a.N) {
     const bool narrow = shape_of((int)cdiv(a.C, Vec<T>::N), a.N, &s);
-    if (narrow) launch_rows<T, DROP>(a, s, bwd, st, &nblk);
-    else if (a.f32_params) launch_wide<T, float, DROP>(a, bwd, st);
-    else launch_wide<T, T, DROP>(a, bwd, st);
+    if (narrow) launch_rows<T, D>(a, s, bwd, st, &nblk);
+    else if (a.f32_params) launch_wide<T, float, D>(a, bwd, st);
+    else launch_wide<T, T, D>(a, bwd, st);
     if (!narrow && bwd && a.part) {
       nblk = (int)(part_rows(a.N) < 128 ? part_rows(a.N) : 128);
-      bwd_wide_weights_kernel<T><<<dim3((uint32_t)cdiv(a.C, NT), (uint32_t)nblk), NT, 0, st>>>(a);
+      bwd_wide_weights_kernel<T, D><<<dim3((uint32_t)cdiv(a.C, NT), (uint32_t)nblk), NT, 0, st>>>(a);
     }
   }
   if (bwd && a.part) {

@@ -22,7 +22,7 @@ int32_t egnn_norm_fwd(const EgnnNormDims* d, const void* x, int64_t ldx, const v
   Args a{};
   a.x = x; a.ldx = ldx; a.r = residual; a.ldr = ldr; a.w = weight; a.b = bias; a.y = y; a.s = residual ? sum : nullptr;
   a.mean = mean; a.rstd = rstd; a.N = d->N; a.C = d->C; a.eps = d->eps; a.f32_params = d->f32_params != 0;
-  return d->dtype == EGNN_BF16 ? launch<egnn::bf16, false>(a, false, (hipStream_t)stream) : launch<float, false>(a, false, (hipStream_t)stream);
+  return d->dtype == EGNN_BF16 ? launch<egnn::bf16, kPlain>(a, false, (hipStream_t)stream) : launch<float, kPlain>(a, false, (hipStream_t)stream);
 }
 
 int32_t egnn_norm_bwd(const EgnnNormDims* d, const void* grad_y, int64_t ldg, const void* sum, int64_t lds, const void* weight,
@@ -42,7 +42,7 @@ int32_t egnn_norm_bwd(const EgnnNormDims* d, const void* grad_y, int64_t ldg, co
   a.gy = grad_y; a.ldg = ldg; a.x = sum; a.ldx = lds; a.w = weight; a.mean = (float*)mean; a.rstd = (float*)rstd;
   a.gsum = grad_sum; a.ldgs = ldgs; a.gx = grad_x; a.gw = grad_weight; a.gb = grad_bias;
   a.part = weights ? (float*)workspace : nullptr; a.N = d->N; a.C = d->C; a.eps = d->eps; a.f32_params = d->f32_params != 0;
-  return d->dtype == EGNN_BF16 ? launch<egnn::bf16, false>(a, true, (hipStream_t)stream) : launch<float, false>(a, true, (hipStream_t)stream);
+  return d->dtype == EGNN_BF16 ? launch<egnn::bf16, kPlain>(a, true, (hipStream_t)stream) : launch<float, kPlain>(a, true, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -164,7 +164,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
 def layer_norm_dropout_forward(x, residual, drop, weight=None, bias=None, eps=1e-5, need_stats=True):
     """``egnn_norm_drop_fwd`` of ``s = residual + dropout(x)``, ``drop`` a :class:`pymolecular_amd.dropout.Dropout`:
-    returns ``(y, s, mean, rstd)`` as :func:`layer_norm_forward` does."""
+    returns ``(y, s, mean, rstd)`` as :func:`layer_norm_forward` does, but that beside float32 parameters the last one is
+    a pair ``(rstd, low)`` where ``s`` is bfloat16: what its rounding lost (int16, opaque), without which float32
+    gradients would be off by 2^-9."""
     r = _capi.ext().norm_drop_forward(x, residual, *drop, weight, bias, eps, need_stats)
     if r is not None:
         return r
@@ -186,12 +188,13 @@ def layer_norm_dropout_forward(x, residual, drop, weight=None, bias=None, eps=1e
     y, s = (torch.empty(shape, dtype=dt, device=dev) for _ in range(2))
     stats = torch.empty((2, n), dtype=torch.float32, device=dev) if need_stats else None
     mean, rstd = (stats[0], stats[1]) if need_stats else (None, None)
+    low = torch.empty(shape, dtype=torch.int16, device=dev) if need_stats and pdt != dt else None
     with torch.cuda.device(dev):
         check("egnn_norm_drop_fwd",
               _capi.lib().egnn_norm_drop_fwd(EgnnNormDims(n, c, _dtype_code(dt), eps, pdt != dt), d, x2.data_ptr(), x2.stride(0),
                                              r2.data_ptr(), r2.stride(0), _ptr(w), _ptr(b), y.data_ptr(), s.data_ptr(),
-                                             _ptr(mean), _ptr(rstd), _stream(dev)))
-    return y, s, mean, rstd
+                                             _ptr(low), _ptr(mean), _ptr(rstd), _stream(dev)))
+    return y, s, mean, rstd if low is None else (rstd, low)
 
 
 def layer_norm_dropout_backward(gy, s, drop, weight, mean, rstd, gsum=None, need_weight=True, need_bias=True, bias_dtype=None):
@@ -200,7 +203,8 @@ def layer_norm_dropout_backward(gy, s, drop, weight, mean, rstd, gsum=None, need
     wdt = s.dtype if weight is None else weight.dtype
     bdt = wdt if bias_dtype is None else bias_dtype
     pdt = _param_dtype(s.dtype, wdt, bdt if need_bias else None)
-    r = _capi.ext().norm_drop_backward(gy, s, *drop, weight, mean, rstd, gsum, need_weight, need_bias, pdt == torch.float32)
+    rstd, low = rstd if isinstance(rstd, tuple) else (rstd, None)
+    r = _capi.ext().norm_drop_backward(gy, s, *drop, weight, mean, rstd, low, gsum, need_weight, need_bias, pdt == torch.float32)
     if r is not None:
         return r[0], r[1], _as(r[2], wdt), _as(r[3], bdt)
     from .dropout import check_drop
@@ -214,6 +218,9 @@ def layer_norm_dropout_backward(gy, s, drop, weight, mean, rstd, gsum=None, need
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.device != dev:
             raise ValueError(f"{name} must be the forward's ({n},) float32 statistics")
+    if low is not None and (dt != torch.bfloat16 or low.dtype != torch.int16 or low.shape != shape or not low.is_contiguous()
+                            or low.device != dev):
+        raise ValueError("rstd must be what the forward returned with s")
     g2 = _rows(gy if gy.dtype == dt else gy.to(dt))
     e2 = None if gsum is None else _rows(gsum if gsum.dtype == dt else gsum.to(dt))
     w = _as(weight, pdt)
@@ -226,7 +233,7 @@ def layer_norm_dropout_backward(gy, s, drop, weight, mean, rstd, gsum=None, need
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with torch.cuda.device(dev):
         check("egnn_norm_drop_bwd",
-              L.egnn_norm_drop_bwd(nd, d, g2.data_ptr(), g2.stride(0), s2.data_ptr(), s2.stride(0), _ptr(w), mean.data_ptr(),
+              L.egnn_norm_drop_bwd(nd, d, g2.data_ptr(), g2.stride(0), s2.data_ptr(), s2.stride(0), _ptr(low), _ptr(w), mean.data_ptr(),
                                    rstd.data_ptr(), _ptr(e2), 0 if e2 is None else e2.stride(0), gx.data_ptr(), gr.data_ptr(),
                                    _ptr(gw), _ptr(gb), _ptr(ws), nbytes, _stream(dev)))
     return gx, gr, _as(gw, wdt), _as(gb, bdt)
@@ -238,7 +245,8 @@ class LayerNormDropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, rng, site, weight, bias, eps):
         y, s, mean, rstd = layer_norm_dropout_forward(x, residual, (p, rng, site), weight, bias, eps)
-        ctx.save_for_backward(s, weight, mean, rstd, rng)
+        rstd, low = rstd if isinstance(rstd, tuple) else (rstd, None)
+        ctx.save_for_backward(s, weight, mean, rstd, low, rng)
         ctx.p, ctx.site = p, site
         ctx.has_b, ctx.bdt = bias is not None, None if bias is None else bias.dtype
         ctx.xdt, ctx.rdt = x.dtype, residual.dtype
@@ -247,7 +255,8 @@ class LayerNormDropoutFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy, gsum=None):
-        s, weight, mean, rstd, rng = ctx.saved_tensors
+        s, weight, mean, rstd, low, rng = ctx.saved_tensors
+        rstd = rstd if low is None else (rstd, low)
         drop = (ctx.p, rng, ctx.site)
         if gy is None:   # only the sum was used, if anything was
             if gsum is None:

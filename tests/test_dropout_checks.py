@@ -69,19 +69,21 @@ def test_dropout_arguments_refused():
 def test_norm_with_dropout_arguments_refused():
     L = _capi.lib()
     dims = lambda **kw: _capi.EgnnNormDims(**{**dict(N=10, C=64, dtype=0, eps=1e-5), **kw})  # noqa: E731
-    fwd = lambda d=None, dr=None, x=BUF, r=BUF, y=BUF, s=BUF, m=BUF, v=BUF, ldr=64, w=BUF: L.egnn_norm_drop_fwd(  # noqa: E731
-        d or dims(), dr or _drop(), x, 64, r, ldr, w, BUF, y, s, m, v, None)
+    fwd = lambda d=None, dr=None, x=BUF, r=BUF, y=BUF, s=BUF, m=BUF, v=BUF, ldr=64, w=BUF, low=None: L.egnn_norm_drop_fwd(  # noqa: E731
+        d or dims(), dr or _drop(), x, 64, r, ldr, w, BUF, y, s, low, m, v, None)
     for d in (dims(C=0), dims(N=1 << 31), dims(eps=-1.0), dims(dtype=5), dims(f32_params=2)):
         assert fwd(d) == 2
     assert fwd(dr=_drop(p=2.0)) == 2
     for kw in (dict(x=None), dict(r=None), dict(y=None), dict(s=None), dict(m=None), dict(dr=_drop(rng=None))):
         assert fwd(**kw) == 1, kw
     assert fwd(ldr=-4) == 3 and fwd(r=BUF + 2) == fwd(s=BUF + 2) == fwd(w=BUF + 2) == fwd(dr=_drop(rng=BUF + 4)) == 4
-    bwd = lambda d=None, dr=None, g=BUF, gx=BUF, gr=BUF, ws=BUF, nb=1 << 30, ldgs=0: L.egnn_norm_drop_bwd(  # noqa: E731
-        d or dims(), dr or _drop(), g, 64, BUF, 64, None, BUF, BUF, BUF, ldgs, gx, gr, BUF, None, ws, nb, None)
+    bwd = lambda d=None, dr=None, g=BUF, gx=BUF, gr=BUF, ws=BUF, nb=1 << 30, ldgs=0, low=None: L.egnn_norm_drop_bwd(  # noqa: E731
+        d or dims(), dr or _drop(), g, 64, BUF, 64, low, None, BUF, BUF, BUF, ldgs, gx, gr, BUF, None, ws, nb, None)
     assert bwd(dims(C=0)) == bwd(dr=_drop(p=-1.0)) == 2 and bwd(g=None) == bwd(gx=None) == bwd(gr=None) == 1
+    assert fwd(low=BUF) == bwd(low=BUF) == 2   # beside float32 rows
+    assert fwd(dims(dtype=1), low=BUF + 1) == bwd(dims(dtype=1), low=BUF + 1) == 4
     assert bwd(ldgs=-1) == 3 and bwd(gr=BUF + 2) == 4 and bwd(ws=None) == bwd(nb=16) == 5
-    assert L.egnn_norm_drop_fwd(dims(), None, *([BUF, 64] * 2), *([BUF] * 6), None) == 1
+    assert L.egnn_norm_drop_fwd(dims(), None, *([BUF, 64] * 2), *([BUF] * 7), None) == 1
 
 
 def test_python_refusals():
