@@ -38,7 +38,9 @@ __device__ __forceinline__ void store_params(void* p, int f, int C, const float*
 }
 
 // ---- forward ------------------------------------------------------------------------------
-constexpr int NT = 256, U = 4;
+constexpr int NT = 256;
+// Up to so many pieces a lane takes one: more workgroups come before more loads in flight
+constexpr int64_t kFewPieces = 1024 * 1024;
 
 struct FwdArgs {
   const void *tokens, *w;
@@ -49,7 +51,7 @@ struct FwdArgs {
   float scale;
 };
 
-template <typename T, typename P, typename I, bool TAIL, bool PAST>
+template <typename T, typename P, typename I, bool TAIL, int U, bool PAST>
 __global__ __launch_bounds__(NT) void fwd_kernel(FwdArgs a) {
   typedef Vec<T, TAIL> V;
   constexpr int VEC = V::N;
@@ -80,10 +82,9 @@ __global__ __launch_bounds__(NT) void fwd_kernel(FwdArgs a) {
     if (in[u]) V::template store<PAST>((T*)a.out + n[u] * a.C, f[u], a.C, v[u]);
 }
 
-template <typename T, typename P, typename I>
+template <typename T, typename P, typename I, bool TAIL, int U, bool PAST>
 static void launch_fwd(FwdArgs a, hipStream_t st) {
-  constexpr int VEC = Vec<T>::N;
-  a.G = (int32_t)cdiv(a.C, VEC);
+  a.G = (int32_t)cdiv(a.C, Vec<T>::N);
   const int tiles = (int)cdiv(a.G, NT * U);
   a.GT = (int32_t)cdiv(a.G, tiles);
   a.R = NT * U / a.GT;
@@ -94,15 +95,14 @@ static void launch_fwd(FwdArgs a, hipStream_t st) {
     a.tokens = (const I*)all.tokens + n;
     a.out = (T*)all.out + n * a.C;
     a.N = N - n < most ? N - n : most;
-    const dim3 grid((uint32_t)cdiv(a.N, a.R), (uint32_t)tiles);
-    if (N * a.C * (int64_t)sizeof(T) >= kPastStore) {
-      if (a.C % VEC) fwd_kernel<T, P, I, true, true><<<grid, NT, 0, st>>>(a);
-      else fwd_kernel<T, P, I, false, true><<<grid, NT, 0, st>>>(a);
-    } else {
-      if (a.C % VEC) fwd_kernel<T, P, I, true, false><<<grid, NT, 0, st>>>(a);
-      else fwd_kernel<T, P, I, false, false><<<grid, NT, 0, st>>>(a);
-    }
+    fwd_kernel<T, P, I, TAIL, U, PAST><<<dim3((uint32_t)cdiv(a.N, a.R), (uint32_t)tiles), NT, 0, st>>>(a);
   }
+}
+template <typename T, typename P, typename I, bool TAIL>
+static void launch_fwd(const FwdArgs& a, hipStream_t st) {
+  if (a.N * cdiv(a.C, Vec<T>::N) < kFewPieces) launch_fwd<T, P, I, TAIL, 1, false>(a, st);
+  else if (a.N * a.C * (int64_t)sizeof(T) < kPastStore) launch_fwd<T, P, I, TAIL, 4, false>(a, st);
+  else launch_fwd<T, P, I, TAIL, 4, true>(a, st);
 }
 
 // ---- backward: sorting inside a workgroup --------------------------------------------------
@@ -748,7 +748,8 @@ static auto by_type(const EgnnEmbedDims* d, A... args) {
 }
 template <typename T, typename P, typename I> struct Fwd {
   static int go(const FwdArgs& a, hipStream_t st) {
-    launch_fwd<T, P, I>(a, st);
+    if (a.C % Vec<T>::N) launch_fwd<T, P, I, true>(a, st);
+    else launch_fwd<T, P, I, false>(a, st);
     return hipGetLastError() == hipSuccess ? EGNN_OK : EGNN_ERR_HIP;
   }
 };

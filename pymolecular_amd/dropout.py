@@ -104,6 +104,10 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: Optional[tor
             site: int = 0) -> torch.Tensor:
     """Dropout of ``x``, or ``residual`` + dropout of ``x`` (module docstring).  Differentiable in ``x`` and the
     residual."""
-    if (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))) or _recorded(x, residual):
-        return DropoutFn.apply(x, p, rng, residual, site)
-    return dropout_forward(x, p, rng, residual, site)
+    if not (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
+        r = _capi.ext().dropout(x, p, rng, site, residual)
+        if r is not None:   # (neither a tensor that needs a conversion, nor a call that has to be recorded)
+            return r
+        if not _recorded(x, residual):
+            return dropout_forward(x, p, rng, residual, site)
+    return DropoutFn.apply(x, p, rng, residual, site)

@@ -118,6 +118,10 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     the weight's).  Differentiable in the weight."""
     if padding is not None and not 0 <= padding < weight.shape[0]:
         raise ValueError(f"padding must be a row of the table, 0 to {weight.shape[0] - 1} (got {padding})")
-    if (torch.is_grad_enabled() and weight.requires_grad) or _recorded(weight):
-        return EmbeddingFn.apply(tokens, weight, scale, padding, dtype)
-    return embedding_forward(tokens, weight, scale, dtype)
+    if not (torch.is_grad_enabled() and weight.requires_grad):
+        r = _capi.ext().embed_forward(tokens, weight, scale, weight.dtype if dtype is None else dtype)
+        if r is not None:   # (neither a tensor that needs a conversion, nor a call that has to be recorded)
+            return r
+        if not _recorded(weight):
+            return embedding_forward(tokens, weight, scale, dtype)
+    return EmbeddingFn.apply(tokens, weight, scale, padding, dtype)

@@ -155,9 +155,14 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
                    eps: float = 1e-6):
     """``(q', k')``: heads normed and turned (module docstring).  Differentiable in q, k and the weights."""
     tensors = (q, k, q_weight, k_weight)
-    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _recorded(*tensors):
-        return QKNormRotaryFn.apply(*tensors, positions, base, rotary_dim, interleaved, eps)
-    return qk_norm_rotary_forward(*tensors, positions, base, rotary_dim, interleaved, eps)
+    how = (base, _rotary(q, positions, rotary_dim), interleaved, eps)
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
+        r = _capi.ext().qk_forward(*tensors, positions, *how)
+        if r is not None:   # (neither a tensor that needs a conversion, nor a call that has to be recorded)
+            return r
+        if not _recorded(*tensors):
+            return qk_norm_rotary_forward(*tensors, positions, *how)
+    return QKNormRotaryFn.apply(*tensors, positions, *how)
 
 
 class QKNormRotaryAttentionFn(torch.autograd.Function):
