@@ -341,23 +341,27 @@ static int lanes_of(const EgnnQkDims* d, bool bwd) {
   while (l * piece_of(d, bwd) < d->D / 2) l *= 2;
   return l;
 }
-// Rows of a tile: enough heads of the side with fewer of them for two of each group of lanes, but a tile for each of 1,024
-// workgroups first
+// Workgroups that small calls are spread over, and partial rows of the weight gradients.  Each costs its start, about 4 ns:
+// with 512, 1,024, 2,048 and 4,096, forward of 4,096 x 8 heads of 32 bf16 5.6, 6.6, 10.8 and 19.0 us, of 32,768 x 10 heads of 64
+// 18.1, 16.7, 19.4 and 25.8; backward with 512, 1,024 and 2,048 10.8, 13.2 and 21.8 us, and 35.0, 29.1 and 34.5.
+static int blocks_for(const EgnnQkDims* d, bool bwd) {
+  const int64_t values = d->N * (d->Hq + d->Hk) * d->D;
+  return values < 1 << 20 ? 256 : values < (bwd ? 4 : 8) << 20 ? 512 : 1024;
+}
+// Rows of a tile: enough heads of the side with fewer of them for two of each group of lanes, but a tile for each workgroup first
 static int tile_rows(const EgnnQkDims* d, bool bwd) {
   const int H = d->Hq < d->Hk ? d->Hq : d->Hk;
   const int groups = NT / lanes_of(d, bwd);
   int64_t tb = groups * 2 / H;
   if (tb > kTable / (d->D / 2 + 2)) tb = kTable / (d->D / 2 + 2);
-  if (tb > cdiv(d->N, 1024)) tb = cdiv(d->N, 1024);
+  if (tb > cdiv(d->N, blocks_for(d, bwd))) tb = cdiv(d->N, blocks_for(d, bwd));
   int m = groups;                            // whole rounds of the groups over the heads
   for (int h = H; h % 2 == 0 && m > 1; h /= 2) m /= 2;
   if (tb > m) tb = tb / m * m;
   return tb < 1 ? 1 : (int)tb;
 }
-// Workgroups of the backward at most, and partial rows of the weight gradients
-constexpr int kBlocks = 1024;
 static int32_t blocks_of(const EgnnQkDims* d, bool bwd) {
-  const int64_t most = bwd ? kBlocks : kMaxGrid;
+  const int64_t most = bwd ? blocks_for(d, true) : kMaxGrid;
   const int64_t tiles = cdiv(d->N, tile_rows(d, bwd));
   return (int32_t)(tiles < most ? tiles : most);
 }
