@@ -1,7 +1,9 @@
 // Dropout of rows, with the residual sum behind it:  y = (residual +) keep ? up x : 0,  the mask of egnn_random.h.
 // The backward is the same kernel on the gradient: gx = keep ? up gy : 0 (the residual's gradient is gy itself).
-// A thread makes the 128 bits of eight columns and takes their values with them, several such groups at once, whose loads
-// are on their way while the bits are made.
+// A thread makes the 128 bits of eight columns and takes their values with them; in large calls four such groups at once, whose
+// loads are on their way while the bits are made.  Bound by HBM: 2,000,000 x 128 bf16 168 us alone and 252 with a residual, 6.1 TB/s,
+// with the vector units busy 0.62 and 0.51 of the time (the generator's products run at a quarter of their rate); 2,432 x 128
+// fp32 2.7 us, a launch.
 #include "egnn_internal.h"
 #include "egnn_random.h"
 #include "egnn_rows.h"
