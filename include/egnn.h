@@ -414,16 +414,16 @@ int32_t egnn_dropout(const EgnnDropout* drop, int32_t dtype, int64_t N, int32_t 
 
 /* egnn_norm_fwd of s = residual + dropout(x), and its backward: grad_residual (N, C)
  * is the gradient of s, grad_x (N, C) its dropout.  The residual and the sum are
- * not optional here; workspace: egnn_norm_bwd_workspace_bytes.  low (N, C) takes
- * what the rounding of a bf16 sum lost, and gives it back to the backward, whose
- * gradients are those of the unrounded sum then; it may be NULL (in both) and has
- * to be beside fp32 rows.  Gradients of fp32 parameters need it: from the rounded
- * sum they are off by 2^-9. */
+ * not optional here; workspace: egnn_norm_bwd_workspace_bytes.  low (N, C), int16
+ * beside fp32 parameters and int8 otherwise, takes what the rounding of a bf16 sum
+ * lost, and gives it back to the backward, whose gradients are those of the
+ * unrounded sum then (to 2^-17 of it with int8).  It may be NULL (in both): the
+ * gradients are those of the stored sum, off by 2^-9; it has to be beside fp32 rows. */
 int32_t egnn_norm_drop_fwd(const EgnnNormDims* dims, const EgnnDropout* drop, const void* x, int64_t ldx, const void* residual,
-                           int64_t ldr, const void* weight, const void* bias, void* y, void* sum, int16_t* low, float* mean,
+                           int64_t ldr, const void* weight, const void* bias, void* y, void* sum, void* low, float* mean,
                            float* rstd, void* stream);
 int32_t egnn_norm_drop_bwd(const EgnnNormDims* dims, const EgnnDropout* drop, const void* grad_y, int64_t ldg, const void* sum,
-                           int64_t lds, const int16_t* low, const void* weight, const float* mean, const float* rstd,
+                           int64_t lds, const void* low, const void* weight, const float* mean, const float* rstd,
                            const void* grad_sum, int64_t ldgs, void* grad_x, void* grad_residual, void* grad_weight, void* grad_bias,
                            void* workspace, size_t workspace_bytes, void* stream);
 

@@ -3,8 +3,8 @@
 //   t = gy w, gs = rstd (t - mean t - xh mean(t xh)) (+ g_sum), gw = sum_rows gy xh, gb = sum_rows gy
 // DROP: s = drop(x) + r with the mask of egnn_random.h, and in the backward gx = drop(gs) beside gs, the residual's gradient:
 // two tensors fewer to write and read again than with a dropout of its own, and the mask is made in registers, twice.  40,961 x
-// 259 fp32, forward and backward 37.6 and 48.4 us, 4.5 and 4.4 TB/s; 19,456 x 128 bf16 7.0 and 7.4 us, launches; 2,000,000 x 128
-// bf16 rows beside fp32 parameters, with what the sum's rounding loses (Low), forward and backward 949 us, 5.9 TB/s.
+// 259 fp32, forward and backward 37.6 and 48.4 us, 4.5 and 4.4 TB/s; 19,456 x 128 bf16 8.4 and 8.1 us, launches; 2,000,000 x 128
+// bf16, with what the sum's rounding loses (Low), forward and backward 906 us, and 943 beside fp32 parameters, 5.7 and 6.0 TB/s.
 // A row lives in the registers of LPR lanes, so it is read once and the variance is taken around the mean.  The backward's
 // blocks walk the rows with a fixed stride; a lane keeps the sums of gw and gb of its columns in fp32 registers, a
 // block's row groups are joined in LDS and its sums leave as one partial row, which a second launch adds up in order.
@@ -34,36 +34,40 @@ struct Args {
   float eps;
   bool f32_params;                           // w, b, gw and gb are fp32 beside bf16 rows
   void* gr;                                  // DROP: the residual's gradient, gs
-  int16_t* low;                              // DROP: what the stored sum's rounding lost (Low), or NULL
+  void* low;                                 // DROP: what the stored sum's rounding lost (Low), or NULL
   int64_t row0;                              // DROP: the first row's number
   DropArgs d;
 };
 
 constexpr int NT = 256;
 
-// What a bf16 sum's rounding lost, in 16 bits: the fp32 value's bits less those of the rounded one, so that the two make it
-// again (but for one unit of 2^-24 at ties).  The gradients of fp32 parameters are sums over all rows, whose own roundings are
-// 2^-24; from the rounded sum they would carry 2^-9.
-template <bool TAIL> struct Low {
-  typedef int16_t type __attribute__((ext_vector_type(8), aligned(2)));
-  typedef int16_t piece __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ int16_t of(float v) {
+// What a bf16 sum's rounding lost: the fp32 value's bits less those of the rounded one, all 16 of them (L = int16_t: the two
+// make the value again, but for one unit of 2^-24 at ties) or the upper 8 (int8_t: to 2^-17).  From the rounded sum alone the
+// gradients would carry its rounding, 2^-9: as much again as their own where they are bf16 (errors of gw 2.5e-3 to 3.9e-3 of its norm,
+// 1.7e-3 with the byte), and 10^4 times as much where the parameters are fp32.
+template <typename L, bool TAIL> struct Low {
+  typedef L type __attribute__((ext_vector_type(8), aligned(sizeof(L))));
+  typedef L piece __attribute__((ext_vector_type(8)));
+  static constexpr int kShift = sizeof(L) == 2 ? 0 : 8, kMost = sizeof(L) == 2 ? 32767 : 127;
+  static __device__ __forceinline__ L of(float v) {
     const int32_t d = (int32_t)(__float_as_uint(v) - __float_as_uint((float)(bf16)v));
-    return (int16_t)min(max(d, -32768), 32767);
+    return (L)min(max(kShift ? (d + 128) >> kShift : d, -kMost - 1), kMost);
   }
-  static __device__ __forceinline__ float with(float rounded, int16_t d) { return __uint_as_float(__float_as_uint(rounded) + (uint32_t)(int32_t)d); }
-  template <bool PAST> static __device__ __forceinline__ piece load(const int16_t* p, int f, int C) {
+  static __device__ __forceinline__ float with(float rounded, L d) {
+    return __uint_as_float(__float_as_uint(rounded) + ((uint32_t)(int32_t)d << kShift));
+  }
+  template <bool PAST> static __device__ __forceinline__ piece load(const L* p, int f, int C) {
     piece t;
     if (!TAIL || C >= 8) {
       if constexpr (PAST) t = __builtin_nontemporal_load(reinterpret_cast<const type*>(p + f));
       else t = *reinterpret_cast<const type*>(p + f);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = i < C ? p[i] : (int16_t)0;
+      for (int i = 0; i < 8; ++i) t[i] = i < C ? p[i] : (L)0;
     }
     return t;
   }
-  static __device__ __forceinline__ void store(int16_t* p, int f, int C, const float* v) {
+  static __device__ __forceinline__ void store(L* p, int f, int C, const float* v) {
     if (!TAIL || C >= 8) {
       type t;
 #pragma unroll
@@ -76,13 +80,16 @@ template <bool TAIL> struct Low {
     }
   }
 };
-// With dropout or without, and with what the sum's rounding lost
-enum { kPlain, kDrop, kDropLow };
+// Without dropout, with it, and with what the sum's rounding lost in 16 or 8 bits
+enum { kPlain, kDrop, kDropLow, kDropByte };
+template <int D> struct LowOf { typedef int16_t type; };
+template <> struct LowOf<kDropByte> { typedef int8_t type; };
 
 template <typename T, typename P, int LPR, int VPL, bool TAIL, int D>
 __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
   typedef Vec<T, TAIL> V;
-  constexpr bool DROP = D != kPlain, LOW = D == kDropLow;
+  constexpr bool DROP = D != kPlain, LOW = D >= kDropLow;
+  typedef typename LowOf<D>::type L;
   constexpr int VEC = V::N;
   const int lane = threadIdx.x % LPR;
   const int64_t n = (int64_t)blockIdx.x * (NT / LPR) + threadIdx.x / LPR;
@@ -115,7 +122,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[p][i] += e[i];
         V::store((T*)a.s + n * a.C, c[p].f, a.C, v[p]);
-        if constexpr (LOW) Low<TAIL>::store(a.low + n * a.C, c[p].f, a.C, v[p]);
+        if constexpr (LOW) Low<L, TAIL>::store((L*)a.low + n * a.C, c[p].f, a.C, v[p]);
       }
   } else if (a.r) {
     typename V::piece r[VPL];
@@ -136,7 +143,11 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
   float mean, rstd;
   auto stats = [&](auto round, float& mean, float& rstd) {
     constexpr bool ROUND = decltype(round)::value;
-    auto at = [&](int p, int i) { return ROUND ? to_f32(from_f32<T>(v[p][i])) : v[p][i]; };
+    auto at = [&](int p, int i) {
+      if (!ROUND) return v[p][i];
+      const float h = to_f32(from_f32<T>(v[p][i]));
+      return LOW ? Low<L, TAIL>::with(h, Low<L, TAIL>::of(v[p][i])) : h;
+    };
     float sum = 0.f;
 #pragma unroll
     for (int p = 0; p < VPL; ++p)
@@ -156,7 +167,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
   stats(std::false_type{}, mean, rstd);
   if (a.mean) {
     float m = mean, rs = rstd;
-    if (sizeof(T) == 2 && !LOW && a.r) {
+    if (sizeof(T) == 2 && a.r) {
       const bool far = mean * mean * rstd * rstd > 1.f;
       if (__ballot(far)) {
         stats(std::true_type{}, m, rs);
@@ -186,7 +197,8 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a) {
 template <typename T, int LPR, int VPL, int PAST, bool TAIL, int D>
 __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
   typedef Vec<T, TAIL> V;
-  constexpr bool DROP = D != kPlain, LOW = D == kDropLow;
+  constexpr bool DROP = D != kPlain, LOW = D >= kDropLow;
+  typedef typename LowOf<D>::type L;
   constexpr int VEC = V::N, RG = NT / LPR, W = LPR * VPL * VEC;
   __shared__ float red[RG][W];
   const int lane = threadIdx.x % LPR, rg = threadIdx.x / LPR;
@@ -205,7 +217,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
   const Mask m = DROP ? mask_of(a.d) : Mask{};
   const int64_t step = (int64_t)gridDim.x * RG;
   typename V::piece pg[VPL], px[VPL], pe[VPL];
-  typename Low<TAIL>::piece pl[LOW ? VPL : 1];
+  typename Low<L, TAIL>::piece pl[LOW ? VPL : 1];
   float mean = 0.f, rstd = 0.f;
   // everything a row needs, requested at once; without branches, which would make the loop wait for the loads they join
   // (2,000,000 x 128 bf16: 409 us, and 326 without).  Past the rows, and in lanes without a piece, what is there is read
@@ -219,7 +231,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
       pg[p] = V::template load<PAST == 2>((const T*)a.gy + n * a.ldg, c[p].f, a.C);
       px[p] = V::template load<PAST == 2>((const T*)a.x + n * a.ldx, c[p].f, a.C);
       if (a.gsum) pe[p] = V::template load<PAST == 2>((const T*)a.gsum + n * a.ldgs, c[p].f, a.C);
-      if constexpr (LOW) pl[p] = Low<TAIL>::template load<PAST == 2>(a.low + n * a.C, c[p].f, a.C);
+      if constexpr (LOW) pl[p] = Low<L, TAIL>::template load<PAST == 2>((const L*)a.low + n * a.C, c[p].f, a.C);
     }
   };
   int64_t n = (int64_t)blockIdx.x * RG + rg;
@@ -238,7 +250,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Args a) {
         V::floats(px[p], xh[p]);
         if constexpr (LOW)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) xh[p][i] = Low<TAIL>::with(xh[p][i], pl[p][i]);
+          for (int i = 0; i < VEC; ++i) xh[p][i] = Low<L, TAIL>::with(xh[p][i], (L)pl[p][i]);
         if (a.gsum) V::floats(pe[p], e[p]);
       }
 #pragma unroll
@@ -303,7 +315,8 @@ template <int S, typename F> __device__ __forceinline__ void columns(int C, F go
 template <typename T, typename P, int D>
 __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
   __shared__ float buf[4];
-  constexpr bool DROP = D != kPlain, LOW = D == kDropLow;
+  constexpr bool DROP = D != kPlain, LOW = D >= kDropLow;
+  typedef typename LowOf<D>::type L;
   constexpr int S = DROP ? 4 : 1;
   const int64_t n = blockIdx.x;
   const T *x = (const T*)a.x + n * a.ldx, *r = a.r ? (const T*)a.r + n * a.ldr : nullptr;
@@ -317,6 +330,10 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
     for (int i = 0; i < S; ++i) v[i] += r && f + i < a.C ? to_f32(r[f + i]) : 0.f;
     return a.C - f < S ? a.C - f : S;
   };
+  auto stored = [&](float x) {
+    const float h = to_f32(from_f32<T>(x));
+    return LOW ? Low<L, true>::with(h, Low<L, true>::of(x)) : h;
+  };
   auto stats = [&](bool round, float& mean, float& rstd) {
     float s = 0.f;
     columns<S>(a.C, [&](int f) {
@@ -324,7 +341,7 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
       const int k = vals(f, v);
 #pragma unroll
       for (int i = 0; i < S; ++i)
-        if (i < k) s += round ? to_f32(from_f32<T>(v[i])) : v[i];
+        if (i < k) s += round ? stored(v[i]) : v[i];
     });
     mean = block_sum(s, buf) / a.C;
     float q = 0.f;
@@ -333,7 +350,7 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
       const int k = vals(f, v);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        const float d = (round ? to_f32(from_f32<T>(v[i])) : v[i]) - mean;
+        const float d = (round ? stored(v[i]) : v[i]) - mean;
         if (i < k) q = __builtin_fmaf(d, d, q);
       }
     });
@@ -343,7 +360,7 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
   stats(false, mean, rstd);
   if (a.mean) {
     float m = mean, rs = rstd;
-    if (sizeof(T) == 2 && !LOW && r && mean * mean * rstd * rstd > 1.f) stats(true, m, rs);
+    if (sizeof(T) == 2 && r && mean * mean * rstd * rstd > 1.f) stats(true, m, rs);
     if (threadIdx.x == 0) { a.mean[n] = m; a.rstd[n] = rs; }
   }
   columns<S>(a.C, [&](int f) {
@@ -354,7 +371,7 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
       if (i >= k) break;
       const float w = a.w ? param<P>(a.w, f + i) : 1.f, b = a.b ? param<P>(a.b, f + i) : 0.f;
       if (r) ((T*)a.s)[n * a.C + f + i] = from_f32<T>(v[i]);
-      if (LOW) a.low[n * a.C + f + i] = Low<true>::of(v[i]);
+      if (LOW) ((L*)a.low)[n * a.C + f + i] = Low<L, true>::of(v[i]);
       ((T*)a.y)[n * a.C + f + i] = from_f32<T>(__builtin_fmaf((v[i] - mean) * rstd, w, b));
     }
   });
@@ -362,11 +379,12 @@ __global__ __launch_bounds__(NT) void fwd_wide_kernel(Args a) {
 template <typename T, typename P, int D>
 __global__ __launch_bounds__(NT) void bwd_wide_kernel(Args a) {
   __shared__ float buf[4];
-  constexpr bool DROP = D != kPlain, LOW = D == kDropLow;
+  constexpr bool DROP = D != kPlain, LOW = D >= kDropLow;
+  typedef typename LowOf<D>::type L;
   const int64_t n = blockIdx.x;
   const T *x = (const T*)a.x + n * a.ldx, *g = (const T*)a.gy + n * a.ldg;
   const float mean = a.mean[n], rstd = a.rstd[n];
-  auto sum_at = [&](int f) { return LOW ? Low<true>::with(to_f32(x[f]), a.low[n * a.C + f]) : to_f32(x[f]); };
+  auto sum_at = [&](int f) { return LOW ? Low<L, true>::with(to_f32(x[f]), ((const L*)a.low)[n * a.C + f]) : to_f32(x[f]); };
   float s1 = 0.f, s2 = 0.f;
   for (int f = threadIdx.x; f < a.C; f += NT) {
     const float t = to_f32(g[f]) * (a.w ? param<P>(a.w, f) : 1.f);
@@ -403,7 +421,7 @@ __global__ __launch_bounds__(NT) void bwd_wide_weights_kernel(Args a) {
   for (int64_t n = blockIdx.y; n < a.N; n += gridDim.y) {
     const float g = to_f32(((const T*)a.gy)[n * a.ldg + f]);
     float v = to_f32(((const T*)a.x)[n * a.ldx + f]);
-    if (D == kDropLow) v = Low<true>::with(v, a.low[n * a.C + f]);
+    if (D >= kDropLow) v = Low<typename LowOf<D>::type, true>::with(v, ((const typename LowOf<D>::type*)a.low)[n * a.C + f]);
     gw = __builtin_fmaf(g, (v - a.mean[n]) * a.rstd[n], gw);
     gb += g;
   }
@@ -470,7 +488,7 @@ static void in_parts(const Args& a, int rows_per_block, Go go) {
     auto at = [&](const void* p, int64_t ld) -> const void* { return p ? (const T*)p + n * ld : nullptr; };
     x.x = at(a.x, a.ldx); x.r = at(a.r, a.ldr); x.gy = at(a.gy, a.ldg); x.gsum = at(a.gsum, a.ldgs);
     x.y = (void*)at(a.y, a.C); x.s = (void*)at(a.s, a.C); x.gx = (void*)at(a.gx, a.C); x.gr = (void*)at(a.gr, a.C);
-    x.low = a.low ? a.low + n * a.C : nullptr;
+    x.low = a.low ? (char*)a.low + n * a.C * (a.f32_params ? 2 : 1) : nullptr;
     x.row0 = n;
     x.mean = a.mean ? a.mean + n : nullptr; x.rstd = a.rstd ? a.rstd + n : nullptr;
     x.N = a.N - n < most ? a.N - n : most;

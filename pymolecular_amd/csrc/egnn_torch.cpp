@@ -362,9 +362,9 @@ pybind11::object norm_drop_forward(const Tensor& x, const Opt& res, double p, co
   const c10::DeviceGuard device(x.device());
   const Tensor y = at::empty(x.sizes(), x.options()), s = at::empty(x.sizes(), x.options());
   const Tensor mean = need_stats ? at::empty({d.N}, stat) : Tensor(), rstd = need_stats ? at::empty({d.N}, stat) : Tensor();
-  const Tensor low = need_stats && d.f32_params ? at::empty(x.sizes(), x.options().dtype(at::kShort)) : Tensor();
+  const Tensor low = need_stats && d.dtype == EGNN_BF16 ? at::empty(x.sizes(), x.options().dtype(d.f32_params ? at::kShort : at::kChar)) : Tensor();
   check("egnn_norm_drop_fwd", egnn_norm_drop_fwd(&d, &dr, ptr(x), d.C, ptr(*res), d.C, ptr(get(w)), ptr(get(b)), ptr(y), ptr(s),
-                                                 ptr<int16_t>(low), ptr<float>(mean), ptr<float>(rstd), stream_of(x)));
+                                                 ptr(low), ptr<float>(mean), ptr<float>(rstd), stream_of(x)));
   if (!need_stats) return pybind11::make_tuple(y, s, pybind11::none(), pybind11::none());
   if (low.defined()) return pybind11::make_tuple(y, s, mean, pybind11::make_tuple(rstd, low));
   return pybind11::make_tuple(y, s, mean, rstd);
@@ -373,7 +373,7 @@ pybind11::object norm_drop_forward(const Tensor& x, const Opt& res, double p, co
 pybind11::object norm_drop_backward(const Tensor& gy, const Tensor& s, double p, const Tensor& rng, int64_t site, const Opt& w,
                                     const Tensor& mean, const Tensor& rstd, const Opt& low, const Opt& gsum, bool need_w, bool need_b, bool f32) {
   if (!norm_ok(s, w, Opt(), 0.0, f32) || !same_rows(gy, s) || (gsum && !same_rows(*gsum, s)) || !drop_ok(s, p, rng) ||
-      (low && (s.scalar_type() != at::kBFloat16 || !plain(*low, s) || low->scalar_type() != at::kShort || low->sizes() != s.sizes() ||
+      (low && (s.scalar_type() != at::kBFloat16 || !plain(*low, s) || low->scalar_type() != (f32 ? at::kShort : at::kChar) || low->sizes() != s.sizes() ||
                !low->is_contiguous())))
     return pybind11::none();
   const EgnnNormDims d = norm_dims(s, 0.0, f32);
@@ -385,7 +385,7 @@ pybind11::object norm_drop_backward(const Tensor& gy, const Tensor& s, double p,
   const Tensor gw = need_w ? at::empty({d.C}, param) : Tensor(), gb = need_b ? at::empty({d.C}, param) : Tensor();
   const size_t nb = need_w || need_b ? egnn_norm_bwd_workspace_bytes(&d) : 0;
   const Tensor ws = workspace(nb, s);
-  check("egnn_norm_drop_bwd", egnn_norm_drop_bwd(&d, &dr, ptr(gy), d.C, ptr(s), d.C, ptr<int16_t>(get(low)), ptr(get(w)), ptr<float>(mean), ptr<float>(rstd),
+  check("egnn_norm_drop_bwd", egnn_norm_drop_bwd(&d, &dr, ptr(gy), d.C, ptr(s), d.C, ptr(get(low)), ptr(get(w)), ptr<float>(mean), ptr<float>(rstd),
                                                  ptr(get(gsum)), d.C, ptr(gx), ptr(gr), ptr(gw), ptr(gb), ptr(ws), nb, stream_of(s)));
   auto out = [](const Tensor& t) -> pybind11::object { return t.defined() ? pybind11::cast(t) : pybind11::none(); };
   return pybind11::make_tuple(gx, gr, out(gw), out(gb));

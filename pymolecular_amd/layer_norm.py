@@ -162,11 +162,15 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     return r[0] if residual is None else (r[0], r[1])
 
 
+def _low_dtype(param_dtype):
+    return torch.int16 if param_dtype == torch.float32 else torch.int8
+
+
 def layer_norm_dropout_forward(x, residual, drop, weight=None, bias=None, eps=1e-5, need_stats=True):
     """``egnn_norm_drop_fwd`` of ``s = residual + dropout(x)``, ``drop`` a :class:`pymolecular_amd.dropout.Dropout`:
-    returns ``(y, s, mean, rstd)`` as :func:`layer_norm_forward` does, but that beside float32 parameters the last one is
-    a pair ``(rstd, low)`` where ``s`` is bfloat16: what its rounding lost (int16, opaque), without which float32
-    gradients would be off by 2^-9."""
+    returns ``(y, s, mean, rstd)`` as :func:`layer_norm_forward` does, but that the last one is a pair ``(rstd, low)``
+    where ``s`` is bfloat16: what its rounding lost (opaque; int16 beside float32 parameters, else int8), without which
+    the gradients would be off by 2^-9."""
     r = _capi.ext().norm_drop_forward(x, residual, *drop, weight, bias, eps, need_stats)
     if r is not None:
         return r
@@ -188,7 +192,7 @@ def layer_norm_dropout_forward(x, residual, drop, weight=None, bias=None, eps=1e
     y, s = (torch.empty(shape, dtype=dt, device=dev) for _ in range(2))
     stats = torch.empty((2, n), dtype=torch.float32, device=dev) if need_stats else None
     mean, rstd = (stats[0], stats[1]) if need_stats else (None, None)
-    low = torch.empty(shape, dtype=torch.int16, device=dev) if need_stats and pdt != dt else None
+    low = torch.empty(shape, dtype=_low_dtype(pdt), device=dev) if need_stats and dt == torch.bfloat16 else None
     with torch.cuda.device(dev):
         check("egnn_norm_drop_fwd",
               _capi.lib().egnn_norm_drop_fwd(EgnnNormDims(n, c, _dtype_code(dt), eps, pdt != dt), d, x2.data_ptr(), x2.stride(0),
@@ -204,6 +208,8 @@ def layer_norm_dropout_backward(gy, s, drop, weight, mean, rstd, gsum=None, need
     bdt = wdt if bias_dtype is None else bias_dtype
     pdt = _param_dtype(s.dtype, wdt, bdt if need_bias else None)
     rstd, low = rstd if isinstance(rstd, tuple) else (rstd, None)
+    if low is not None and low.dtype == torch.int16:   # (the forward had a float32 bias alone)
+        pdt = torch.float32
     r = _capi.ext().norm_drop_backward(gy, s, *drop, weight, mean, rstd, low, gsum, need_weight, need_bias, pdt == torch.float32)
     if r is not None:
         return r[0], r[1], _as(r[2], wdt), _as(r[3], bdt)
@@ -218,7 +224,7 @@ def layer_norm_dropout_backward(gy, s, drop, weight, mean, rstd, gsum=None, need
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.device != dev:
             raise ValueError(f"{name} must be the forward's ({n},) float32 statistics")
-    if low is not None and (dt != torch.bfloat16 or low.dtype != torch.int16 or low.shape != shape or not low.is_contiguous()
+    if low is not None and (dt != torch.bfloat16 or low.dtype != _low_dtype(pdt) or low.shape != shape or not low.is_contiguous()
                             or low.device != dev):
         raise ValueError("rstd must be what the forward returned with s")
     g2 = _rows(gy if gy.dtype == dt else gy.to(dt))

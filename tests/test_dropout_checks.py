@@ -81,7 +81,7 @@ def test_norm_with_dropout_arguments_refused():
         d or dims(), dr or _drop(), g, 64, BUF, 64, low, None, BUF, BUF, BUF, ldgs, gx, gr, BUF, None, ws, nb, None)
     assert bwd(dims(C=0)) == bwd(dr=_drop(p=-1.0)) == 2 and bwd(g=None) == bwd(gx=None) == bwd(gr=None) == 1
     assert fwd(low=BUF) == bwd(low=BUF) == 2   # beside float32 rows
-    assert fwd(dims(dtype=1), low=BUF + 1) == bwd(dims(dtype=1), low=BUF + 1) == 4
+    assert fwd(dims(dtype=1, f32_params=1), low=BUF + 1) == bwd(dims(dtype=1, f32_params=1), low=BUF + 1) == 4
     assert bwd(ldgs=-1) == 3 and bwd(gr=BUF + 2) == 4 and bwd(ws=None) == bwd(nb=16) == 5
     assert L.egnn_norm_drop_fwd(dims(), None, *([BUF, 64] * 2), *([BUF] * 7), None) == 1
 

@@ -2,8 +2,9 @@
 
 Bounds.  A value that stays is x up: up is rounded to float32 (2^-24 of it at most; exact for p = 0 and 1/2), the product
 (2^-24), the sum with the residual (2^-24 of the sum), and the result to its dtype (half a step, eps / 2).  fp32 norms and
-gradients are held to 2e-6 normwise and bf16 gradients, which are made from the sum as it is stored, to 2 x 2^-9, as in
-test_layer_norm_gpu.py.
+gradients are held to 2e-6 normwise and bf16 ones to 2 x 2^-9, as in test_layer_norm_gpu.py.  Gradients are those of the sum
+before it is rounded: exactly beside float32 parameters, else to 2^-17 of it, which adds up to 2^-16 |mean| / std beside a
+rounding of 2^-8.
 """
 import numpy as np
 import pytest
@@ -141,14 +142,45 @@ def test_norm(n, c, dtype, params):
         assert rel(y, y_ref) <= tol
     for gsum in (None, gs):
         grads = layer_norm_dropout_backward(gy, s, drop, w, mean, rstd, gsum)
-        # from the sum as it is stored, or (float32 parameters) as it was
-        gr, gw, gb = ref.layer_norm_grads_ref(_np(gy), _np(s) if params == dtype else s_ref, _np(w), 1e-5, _np(gsum))
+        gr, gw, gb = ref.layer_norm_grads_ref(_np(gy), s_ref, _np(w), 1e-5, _np(gsum))
         gx = dropout_grad_ref(gr, 0.1, SEED, OFFSET + 5)
         assert [t.dtype for t in grads] == [dtype, dtype, params, params]
         errs = [rel(a, t) for a, t in zip(grads, (gx, gr, gw, gb))] if c > 1 else [0.0]
         print([f"{e:.1e}" for e in errs], flush=True)
         assert max(errs) <= tol and max(errs[2:], default=0.0) <= (2e-6 if params == F32 else tol)
         assert np.array_equal(_np(grads[0]) == 0, (gx == 0) | (_np(grads[1]) == 0))
+
+
+@pytest.mark.parametrize("params", [BF16, F32])
+@pytest.mark.parametrize("n,c", [(3000, 40), (3000, 259), (300, 4099)])
+def test_gradients_of_the_unrounded_sum(n, c, params):
+    # rows whose mean is four times their deviation: the stored sum's rounding would be 1e-2 of them
+    from pymolecular_amd.dropout import Dropout
+    from pymolecular_amd.layer_norm import layer_norm_dropout_backward, layer_norm_dropout_forward
+    x, gy = (_rand(i, n, c, dtype=BF16) for i in (1, 2))
+    r = (_rand(3, n, c) + 4 * _rand(4, n, 1).sign()).to(BF16)
+    w, b = (1 + 0.2 * _rand(5, c)).to(params), _rand(6, c).to(params)
+    drop = Dropout(0.25, _rng(), 1)
+    y, s, mean, rstd = layer_norm_dropout_forward(x, r, drop, w, b)
+    s_ref = dropout_ref(_np(x), 0.25, SEED, OFFSET + 1, _np(r))
+    gr, gw, gb = ref.layer_norm_grads_ref(_np(gy), s_ref, _np(w))
+    got = layer_norm_dropout_backward(gy, s, drop, w, mean, rstd)
+    rel = lambda a, t: np.linalg.norm(_np(a) - t) / np.linalg.norm(t)  # noqa: E731
+    # one rounding of the result, at most half a step; the statistics' 2^-24 |mean| / std, the sum's 2^-17 |mean| / std
+    half = 2.0 ** -8 if params == BF16 else 0.0
+    assert rel(got[1], gr) <= 2.0 ** -8 + 2.0 ** -14
+    assert rel(got[2], gw) <= half + (2.0 ** -14 if params == BF16 else 4e-6) and rel(got[3], gb) <= half + 2e-6
+    # rows of one value (no deviation): the gradient is 0 but for the gradient of the sum
+    one = torch.full((n, 1), 1.37, dtype=BF16, device="cuda")
+    y, s, mean, rstd = layer_norm_dropout_forward(x[:, :1].contiguous(), one, drop, w[:1], b[:1])
+    got = layer_norm_dropout_backward(gy[:, :1].contiguous(), s, drop, w[:1], mean, rstd)
+    assert float(got[1].float().abs().max()) == 0.0 == float(got[2].float().abs().max())
+    # a bias alone, and what another call returned
+    y, s, mean, rstd = layer_norm_dropout_forward(x, r, drop, None, b)
+    assert torch.equal(layer_norm_dropout_backward(gy, s, drop, None, mean, rstd, bias_dtype=params)[1],
+                       layer_norm_dropout_backward(gy, s, drop, None, mean, rstd, need_bias=False)[1])
+    with pytest.raises(ValueError, match="rstd"):
+        layer_norm_dropout_backward(gy, s, drop, None, mean, (rstd[0], rstd[1][:1]))
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
