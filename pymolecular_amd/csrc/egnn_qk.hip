@@ -13,17 +13,12 @@
 // a head's pieces are half lines.  Small calls are bound by the launch, the positions, the barrier behind the angles and the rows:
 // 64 x 10 heads of 64, forward 5.8 us.
 #include "egnn_internal.h"
+#include "egnn_qk_plan.h"
 #include "egnn_rows.h"
 #include <cmath>
 
 namespace egnn {
 namespace qk {
-
-constexpr int NT = 256;
-constexpr int kPairs = 64;                   // pairs of a head at most
-constexpr int kTable = 2304;                 // cos and sin of a tile at most: 18 KB
-constexpr int kHeads = 4096;
-constexpr int64_t kMaxGrid = int64_t(1) << 20;
 
 struct Side {
   const void *x, *w, *g;
@@ -32,7 +27,7 @@ struct Side {
   float* part;                               // [blocks][D] sums of gw
   int64_t xr, xh, gr, gh, yr, yh;            // strides of rows and heads
   int32_t H;                                 // heads
-  uint32_t magic;                            // u / H = the high word of u magic (H > 1)
+  uint32_t magic;                            // reciprocal(H)
 };
 struct Args {
   Side s[2];
@@ -333,45 +328,6 @@ template <typename P> __global__ __launch_bounds__(1024) void sum_kernel(Args a)
   if (!k && f < a.D && s.gw) ((P*)s.gw)[f] = from_f32<P>(red[0][c]);
 }
 
-// Widest piece that fits 16 bytes (8 in the backward) and never lies across the rotated part's middle or end.  The backward
-// with pieces of 8 bf16 holds 184 registers, two waves a SIMD, with 4 it holds 113: 32,768 x 8 heads of 32, 24.5 and 16.3 us;
-// 1,048,576 x 3 heads of 128, 757 and 613; only the largest tensors of narrow heads lose, 2,000,000 x 8 heads of 32, 660 and 712.
-static int piece_of(const EgnnQkDims* d, bool bwd) {
-  int v = d->dtype == EGNN_F32 || bwd ? 4 : 8;
-  const int half = d->D / 2, r = d->rotary / 2;
-  while (v > 1 && (half % v || (!d->interleaved && r % v))) v /= 2;
-  return v;
-}
-static int lanes_of(const EgnnQkDims* d, bool bwd) {
-  int l = 1;
-  while (l * piece_of(d, bwd) < d->D / 2) l *= 2;
-  return l;
-}
-// Workgroups that small calls are spread over, and partial rows of the weight gradients.  Each costs its start, about 4 ns:
-// with 512, 1,024, 2,048 and 4,096, forward of 4,096 x 8 heads of 32 bf16 5.6, 6.6, 10.8 and 19.0 us, of 32,768 x 10 heads of 64
-// 18.1, 16.7, 19.4 and 25.8; backward with 512, 1,024 and 2,048 10.8, 13.2 and 21.8 us, and 35.0, 29.1 and 34.5.
-static int blocks_for(const EgnnQkDims* d, bool bwd) {
-  const int64_t values = d->N * (d->Hq + d->Hk) * d->D;
-  return values < 1 << 20 ? 256 : values < (bwd ? 4 : 8) << 20 ? 512 : 1024;
-}
-// Rows of a tile: enough heads of the side with fewer of them for two of each group of lanes, but a tile for each workgroup first
-static int tile_rows(const EgnnQkDims* d, bool bwd) {
-  const int H = d->Hq < d->Hk ? d->Hq : d->Hk;
-  const int groups = NT / lanes_of(d, bwd);
-  int64_t tb = groups * 2 / H;
-  if (tb > kTable / (d->D / 2 + 2)) tb = kTable / (d->D / 2 + 2);
-  if (tb > cdiv(d->N, blocks_for(d, bwd))) tb = cdiv(d->N, blocks_for(d, bwd));
-  int m = groups;                            // whole rounds of the groups over the heads
-  for (int h = H; h % 2 == 0 && m > 1; h /= 2) m /= 2;
-  if (tb > m) tb = tb / m * m;
-  return tb < 1 ? 1 : (int)tb;
-}
-static int32_t blocks_of(const EgnnQkDims* d, bool bwd) {
-  const int64_t most = bwd ? blocks_for(d, true) : kMaxGrid;
-  const int64_t tiles = cdiv(d->N, tile_rows(d, bwd));
-  return (int32_t)(tiles < most ? tiles : most);
-}
-
 template <typename T, int VEC>
 static void launch(const Args& a, bool bwd, hipStream_t st) {
   const uint32_t grid = (uint32_t)a.blocks;
@@ -397,7 +353,7 @@ static int run(const EgnnQkDims* d, Args& a, bool bwd, hipStream_t st) {
   for (int i = 0; i < 2; ++i) {
     Side& s = a.s[i];
     s.H = i ? d->Hk : d->Hq;
-    s.magic = s.H > 1 ? (uint32_t)(((uint64_t(1) << 32) + s.H - 1) / s.H) : 0;
+    s.magic = reciprocal(s.H);
   }
   a.inv = 1.f / d->D;
   a.TB = tile_rows(d, bwd);
