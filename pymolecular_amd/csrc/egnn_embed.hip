@@ -562,11 +562,11 @@ __global__ __launch_bounds__(FT) void fix_kernel(BwdArgs a, const uint32_t* tota
         for (int i = 0; i < nv; ++i) at[i + 1] = at[i] + (int32_t)total[v0 + i];
       }
     } else if (s1 - s0 <= kFew) {            // few tokens: each looks whether it begins the next rows
-      for (int32_t p = s0 + threadIdx.x; p <= s1; p += FT) {
+      for (int64_t p = s0 + (int64_t)threadIdx.x; p <= s1; p += FT) {   // (past s1 it may pass 2^31)
         // (tokens of the digit's rows before and behind these count as one row there)
         const int64_t v = p < s1 ? (int64_t)(a.sorted[p] >> 32) - v0 : nv;
         const int64_t u = p > s0 ? (int64_t)(a.sorted[p - 1] >> 32) - v0 + 1 : 0;
-        for (int r = (int)(u > 0 ? u : 0); r <= (v < nv ? v : nv); ++r) at[r] = p;
+        for (int r = (int)(u > 0 ? u : 0); r <= (v < nv ? v : nv); ++r) at[r] = (int32_t)p;
       }
     } else if ((int)threadIdx.x <= nv) {     // many: by halving
       int32_t lo = s0, hi = s1;
