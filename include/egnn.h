@@ -444,7 +444,8 @@ typedef struct EgnnEmbedDims {
 int32_t egnn_embed_fwd(const EgnnEmbedDims* dims, const void* tokens, const void* weight, int64_t ldw, void* out, void* stream);
 size_t egnn_embed_bwd_workspace_bytes(const EgnnEmbedDims* dims);
 /* Writes grad_weight (V, C), contiguous; the row of `padding` (-1: none) becomes 0.
- * fp32 sums in a fixed order, no atomics on values. */
+ * fp32 sums of parts, those of long runs added up in 64 bits: in a fixed order, no
+ * atomics on values. */
 int32_t egnn_embed_bwd(const EgnnEmbedDims* dims, int64_t padding, const void* grad_out, int64_t ldg, const void* tokens,
                        void* grad_weight, void* workspace, size_t workspace_bytes, void* stream);
 
