@@ -21,7 +21,7 @@ from ...dropout import Dropout, dropout
 from ...embedding import embedding
 from ...layer_norm import layer_norm, layer_norm_dropout
 from ...node_update import dense
-from ...qk_norm_rotary import qk_norm_rotary_attention
+from ...qk_norm_rotary import MAX_HEAD_DIM, qk_norm_rotary_attention
 from ...segment_attention import segment_attention, segment_attention_qkv
 from .egnn_clean import E_GCL, _csr_cache
 
@@ -58,6 +58,9 @@ class GlobalAttention(nn.Module):
         super().__init__()
         self.heads, self.kv_heads = heads, heads if kv_heads is None else kv_heads
         d = _head_dim(hidden_nf, heads, self.kv_heads)
+        if qk_norm and (d % 2 or d > MAX_HEAD_DIM):
+            raise ValueError(f"qk_norm needs heads of an even width up to {MAX_HEAD_DIM} (hidden_nf {hidden_nf} / heads "
+                             f"{heads} is {d})")
         self.qkv = nn.Linear(hidden_nf, (heads + 2 * self.kv_heads) * d)
         self.out = nn.Linear(hidden_nf, hidden_nf)
         self.qk_norm, self.rotary_base = qk_norm, rotary_base
