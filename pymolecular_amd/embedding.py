@@ -5,8 +5,9 @@
 Tokens (int32 or int64, any shape) name node types, elements, residues or fragments.  The gradient sorts them first, so that
 each row of ``grad_out`` is read once and each row of the table is written once, with sums in a fixed order (float32; the
 parts of a long run in 64 bits).  A token outside the table has a row of zeros and no gradient; the row ``padding`` is read
-as any other and gets no gradient.  Rows are float32 or bfloat16; a float32 table beside bfloat16 rows keeps the gradients in float32
-(``egnn_embed_fwd`` / ``egnn_embed_bwd`` in include/egnn.h).  There is no reference function for this step, and no CPU path: ROCm tensors only.
+as any other and gets no gradient.  Rows are float32 or bfloat16; a float32 table beside bfloat16 rows keeps the gradients in
+float32 (``egnn_embed_fwd`` / ``egnn_embed_bwd`` in include/egnn.h).  There is no reference function for this step, and no CPU
+path: ROCm tensors only.
 """
 from __future__ import annotations
 
