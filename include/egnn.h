@@ -417,8 +417,9 @@ int32_t egnn_dropout(const EgnnDropout* drop, int32_t dtype, int64_t N, int32_t 
  * not optional here; workspace: egnn_norm_bwd_workspace_bytes.  low (N, C), int16
  * beside fp32 parameters and int8 otherwise, takes what the rounding of a bf16 sum
  * lost, and gives it back to the backward, whose gradients are those of the
- * unrounded sum then (to 2^-17 of it with int8).  It may be NULL (in both): the
- * gradients are those of the stored sum, off by 2^-9; it has to be beside fp32 rows. */
+ * unrounded sum then (with int8, of one within 2^-16 of it, within 2^-15 for one
+ * value in 512).  It may be NULL (in both): the gradients are those of the stored
+ * sum, off by up to 2^-8; it has to be beside fp32 rows. */
 int32_t egnn_norm_drop_fwd(const EgnnNormDims* dims, const EgnnDropout* drop, const void* x, int64_t ldx, const void* residual,
                            int64_t ldr, const void* weight, const void* bias, void* y, void* sum, void* low, float* mean,
                            float* rstd, void* stream);

@@ -41,9 +41,11 @@ struct Args {
 
 constexpr int NT = 256;
 
-// What a bf16 sum's rounding lost: the fp32 value's bits less those of the rounded one, all 16 of them (L = int16_t: the two
-// make the value again, but for one unit of 2^-24 at ties) or the upper 8 (int8_t: to 2^-17).  From the rounded sum alone the
-// gradients would carry its rounding, 2^-9: as much again as their own where they are bf16 (errors of gw 2.5e-3 to 3.9e-3 of its norm,
+// What a bf16 sum's rounding lost: the fp32 value's bits less those of the rounded one, -32,768 to 32,768 of them, in full (L =
+// int16_t: the two make the value again, but for one unit in 2^23 at ties) or in steps of 256 (int8_t: to 128 units, 2^-16 of
+// the value at most, and to 256 in the one of 512 values that lie past the byte's 127 steps; in steps of 257 none would, but sums
+// that cancelled, whose last 8 bits are 0, would no longer come back whole).  From the rounded sum alone the gradients would
+// carry its rounding, up to 2^-8: as much again as their own where they are bf16 (errors of gw 2.5e-3 to 3.9e-3 of its norm,
 // 1.7e-3 with the byte), and 10^4 times as much where the parameters are fp32.
 template <typename L, bool TAIL> struct Low {
   typedef L type __attribute__((ext_vector_type(8), aligned(sizeof(L))));

@@ -170,7 +170,7 @@ def layer_norm_dropout_forward(x, residual, drop, weight=None, bias=None, eps=1e
     """``egnn_norm_drop_fwd`` of ``s = residual + dropout(x)``, ``drop`` a :class:`pymolecular_amd.dropout.Dropout`:
     returns ``(y, s, mean, rstd)`` as :func:`layer_norm_forward` does, but that the last one is a pair ``(rstd, low)``
     where ``s`` is bfloat16: what its rounding lost (opaque; int16 beside float32 parameters, else int8), without which
-    the gradients would be off by 2^-9."""
+    the gradients would be off by up to 2^-8."""
     r = _capi.ext().norm_drop_forward(x, residual, *drop, weight, bias, eps, need_stats)
     if r is not None:
         return r
