@@ -457,8 +457,9 @@ int32_t egnn_embed_bwd(const EgnnEmbedDims* dims, int64_t padding, const void* g
  * then the pairs (a, b) of its first `rotary` values are turned by the angle
  * position base^(-2 i / rotary), i the pair's number: (a cos - b sin, b cos + a sin).
  * Pairs are (y_i, y_{i + rotary / 2}), or neighbours (y_2i, y_2i+1) if interleaved.
- * The angle is position times frequency to 2^-30 turns for positions up to 2^32 in
- * magnitude: their product is made in 64-bit fixed point.  The weights may be NULL
+ * Position times frequency is made in 64-bit fixed point, to 2^-29 turns for
+ * positions up to 2^32 in magnitude (further ones lose in proportion, and nearer ones
+ * less), and its fraction of a turn is rounded to fp32.  The weights may be NULL
  * (1), and the positions where nothing is turned. */
 typedef struct EgnnQkDims {
   int64_t N;             /* rows, below 2^31 */

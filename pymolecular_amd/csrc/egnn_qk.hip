@@ -4,8 +4,9 @@
 // One pass: a head lives in the registers of a few lanes, each of which holds both values of its pairs, so that nothing but
 // the two row sums crosses lanes.  The angles depend on the row alone: a workgroup makes cos and sin of its rows once, in LDS,
 // for all its heads, queries' and keys'; a thread has one pair's frequency and takes every so many rows.  An angle is position
-// times frequency in turns, as a 64-bit fixed-point product whose overflow is the whole turns: exact for any position, with no
-// large argument to reduce.  cos and sin come from their Taylor series on an eighth of a turn to either side.
+// times frequency in turns, as a 64-bit fixed-point product whose overflow is the whole turns, so there is no large argument to
+// reduce; the frequency is rounded to such a fixed-point number, and the position multiplies what that loses (frequencies()).
+// cos and sin come from their Taylor series on an eighth of a turn to either side.
 // Bound by HBM where there are many rows: 2,000,000 x 8 heads of 32 bf16, forward 394 us and backward 681 us, 5.2 and 4.5 TB/s (a
 // large copy 5.3; queries and keys in workgroups of their own, which makes the angles twice, 600 and 783).  The backward holds
 // weights and their gradients of both sides, 113 to 117 registers: four waves a SIMD; two heads at once instead of one take 138,
@@ -15,7 +16,6 @@
 #include "egnn_internal.h"
 #include "egnn_qk_plan.h"
 #include "egnn_rows.h"
-#include <cmath>
 
 namespace egnn {
 namespace qk {
@@ -346,10 +346,7 @@ static int run(const EgnnQkDims* d, Args& a, bool bwd, hipStream_t st) {
   const int vec = piece_of(d, bwd), half = d->D / 2;
   a.N = d->N; a.D = d->D; a.rot = d->rotary; a.lanes = lanes_of(d, bwd); a.act = half / vec; a.eps = d->eps;
   a.il = d->interleaved; a.f32 = d->f32_params; a.i64 = d->index64;
-  // base^(-2 i / rotary) / 2 pi in units of 2^-64, by repeated multiplication in extended precision
-  const long double step = d->rotary ? powl((long double)d->base, -2.0L / d->rotary) : 1.0L;
-  long double f = 18446744073709551616.0L / 6.283185307179586476925286766559L;
-  for (int i = 0; i < d->rotary / 2; ++i, f *= step) a.freq[i] = (uint64_t)(f + 0.5L);
+  frequencies(d, a.freq);
   for (int i = 0; i < 2; ++i) {
     Side& s = a.s[i];
     s.H = i ? d->Hk : d->Hq;

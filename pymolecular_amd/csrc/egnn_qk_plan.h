@@ -1,6 +1,7 @@
 // How a call of the head norm with rotation is cut into pieces, tiles and workgroups: host arithmetic alone.
 #pragma once
 #include "../../include/egnn.h"
+#include <cmath>
 
 namespace egnn {
 namespace qk {
@@ -56,6 +57,15 @@ inline int32_t blocks_of(const EgnnQkDims* d, bool bwd) {
   const int64_t most = bwd ? blocks_for(d, true) : kMaxGrid;
   const int64_t tiles = ceil_div(d->N, tile_rows(d, bwd));
   return (int32_t)(tiles < most ? tiles : most);
+}
+
+// base^(-2 i / rotary) / 2 pi for the rotary / 2 pairs, turns a position, in units of 2^-64: by repeated multiplication in
+// extended precision (one power instead of 64), whose roundings make them wrong by up to 5 units for bases near 1, by less than
+// one from 100 on.  A position of 2^32 makes 2^-29 turns of the 5, one of 2^20 2^-41.
+inline void frequencies(const EgnnQkDims* d, uint64_t* freq) {
+  const long double step = d->rotary ? powl((long double)d->base, -2.0L / d->rotary) : 1.0L;
+  long double f = 18446744073709551616.0L / 6.283185307179586476925286766559L;
+  for (int i = 0; i < d->rotary / 2; ++i, f *= step) freq[i] = (uint64_t)(f + 0.5L);
 }
 
 }  // namespace qk

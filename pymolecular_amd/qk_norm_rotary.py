@@ -5,10 +5,10 @@
 ``q`` is (N, heads, d), ``k`` (N, kv_heads, d), with a weight (d,) each (None: 1).  The first ``rotary_dim`` values of a head
 (None: all of them) are turned by ``positions[n] * base ** (-2 i / rotary_dim)``, i the pair's number, so that the product of
 a query and a key depends on how far apart they are: residues of a chain.  Pairs are the first half and the second half of
-those values, or neighbours if ``interleaved``.  Positions are int32 or int64 and may be far (|position| <= 2^32 to 2^-30
-turns); without positions nothing is turned.  float32 or bfloat16 with fp32 sums, even head widths up to 128, parts of one
-projection's rows (``qkv[:, :heads]``) read where they lie.  The backward recomputes what it needs from the inputs
-(``egnn_qk_fwd`` / ``egnn_qk_bwd`` in include/egnn.h).  :func:`qk_norm_rotary_attention` puts
+those values, or neighbours if ``interleaved``.  Positions are int32 or int64 and may be far (|position| <= 2^32 to 2^-29
+turns, further ones in proportion); without positions nothing is turned.  float32 or bfloat16 with fp32 sums, even head widths
+up to 128, parts of one projection's rows (``qkv[:, :heads]``) read where they lie.  The backward recomputes what it needs from
+the inputs (``egnn_qk_fwd`` / ``egnn_qk_bwd`` in include/egnn.h).  :func:`qk_norm_rotary_attention` puts
 :func:`pymolecular_amd.segment_attention.segment_attention` behind it.  There is no reference function for this step, and no
 CPU path: ROCm tensors only.
 """

@@ -1,5 +1,8 @@
 """How a call of the head norm with rotation is cut into tiles: the host's rules (egnn_qk_plan.h), compiled for the CPU."""
 import subprocess
+from decimal import Decimal, getcontext
+
+import pytest
 
 from pymolecular_amd import _build
 
@@ -39,14 +42,46 @@ int main() {
 """
 
 
-def _run(tmp_path, program, *flags):
+def _run(tmp_path, program, *args):
     src, exe = tmp_path / "plan.cpp", tmp_path / "plan"
     src.write_text(program)
-    subprocess.run(["g++", "-O2", "-std=c++17", "-I", str(_build.CSRC), *flags, str(src), "-o", str(exe)], check=True)
-    return subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", str(_build.CSRC), str(src), "-o", str(exe)], check=True)
+    return subprocess.run([str(exe), *args], capture_output=True, text=True, timeout=120)
 
 
 def test_rows_of_a_tile_are_divided_exactly(tmp_path):
     r = _run(tmp_path, DIVISIONS)
     assert r.returncode == 0, r.stdout
     assert int(r.stdout) > 10 ** 7
+
+
+FREQUENCIES = r"""
+#include <cstdio>
+#include <cstdlib>
+#include "egnn_qk_plan.h"
+int main(int n, char** v) {
+  EgnnQkDims d{};
+  d.base = strtod(v[1], nullptr);
+  for (d.rotary = 2; d.rotary <= 128; d.rotary += 2) {
+    uint64_t f[64];
+    egnn::qk::frequencies(&d, f);
+    for (int i = 0; i < d.rotary / 2; ++i) printf("%d %d %llu\n", d.rotary, i, (unsigned long long)f[i]);
+  }
+}
+"""
+
+
+# extended precision carries 2^-64 of a frequency a rounding: of the power, i times over, and of i products; (2 i + 1) 2^-64
+# base^(-2 i / rotary) / 2 pi, and half a unit for the fixed point
+@pytest.mark.parametrize("base", ["1", "1.0001", "1.1", "2", "10", "100", "10000", "500000", "1e12"])
+def test_frequencies(tmp_path, base):
+    getcontext().prec = 50
+    unit = Decimal(2) ** 64 / (2 * Decimal("3.14159265358979323846264338327950288419716939937511"))
+    log, worst = Decimal(float(base)).ln(), 0
+    for line in _run(tmp_path, FREQUENCIES, base).stdout.split("\n")[:-1]:
+        rotary, i, f = map(int, line.split())
+        want = unit * (log * -2 * i / rotary).exp()
+        err = abs(f - want)
+        assert err <= Decimal("0.5") + (2 * i + 1) * want / 2 ** 64, (base, rotary, i)
+        worst = max(worst, err)
+    assert worst < (1 if float(base) >= 100 else 8)      # 2^-32 and 2^-29 turns at a position of 2^32
