@@ -486,7 +486,8 @@ int32_t egnn_qk_fwd(const EgnnQkDims* dims, const EgnnQkStrides* strides, const 
                     const void* k_weight, const void* positions, void* q_out, void* k_out, void* stream);
 size_t egnn_qk_bwd_workspace_bytes(const EgnnQkDims* dims);
 /* Backward from the inputs.  grad_q_weight and grad_k_weight (D) may be NULL, and
- * need the workspace otherwise; fixed-order sums, no atomics. */
+ * need the workspace otherwise; fixed-order sums, no atomics.  A head whose gradient
+ * is 0 throughout gets 0 and reaches nothing, whatever it holds. */
 int32_t egnn_qk_bwd(const EgnnQkDims* dims, const EgnnQkStrides* strides, const void* grad_q_out, const void* grad_k_out,
                     const void* q, const void* k, const void* q_weight, const void* k_weight, const void* positions,
                     void* grad_q, void* grad_k, void* grad_q_weight, void* grad_k_weight, void* workspace,

@@ -185,7 +185,7 @@ __global__ __launch_bounds__(NT) void qk_kernel(Args a) {
       }
       sum = lives ? sum : 0.f;
       for (int m = lanes / 2; m; m >>= 1) sum += shfl_xor(sum, m);
-      const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(sum, a.inv, a.eps));   // (to one unit of 2^-23)
+      float r = __builtin_amdgcn_rsqf(__builtin_fmaf(sum, a.inv, a.eps));   // (to one unit of 2^-23)
       float oa[VEC], ob[VEC];
       if constexpr (!BWD) {
 #pragma unroll
@@ -197,6 +197,20 @@ __global__ __launch_bounds__(NT) void qk_kernel(Args a) {
       } else {
         float ta[VEC], tb[VEC], dot = 0.f;
         to_pairs<VEC, IL>(raw[u].g0, raw[u].g1, ta, tb);
+        // A head whose gradient is 0 throughout takes no part, NaN and infinities of it neither: what an attention leaves out may
+        // hold anything.  (0 times a finite head is 0 anyway.)
+        if (__ballot(!(sum < __builtin_inff()))) {
+          float some = 0.f;                   // (how many of the gradient's pairs are not 0)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) some += (ta[i] != 0.f || tb[i] != 0.f) ? 1.f : 0.f;
+          some = lives ? some : 0.f;
+          for (int m = lanes / 2; m; m >>= 1) some += shfl_xor(some, m);
+          if (some == 0.f) {
+            r = 0.f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) va[i] = vb[i] = 0.f;
+          }
+        }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const float na = ta[i] * c[i] + tb[i] * sn[i], nb = tb[i] * c[i] - ta[i] * sn[i];

@@ -8,9 +8,10 @@ a query and a key depends on how far apart they are: residues of a chain.  Pairs
 those values, or neighbours if ``interleaved``.  Positions are int32 or int64 and may be far (|position| <= 2^32 to 2^-29
 turns, further ones in proportion); without positions nothing is turned.  float32 or bfloat16 with fp32 sums, even head widths
 up to 128, parts of one projection's rows (``qkv[:, :heads]``) read where they lie.  The backward recomputes what it needs from
-the inputs (``egnn_qk_fwd`` / ``egnn_qk_bwd`` in include/egnn.h).  :func:`qk_norm_rotary_attention` puts
-:func:`pymolecular_amd.segment_attention.segment_attention` behind it.  There is no reference function for this step, and no
-CPU path: ROCm tensors only.
+the inputs (``egnn_qk_fwd`` / ``egnn_qk_bwd`` in include/egnn.h); a head whose gradient is 0 throughout takes no part in it and
+may hold anything.  :func:`qk_norm_rotary_attention` puts :func:`pymolecular_amd.segment_attention.segment_attention` behind it,
+where masked keys and rows outside every segment are such heads.  There is no reference function for this step, and no CPU path:
+ROCm tensors only.
 """
 from __future__ import annotations
 
