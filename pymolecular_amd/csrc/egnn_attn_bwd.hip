@@ -5,7 +5,7 @@
 // heads of the group); each sum is made by one owner in a fixed order, so there are no atomics.  That takes seven products
 // (eight in bf16, below) where one kernel with atomics on dq would take five.
 //
-// delta.  o is the rounded output, so in bf16 do . o is off by up to 2^-9 |do| |o|, and the ds made with it sum to that
+// delta.  o is the rounded output, so in bf16 do . o is off by up to 2^-8 |do| |o|, and the ds made with it sum to that
 // instead of 0.  Where keys and values have a common part (a projection's bias), o has it too and dq takes the error times
 // that of the keys: with three times the spread of the values in both, dq was off by 7 % of its norm at 512 keys and by 13 %
 // at 4,000, with ten times by as much as it is long.  As sum_j p_ij = 1, delta is also sum_j p_ij dp_ij, and the ds made with

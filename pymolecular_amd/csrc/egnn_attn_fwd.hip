@@ -5,7 +5,7 @@
 // precision in floating point, so that a step costs no maximum, no shuffle and no rescaling of the output.  A step whose
 // sum passes 2^10 (the first one always: m starts at the lowest float) is made again with its maximum as the reference.
 // The sum takes the unrounded probabilities (one more product, against ones, would sum the rounded ones at less
-// cost, and put up to 2^-9 into lse).
+// cost, and put up to 2^-8 into lse).
 //
 // Measured (the kernel alone, called back to back): 12,289 rows, 4 heads of 64, bf16, 196 us, 0.79 PFLOP/s, bound by vector
 // and MFMA issue, which do not overlap (0.50 and 0.32 of the cycles); one query of 8 heads on 2 over 2,000,000 keys 183 us,

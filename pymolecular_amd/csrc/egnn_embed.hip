@@ -11,7 +11,7 @@
 //    us, floor 97; 19,456 x 128 9.7 + 3.9 us, where it waits for two rounds of tokens, one of rows and the barriers between.
 //  - sorted: counting sorts of (token, row) by digits of up to 11 bits, then the sums over tiles of the sorted order, and a launch
 //    that joins the runs that cross tiles and clears the rows that no token names.  40,961 x 259 fp32 over 50,021 rows 54 us: two
-//    sorts of three launches 27, the sums 18, the rest 15; its floor is 18, and each of the eight launches waits on memory two or
+//    sorts of three launches 25, the sums 18, the rest 14; its floor is 18, and each of the eight launches waits on memory two or
 //    three times.  Counts that a scatter adds up by itself instead of scan_kernel cost as much (66 us and 64).
 #include "egnn_internal.h"
 #include "egnn_rows.h"
@@ -659,7 +659,8 @@ static Plan plan_of(const EgnnEmbedDims* d) {
   if (p.local) {
     // Partial tables: at most half as many rows as there are tokens, and none up to 4,096 tokens.  Chunks of 256 tokens or more,
     // of 512 among many (100,000 x 128 bf16 over 119 rows, 21.4 and 19.5 us; 19,456 x 128 with the forward 16.2 and 16.6), and
-    // up to 1,024 of them (2,000,000 x 128 over 119 rows 133 us, with 512 chunks 129; x 32 over 8 rows 46, and 51)
+    // up to 1,024 of them, which costs the wide rows less than it gives the narrow ones (2,000,000 x 128 over 119 rows 133 us, with
+    // 512 chunks 129; x 32 over 8 rows 46, and 51)
     int64_t K = N <= 4096 ? 1 : N / (2 * V);
     const int64_t least_chunk = N <= 65536 ? 256 : 512;
     if (K > cdiv(N, least_chunk)) K = cdiv(N, least_chunk);

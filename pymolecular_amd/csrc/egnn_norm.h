@@ -11,7 +11,7 @@
 // y is made from the sum as it is, before it is rounded to the type it is stored in.  The backward reads the stored one, so
 // where the mean exceeds the deviation the statistics kept for it are those of the stored one: with the others a row whose
 // values differ by less than their rounding would get any gradient (one column of bf16: hundreds of times too large, instead
-// of 0).  Elsewhere the two agree to 2^-9 of the deviation.  (For every row: 402 us instead of 360, 2,000,000 x 128 bf16.)
+// of 0).  Elsewhere the two agree to 2^-8 of the deviation.  (For every row: 402 us instead of 360, 2,000,000 x 128 bf16.)
 // Bound by HBM where the tensors are large: 2,000,000 x 128 bf16 with a residual, forward 337 us and backward 323 us, 6.1 and
 // 6.3 TB/s (each kernel alone, called back to back); 40,961 x 259 fp32, rows that cross lines, 18.4 and 23.6 us, 4.6 and 5.4
 // TB/s.  By its launches where they are small: 2,432 x 128 fp32, forward, 2.8 us.  Rows wider than a wave's registers are read

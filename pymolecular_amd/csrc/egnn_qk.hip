@@ -7,9 +7,9 @@
 // times frequency in turns, as a 64-bit fixed-point product whose overflow is the whole turns, so there is no large argument to
 // reduce; the frequency is rounded to such a fixed-point number, and the position multiplies what that loses (frequencies()).
 // cos and sin come from their Taylor series on an eighth of a turn to either side.
-// Bound by HBM where there are many rows: 2,000,000 x 8 heads of 32 bf16, forward 394 us and backward 681 us, 5.2 and 4.5 TB/s (a
+// Bound by HBM where there are many rows: 2,000,000 x 8 heads of 32 bf16, forward 394 us and backward 686 us, 5.2 and 4.5 TB/s (a
 // large copy 5.3; queries and keys in workgroups of their own, which makes the angles twice, 600 and 783).  The backward holds
-// weights and their gradients of both sides, 113 to 117 registers: four waves a SIMD; two heads at once instead of one take 138,
+// weights and their gradients of both sides, 104 to 121 registers: four waves a SIMD; two heads at once instead of one take 138,
 // three waves, and 445 instead of 356 us for 1,000,000 rows.  Loads and stores past the cache are slower here (476 us forward):
 // a head's pieces are half lines.  Small calls are bound by the launch, the positions, the barrier behind the angles and the rows:
 // 64 x 10 heads of 64, forward 5.8 us.

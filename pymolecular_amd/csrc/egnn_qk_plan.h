@@ -19,7 +19,7 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline uint32_t reciprocal(int32_t H) { return H > 1 ? (uint32_t)(((uint64_t(1) << 32) + H - 1) / H) : 0; }
 
 // Widest piece that fits 16 bytes (8 in the backward) and never lies across the rotated part's middle or end.  The backward
-// with pieces of 8 bf16 holds 184 registers, two waves a SIMD, with 4 it holds 113: 32,768 x 8 heads of 32, 24.5 and 16.3 us;
+// with pieces of 8 bf16 holds 184 registers, two waves a SIMD, with 4 it holds 116: 32,768 x 8 heads of 32, 24.5 and 16.3 us;
 // 1,048,576 x 3 heads of 128, 757 and 613; only the largest tensors of narrow heads lose, 2,000,000 x 8 heads of 32, 660 and 712.
 inline int piece_of(const EgnnQkDims* d, bool bwd) {
   int v = d->dtype == EGNN_F32 || bwd ? 4 : 8;

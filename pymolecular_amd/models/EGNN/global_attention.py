@@ -38,7 +38,8 @@ def _head_dim(hidden_nf, heads, kv_heads):
 class TypeEmbedding(nn.Module):
     """One vector a node type: hidden_nf ** 0.5 times a row of a table whose rows have length of about 1.  ``dtype``: of
     the vectors (None: the table's; bfloat16 beside a float32 table keeps its gradients in float32).  The row
-    ``padding_type`` gets no gradient."""
+    ``padding_type`` gets no gradient.  A type outside the table has a vector of zeros and no gradient; it is not an error,
+    which would have to wait for the device."""
 
     def __init__(self, n_types, hidden_nf, padding_type=None, dtype=None):
         super().__init__()
