@@ -198,8 +198,9 @@ __global__ __launch_bounds__(NT) void qk_kernel(Args a) {
         float ta[VEC], tb[VEC], dot = 0.f;
         to_pairs<VEC, IL>(raw[u].g0, raw[u].g1, ta, tb);
         // A head whose gradient is 0 throughout takes no part, NaN and infinities of it neither: what an attention leaves out may
-        // hold anything.  (0 times a finite head is 0 anyway.)
-        if (__ballot(!(sum < __builtin_inff()))) {
+        // hold anything.  (0 times a finite head is 0 anyway, but for one of zeros without eps, whose r is infinite; that of NaN is
+        // NaN, that of infinities 0.)
+        if (__ballot(!(r > 0.f && r < __builtin_inff()))) {
           float some = 0.f;                   // (how many of the gradient's pairs are not 0)
 #pragma unroll
           for (int i = 0; i < VEC; ++i) some += (ta[i] != 0.f || tb[i] != 0.f) ? 1.f : 0.f;

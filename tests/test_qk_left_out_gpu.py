@@ -63,3 +63,16 @@ def test_left_out_by_the_attention(rows, d, heads, kv):
     got, want = run(bad), run(qkv)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert not got[0][outside].any() and not got[1][outside].any() and not got[1][~mask, heads:].any()
+
+
+@pytest.mark.parametrize("rows", [F32, BF16])
+@pytest.mark.parametrize("d", [32, 10])
+def test_heads_of_zeros_without_eps(rows, d):
+    # 0 / 0 in the forward, as the formula has it; without a gradient (a batch padded with zeros) such heads get 0
+    from pymolecular_amd.qk_norm_rotary import qk_norm_rotary_backward
+    q, gq, w, pos = _rand(1, 90, 4, d, dtype=rows), _rand(2, 90, 4, d, dtype=rows), _rand(3, 2, d, dtype=rows), torch.arange(90, device="cuda")
+    gq[70:], gq[:, 3] = 0, 0
+    want = qk_norm_rotary_backward(gq, gq, q, q, w[0], w[1], pos, eps=0.0)
+    q[70:], q[::2, 3] = 0, 0
+    got = qk_norm_rotary_backward(gq, gq, q, q, w[0], w[1], pos, eps=0.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not got[0][70:].any()
